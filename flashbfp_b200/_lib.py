@@ -79,6 +79,13 @@ _PROTOS = {
                                     _vp]),
     "fbfp_expand_x15": (_c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _vp, _vp,
                                  _c_i64, _vp, _c_i64, _vp]),
+    "fbfp_fp8_scale_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "fbfp_fp8_quantize": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "fbfp_fp8_rmsnorm": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, ctypes.c_float,
+                                  _vp, _c_i64, _vp, _vp]),
+    "fbfp_fp8_geglu": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "fbfp_fp8_linear": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _vp,
+                                 _c_int, _c_i64, _vp, _vp]),
     "fbfp_compress_scratch_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "fbfp_compress_threshold": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
     "fbfp_compress_pack": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp,

@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "pdl.cuh"
 #include "sm100.cuh"
 
 namespace fbfp {
@@ -61,28 +62,6 @@ __device__ float block_max(float v, float* red) {
 }
 
 constexpr int kNormThreads = 512;
-
-__device__ __forceinline__ void pdl_prologue() {
-  sm100::grid_dependency_wait();
-  sm100::grid_launch_dependents();
-}
-
-// Launch with programmatic stream serialisation (see the top of this file).
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                              cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // Row r of every kernel below is the token at position *pos + r (M rows: a prompt chunk, or
 // one token when decoding).

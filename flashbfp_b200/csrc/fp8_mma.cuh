@@ -1,0 +1,94 @@
+// fp8_mma.cuh — the sm_100a instructions of the block-scaled e4m3 product: tcgen05.mma with scale
+// factors in tensor memory, and the copies that bring those there.
+//
+// kind::mxf8f6f4 multiplies a 32-wide K slice by one power-of-two scale per row of each operand.
+// Tensor memory holds the scales of 128 rows in 4 columns: row r in lane r % 32, column r / 32,
+// one 32-bit word of 4 scales per row (the same words in all four lane quarters); the instruction
+// descriptor picks the byte. One 512-byte tile (32 x 16 bytes) in shared memory is exactly that,
+// and one tcgen05.cp places it. With one scale per 128 values a word covers 512 values of K: the
+// four K slices of block b use byte b % 4.
+#pragma once
+#include <stdint.h>
+
+#include "sm100.cuh"
+
+namespace fbfp {
+namespace sm100 {
+
+// Instruction descriptor of kind::mxf8f6f4: e4m3 A and B, both K-major, fp32 D, UE8M0 scales,
+// without the scale bytes' ids.
+__host__ __device__ constexpr uint32_t idesc_mxf8(uint32_t m, uint32_t n) {
+  return ((n >> 3) << 17)                // N / 8
+       | (1u << 23)                      // scales: UE8M0
+       | ((m >> 4) << 24);               // M / 16
+}
+// The same with byte `id` (0..3) of both operands' scale words.
+__device__ __forceinline__ uint32_t idesc_mxf8_id(uint32_t idesc, uint32_t id) {
+  return idesc | (id << 4) | (id << 29);
+}
+
+// Shared-memory descriptor of a 512-byte scale tile: 32 rows of 16 bytes, no swizzle, 8-row
+// groups 128 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;                 // descriptor version for sm_100
+  return d;
+}
+
+// 32 lanes x 16 bytes to 4 columns of tensor memory, repeated in the four lane quarters. Copies and
+// MMAs of one thread execute in order.
+template <int CG>
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// D[tmem] (+)= (A[smem] * scale_A) * (B[smem] * scale_B).
+template <int CG>
+__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
+
+// ---------------------------------------------------------------- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n"
+      "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// Address of this CTA's shared-memory address `saddr` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_shared(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+}  // namespace sm100
+}  // namespace fbfp

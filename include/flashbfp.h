@@ -377,6 +377,40 @@ int fbfp_decode_attention_step(const void* qkv, int64_t b, int64_t nh, int64_t n
                                void* stream);
 int fbfp_advance_positions(int32_t* pos, int64_t b, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Block-scaled 8-bit linears (no counterpart in the reference). A row operand is `values`, e4m3
+ * rows (row pitch ldv / ldx / ldw bytes, a multiple of 16, 16-byte aligned), and `scales`,
+ * fbfp_fp8_scale_bytes(rows, k) bytes (16-byte aligned): one byte c per row and 128 values, worth
+ * 2^(c - 127), in tiles of 128 rows x 4 blocks of 512 bytes each: the scale of (row r, block b)
+ * is byte ((r / 128) * ceil(k / 512) + b / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4.
+ * c is the smallest integer >= 0 with max|block| / 2^(c - 127) <= 448; values are rounded to
+ * nearest even. A block with an infinity or NaN gets c = 255 and NaN values. Tile bytes past the
+ * last row or block are written as 0.
+ *
+ * fbfp_fp8_quantize: rows x[m][k] (any fbfp_dtype, row stride ldx elements).
+ * fbfp_fp8_rmsnorm: RMSNorm(h; w) = h * rsqrt(mean(h^2) + eps) * (1 + w) quantised, with h = x
+ *   (resid null), x + resid (w_post null) or RMSNorm(x; w_post) + resid; with resid, h rounded to
+ *   its type replaces resid (the norm reads the unrounded h). All of one dtype, k <= 32768; x may
+ *   be resid itself.
+ * fbfp_fp8_geglu: gelu_tanh(gate) * up quantised, for rows [gate (inter) | up (inter)].
+ * fbfp_fp8_linear: y[m][n] = sum_k x[m][k] w[n][k] (+ bias[n]), scales applied, fp32 accumulation
+ *   on the tensor cores (tcgen05 block-scaled MMA), rounded once to y_dtype. `workspace`: 4 bytes
+ *   of zeroed device memory that record a bounded device-side wait that gave up (fbfp_gemv_check
+ *   reads and clears them); calls on any streams may share them.
+ * The outputs of one call must not overlap its inputs, apart from resid.
+ * ---------------------------------------------------------------------------------- */
+int64_t fbfp_fp8_scale_bytes(int64_t rows, int64_t k);
+int fbfp_fp8_quantize(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, void* values,
+                      int64_t ldv, void* scales, void* stream);
+int fbfp_fp8_rmsnorm(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, const void* w,
+                     const void* w_post, void* resid, int64_t ldr, float eps, void* values,
+                     int64_t ldv, void* scales, void* stream);
+int fbfp_fp8_geglu(const void* gate_up, int dtype, int64_t m, int64_t inter, int64_t ldx,
+                   void* values, int64_t ldv, void* scales, void* stream);
+int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void* x_scales,
+                    const void* w, int64_t n, int64_t ldw, const void* w_scales, const void* bias,
+                    int bias_dtype, void* y, int y_dtype, int64_t ldy, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
