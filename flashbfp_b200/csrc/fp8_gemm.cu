@@ -237,6 +237,268 @@ int launch_few(const Fp8Args& a, const Fp8Maps& M, int dev, int splits, cudaStre
   return FBFP_OK;
 }
 
+// ---------------------------------------------------------------------------------------
+// Many tokens. Persistent CTA pairs (cta_group::2): a pair takes tiles of 256 tokens x BN features,
+// tokens on the MMA's M side (128 per CTA), features on its N side (half of the weight rows in each
+// CTA's shared memory), so that each SM loads 128 + BN / 2 rows of 128 bytes per K block for
+// 128 x BN x 128 multiply-adds. Scale tiles are loaded once per 512 values of K, with the stage of
+// the group's first K block, and copied to one of kSfSlots slots of tensor memory; a slot is
+// written again only when MMAs of at least kStages later K blocks (or of a drained accumulator)
+// are due, so the MMAs that read it have completed. A tile starts on a whole scale tile (features
+// in steps of 128), which keeps the scales' tensor-memory addresses on multiples of 4 columns.
+template <int BN>
+struct Many {
+  static constexpr int kHalfN = BN / 2;
+  static constexpr int kChunks = BN / 128;                       // scale tiles of the features
+  static constexpr int kA = 128 * 128, kB = kHalfN * 128, kSf = 512 * (1 + kChunks);
+  static constexpr int kStage = kA + kB + 2048;
+  static constexpr int kStages = 6;
+  static constexpr int kBufs = BN == 256 ? 1 : 2;                // accumulators
+  static constexpr int kSfCols = 4 * (1 + kChunks), kSfSlots = 4;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 32 * (4 + kEpiWarps);
+  static constexpr uint32_t kTmemCols = 512, kSfCol0 = kBufs * BN;
+  static constexpr int kData = kStages * kStage;
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 1;
+  static constexpr size_t kSmem = kData + kBars * 8 + 16 + 1024;
+  static_assert(BN % 128 == 0 && kSf <= 2048, "features in whole scale tiles");
+  static_assert(kSfCol0 + kSfSlots * kSfCols <= (int)kTmemCols, "tensor memory budget");
+  static_assert(kSmem <= 232448, "shared memory budget");
+};
+
+struct ManyShared {
+  volatile int* abort_flag;
+  int32_t* err;
+};
+
+__device__ __forceinline__ bool many_wait(uint64_t* bar, uint32_t parity, const ManyShared& S, int site) {
+  for (uint32_t it = 0; it < (1u << 16); ++it) {
+    if (mbar_try_wait_cluster(bar, parity, 20000u)) return true;
+    if ((it & 15) == 15 && *S.abort_flag) return false;
+  }
+  *S.abort_flag = 1;
+  atomicExch(S.err, site);
+  return false;
+}
+
+// 32 consecutive features of one token. vec: y's rows and base are 32-byte aligned.
+__device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t row, int64_t f0, const float (&v)[32], bool vec) {
+  if (vec && f0 + 32 <= a.n) {
+    if (a.y_dtype == FBFP_F32) {
+      float* p = reinterpret_cast<float*>(a.y) + row * a.ldy + f0;
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p + 8 * h), "f"(v[8 * h]),
+                     "f"(v[8 * h + 1]), "f"(v[8 * h + 2]), "f"(v[8 * h + 3]), "f"(v[8 * h + 4]), "f"(v[8 * h + 5]),
+                     "f"(v[8 * h + 6]), "f"(v[8 * h + 7]) : "memory");
+    } else {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (a.y_dtype == FBFP_BF16) {
+          const __nv_bfloat162 h = __float22bfloat162_rn(make_float2(v[2 * i], v[2 * i + 1]));
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __half2 h = __float22half2_rn(make_float2(v[2 * i], v[2 * i + 1]));
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      uint16_t* p = reinterpret_cast<uint16_t*>(a.y) + row * a.ldy + f0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p + 16 * h), "r"(w[8 * h]),
+                     "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
+                     "r"(w[8 * h + 6]), "r"(w[8 * h + 7]) : "memory");
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (f0 + i < a.n) store_from_float(a.y, a.y_dtype, row * a.ldy + f0 + i, v[i]);
+  }
+}
+
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many<BN>::kThreads, 1)
+fp8_many_kernel(const Fp8Args a, const __grid_constant__ Fp8Maps M) {
+  using C = Many<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kData);   // used in CTA 0
+  uint64_t* empty = full + C::kStages;
+  uint64_t* acc_full = empty + C::kStages;
+  uint64_t* acc_empty = acc_full + 2;                               // used in CTA 0
+  uint64_t* tail = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 1);
+  ManyShared S;
+  S.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  S.err = a.err;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int64_t tiles = (a.n + BN - 1) / BN * a.n_tt;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * C::kEpiWarps); }
+    mbar_init(tail, 1);
+    *S.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, C::kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                                        // the peer's barriers are ready
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_prologue();
+
+  if (warp == 0) {
+    if (elect_one_sync()) {
+      prefetch_tmap(&M.w); prefetch_tmap(&M.x); prefetch_tmap(&M.ws); prefetch_tmap(&M.xs);
+      const uint32_t sbase = smem_u32(smem);
+      int s = 0;
+      uint32_t ph = 0;
+      int64_t issued = 0;
+      bool ok = true;
+      for (int64_t t = pair; t < tiles && ok; t += pairs) {
+        const int64_t m0 = t % a.n_tt * 256 + 128 * rank, n0 = t / a.n_tt * BN;
+        for (int kb = 0; kb < a.nkb; ++kb) {
+          if (!(ok = many_wait(&empty[s], ph ^ 1, S, 23))) break;
+          const uint32_t st = sbase + (uint32_t)s * C::kStage;
+          const uint32_t bar = map_shared(smem_u32(&full[s]), 0);
+          const bool sf = (kb & 3) == 0;
+          // CTA 0 expects both CTAs' bytes
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * (C::kA + C::kB + (sf ? C::kSf : 0)));
+          tma_2d_g2s_pair(st, &M.x, kb * 128, (int)m0, bar);
+          tma_2d_g2s_pair(st + C::kA, &M.w, kb * 128, (int)(n0 + rank * C::kHalfN), bar);
+          if (sf) {
+            tma_2d_g2s_pair(st + C::kA + C::kB, &M.xs, 0, (int)(m0 / 128 * a.kgroups + kb / 4), bar);
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c)         // tiles past the last one read as zero
+              tma_2d_g2s_pair(st + C::kA + C::kB + 512 * (1 + c), &M.ws, 0,
+                              (int)((n0 / 128 + c) * a.kgroups + kb / 4), bar);
+          }
+          ++issued;
+          if (++s == C::kStages) { s = 0; ph ^= 1; }
+        }
+      }
+      if (!ok) {                                         // copies in flight land before the pair exits
+        if (rank == 0)
+          for (int64_t j = issued > C::kStages ? issued - C::kStages : 0; j < issued; ++j)
+            mbar_wait(&full[j % C::kStages], (uint32_t)(j / C::kStages) & 1, 1u << 16);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1 && rank == 0) {
+    if (elect_one_sync()) {
+      constexpr uint32_t kIdesc = idesc_mxf8(256, BN);
+      const uint32_t sbase = smem_u32(smem);
+      const int64_t mine = pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0;
+      const int64_t total = mine * a.nkb;
+      int64_t it = 0;
+      int s = 0, buf = 0, slot = C::kSfSlots - 1;
+      uint32_t ph = 0, aph = 0;
+      bool ok = true;
+      for (int64_t t = pair; t < tiles && ok; t += pairs) {
+        if (!(ok = many_wait(&acc_empty[buf], aph ^ 1, S, 24))) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        uint32_t acc = 0, sfa = 0;
+        for (int kb = 0; kb < a.nkb; ++kb) {
+          if (!(ok = many_wait(&full[s], ph, S, 25))) break;
+          tc_fence_after();
+          const uint32_t st = sbase + (uint32_t)s * C::kStage;
+          if ((kb & 3) == 0) {
+            slot = slot == C::kSfSlots - 1 ? 0 : slot + 1;
+            sfa = tmem + C::kSfCol0 + slot * C::kSfCols;
+#pragma unroll
+            for (int c = 0; c < 1 + C::kChunks; ++c)
+              scales_to_tmem<2>(sfa + 4 * c, smem_desc_scales(st + C::kA + C::kB + 512 * c));
+          }
+          const uint64_t da = smem_desc_sw128(st, 1024), db = smem_desc_sw128(st + C::kA, 1024);
+          const uint32_t id = idesc_mxf8_id(kIdesc, kb & 3);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            mma_mxf8<2>(d, da + 2 * k, db + 2 * k, id, sfa, sfa + 4, acc);
+            acc = 1;
+          }
+          if (it + C::kStages < total) mma_commit_pair(&empty[s]);   // only where the producers wait for it
+          ++it;
+          if (++s == C::kStages) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+        mma_commit_pair(&acc_full[buf]);
+        if (++buf == C::kBufs) { buf = 0; aph ^= 1; }
+      }
+      if (!ok) {                                         // MMAs in flight end before the memory goes
+        mma_commit_pair(tail);
+        mbar_wait(tail, 0, 1u << 16);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // two warps per lane quarter, half of the columns each: the sums go to registers first, so that
+    // the accumulator is free again after the loads
+    constexpr int kCols = BN / 2;
+    const int q4 = warp & 3, row = q4 * 32 + lane, col0 = ((warp - 4) >> 2) * kCols;
+    const bool vec = ((uintptr_t)a.y & 31) == 0 && (a.ldy * (a.y_dtype == FBFP_F32 ? 4 : 2)) % 32 == 0;
+    int buf = 0;
+    uint32_t ph = 0;
+    for (int64_t t = pair; t < tiles; t += pairs) {
+      const int64_t tok = t % a.n_tt * 256 + 128 * rank + row, n0 = t / a.n_tt * BN + col0;
+      if (!__all_sync(0xffffffffu, many_wait(&acc_full[buf], ph, S, 26))) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + buf * BN + col0 + ((uint32_t)(q4 * 32) << 16);
+      float v[kCols / 32][32];
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, v[c]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[buf]), 0));
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        const int64_t f0 = n0 + 32 * c;
+        if (f0 >= a.n) break;                            // whole warps
+        if (a.bias) {
+          const float b = f0 + lane < a.n ? load_as_float(a.bias, a.bias_dtype, f0 + lane) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c][i] += __shfl_sync(0xffffffffu, b, i);
+        }
+        if (tok < a.m) store_y32(a, tok, f0, v[c], vec);
+      }
+      if (++buf == C::kBufs) { buf = 0; ph ^= 1; }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();                                        // no CTA leaves while its pair may still reach it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, C::kTmemCols);
+  }
+}
+
+template <int BN>
+int launch_many(const Fp8Args& a, const Fp8Maps& M, int dev, int nsm, cudaStream_t st) {
+  using C = Many<BN>;
+  static bool attr_set[64] = {false};
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    FBFP_CUDA_TRY(cudaFuncSetAttribute(fp8_many_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)C::kSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const int64_t tiles = (a.n + BN - 1) / BN * a.n_tt;
+  const int64_t pairs = tiles < nsm / 2 ? tiles : nsm / 2;
+  FBFP_CUDA_TRY(launch_pdl(fp8_many_kernel<BN>, dim3((unsigned)(2 * pairs)), dim3(C::kThreads), C::kSmem, st, a, M));
+  FBFP_LAUNCH_CHECK("fp8_many_kernel");
+  return FBFP_OK;
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -268,26 +530,29 @@ extern "C" int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx,
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
   const int nsm = sm_count(dev);
 
-  const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  a.n_tt = (m + bn - 1) / bn;
+  constexpr int kManyN = 256;
+  const bool many = m > 128;
+  const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;   // token rows of a tile (per CTA)
+  a.n_tt = many ? (m + 255) / 256 : (m + bn - 1) / bn;
   const int64_t xt = (m + 127) / 128 * a.kgroups, wt = (n + 127) / 128 * a.kgroups;
   FBFP_CHECK_ARG(xt < ((int64_t)1 << 31) && wt < ((int64_t)1 << 31), "too many scale tiles");
   Fp8Maps M;
   int rc;
   if ((rc = encode_2d(&M.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)k, (uint64_t)m, (uint64_t)ldx, 128,
                       (uint32_t)bn, CU_TENSOR_MAP_SWIZZLE_128B)) != FBFP_OK) return rc;
-  if ((rc = encode_2d(&M.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, (uint64_t)k, (uint64_t)n, (uint64_t)ldw, 128, 128,
-                      CU_TENSOR_MAP_SWIZZLE_128B)) != FBFP_OK) return rc;
+  if ((rc = encode_2d(&M.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, (uint64_t)k, (uint64_t)n, (uint64_t)ldw, 128,
+                      many ? kManyN / 2 : 128, CU_TENSOR_MAP_SWIZZLE_128B)) != FBFP_OK) return rc;
   if ((rc = encode_2d(&M.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, x_scales, 128, (uint64_t)xt, 512, 128, 1,
                       CU_TENSOR_MAP_SWIZZLE_NONE)) != FBFP_OK) return rc;
   if ((rc = encode_2d(&M.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, w_scales, 128, (uint64_t)wt, 512, 128, 1,
                       CU_TENSOR_MAP_SWIZZLE_NONE)) != FBFP_OK) return rc;
 
+  const cudaStream_t st = as_stream(stream);
+  if (many) return launch_many<kManyN>(a, M, dev, nsm, st);
   // split K over a cluster while that still fills idle SMs (two CTAs fit an SM)
   const int64_t tiles = (n + 127) / 128 * a.n_tt;
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= 2 * nsm && a.nkb >= splits * 4) splits *= 2;
-  const cudaStream_t st = as_stream(stream);
   switch (bn) {
     case 16: return launch_few<16>(a, M, dev, splits, st);
     case 32: return launch_few<32>(a, M, dev, splits, st);
