@@ -20,79 +20,93 @@ struct Fp8Args {
   const void* bias;
   int bias_dtype;
   void* y;
-  int y_dtype;
   int64_t ldy;
   int32_t* err;
   int64_t n_tt;            // token tiles
+  int stages;              // depth of the operand ring
 };
 
 struct Fp8Maps {
-  CUtensorMap x, w, xs, ws;       // the scales' maps: many tokens only
+  CUtensorMap x, w, xs, ws;       // the scales' maps: tiles of 128 tokens and more only
 };
 
-// Bounded wait (about a second), giving up early once another role of the CTA has.
-__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err,
-                                         int site) {
-  if (mbar_try_wait(bar, parity)) return true;
+constexpr int kMaxStages = 8;
+// Shared memory a CTA may take so that one or two fit an SM (228 KB, 1 KB of it per CTA reserved).
+constexpr int kSmemOne = 232448, kSmemTwo = 115712;
+
+// Where a role of a CTA gave up, and whom it tells.
+struct Abort {
+  volatile int* flag;
+  int32_t* err;
+};
+
+// Bounded wait (about a second), giving up early once another role of the CTA has. CLUSTER: other
+// CTAs arrive on the barrier too.
+template <bool CLUSTER>
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, const Abort& A, int site) {
   for (uint32_t it = 0; it < (1u << 16); ++it) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if ((it & 15) == 15 && *abort_flag) return false;
+    if (CLUSTER ? mbar_try_wait_cluster(bar, parity, 20000u) : mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    if ((it & 15) == 15 && *A.flag) return false;
   }
-  *abort_flag = 1;
-  atomicExch(err, site);
+  *A.flag = 1;
+  atomicExch(A.err, site);
   return false;
 }
 
-// Four consecutive features (the first is `feat`) at element `at` of y; vec: all four exist and
-// the address is aligned for one store.
-__device__ __forceinline__ void store4(const Fp8Args& a, int64_t at, int64_t feat, float v0, float v1, float v2,
-                                       float v3, bool vec) {
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(make_float2(a, b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 h = __float22half2_rn(make_float2(a, b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void round_to(float v, float& o) { o = v; }
+__device__ __forceinline__ void round_to(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void round_to(float v, __half& o) { o = __float2half_rn(v); }
+
+// Four consecutive features at p; n of them exist; vec: all four, and p is aligned for one store.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int n, const float4& v, bool vec) {
   if (vec) {
-    if (a.y_dtype == FBFP_F32) {
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.y) + at) = make_float4(v0, v1, v2, v3);
-    } else if (a.y_dtype == FBFP_BF16) {
-      const __nv_bfloat162 h[2] = {__float22bfloat162_rn(make_float2(v0, v1)),
-                                   __float22bfloat162_rn(make_float2(v2, v3))};
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.y) + at) = *reinterpret_cast<const uint2*>(h);
-    } else {
-      const __half2 h[2] = {__float22half2_rn(make_float2(v0, v1)), __float22half2_rn(make_float2(v2, v3))};
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.y) + at) = *reinterpret_cast<const uint2*>(h);
-    }
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(p) = v;
+    else
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v.x, v.y, p), pack2(v.z, v.w, p));
   } else {
-    const float v[4] = {v0, v1, v2, v3};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (feat + i < a.n) store_from_float(a.y, a.y_dtype, at + i, v[i]);
+    if (n > 0) round_to(v.x, p[0]);
+    if (n > 1) round_to(v.y, p[1]);
+    if (n > 2) round_to(v.z, p[2]);
+    if (n > 3) round_to(v.w, p[3]);
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// Few tokens. A CTA takes 128 output features (the MMA's M side: 128 weight rows) x BN tokens
-// (its N side) and a contiguous range of the K blocks; the CTAs of a cluster (up to 8) share a tile
-// and split its K blocks. Per K block one stage: 128 x 128 weight bytes, BN x 128 token bytes
-// (128-byte swizzle) and both scale tiles. Warp 0 loads, warp 1 copies the scales to tensor memory
-// and issues four MMAs, warps 2-5 read the sums back (a feature per lane). With a split each CTA
-// owns some of the tile's tokens: every CTA writes its fp32 partial sums straight into the owners'
-// shared memory, and after one cluster barrier the owners add them in rank order (a fixed
-// order: same bits every time) and write y.
+// Few tokens (up to 64). A CTA takes 128 output features (the MMA's M side: 128 weight rows) x BN
+// tokens (its N side) and a contiguous range of the K blocks; the CTAs of a cluster (up to 8) share
+// a tile and split its K blocks. Per K block one stage: 128 x 128 weight bytes, BN x 128 token
+// bytes (128-byte swizzle) and both scale tiles. Warp 0 loads, warp 1 copies the scales to tensor
+// memory and issues four MMAs, warps 2-5 read the sums back (a feature per lane) into shared
+// memory. With a split each CTA owns some of the tile's tokens: the others store their fp32
+// partial sums straight into its shared memory, and it adds them in rank order (a fixed order: same
+// bits every time).
 template <int BN>
 struct Few {
   static constexpr int kA = 128 * 128, kB = BN * 128, kSf = 512;
   static constexpr int kStage = kA + kB + 2 * kSf;
-  static constexpr int kMaxStages = 8;
   static constexpr int kSums = (BN + 8) * 512;          // partial sums of the tokens a CTA owns
   static constexpr int kThreads = 192;
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
-  static constexpr uint32_t kTmemCols = kAccCols + 8 * kMaxStages <= 128 ? 128 : 256;
+  static constexpr uint32_t kTmemCols = 128;
   static constexpr int kBars = (2 * kMaxStages + 1) * 8 + 16;
-  static constexpr int kFixed = kBars + 1024;           // barriers, and stages start on 1 KB
+  static constexpr int kFixed = kBars + 1024;           // stages start on 1 KB
   static_assert(kStage % 1024 == 0, "swizzled stages start on 1 KB");
-  static_assert(BN * 512 <= 3 * kStage, "unsplit sums take the place of the stages (at least 3)");
+  static_assert(kSums <= 3 * kStage, "unsplit, the sums take the place of the stages (at least 3)");
   static_assert(kAccCols + 8 * kMaxStages <= (int)kTmemCols, "tensor memory budget");
 };
 
-template <int BN>
-__global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Args a, const int stages,
+template <int BN, typename T>
+__global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Args a,
                                                                     const __grid_constant__ Fp8Maps M) {
   using C = Few<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -100,13 +114,14 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
   uint32_t splits, rank;
   asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(splits));
   rank = cluster_rank();
-  // partial sums: behind the stages, or (no split: nobody else writes them) in their place
+  const int stages = a.stages;
+  // [rank][owned token][feature]: behind the stages, or in their place (one CTA: the MMAs are done)
   float* sums = reinterpret_cast<float*>(smem + (splits > 1 ? stages * C::kStage : 0));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * C::kStage + (splits > 1 ? C::kSums : 0));
-  uint64_t* empty = full + C::kMaxStages;
-  uint64_t* done = empty + C::kMaxStages;
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* done = empty + kMaxStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   const int64_t tile = blockIdx.x / splits;
@@ -114,6 +129,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
   const int kb0 = (int)((int64_t)a.nkb * rank / splits), kb1 = (int)((int64_t)a.nkb * (rank + 1) / splits);
   const int ntok = (int)(a.m - m0 < BN ? a.m - m0 : BN);
   const int own = (int)((ntok + splits - 1) / splits);   // tokens a CTA of the cluster owns
+  const int t1 = min(own, ntok - (int)rank * own);       // this one (none: <= 0)
 
   if (warp == 0 && elect_one_sync()) {
     // the first weights on their way to L2 while the previous kernel of the stream ends
@@ -123,7 +139,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
   if (threadIdx.x == 32) {
     for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(done, 1);
-    *abort_flag = 0;
+    *A.flag = 0;
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -143,7 +159,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
       uint32_t ph = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = fp8_wait(&empty[s], ph ^ 1, abort_flag, a.err, 20))) break;
+        if (!(ok = fp8_wait<false>(&empty[s], ph ^ 1, A, 20))) break;
         uint8_t* st = smem + (size_t)s * C::kStage;
         mbar_arrive_expect_tx(&full[s], C::kStage);
         tma_2d_g2s(st, &M.w, kb * 128, (int)n0, &full[s]);
@@ -167,7 +183,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
       uint32_t ph = 0, acc = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = fp8_wait(&full[s], ph, abort_flag, a.err, 21))) break;
+        if (!(ok = fp8_wait<false>(&full[s], ph, A, 21))) break;
         tc_fence_after();
         const uint32_t st = sbase + s * C::kStage;
         const uint32_t sfa = tmem + C::kAccCols + s * 8, sfb = sfa + 4;
@@ -189,193 +205,130 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
     __syncwarp();
   }
   if (splits > 1) cluster_wait();                        // every CTA of the cluster runs
-  if (warp >= 2 && __all_sync(0xffffffffu, fp8_wait(done, 0, abort_flag, a.err, 22))) {
+  if (warp >= 2 && __all_sync(0xffffffffu, fp8_wait<false>(done, 0, A, 22))) {
     tc_fence_after();
     const int q4 = warp & 3, row = q4 * 32 + lane;       // tensor-memory lane = feature n0 + row
     const uint32_t taddr = tmem + ((uint32_t)(q4 * 32) << 16);
-    const uint32_t mine = smem_u32(sums) + (rank * own * 128 + row) * 4;   // this rank's slot in an owner's sums
-    int owner = 0, slot = 0;
-    uint32_t dst = splits > 1 ? map_shared(mine, 0) : 0;
-    constexpr int kCols = BN < 32 ? 16 : 32;
-    for (int c0 = 0; c0 < ntok; c0 += kCols) {
-      float v[kCols];
-      if constexpr (kCols == 16) tmem_ld_32x32b_x16(taddr + c0, v);
-      else tmem_ld_32x32b_x32(taddr + c0, v);
-      tmem_wait_ld();
-      if (splits > 1) {
+    const uint32_t slot = smem_u32(sums + rank * own * 128 + row);
+    // owner by owner, 16 tokens at a time (columns past the accumulator's are not used)
+#pragma unroll 1
+    for (int o = 0; o < (int)splits; ++o) {
+      const int t0 = o * own, cnt = min(own, ntok - t0);
+      const uint32_t dst = splits > 1 ? map_shared(slot, o) : slot;
+#pragma unroll 1
+      for (int c = 0; c < cnt; c += 16) {
+        float v[16];
+        tmem_ld_32x32b_x16(taddr + t0 + c, v);
+        tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          if (c0 + j >= ntok) break;
-          st_shared_cluster(dst + slot * 512, v[j]);
-          if (++slot == own) { slot = 0; dst = map_shared(mine, min(++owner, (int)splits - 1)); }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) sums[(c0 + j) * 128 + row] = v[j];   // c0 + j < BN
+        for (int j = 0; j < 16; ++j)
+          if (c + j < cnt) st_shared_cluster(dst + (c + j) * 512, v[j]);
       }
     }
   }
-
   tc_fence_before();
   __syncwarp();
-  if (splits > 1) cluster_sync();                        // every partial sum has landed
-  else __syncthreads();
+  if (splits > 1) {                                      // every partial sum has landed
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   // a warp per owned token, 4 features per lane
-  const int f = lane * 4;
+  const int f = lane * 4, nf = (int)(a.n - n0 - f < 4 ? a.n - n0 - f : 4);
   const bool vec = n0 + 128 <= a.n && a.ldy % 4 == 0 && ((uintptr_t)a.y & 15) == 0;
   float bias[4] = {0.f, 0.f, 0.f, 0.f};
   if (a.bias)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n0 + f + i < a.n) bias[i] = load_as_float(a.bias, a.bias_dtype, n0 + f + i);
-  const int t1 = min(own, ntok - (int)rank * own);
-#pragma unroll 4
+      if (i < nf) bias[i] = load_as_float(a.bias, a.bias_dtype, n0 + f + i);
+  T* y = reinterpret_cast<T*>(a.y) + (m0 + (int)rank * own) * a.ldy + n0 + f;
+#pragma unroll 1
   for (int t = warp; t < t1; t += C::kThreads / 32) {
-    float4 p = *reinterpret_cast<const float4*>(sums + t * 128 + f);
-    for (uint32_t r = 1; r < splits; ++r) {
-      const float4 q = *reinterpret_cast<const float4*>(sums + (r * own + t) * 128 + f);
+    float4 p = make_float4(bias[0], bias[1], bias[2], bias[3]);
+    const float* from = sums + t * 128 + f;
+#pragma unroll 4
+    for (int r = 0; r < (int)splits; ++r) {
+      const float4 q = *reinterpret_cast<const float4*>(from + r * own * 128);
       p.x += q.x; p.y += q.y; p.z += q.z; p.w += q.w;
     }
-    const int64_t at = (m0 + (int)rank * own + t) * a.ldy + n0 + f;
-    store4(a, at, n0 + f, p.x + bias[0], p.y + bias[1], p.z + bias[2], p.w + bias[3], vec);
+    store4(y + t * a.ldy, nf, p, vec);
   }
-  __syncthreads();
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
 }
 
-// Shared memory a CTA may take so that one or two fit an SM (228 KB, 1 KB of it per CTA reserved).
-constexpr int kSmemOne = 232448, kSmemTwo = 115712;
-
-// Which split and pipeline a tile count gets: K is split over a cluster while that fills idle
-// CTA slots and leaves every CTA at least 4 K blocks. Two CTAs per SM, but for 128-token tiles with a
-// split, whose stages and partial sums take more than half an SM.
-template <int BN>
-int launch_few(const Fp8Args& a, const Fp8Maps& M, int dev, int nsm, cudaStream_t st) {
-  using C = Few<BN>;
-  static bool attr_set[64] = {false};
-  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    FBFP_CUDA_TRY(cudaFuncSetAttribute(fp8_few_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOne));
-    if (dev >= 0 && dev < 64) attr_set[dev] = true;
-  }
-  const int64_t tiles = (a.n + 127) / 128 * a.n_tt;
-  const int slots = BN == 128 ? nsm : 2 * nsm;
-  int splits = (int)(slots / tiles < 8 ? slots / tiles : 8);
-  if (splits > a.nkb / 4) splits = a.nkb / 4;
-  if (splits < 1) splits = 1;
-  const int sums = splits > 1 ? C::kSums : 0;
-  const int room = (BN == 128 && tiles * splits <= nsm ? kSmemOne : kSmemTwo) - C::kFixed - sums;
-  int stages = room / C::kStage < C::kMaxStages ? room / C::kStage : C::kMaxStages;
-  const size_t smem = (size_t)stages * C::kStage + sums + C::kFixed;
-  const int64_t grid = tiles * splits;
-  FBFP_CHECK_ARG(grid < ((int64_t)1 << 31), "too many output tiles");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)splits;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  FBFP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp8_few_kernel<BN>, a, stages, M));
-  FBFP_LAUNCH_CHECK("fp8_few_kernel");
-  return FBFP_OK;
-}
-
 // ---------------------------------------------------------------------------------------
-// Many tokens. Persistent CTA pairs (cta_group::2): a pair takes tiles of 256 tokens x BN features,
-// tokens on the MMA's M side (128 per CTA), features on its N side (half of the weight rows in each
-// CTA's shared memory), so that each SM loads 128 + BN / 2 rows of 128 bytes per K block for
-// 128 x BN x 128 multiply-adds. Scale tiles are loaded once per 512 values of K, with the stage of
-// the group's first K block, and copied to one of four slots of tensor memory in turn. A slot is
-// written again 10 or more K blocks later where a tile has more than 8 (more than the stages in
-// flight), else at least two tiles later (whose accumulator had to be drained first): either way
-// the MMAs that read it have completed. A tile starts on a whole scale tile (features
-// in steps of 128), which keeps the scales' tensor-memory addresses on multiples of 4 columns.
-template <int BN>
+// Many tokens (more than 64): tokens on the MMA's M side. CG = 1: a CTA takes tiles of 128 tokens x BN
+// features. CG = 2: a CTA pair (cta_group::2) takes tiles of 256 tokens x BN features, with 128
+// tokens and half of the weight rows in each CTA's shared memory, so that each SM loads
+// 128 + BN / 2 rows of 128 bytes per K block for 128 x BN x 128 multiply-adds. Persistent, or with a
+// split: the CTAs (pairs) of a cluster share a tile and split its K blocks.
+//
+// Scale tiles are loaded once per 512 values of K, with the stage of the group's first K block, and
+// copied to one of four slots of tensor memory in turn. A slot is written again 10 or more K
+// blocks later where a tile has more than 8 (more than the stages in flight), else at least two
+// tiles later (whose accumulator had to be drained first): either way the MMAs that read it have
+// completed. A tile starts on a whole scale tile (features in steps of 128), which keeps the
+// scales' tensor-memory addresses on multiples of 4 columns.
+//
+// Epilogue: eight warps, each a unit of 32 tokens (a lane quarter; a token per lane) x BN / 2
+// features. The sums go to registers first, so that the accumulator is free again after the
+// loads. With a split every unit has an owner among the cluster's CTAs: the others store their
+// sums into its shared memory (rows padded to 17 x 16 bytes, free of bank conflicts), and it adds
+// them to its own in rank order.
+template <int CG, int BN>
 struct Many {
-  static constexpr int kHalfN = BN / 2;
+  static constexpr int kRowsB = BN / CG;
   static constexpr int kChunks = BN / 128;                       // scale tiles of the features
-  static constexpr int kA = 128 * 128, kB = kHalfN * 128, kSf = 512 * (1 + kChunks);
+  static constexpr int kA = 128 * 128, kB = kRowsB * 128, kSf = 512 * (1 + kChunks);
   static constexpr int kStage = kA + kB + (kSf + 1023) / 1024 * 1024;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
-  static constexpr int kTurn = 32 * 17 * 4;                      // a warp's 32 x 16 words, rows 17 apart
-  static constexpr int kBufs = BN == 256 ? 1 : 2;                // accumulators
+  static constexpr int kBufs = CG == 2 && BN == 128 ? 2 : 1;     // accumulators
   static constexpr int kSfCols = 4 * (1 + kChunks), kSfSlots = 4;
-  static constexpr int kEpiWarps = 8;
-  static constexpr int kThreads = 32 * (4 + kEpiWarps);
-  static constexpr uint32_t kTmemCols = 512, kSfCol0 = kBufs * BN;
-  static constexpr int kData = kStages * kStage;
-  static constexpr int kBarOff = kData + kEpiWarps * kTurn;
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 1;
-  static constexpr size_t kSmem = kBarOff + kBars * 8 + 16 + 1024;
-  static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 8 == 0, "features in whole scale tiles");
-  static_assert(kSfCol0 + kSfSlots * kSfCols <= (int)kTmemCols, "tensor memory budget");
-  static_assert(kSmem <= 232448, "shared memory budget");
+  static constexpr uint32_t kSfCol0 = kBufs * BN;
+  static constexpr uint32_t kTmemCols = kSfCol0 + kSfSlots * kSfCols <= 256 ? 256 : 512;
+  static constexpr int kEpiWarps = 8, kThreads = 32 * (4 + kEpiWarps);
+  static constexpr int kCols = BN / 2;                           // columns of a unit
+  static constexpr int kTurn = 32 * 17 * 4;                      // a warp's 32 x 16 words, rows 17 apart
+  static constexpr int kTurns = kEpiWarps * kTurn;
+  static constexpr int kSumRow = kCols + 4;                      // floats
+  static constexpr int kUnit = 32 * kSumRow * 4;
+  static constexpr int kSums = 7 * kUnit;                        // at most 7 units from other CTAs
+  static constexpr int kBars = (2 * kMaxStages + 2 + 2 + 2) * 8 + 16;
+  static constexpr int kFixed = kBars + 1024;                    // stages start on 1 KB
+  static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kUnit % 16 == 0, "alignment");
+  static_assert(kSfCol0 + kSfSlots * kSfCols <= kTmemCols, "tensor memory budget");
 };
-
-struct ManyShared {
-  volatile int* abort_flag;
-  int32_t* err;
-};
-
-__device__ __forceinline__ bool many_wait(uint64_t* bar, uint32_t parity, const ManyShared& S, int site) {
-  for (uint32_t it = 0; it < (1u << 16); ++it) {
-    if (mbar_try_wait_cluster(bar, parity, 20000u)) return true;
-    if ((it & 15) == 15 && *S.abort_flag) return false;
-  }
-  *S.abort_flag = 1;
-  atomicExch(S.err, site);
-  return false;
-}
 
 // One warp: 32 consecutive features, the first f0, of 32 consecutive tokens, one per lane (the
-// first tok0; tokens from a.m on are not stored). vec: y's base and rows are 32-byte aligned, so
-// each lane stores whole 32-byte sectors of its row; else the values turn through shared memory
-// (`turn`) and the lanes store along the rows.
-__device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_t f0, const float (&v)[32], bool vec,
+// first tok0; tokens from a.m on are not stored). vec, the bytes that y's base and rows are
+// aligned to: at 32 each lane stores whole sectors of its row, at 16 halves of them; else the
+// values turn through shared memory (`turn`) and the lanes store along the rows.
+template <typename T>
+__device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_t f0, const float (&v)[32], int vec,
                                           uint32_t* turn) {
   const int lane = threadIdx.x & 31;
   const int64_t row = tok0 + lane;
-  uint32_t w[16];
-  if (a.y_dtype != FBFP_F32) {
+  T* y = reinterpret_cast<T*>(a.y);
+  if constexpr (sizeof(T) == 4) {
+    if (vec && f0 + 32 <= a.n) {
+      if (row >= a.m) return;
+      T* p = y + row * a.ldy + f0;
+      if (vec == 16) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (a.y_dtype == FBFP_BF16) {
-        const __nv_bfloat162 h = __float22bfloat162_rn(make_float2(v[2 * i], v[2 * i + 1]));
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __half2 h = __float22half2_rn(make_float2(v[2 * i], v[2 * i + 1]));
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int h = 0; h < 8; ++h)
+          reinterpret_cast<float4*>(p)[h] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+        return;
       }
-    }
-  }
-  if (vec && f0 + 32 <= a.n) {
-    if (row >= a.m) return;
-    if (a.y_dtype == FBFP_F32) {
-      float* p = reinterpret_cast<float*>(a.y) + row * a.ldy + f0;
 #pragma unroll
       for (int h = 0; h < 4; ++h)
         asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p + 8 * h), "f"(v[8 * h]),
                      "f"(v[8 * h + 1]), "f"(v[8 * h + 2]), "f"(v[8 * h + 3]), "f"(v[8 * h + 4]), "f"(v[8 * h + 5]),
                      "f"(v[8 * h + 6]), "f"(v[8 * h + 7]) : "memory");
-    } else {
-      uint16_t* p = reinterpret_cast<uint16_t*>(a.y) + row * a.ldy + f0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p + 16 * h), "r"(w[8 * h]),
-                     "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
-                     "r"(w[8 * h + 6]), "r"(w[8 * h + 7]) : "memory");
+      return;
     }
-  } else if (a.y_dtype == FBFP_F32) {
-    float* y = reinterpret_cast<float*>(a.y);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {                        // 16 columns at a time, two rows per store
       __syncwarp();
@@ -388,7 +341,25 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
         if (tok0 + r < a.m && f < a.n) y[(tok0 + r) * a.ldy + f] = __uint_as_float(turn[r * 17 + (lane & 15)]);
     }
   } else {
-    uint16_t* y = reinterpret_cast<uint16_t*>(a.y);
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], y);
+    if (vec && f0 + 32 <= a.n) {
+      if (row >= a.m) return;
+      T* p = y + row * a.ldy + f0;
+      if (vec == 16) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          reinterpret_cast<uint4*>(p)[h] = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+        return;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p + 16 * h), "r"(w[8 * h]),
+                     "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
+                     "r"(w[8 * h + 6]), "r"(w[8 * h + 7]) : "memory");
+      return;
+    }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; ++i) turn[lane * 17 + i] = w[i];
@@ -396,194 +367,370 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
 #pragma unroll 4
     for (int r = 0; r < 32; ++r)
       if (tok0 + r < a.m && f0 + lane < a.n)
-        y[(tok0 + r) * a.ldy + f0 + lane] = reinterpret_cast<const uint16_t*>(turn + r * 17)[lane];
+        y[(tok0 + r) * a.ldy + f0 + lane] = reinterpret_cast<const T*>(turn + r * 17)[lane];
   }
 }
 
-template <int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Many<BN>::kThreads, 1)
-fp8_many_kernel(const Fp8Args a, const __grid_constant__ Fp8Maps M) {
-  using C = Many<BN>;
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar, uint16_t pair_mask) {
+  if constexpr (CG == 1) mma_commit(bar);
+  else mma_commit_pair(bar, pair_mask);
+}
+template <int CG>
+__device__ __forceinline__ void load_tile(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 1) tma_2d_g2s(dst, map, x, y, bar);
+  else tma_2d_g2s_pair(dst, map, x, y, bar);
+}
+
+template <int CG, int BN, typename T>
+__global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(const Fp8Args a, const int splits,
+                                                                              const __grid_constant__ Fp8Maps M) {
+  using C = Many<CG, BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);   // used in CTA 0
-  uint64_t* empty = full + C::kStages;
-  uint64_t* acc_full = empty + C::kStages;
-  uint64_t* acc_empty = acc_full + 2;                               // used in CTA 0
+  const int stages = a.stages;
+  // behind the stages: the other CTAs' sums (split) or the epilogue's turning room; a split's
+  // epilogue turns in the stages' place, its MMAs being done by then
+  uint8_t* sums = smem + stages * C::kStage;
+  uint8_t* turns = splits > 1 ? smem : sums;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sums + (splits > 1 ? C::kSums : C::kTurns));   // used in a pair's CTA 0
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* acc_full = empty + kMaxStages;
+  uint64_t* acc_empty = acc_full + 2;                               // used in a pair's CTA 0
   uint64_t* tail = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 1);
-  ManyShared S;
-  S.abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  S.err = a.err;
+  uint64_t* landed = tail + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 1);
+  const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t rank = cluster_rank(), pr = rank % CG, lead = rank - pr;
+  const int sp = (int)(rank / CG);                                  // which split of the K blocks
+  const uint16_t pair_mask = (uint16_t)(3u << lead);
+  const int64_t team = blockIdx.x / (CG * splits), teams = gridDim.x / (CG * splits);
   const int64_t tiles = (a.n + BN - 1) / BN * a.n_tt;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * C::kEpiWarps); }
+  const int kb0 = (int)((int64_t)a.nkb * sp / splits), kb1 = (int)((int64_t)a.nkb * (sp + 1) / splits);
+  const int per = 8 / splits;                                       // units a CTA owns
+  if (warp == 0 && elect_one_sync()) {
+    // the first weights on their way to L2 while the previous kernel of the stream ends
+    prefetch_tmap(&M.w); prefetch_tmap(&M.x); prefetch_tmap(&M.ws); prefetch_tmap(&M.xs);
+    for (int kb = kb0; kb < kb1 && kb < kb0 + stages; ++kb)
+      tma_2d_prefetch(&M.w, kb * 128, (int)(team / a.n_tt * BN + pr * C::kRowsB));
+  }
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], CG * C::kEpiWarps); }
     mbar_init(tail, 1);
-    *S.abort_flag = 0;
+    mbar_init(landed, 1);
+    *A.flag = 0;
     fence_mbar_init();
+    if (splits > 1) {                                    // units of this CTA that have tokens
+      int live = 0;
+      for (int u = sp * per; u < (sp + 1) * per; ++u)
+        live += team % a.n_tt * (128 * CG) + 128 * pr + (u >> 1) * 32 < a.m;
+      if (live) mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * C::kCols * 4));
+    }
   }
-  if (warp == 1) {
-    tmem_alloc_pair(tmem_slot, C::kTmemCols);
-    tmem_relinquish_pair();
+  if (warp == 2) {
+    if constexpr (CG == 1) { tmem_alloc(tmem_slot, C::kTmemCols); tmem_relinquish(); }
+    else { tmem_alloc_pair(tmem_slot, C::kTmemCols); tmem_relinquish_pair(); }
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
-  cluster_sync();                                        // the peer's barriers are ready
+  cluster_arrive();
+  cluster_wait();                                        // every CTA of the cluster runs, its barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_prologue();
 
   if (warp == 0) {
     if (elect_one_sync()) {
-      prefetch_tmap(&M.w); prefetch_tmap(&M.x); prefetch_tmap(&M.ws); prefetch_tmap(&M.xs);
       const uint32_t sbase = smem_u32(smem);
       int s = 0;
       uint32_t ph = 0;
       int64_t issued = 0;
       bool ok = true;
-      for (int64_t t = pair; t < tiles && ok; t += pairs) {
-        const int64_t m0 = t % a.n_tt * 256 + 128 * rank, n0 = t / a.n_tt * BN;
-        for (int kb = 0; kb < a.nkb; ++kb) {
-          if (!(ok = many_wait(&empty[s], ph ^ 1, S, 23))) break;
+      for (int64_t t = team; t < tiles && ok; t += teams) {
+        const int64_t m0 = t % a.n_tt * (128 * CG) + 128 * pr, n0 = t / a.n_tt * BN;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = fp8_wait<CG == 2>(&empty[s], ph ^ 1, A, 23))) break;
           const uint32_t st = sbase + (uint32_t)s * C::kStage;
-          const uint32_t bar = map_shared(smem_u32(&full[s]), 0);
-          const bool sf = (kb & 3) == 0;
-          // CTA 0 expects both CTAs' bytes
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * (C::kA + C::kB + (sf ? C::kSf : 0)));
-          tma_2d_g2s_pair(st, &M.x, kb * 128, (int)m0, bar);
-          tma_2d_g2s_pair(st + C::kA, &M.w, kb * 128, (int)(n0 + rank * C::kHalfN), bar);
-          if (sf) {
-            tma_2d_g2s_pair(st + C::kA + C::kB, &M.xs, 0, (int)(m0 / 128 * a.kgroups + kb / 4), bar);
+          const uint32_t bar = CG == 1 ? smem_u32(&full[s]) : map_shared(smem_u32(&full[s]), lead);
+          const bool sf = (kb & 3) == 0 || kb == kb0;
+          // a pair's CTA 0 expects both CTAs' bytes
+          if (pr == 0) mbar_arrive_expect_tx(&full[s], CG * (C::kA + C::kB + (sf ? C::kSf : 0)));
+          load_tile<CG>(st, &M.x, kb * 128, (int)m0, bar);
+          load_tile<CG>(st + C::kA, &M.w, kb * 128, (int)(n0 + pr * C::kRowsB), bar);
+          if (sf) {                                      // tiles past the last one read as zero
+            load_tile<CG>(st + C::kA + C::kB, &M.xs, 0, (int)(m0 / 128 * a.kgroups + kb / 4), bar);
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)         // tiles past the last one read as zero
-              tma_2d_g2s_pair(st + C::kA + C::kB + 512 * (1 + c), &M.ws, 0,
-                              (int)((n0 / 128 + c) * a.kgroups + kb / 4), bar);
+            for (int c = 0; c < C::kChunks; ++c)
+              load_tile<CG>(st + C::kA + C::kB + 512 * (1 + c), &M.ws, 0,
+                            (int)((n0 / 128 + c) * a.kgroups + kb / 4), bar);
           }
           ++issued;
-          if (++s == C::kStages) { s = 0; ph ^= 1; }
+          if (++s == stages) { s = 0; ph ^= 1; }
         }
       }
-      if (!ok) {                                         // copies in flight land before the pair exits
-        if (rank == 0)
-          for (int64_t j = issued > C::kStages ? issued - C::kStages : 0; j < issued; ++j)
-            mbar_wait(&full[j % C::kStages], (uint32_t)(j / C::kStages) & 1, 1u << 16);
+      if (!ok) {                                         // copies in flight land before the CTA exits
+        if (pr == 0)
+          for (int64_t j = issued > stages ? issued - stages : 0; j < issued; ++j)
+            mbar_wait(&full[j % stages], (uint32_t)(j / stages) & 1, 1u << 16);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
       }
     }
     __syncwarp();
-  } else if (warp == 1 && rank == 0) {
+  } else if (warp == 1 && pr == 0) {
     if (elect_one_sync()) {
-      constexpr uint32_t kIdesc = idesc_mxf8(256, BN);
+      constexpr uint32_t kIdesc = idesc_mxf8(128 * CG, BN);
       const uint32_t sbase = smem_u32(smem);
-      const int64_t mine = pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0;
-      const int64_t total = mine * a.nkb;
+      const int64_t mine = team < tiles ? (tiles - team + teams - 1) / teams : 0;
+      const int64_t total = mine * (kb1 - kb0);
       int64_t it = 0;
       int s = 0, buf = 0, slot = C::kSfSlots - 1;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
-      for (int64_t t = pair; t < tiles && ok; t += pairs) {
-        if (!(ok = many_wait(&acc_empty[buf], aph ^ 1, S, 24))) break;
+      for (int64_t t = team; t < tiles && ok; t += teams) {
+        if (!(ok = fp8_wait<CG == 2>(&acc_empty[buf], aph ^ 1, A, 24))) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
         uint32_t acc = 0, sfa = 0;
-        for (int kb = 0; kb < a.nkb; ++kb) {
-          if (!(ok = many_wait(&full[s], ph, S, 25))) break;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = fp8_wait<CG == 2>(&full[s], ph, A, 25))) break;
           tc_fence_after();
           const uint32_t st = sbase + (uint32_t)s * C::kStage;
-          if ((kb & 3) == 0) {
+          if ((kb & 3) == 0 || kb == kb0) {
             slot = slot == C::kSfSlots - 1 ? 0 : slot + 1;
             sfa = tmem + C::kSfCol0 + slot * C::kSfCols;
 #pragma unroll
             for (int c = 0; c < 1 + C::kChunks; ++c)
-              scales_to_tmem<2>(sfa + 4 * c, smem_desc_scales(st + C::kA + C::kB + 512 * c));
+              scales_to_tmem<CG>(sfa + 4 * c, smem_desc_scales(st + C::kA + C::kB + 512 * c));
           }
           const uint64_t da = smem_desc_sw128(st, 1024), db = smem_desc_sw128(st + C::kA, 1024);
           const uint32_t id = idesc_mxf8_id(kIdesc, kb & 3);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            mma_mxf8<2>(d, da + 2 * k, db + 2 * k, id, sfa, sfa + 4, acc);
+          for (int k = 0; k < 4; ++k) {                  // 32 values = 32 bytes per step
+            mma_mxf8<CG>(d, da + 2 * k, db + 2 * k, id, sfa, sfa + 4, acc);
             acc = 1;
           }
-          if (it + C::kStages < total) mma_commit_pair(&empty[s]);   // only where the producers wait for it
+          if (it + stages < total) commit<CG>(&empty[s], pair_mask);   // only where the producers wait for it
           ++it;
-          if (++s == C::kStages) { s = 0; ph ^= 1; }
+          if (++s == stages) { s = 0; ph ^= 1; }
         }
         if (!ok) break;
-        mma_commit_pair(&acc_full[buf]);
+        commit<CG>(&acc_full[buf], pair_mask);
         if (++buf == C::kBufs) { buf = 0; aph ^= 1; }
       }
       if (!ok) {                                         // MMAs in flight end before the memory goes
-        mma_commit_pair(tail);
+        commit<CG>(tail, pair_mask);
         mbar_wait(tail, 0, 1u << 16);
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
-    // two warps per lane quarter, half of the columns each: the sums go to registers first, so that
-    // the accumulator is free again after the loads
-    constexpr int kCols = BN / 2;
-    const int q4 = warp & 3, col0 = ((warp - 4) >> 2) * kCols;
-    uint32_t* turn = reinterpret_cast<uint32_t*>(smem + C::kData + (warp - 4) * C::kTurn);
-    const bool vec = ((uintptr_t)a.y & 31) == 0 && (a.ldy * (a.y_dtype == FBFP_F32 ? 4 : 2)) % 32 == 0;
+    const int q4 = warp & 3, half = (warp - 4) >> 2, col0 = half * C::kCols;
+    const int unit = 2 * q4 + half, owner = unit / per;
+    uint32_t* turn = reinterpret_cast<uint32_t*>(turns + (warp - 4) * C::kTurn);
+    const uint64_t bits = (uint64_t)(uintptr_t)a.y | (uint64_t)a.ldy * sizeof(T);
+    const int vec = (bits & 31) == 0 ? 32 : (bits & 15) == 0 ? 16 : 0;
     int buf = 0;
     uint32_t ph = 0;
-    for (int64_t t = pair; t < tiles; t += pairs) {
-      const int64_t tok0 = t % a.n_tt * 256 + 128 * rank + q4 * 32, n0 = t / a.n_tt * BN + col0;
-      if (!__all_sync(0xffffffffu, many_wait(&acc_full[buf], ph, S, 26))) break;
+#pragma unroll 1
+    for (int64_t t = team; t < tiles; t += teams) {
+      const int64_t tok0 = t % a.n_tt * (128 * CG) + 128 * pr + q4 * 32, n0 = t / a.n_tt * BN + col0;
+      if (!__all_sync(0xffffffffu, fp8_wait<CG == 2>(&acc_full[buf], ph, A, 26))) break;
       tc_fence_after();
       const uint32_t taddr = tmem + buf * BN + col0 + ((uint32_t)(q4 * 32) << 16);
-      float v[kCols / 32][32];
+      float v[C::kCols / 32][32];
 #pragma unroll
-      for (int c = 0; c < kCols / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, v[c]);
+      for (int c = 0; c < C::kCols / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, v[c]);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[buf]), 0));
+      if (lane == 0) {
+        if constexpr (CG == 1) mbar_arrive(&acc_empty[buf]);
+        else mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[buf]), lead));
+      }
+      if constexpr (BN == 128) {
+        if (splits > 1 && tok0 < a.m) {
+          if (owner != sp) {
+            // into the owner's room for this unit and split
+            const int from = sp < owner ? sp : sp - 1, to = owner * CG + pr;
+            const uint32_t dst = map_shared(smem_u32(sums) + (unit % per * (splits - 1) + from) * C::kUnit +
+                                                lane * C::kSumRow * 4, to);
+            const uint32_t bar = map_shared(smem_u32(landed), to);
 #pragma unroll
-      for (int c = 0; c < kCols / 32; ++c) {
+            for (int c = 0; c < C::kCols; c += 4)
+              st_async_v4(dst + c * 4, v[c / 32][c % 32], v[c / 32][c % 32 + 1], v[c / 32][c % 32 + 2],
+                          v[c / 32][c % 32 + 3], bar);
+            continue;
+          }
+          if (!__all_sync(0xffffffffu, fp8_wait<true>(landed, 0, A, 27))) break;
+#pragma unroll 1
+          for (int r = 0; r < splits - 1; ++r) {
+            const float* p = reinterpret_cast<const float*>(sums + (unit % per * (splits - 1) + r) * C::kUnit) +
+                             lane * C::kSumRow;
+#pragma unroll
+            for (int c = 0; c < C::kCols; c += 4) {
+              const float4 q = *reinterpret_cast<const float4*>(p + c);
+              v[c / 32][c % 32] += q.x; v[c / 32][c % 32 + 1] += q.y;
+              v[c / 32][c % 32 + 2] += q.z; v[c / 32][c % 32 + 3] += q.w;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C::kCols / 32; ++c) {
         const int64_t f0 = n0 + 32 * c;
-        if (f0 >= a.n) break;                            // whole warps
+        if (f0 >= a.n || tok0 >= a.m) break;             // whole warps
         if (a.bias) {
           const float b = f0 + lane < a.n ? load_as_float(a.bias, a.bias_dtype, f0 + lane) : 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[c][i] += __shfl_sync(0xffffffffu, b, i);
         }
-        if (tok0 < a.m) store_y32(a, tok0, f0, v[c], vec, turn);
+        store_y32<T>(a, tok0, f0, v[c], vec, turn);
       }
       if (++buf == C::kBufs) { buf = 0; ph ^= 1; }
     }
   }
   __syncwarp();
   tc_fence_before();
-  cluster_sync();                                        // no CTA leaves while its pair may still reach it
-  if (warp == 1) {
+  cluster_arrive_relaxed();
+  cluster_wait();                                        // no CTA leaves while another may still reach it
+  if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, C::kTmemCols);
+    if constexpr (CG == 1) tmem_dealloc(tmem, C::kTmemCols);
+    else tmem_dealloc_pair(tmem, C::kTmemCols);
   }
 }
 
-template <int BN>
-int launch_many(const Fp8Args& a, const Fp8Maps& M, int dev, int nsm, cudaStream_t st) {
-  using C = Many<BN>;
-  static bool attr_set[64] = {false};
+// ---------------------------------------------------------------------------------------
+// Launch with programmatic stream serialisation and a cluster of `cluster` CTAs.
+template <typename... KArgs, typename... Args>
+int launch_cluster(void (*kernel)(KArgs...), int dev, bool (&attr_set)[64], int64_t grid, int cluster, int threads,
+                   size_t smem, cudaStream_t st, Args... args) {
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    FBFP_CUDA_TRY(cudaFuncSetAttribute(fp8_many_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)C::kSmem));
+    FBFP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOne));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  const int64_t tiles = (a.n + BN - 1) / BN * a.n_tt;
-  const int64_t pairs = tiles < nsm / 2 ? tiles : nsm / 2;
-  FBFP_CUDA_TRY(launch_pdl(fp8_many_kernel<BN>, dim3((unsigned)(2 * pairs)), dim3(C::kThreads), C::kSmem, st, a, M));
-  FBFP_LAUNCH_CHECK("fp8_many_kernel");
+  FBFP_CHECK_ARG(grid < ((int64_t)1 << 31), "too many output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FBFP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  FBFP_LAUNCH_CHECK("fp8_linear");
   return FBFP_OK;
 }
 
+// K is split over a cluster while that fills idle CTA slots (two per SM) and leaves every CTA at
+// least 4 K blocks.
+template <int BN, typename T>
+int launch_few(Fp8Args a, const Fp8Maps& M, int dev, int nsm, cudaStream_t st) {
+  using C = Few<BN>;
+  static bool attr_set[64] = {false};
+  const int64_t tiles = (a.n + 127) / 128 * a.n_tt;
+  int splits = (int)(2 * nsm / tiles < 8 ? 2 * nsm / tiles : 8);
+  if (splits > a.nkb / 4) splits = a.nkb / 4;
+  if (splits < 1) splits = 1;
+  const int extra = splits > 1 ? C::kSums : 0;
+  const int fit = (kSmemTwo - C::kFixed - extra) / C::kStage;
+  a.stages = fit < kMaxStages ? fit : kMaxStages;
+  return launch_cluster(fp8_few_kernel<BN, T>, dev, attr_set, tiles * splits, splits, C::kThreads,
+                        (size_t)a.stages * C::kStage + extra + C::kFixed, st, a, M);
+}
+
+template <int CG, int BN, typename T>
+int launch_many(Fp8Args a, const Fp8Maps& M, int dev, int teams, int splits, cudaStream_t st) {
+  using C = Many<CG, BN>;
+  static bool attr_set[64] = {false};
+  const int extra = splits > 1 ? C::kSums : C::kTurns;
+  const int fit = (kSmemOne - C::kFixed - extra) / C::kStage;
+  a.stages = fit < kMaxStages ? fit : kMaxStages;
+  return launch_cluster(fp8_many_kernel<CG, BN, T>, dev, attr_set, (int64_t)teams * CG * splits, CG * splits,
+                        C::kThreads, (size_t)a.stages * C::kStage + extra + C::kFixed, st, a, splits, M);
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+struct Fp8Operands {
+  const void *x, *w;
+  int64_t k, ldx, ldw;
+};
+
+int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t ld, int box) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)k, (uint64_t)rows, (uint64_t)ld, 128,
+                   (uint32_t)box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int encode_scales(CUtensorMap* map, const void* base, int64_t tiles) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, (uint64_t)tiles, 512, 128, 1,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+// Which tile and split: the least of an estimate in SM cycles, rounds of tiles x (K blocks x
+// cycles per block + 2500 for a tile's fill and drain) + 6000 for a split's exchange of partial
+// sums. Cycles per K block: 128 x BN x 128 multiply-adds take 2 BN, and the operand rows come
+// in at about 64 bytes a cycle: measured 512 (one CTA, 128 features; bound by the loads), 768 (256
+// features), 400 and 560 (a pair; loads and MMAs nearly even). Measured against the alternatives: 512
+// tokens x 8192 x 3840 16.5 us on 256-wide pair tiles and 18.7 on 128-wide ones, 512 x 3840 x
+// 15360 the other way around (41.0 and 31.5 us: 30 and 60 tiles for 74 pairs), 128 x 3840 x 15360
+// 19.7 us split four ways, 22.0 in two pairs, 29.1 unsplit.
+struct ManyPlan {
+  int cg, bn, splits, teams;
+  int64_t token_tiles;
+};
+ManyPlan plan_many(int64_t m, int64_t n, int nkb, int nsm) {
+  ManyPlan best{};
+  double least = 0;
+  for (int cg = m <= 128 ? 1 : 2; cg <= 2; ++cg)
+    for (int bn = 128; bn <= 256; bn += 128)
+      for (int splits = 1; splits * cg <= 8 && (splits == 1 || (bn == 128 && nkb >= 4 * splits)); splits *= 2) {
+        const int64_t tt = (m + 128 * cg - 1) / (128 * cg), tiles = (n + bn - 1) / bn * tt;
+        const int64_t slots = nsm / (cg * splits);       // teams that run at a time
+        if (splits > 1 && tiles > slots) continue;
+        const int64_t rounds = (tiles + slots - 1) / slots;
+        const double per_kb = cg == 1 ? (bn == 128 ? 512 : 768) : (bn == 128 ? 400 : 560);
+        const double cost = (double)rounds * ((nkb + splits - 1) / splits * per_kb + 2500) + (splits > 1 ? 6000 : 0);
+        if (best.cg == 0 || cost < least) {
+          least = cost;
+          best = ManyPlan{cg, bn, splits, (int)(tiles < slots ? tiles : slots), tt};
+        }
+      }
+  return best;
+}
+
+template <typename T>
+int fp8_dispatch(Fp8Args& a, const Fp8Operands& o, int dev, int nsm, cudaStream_t st) {
+  Fp8Maps M;
+  int rc;
+  if (a.m <= 64) {
+    const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64;
+    a.n_tt = 1;
+    if ((rc = encode_rows(&M.x, o.x, a.m, o.k, o.ldx, bn)) != FBFP_OK) return rc;
+    if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, 128)) != FBFP_OK) return rc;
+    return bn == 16   ? launch_few<16, T>(a, M, dev, nsm, st)
+           : bn == 32 ? launch_few<32, T>(a, M, dev, nsm, st)
+                      : launch_few<64, T>(a, M, dev, nsm, st);
+  }
+  const ManyPlan p = plan_many(a.m, a.n, a.nkb, nsm);
+  a.n_tt = p.token_tiles;
+  if ((rc = encode_rows(&M.x, o.x, a.m, o.k, o.ldx, 128)) != FBFP_OK) return rc;
+  if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, p.bn / p.cg)) != FBFP_OK) return rc;
+  if ((rc = encode_scales(&M.xs, a.x_scales, (a.m + 127) / 128 * a.kgroups)) != FBFP_OK) return rc;
+  if ((rc = encode_scales(&M.ws, a.w_scales, (a.n + 127) / 128 * a.kgroups)) != FBFP_OK) return rc;
+  if (p.cg == 1)
+    return p.bn == 128 ? launch_many<1, 128, T>(a, M, dev, p.teams, p.splits, st)
+                       : launch_many<1, 256, T>(a, M, dev, p.teams, p.splits, st);
+  return p.bn == 128 ? launch_many<2, 128, T>(a, M, dev, p.teams, p.splits, st)
+                     : launch_many<2, 256, T>(a, M, dev, p.teams, p.splits, st);
+}
 
 }  // namespace
 }  // namespace fbfp
@@ -607,39 +754,19 @@ extern "C" int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx,
   a.m = m; a.n = n;
   a.nkb = (int)((k + 127) / 128);
   a.kgroups = (int)((k + 511) / 512);
+  FBFP_CHECK_ARG((m + 127) / 128 * a.kgroups < ((int64_t)1 << 31) && (n + 127) / 128 * a.kgroups < ((int64_t)1 << 31),
+                 "too many scale tiles");
   a.x_scales = reinterpret_cast<const uint8_t*>(x_scales);
   a.w_scales = reinterpret_cast<const uint8_t*>(w_scales);
   a.bias = bias; a.bias_dtype = bias_dtype;
-  a.y = y; a.y_dtype = y_dtype; a.ldy = ldy;
+  a.y = y; a.ldy = ldy;
   a.err = reinterpret_cast<int32_t*>(workspace);
+  const Fp8Operands o{x, w, k, ldx, ldw};
   int dev = 0;
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
   const int nsm = sm_count(dev);
-
-  constexpr int kManyN = 256;
-  const bool many = m > 128;
-  const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;   // token rows of a tile (per CTA)
-  a.n_tt = many ? (m + 255) / 256 : (m + bn - 1) / bn;
-  const int64_t xt = (m + 127) / 128 * a.kgroups, wt = (n + 127) / 128 * a.kgroups;
-  FBFP_CHECK_ARG(xt < ((int64_t)1 << 31) && wt < ((int64_t)1 << 31), "too many scale tiles");
-  Fp8Maps M;
-  int rc;
-  if ((rc = encode_2d(&M.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, x, (uint64_t)k, (uint64_t)m, (uint64_t)ldx, 128,
-                      (uint32_t)bn, CU_TENSOR_MAP_SWIZZLE_128B)) != FBFP_OK) return rc;
-  if ((rc = encode_2d(&M.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, (uint64_t)k, (uint64_t)n, (uint64_t)ldw, 128,
-                      many ? kManyN / 2 : 128, CU_TENSOR_MAP_SWIZZLE_128B)) != FBFP_OK) return rc;
   const cudaStream_t st = as_stream(stream);
-  if (many) {
-    if ((rc = encode_2d(&M.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, x_scales, 128, (uint64_t)xt, 512, 128, 1,
-                        CU_TENSOR_MAP_SWIZZLE_NONE)) != FBFP_OK) return rc;
-    if ((rc = encode_2d(&M.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, w_scales, 128, (uint64_t)wt, 512, 128, 1,
-                        CU_TENSOR_MAP_SWIZZLE_NONE)) != FBFP_OK) return rc;
-    return launch_many<kManyN>(a, M, dev, nsm, st);
-  }
-  switch (bn) {
-    case 16: return launch_few<16>(a, M, dev, nsm, st);
-    case 32: return launch_few<32>(a, M, dev, nsm, st);
-    case 64: return launch_few<64>(a, M, dev, nsm, st);
-    default: return launch_few<128>(a, M, dev, nsm, st);
-  }
+  return y_dtype == FBFP_BF16  ? fp8_dispatch<__nv_bfloat16>(a, o, dev, nsm, st)
+         : y_dtype == FBFP_F16 ? fp8_dispatch<__half>(a, o, dev, nsm, st)
+                               : fp8_dispatch<float>(a, o, dev, nsm, st);
 }

@@ -80,13 +80,20 @@ __device__ __forceinline__ void tmem_relinquish_pair() {
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// Arrive once on `bar` in both CTAs when every tcgen05 operation issued so far has completed.
-__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+// Arrive once on `bar` in both CTAs (`mask`: their bits by cluster rank) when every tcgen05
+// operation issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar, uint16_t mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
-      ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+      ::"r"(smem_u32(bar)), "h"(mask) : "memory");
 }
-// Tensor copy into this CTA's shared memory that completes on a barrier of either CTA of the pair
+// Tensor copy into this CTA's shared memory, by address.
+__device__ __forceinline__ void tma_2d_g2s(uint32_t dst_smem, const void* tmap, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+      ::"r"(dst_smem), "l"(tmap), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// The same, completing on a barrier of either CTA of the pair
 // (`bar`: a shared::cluster address).
 __device__ __forceinline__ void tma_2d_g2s_pair(uint32_t dst_smem, const void* tmap, int x, int y, uint32_t bar) {
   asm volatile(
@@ -127,17 +134,16 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
-// The two halves of cluster_sync (every thread takes both, in this order, before the next one).
+// The two halves of a barrier over the cluster (every thread takes both, in this order).
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
 }
+// Without ordering memory (a release would wait for the thread's global stores).
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile(
-      "barrier.cluster.arrive.release.aligned;\n"
-      "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 // Address of this CTA's shared-memory address `saddr` in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_shared(uint32_t saddr, uint32_t rank) {
@@ -147,6 +153,12 @@ __device__ __forceinline__ uint32_t map_shared(uint32_t saddr, uint32_t rank) {
 }
 __device__ __forceinline__ void st_shared_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory");
+}
+// Store to another CTA's shared memory that completes on a barrier there (shared::cluster
+// addresses of that CTA).
+__device__ __forceinline__ void st_async_v4(uint32_t addr, float v0, float v1, float v2, float v3, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1,%2,%3,%4}, [%5];\n"
+               ::"r"(addr), "f"(v0), "f"(v1), "f"(v2), "f"(v3), "r"(bar) : "memory");
 }
 // Bring a tensor-map box into L2 (coherent with whatever still writes it, so it may run ahead of
 // the kernel that produces the data).

@@ -253,7 +253,8 @@ def integer_rows(m, k, seed, lim=3):
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 200, 3840), (2, 129, 127), (3, 1000, 129), (16, 256, 512), (17, 130, 640),
           (31, 512, 1030), (33, 384, 2000), (64, 300, 4096), (65, 129, 300), (100, 1024, 1024), (128, 128, 16),
           (129, 257, 1500), (200, 640, 384), (256, 512, 512), (257, 1100, 900), (333, 1999, 4090), (512, 768, 2048),
-          (700, 513, 260), (1024, 2048, 1280), (1500, 300, 100)]
+          (700, 513, 260), (1024, 2048, 1280), (1500, 300, 100), (90, 200, 8200), (128, 3840, 3000),
+          (300, 1000, 8200), (130, 2000, 128), (2100, 1240, 700)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
