@@ -16,12 +16,14 @@
 
 #include "common.cuh"
 #include "pdl.cuh"
+#include "tc_host.h"
 
 namespace fbfp {
 namespace {
 
 constexpr int kSeg = 512;            // values a warp takes
-constexpr int kLane = 16;            // values a lane takes
+constexpr int kLane = 16;            // values a lane takes, as pairs (the fp32 arithmetic is paired)
+constexpr int kPairs = kLane / 2;
 constexpr int kNormMaxK = 32768;     // the longest row of the norm kernel (1024 threads x 2 chunks)
 
 struct RowsOut {
@@ -36,212 +38,359 @@ __device__ __forceinline__ int64_t scale_word(int64_t row, int seg, int segs) {
   return ((row >> 7) * segs + seg) * 128 + (row & 31) * 4 + ((row & 127) >> 5);
 }
 
-__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b, const __nv_bfloat16*) {
-  a = __uint_as_float(u << 16);
-  b = __uint_as_float(u & 0xFFFF0000u);
+__device__ __forceinline__ float2 unpack2(uint32_t u, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
-__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b, const __half*) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-  a = f.x;
-  b = f.y;
+__device__ __forceinline__ float2 unpack2(uint32_t u, const __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_float(float v, float& o) { o = v; }
-__device__ __forceinline__ void from_float(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_float(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ uint32_t pack2(float2 f, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float2 f, const __half*) {
+  const __half2 h = __float22half2_rn(f);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-// 16 values from p (n of them exist, the others read as zero); vec: p is 16-byte aligned.
+__device__ __forceinline__ void ld32(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p) : "memory");
+}
+__device__ __forceinline__ void st32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// A lane's 16 values of a segment as they lie in memory: loaded early, unpacked where they are
+// needed. VEC: values 16 lane .. 16 lane + 15, in whole 32-byte sectors, for rows that start on 32
+// bytes and hold a multiple of 16 values. Not VEC: values lane + 32 i, so that rows of any
+// alignment and length are read and written along the lanes. (One kernel for both would run a
+// third slower: its branches cost instruction fetches that short rows cannot hide.)
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, int n, bool vec, float (&v)[kLane]) {
-  if (vec && n >= kLane) {
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) unpack2(w[i], v[8 * h + 2 * i], v[8 * h + 2 * i + 1], p);
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const float4 f = reinterpret_cast<const float4*>(p)[h];
-        v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) v[i] = i < n ? to_float(p[i]) : 0.f;
-  }
-}
+struct Raw16 {
+  uint32_t w[kLane * sizeof(T) / 4];
+};
 
-template <typename T>
-__device__ __forceinline__ void store16(T* p, int n, bool vec, const float (&v)[kLane]) {
-  if (vec && n >= kLane) {
-    constexpr int per = 16 / sizeof(T);
-#pragma unroll
-    for (int h = 0; h < kLane / per; ++h) {
-      __align__(16) T o[per];
-#pragma unroll
-      for (int i = 0; i < per; ++i) from_float(v[per * h + i], o[i]);
-      reinterpret_cast<uint4*>(p)[h] = *reinterpret_cast<const uint4*>(o);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kLane; ++i)
-      if (i < n) from_float(v[i], p[i]);
-  }
-}
-
-// One warp: quantise its 512 values (16 per lane, zeros past the row's end) of segment `seg` of
-// `row` and store values and scale word. Called by whole warps.
-__device__ __forceinline__ void quantise_segment(const float (&v)[kLane], int64_t row, int seg, const RowsOut& o) {
+template <bool VEC>
+__device__ __forceinline__ int place(int i) {
   const int lane = threadIdx.x & 31;
-  // maximum of |v| as bits: ordered like the values, with NaN above infinity above all others
-  uint32_t amax = 0;
+  return VEC ? lane * kLane + i : lane + 32 * i;
+}
+
+// p: the segment's first value; n of the segment's values exist (the others read as zero).
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw16<T> load16(const T* p, int n) {
+  Raw16<T> r;
+  constexpr int words = kLane * sizeof(T) / 4;
 #pragma unroll
-  for (int i = 0; i < kLane; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < words; ++i) r.w[i] = 0;
+  if constexpr (VEC) {
+    if (place<VEC>(0) < n) {
 #pragma unroll
-  for (int s = 4; s > 0; s >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, s));
-  // 448 = 1.75 * 2^8: the exponent goes up by one where the mantissa is above 1.75
-  int c = (int)((amax + 0x1FFFFFu) >> 23) - 8;
-  c = amax >= 0x7F800000u ? 255 : (c < 0 ? 0 : c);
-  const float inv = c == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(254 - c) << 23);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE,
-                                                 __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    w[i] = lo | (hi << 16);
-  }
-  const int64_t k0 = (int64_t)seg * kSeg + lane * kLane;
-  uint8_t* q = o.q + row * o.ldq + k0;
-  if (k0 + kLane <= o.k) {
-    *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int h = 0; h < words; h += 8) ld32(reinterpret_cast<const uint32_t*>(p + place<VEC>(0)) + h, r.w + h);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < kLane; ++i)
-      if (k0 + i < o.k) q[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    for (int i = 0; i < kLane; ++i) {
+      if (place<VEC>(i) < n) {
+        if constexpr (sizeof(T) == 4)
+          r.w[i] = __float_as_uint(p[place<VEC>(i)]);
+        else
+          r.w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[place<VEC>(i)] << (16 * (i & 1));
+      }
+    }
   }
-  uint32_t word = (uint32_t)c;
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const Raw16<T>& r, float2 (&v)[kPairs]) {
 #pragma unroll
-  for (int b = 1; b < 4; ++b) word |= (uint32_t)__shfl_sync(0xffffffffu, c, 8 * b) << (8 * b);
-  // lane 0 holds block 0's byte; past the row's last block the values are zero and c is 0
+  for (int i = 0; i < kPairs; ++i) {
+    if constexpr (sizeof(T) == 4)
+      v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else
+      v[i] = unpack2(r.w[i], (const T*)nullptr);
+  }
+}
+
+template <bool VEC, typename T>
+__device__ __forceinline__ void store16(T* p, int n, const float2 (&v)[kPairs]) {
+  constexpr int words = kLane * sizeof(T) / 4;
+  uint32_t w[words];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[2 * i] = __float_as_uint(v[i].x);
+      w[2 * i + 1] = __float_as_uint(v[i].y);
+    } else {
+      w[i] = pack2(v[i], (const T*)nullptr);
+    }
+  }
+  if constexpr (VEC) {
+    if (place<VEC>(0) < n) {
+#pragma unroll
+      for (int h = 0; h < words; h += 8) st32(reinterpret_cast<uint32_t*>(p + place<VEC>(0)) + h, w + h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      if (place<VEC>(i) < n) {
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[place<VEC>(i)] = w[i];
+        else reinterpret_cast<uint16_t*>(p)[place<VEC>(i)] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Scale byte of a block whose values' magnitude bits have the maximum amax, and the factor
+// 2^(127 - c). 448 = 1.75 * 2^8: the exponent goes up by one where the mantissa is above 1.75.
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  const int c = (int)((amax + 0x1FFFFFu) >> 23) - 8;
+  return amax >= 0x7F800000u ? 255 : (c < 0 ? 0 : c);
+}
+__device__ __forceinline__ float scale_inverse(int c) {
+  return c == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(254 - c) << 23);
+}
+
+// One warp: quantise its 512 values (zeros past the row's end) of segment `seg` of `row` and store
+// values and scale word. Called by whole warps. Across lanes the maximum of |v| is taken on its
+// bits, which are ordered like the values, with NaN above infinity above all others.
+template <bool VEC>
+__device__ __forceinline__ void quantise_segment(const float2 (&v)[kPairs], int64_t row, int seg, const RowsOut& o) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* q = o.q + row * o.ldq + (int64_t)seg * kSeg;
+  const int n = (int)(o.k - (int64_t)seg * kSeg < kSeg ? o.k - (int64_t)seg * kSeg : kSeg);
+  uint32_t word;
+  if constexpr (VEC) {                                   // a block lies in 8 lanes
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) top = amax3(top, v[i].x, v[i].y);
+    uint32_t amax = __float_as_uint(top);
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+    const int c = scale_byte(amax);
+    const float2 inv = make_float2(scale_inverse(c), scale_inverse(c));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i], inv), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i + 1], inv), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | (hi << 16);
+    }
+    if (place<VEC>(0) < n) *reinterpret_cast<uint4*>(q + place<VEC>(0)) = make_uint4(w[0], w[1], w[2], w[3]);
+    word = (uint32_t)c;
+#pragma unroll
+    for (int b = 1; b < 4; ++b) word |= (uint32_t)__shfl_sync(0xffffffffu, c, 8 * b) << (8 * b);
+  } else {                                               // a block is four values of every lane
+    word = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float top = amax3(amax3(0.f, v[2 * b].x, v[2 * b].y), v[2 * b + 1].x, v[2 * b + 1].y);
+      const int c = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      const float2 inv = make_float2(scale_inverse(c), scale_inverse(c));
+      word |= (uint32_t)c << (8 * b);
+#pragma unroll
+      for (int i = 2 * b; i < 2 * b + 2; ++i) {
+        const uint32_t e = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[i], inv), __NV_SATFINITE, __NV_E4M3);
+        if (place<VEC>(2 * i) < n) q[place<VEC>(2 * i)] = (uint8_t)e;
+        if (place<VEC>(2 * i + 1) < n) q[place<VEC>(2 * i + 1)] = (uint8_t)(e >> 8);
+      }
+    }
+  }
+  // lane 0's word is right; past the row's last block the values are zero and so are the bytes
   if (lane == 0) o.sc[scale_word(row, seg, o.segs)] = word;
   // the last row also zeroes the tile's rows behind it, so that every scale byte is defined
   if (row == o.m - 1)
     for (int64_t r = o.m + lane; r < ((o.m + 127) & ~(int64_t)127); r += 32) o.sc[scale_word(r, seg, o.segs)] = 0u;
 }
 
+__device__ __forceinline__ int left_of(int64_t k, int seg) {   // values of the row from segment `seg` on
+  const int64_t n = k - (int64_t)seg * kSeg;
+  return n > kSeg ? kSeg : (int)n;                             // 0 or less: none
+}
+
 // ------------------------------------------------------------------------------- quantise, GeGLU
 constexpr int kFlatThreads = 256;
 
+// gelu_tanh(g) = g (1 + tanh t) / 2 = g / (1 + exp(-2 t)), t = sqrt(2 / pi) (g + 0.044715 g^3): no
+// cancellation for negative g. The exponent is taken to base 2, log2(e) in its constants; where the
+// power overflows the quotient is 0, as it should be.
+__device__ __forceinline__ float2 gelu_tanh(float2 g) {
+  const float c1 = 2.302208198144325f, c2 = 0.1029432395800235f;   // 2 log2(e) sqrt(2 / pi) (1, 0.044715)
+  const float2 t = __fmul2_rn(g, __ffma2_rn(make_float2(-c2, -c2), __fmul2_rn(g, g), make_float2(-c1, -c1)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  e = __fadd2_rn(e, make_float2(1.f, 1.f));
+  return make_float2(__fdividef(g.x, e.x), __fdividef(g.y, e.y));
+}
+
 // One warp per (row, segment). GEGLU: the row holds gate | up, `k` values each.
-template <typename T, bool GEGLU>
-__global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int64_t ldx, bool vec, const RowsOut o) {
+template <typename T, bool GEGLU, bool VEC>
+__global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int64_t ldx, const RowsOut o) {
   pdl_prologue();
-  const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * (kFlatThreads / 32) + (threadIdx.x >> 5);
   const int64_t row = unit / o.segs;
   if (row >= o.m) return;                              // whole warps
-  const int seg = (int)(unit - row * o.segs);
-  const int64_t k0 = (int64_t)seg * kSeg + lane * kLane;
-  const int n = (int)(o.k - k0 < kLane ? o.k - k0 : kLane);
-  const T* p = x + row * ldx + k0;
-  float v[kLane];
-  load16(p, n, vec, v);
+  const int seg = (int)(unit - row * o.segs), n = left_of(o.k, seg);
+  const T* p = x + row * ldx + (int64_t)seg * kSeg;
+  float2 v[kPairs];
   if constexpr (GEGLU) {
-    float u[kLane];
-    load16(p + o.k, n, vec, u);
+    const Raw16<T> gr = load16<VEC>(p, n), ur = load16<VEC>(p + o.k, n);
+    float2 u[kPairs];
+    unpack16(gr, v);
+    unpack16(ur, u);
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      // gelu_tanh(g) = g (1 + tanh t) / 2 = g / (1 + exp(-2 t)): no cancellation for g < 0
-      const float g = v[i];
-      const float t2 = 1.5957691216057308f * (g + 0.044715f * g * g * g);   // 2 sqrt(2 / pi) (..)
-      v[i] = g / (1.f + expf(-t2)) * u[i];
-    }
+    for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(gelu_tanh(v[i]), u[i]);
+  } else {
+    unpack16(load16<VEC>(p, n), v);
   }
-  quantise_segment(v, row, seg, o);
+  quantise_segment<VEC>(v, row, seg, o);
 }
 
 // ------------------------------------------------------------------------------- RMSNorm
-__device__ __forceinline__ float cta_sum(float v, float* red) {
+// A team of warps takes a row, a warp NV segments of it, in registers; a CTA has one team or
+// several and goes on to further rows, whose values are on their way while a row is worked on
+// (kEarly: all but rows above 16384 values, whose 1024 threads have 64 registers each, and long
+// fp32 rows). The weights come from L1. MODE 0: RMSNorm(x; w). MODE 1: h = x + resid first,
+// MODE 2: h = RMSNorm(x; w_post) + resid; both store round(h) to resid and normalise the
+// unrounded h.
+struct NormArgs {
+  int64_t ldx, ldr;
+  float eps, inv_k;
+  int team;                                              // warps per row
+};
+
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+// Sum over the warps of a team; red: MAXW floats of the team, zero where it has fewer warps.
+template <int MAXW>
+__device__ __forceinline__ float team_sum(float2 p, float* red, int warp) {
+  float v = p.x + p.y;
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
-  float t = 0.f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += red[w];
-  return t;
+  float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < MAXW; w += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(red + w);
+    t = __fadd2_rn(t, __fadd2_rn(make_float2(q.x, q.y), make_float2(q.z, q.w)));
+  }
+  return t.x + t.y;
 }
 
-// One CTA per row, its values in registers (NV chunks of 16 per thread; a warp's chunks are 512
-// consecutive values). MODE 0: RMSNorm(x; w). MODE 1: h = x + resid first, MODE 2:
-// h = RMSNorm(x; w_post) + resid; both store round(h) to resid and normalise the unrounded h.
-template <typename T, int NV, int MODE>
-__global__ void __launch_bounds__(1024) fp8_rmsnorm_kernel(const T* x, int64_t ldx, const T* w, const T* w_post,
-                                                           T* resid, int64_t ldr, float eps, bool vec,
-                                                           const RowsOut o) {
+template <typename T, int NV, int MODE, int THREADS, int MINB, bool VEC>
+__global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, const T* w, const T* w_post, T* resid,
+                                                                    const NormArgs a, const RowsOut o) {
   pdl_prologue();
-  __shared__ float red[2][32];
-  const int64_t row = blockIdx.x;
-  const float rk = (float)o.k;
-  float v[NV][kLane];
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t k0 = (int64_t)(threadIdx.x + i * blockDim.x) * kLane;
-    const int n = (int)(o.k - k0 < kLane ? o.k - k0 : kLane);
-    load16(x + row * ldx + k0, n, vec, v[i]);
-    if constexpr (MODE == 1) {
-      float r[kLane];
-      load16((const T*)resid + row * ldr + k0, n, vec, r);
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) v[i][e] += r[e];
-      store16(resid + row * ldr + k0, n, vec, v[i]);
-    }
-#pragma unroll
-    for (int e = 0; e < kLane; ++e) ss += v[i][e] * v[i][e];
-  }
-  float rs = rsqrtf(cta_sum(ss, red[0]) / rk + eps);
-  if constexpr (MODE == 2) {
-    ss = 0.f;
+  constexpr bool kEarly = THREADS < 1024 && (sizeof(T) == 2 || NV == 1);
+  constexpr int kWarps = THREADS / 32, kTeams = THREADS == 256 ? 8 : 1;   // at most, a CTA
+  __shared__ __align__(16) float reds[2][kTeams * kWarps];
+  for (int i = threadIdx.x; i < 2 * kTeams * kWarps; i += blockDim.x) (&reds[0][0])[i] = 0.f;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, teams = (int)(blockDim.x >> 5) / a.team;
+  const int seg0 = warp % a.team;                        // this warp's segments: seg0 + i * team
+  float* red = reds[0] + warp / a.team * kWarps;         // this team's sums, two rooms in turn
+  const int64_t step = (int64_t)gridDim.x * teams;
+  int64_t row = (int64_t)blockIdx.x * teams + warp / a.team;
+  const T *xp = x + row * a.ldx, *rp = resid + row * a.ldr;
+  Raw16<T> xr[NV], rr[NV];
+  if constexpr (kEarly) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t k0 = (int64_t)(threadIdx.x + i * blockDim.x) * kLane;
-      const int n = (int)(o.k - k0 < kLane ? o.k - k0 : kLane);
-      float wv[kLane], r[kLane];
-      load16(w_post + k0, n, vec, wv);
-      load16((const T*)resid + row * ldr + k0, n, vec, r);
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        v[i][e] = v[i][e] * rs * (1.f + wv[e]) + r[e];
-        ss += v[i][e] * v[i][e];
-      }
-      store16(resid + row * ldr + k0, n, vec, v[i]);
+      const int seg = seg0 + i * a.team, n = row < o.m ? left_of(o.k, seg) : 0;
+      xr[i] = load16<VEC>(xp + seg * kSeg, n);
+      if constexpr (MODE > 0) rr[i] = load16<VEC>(rp + seg * kSeg, n);
     }
-    rs = rsqrtf(cta_sum(ss, red[1]) / rk + eps);
   }
+  int turn = 0;
+#pragma unroll 1
+  for (int64_t base = (int64_t)blockIdx.x * teams; base < o.m; base += step, row += step) {
+    const bool live = row < o.m, more = row + step < o.m;   // a team past the last row takes part in the sums only
+    T* const now = resid + row * a.ldr;                      // this row of the residual
+    float2 v[NV][kPairs];
+    float2 ss = make_float2(0.f, 0.f);
+    if constexpr (kEarly) xp += step * a.ldx;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int chunk = threadIdx.x + i * blockDim.x;
-    const int seg = chunk >> 5;
-    if (seg >= o.segs) break;                          // whole warps
-    const int64_t k0 = (int64_t)chunk * kLane;
-    const int n = (int)(o.k - k0 < kLane ? o.k - k0 : kLane);
-    float wv[kLane];
-    load16(w + k0, n, vec, wv);
+    for (int i = 0; i < NV; ++i) {
+      const int seg = seg0 + i * a.team, all = left_of(o.k, seg), n = live ? all : 0;
+      if constexpr (!kEarly) xr[i] = load16<VEC>(x + row * a.ldx + seg * kSeg, n);
+      unpack16(xr[i], v[i]);
+      if constexpr (kEarly) xr[i] = load16<VEC>(xp + seg * kSeg, more ? all : 0);
+      if constexpr (MODE == 1) {
+        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n);
+        float2 r[kPairs];
+        unpack16(rr[i], r);
+        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0);
 #pragma unroll
-    for (int e = 0; e < kLane; ++e) v[i][e] = v[i][e] * rs * (1.f + wv[e]);
-    quantise_segment(v[i], row, seg, o);
+        for (int e = 0; e < kPairs; ++e) v[i][e] = __fadd2_rn(v[i][e], r[e]);
+        store16<VEC>(now + seg * kSeg, n, v[i]);
+      }
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) ss = __ffma2_rn(v[i][e], v[i][e], ss);
+    }
+    float rs = rsqrtf(team_sum<kWarps>(ss, red + turn, seg0) * a.inv_k + a.eps);
+    turn ^= kTeams * kWarps;
+    if constexpr (MODE == 2) {
+      ss = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int seg = seg0 + i * a.team, all = left_of(o.k, seg), n = live ? all : 0;
+        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n);
+        float2 wv[kPairs];
+        unpack16(load16<VEC>(w_post + seg * kSeg, n), wv);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {               // y = v rs, y + y w
+          v[i][e] = __fmul2_rn(v[i][e], both(rs));
+          v[i][e] = __ffma2_rn(v[i][e], wv[e], v[i][e]);
+        }
+        unpack16(rr[i], wv);
+        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          v[i][e] = __fadd2_rn(v[i][e], wv[e]);
+          ss = __ffma2_rn(v[i][e], v[i][e], ss);
+        }
+        store16<VEC>(now + seg * kSeg, n, v[i]);
+      }
+      rs = rsqrtf(team_sum<kWarps>(ss, red + turn, seg0) * a.inv_k + a.eps);
+      turn ^= kTeams * kWarps;
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int seg = seg0 + i * a.team;
+        if (seg >= o.segs) break;                        // whole warps
+        float2 wv[kPairs];
+        unpack16(load16<VEC>(w + seg * kSeg, left_of(o.k, seg)), wv);
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+          v[i][e] = __fmul2_rn(v[i][e], both(rs));
+          v[i][e] = __ffma2_rn(v[i][e], wv[e], v[i][e]);
+        }
+        quantise_segment<VEC>(v[i], row, seg, o);
+      }
+    }
   }
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Whether rows whose addresses and byte strides (or'ed) are these start on 32 bytes and hold whole
+// lanes' values.
+bool whole_sectors(uint64_t bits, int64_t k) { return (bits & 31) == 0 && k % kLane == 0; }
+uint64_t bits_of(const void* p) { return (uint64_t)(uintptr_t)p; }
 
 // Arguments common to the three entries; fills o.
 int rows_out(int64_t m, int64_t k, void* values, int64_t ldv, void* scales, RowsOut& o) {
@@ -262,38 +411,51 @@ int rows_out(int64_t m, int64_t k, void* values, int64_t ldv, void* scales, Rows
 
 template <typename T, bool GEGLU>
 cudaError_t launch_flat(const void* x, int64_t ldx, const RowsOut& o, cudaStream_t st) {
-  const bool vec = aligned16(x) && (ldx * sizeof(T)) % 16 == 0 && (!GEGLU || (o.k * sizeof(T)) % 16 == 0);
+  const bool vec = whole_sectors(bits_of(x) | (uint64_t)ldx * sizeof(T), o.k);
   const int64_t units = o.m * o.segs, per = kFlatThreads / 32;
-  return launch_pdl(fp8_rows_kernel<T, GEGLU>, dim3((unsigned)((units + per - 1) / per)), dim3(kFlatThreads), 0, st,
-                    reinterpret_cast<const T*>(x), ldx, vec, o);
+  return launch_pdl(vec ? fp8_rows_kernel<T, GEGLU, true> : fp8_rows_kernel<T, GEGLU, false>,
+                    dim3((unsigned)((units + per - 1) / per)), dim3(kFlatThreads), 0, st,
+                    reinterpret_cast<const T*>(x), ldx, o);
 }
 
-template <typename T, int NV, int MODE>
-cudaError_t launch_norm(const void* x, int64_t ldx, const void* w, const void* w_post, void* resid, int64_t ldr,
-                        float eps, const RowsOut& o, cudaStream_t st) {
-  const bool vec = aligned16(x) && aligned16(w) && (ldx * sizeof(T)) % 16 == 0 &&
-                   (MODE == 0 || (aligned16(resid) && (ldr * sizeof(T)) % 16 == 0)) &&
-                   (MODE != 2 || aligned16(w_post));
-  const int warps = (o.segs + NV - 1) / NV;
-  return launch_pdl(fp8_rmsnorm_kernel<T, NV, MODE>, dim3((unsigned)o.m), dim3(32 * warps), 0, st,
-                    reinterpret_cast<const T*>(x), ldx, reinterpret_cast<const T*>(w),
-                    reinterpret_cast<const T*>(w_post), reinterpret_cast<T*>(resid), ldr, eps, vec, o);
+struct NormPtrs {
+  const void *x, *w, *w_post;
+  void* resid;
+};
+
+template <typename T, int NV, int MODE, int THREADS, int MINB, bool VEC>
+cudaError_t launch_norm(const NormPtrs& p, NormArgs a, const RowsOut& o, int nsm, cudaStream_t st) {
+  a.team = (o.segs + NV - 1) / NV;
+  const int teams = THREADS == 256 ? 8 / a.team : 1;     // rows of a CTA at a time
+  const int64_t want = (o.m + teams - 1) / teams;
+  const int64_t room = (int64_t)nsm * MINB;
+  return launch_pdl(fp8_rmsnorm_kernel<T, NV, MODE, THREADS, MINB, VEC>, dim3((unsigned)(want < room ? want : room)),
+                    dim3(32 * a.team * teams), 0, st, reinterpret_cast<const T*>(p.x),
+                    reinterpret_cast<const T*>(p.w), reinterpret_cast<const T*>(p.w_post),
+                    reinterpret_cast<T*>(p.resid), a, o);
 }
 
 template <typename T, int MODE>
-cudaError_t norm_by_size(const void* x, int64_t ldx, const void* w, const void* w_post, void* resid, int64_t ldr,
-                         float eps, const RowsOut& o, cudaStream_t st) {
-  // up to 16384 values a row fits one chunk per thread
-  return o.segs <= 32 ? launch_norm<T, 1, MODE>(x, ldx, w, w_post, resid, ldr, eps, o, st)
-                      : launch_norm<T, 2, MODE>(x, ldx, w, w_post, resid, ldr, eps, o, st);
+cudaError_t norm_by_size(const NormPtrs& p, NormArgs a, const RowsOut& o, int nsm, cudaStream_t st) {
+  const bool vec = whole_sectors(bits_of(p.x) | bits_of(p.w) | bits_of(p.resid) | bits_of(p.w_post) |
+                                     (uint64_t)a.ldx * sizeof(T) | (MODE ? (uint64_t)a.ldr * sizeof(T) : 0),
+                                 o.k);
+  // CTAs per SM by the registers of a row's 16 values a thread (twice as many words in fp32)
+  constexpr int kThree = sizeof(T) == 2 ? 3 : 2, kTwo = sizeof(T) == 2 ? 2 : 1;
+  if (!vec)
+    return o.segs <= 8 ? launch_norm<T, 1, MODE, 256, kThree, false>(p, a, o, nsm, st)
+                       : launch_norm<T, 2, MODE, 1024, 1, false>(p, a, o, nsm, st);
+  return o.segs <= 8    ? launch_norm<T, 1, MODE, 256, kThree, true>(p, a, o, nsm, st)
+         : o.segs <= 16 ? launch_norm<T, 1, MODE, 512, kTwo, true>(p, a, o, nsm, st)
+         : o.segs <= 32 ? launch_norm<T, 2, MODE, 512, 1, true>(p, a, o, nsm, st)
+                        : launch_norm<T, 2, MODE, 1024, 1, true>(p, a, o, nsm, st);
 }
 
 template <typename T>
-cudaError_t norm_by_mode(const void* x, int64_t ldx, const void* w, const void* w_post, void* resid, int64_t ldr,
-                         float eps, const RowsOut& o, cudaStream_t st) {
-  return !resid ? norm_by_size<T, 0>(x, ldx, w, w_post, resid, ldr, eps, o, st)
-         : w_post ? norm_by_size<T, 2>(x, ldx, w, w_post, resid, ldr, eps, o, st)
-                  : norm_by_size<T, 1>(x, ldx, w, w_post, resid, ldr, eps, o, st);
+cudaError_t norm_by_mode(const NormPtrs& p, const NormArgs& a, const RowsOut& o, int nsm, cudaStream_t st) {
+  return !p.resid ? norm_by_size<T, 0>(p, a, o, nsm, st)
+         : p.w_post ? norm_by_size<T, 2>(p, a, o, nsm, st)
+                    : norm_by_size<T, 1>(p, a, o, nsm, st);
 }
 
 template <bool GEGLU>
@@ -347,10 +509,15 @@ extern "C" int fbfp_fp8_rmsnorm(const void* x, int dtype, int64_t m, int64_t k, 
   FBFP_CHECK_ARG(k <= kNormMaxK, "rows of at most %d values (got %lld)", kNormMaxK, (long long)k);
   FBFP_CHECK_ARG(ldx >= 0 && (!resid || m == 1 || ldr >= k), "bad row stride (ldx %lld, ldr %lld)", (long long)ldx,
                  (long long)ldr);
+  int dev = 0;
+  FBFP_CUDA_TRY(cudaGetDevice(&dev));
+  const NormPtrs p{x, w, w_post, resid};
+  const NormArgs a{ldx, ldr, eps, 1.f / (float)k, 0};
+  const int nsm = sm_count(dev);
   const cudaStream_t st = as_stream(stream);
-  FBFP_CUDA_TRY(dtype == FBFP_BF16 ? norm_by_mode<__nv_bfloat16>(x, ldx, w, w_post, resid, ldr, eps, o, st)
-                : dtype == FBFP_F16 ? norm_by_mode<__half>(x, ldx, w, w_post, resid, ldr, eps, o, st)
-                                    : norm_by_mode<float>(x, ldx, w, w_post, resid, ldr, eps, o, st));
+  FBFP_CUDA_TRY(dtype == FBFP_BF16  ? norm_by_mode<__nv_bfloat16>(p, a, o, nsm, st)
+                : dtype == FBFP_F16 ? norm_by_mode<__half>(p, a, o, nsm, st)
+                                    : norm_by_mode<float>(p, a, o, nsm, st));
   FBFP_LAUNCH_CHECK("fp8_rmsnorm_kernel");
   return FBFP_OK;
 }
