@@ -145,11 +145,6 @@ def stream_ptr(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def raw_stream(index: int) -> int:
-    """The handle of device `index`'s current stream (without building a Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def require_cuda(t: torch.Tensor, what: str) -> None:
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise RuntimeError(f"{what} must be a CUDA tensor: FlashBFP-B200 runs only on the GPU "

@@ -1,8 +1,8 @@
-"""Build libflashbfp.so (sm_100a) in-tree with nvcc.
+"""Build libflashbfp.so (sm_100a) in-tree with nvcc, and the Python module _fp8_bind with g++.
 
     python -m flashbfp_b200.build          # or flashbfp_b200.build.build()
 
-The shared library lands next to this file so that it travels with the source tree.
+Both land next to this file so that they travel with the source tree.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libflashbfp.so")
+BIND = os.path.join(HERE, "_fp8_bind.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -33,8 +34,32 @@ def _stale() -> bool:
     return any(os.path.getmtime(p) > t for p in deps)
 
 
+def _build_bind(force: bool, verbose: bool) -> None:
+    """_fp8_bind.so: the Python entry points that check their tensors and call the library."""
+    src = os.path.join(CSRC, "fp8_bind.cpp")
+    header = os.path.join(os.path.dirname(HERE), "include", "flashbfp.h")
+    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) > max(map(os.path.getmtime, (src, header))):
+        return
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), sysconfig.get_paths()["include"]]
+    tmp = BIND + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[a for i in inc for a in ("-isystem", i)], src, "-o", tmp, "-L" + HERE, "-l:libflashbfp.so",
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(root, "lib")]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BIND)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
+        _build_bind(force, verbose)
         return LIB
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -53,6 +78,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
+    _build_bind(force, verbose)
     return LIB
 
 
