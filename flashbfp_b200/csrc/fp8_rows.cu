@@ -232,7 +232,10 @@ __device__ __forceinline__ float2 gelu_tanh(float2 g) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
   e = __fadd2_rn(e, make_float2(1.f, 1.f));
-  return make_float2(__fdividef(g.x, e.x), __fdividef(g.y, e.y));
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+  return __fmul2_rn(g, r);
 }
 
 // One warp per (row, segment). GEGLU: the row holds gate | up, `k` values each.
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
                                                                     const NormArgs a, const RowsOut o) {
   pdl_prologue();
   constexpr bool kEarly = THREADS < 1024 && (sizeof(T) == 2 || NV == 1);
-  constexpr int kWarps = THREADS / 32, kTeams = THREADS == 256 ? 8 : 1;   // at most, a CTA
+  constexpr int kWarps = THREADS / 32, kTeams = THREADS <= 256 ? kWarps : 1;   // at most, a CTA
   __shared__ __align__(16) float reds[2][kTeams * kWarps];
   for (int i = threadIdx.x; i < 2 * kTeams * kWarps; i += blockDim.x) (&reds[0][0])[i] = 0.f;
   __syncthreads();
@@ -426,7 +429,7 @@ struct NormPtrs {
 template <typename T, int NV, int MODE, int THREADS, int MINB, bool VEC>
 cudaError_t launch_norm(const NormPtrs& p, NormArgs a, const RowsOut& o, int nsm, cudaStream_t st) {
   a.team = (o.segs + NV - 1) / NV;
-  const int teams = THREADS == 256 ? 8 / a.team : 1;     // rows of a CTA at a time
+  const int teams = THREADS <= 256 ? THREADS / 32 / a.team : 1;   // rows of a CTA at a time
   const int64_t want = (o.m + teams - 1) / teams;
   const int64_t room = (int64_t)nsm * MINB;
   return launch_pdl(fp8_rmsnorm_kernel<T, NV, MODE, THREADS, MINB, VEC>, dim3((unsigned)(want < room ? want : room)),

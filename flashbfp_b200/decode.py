@@ -16,6 +16,12 @@ prefill GEMM once M > 16), and logits for the last row only.
 ``GemmaDecoder.from_hf`` takes a Hugging Face Gemma-3 causal LM after ``compress_gemma_model``;
 ``GemmaDecoder(...)`` takes the parts directly (used by the benchmark's random-init 12B-class
 model).
+
+With ``from_hf(..., weights="fp8")`` (an uncompressed model) or layers that hold ``fp8.Fp8Rows`` the
+linears run as block-scaled 8-bit products (``fp8.py``): the norms between a layer's halves, the
+GeGLU activation and the attention output leave as e4m3 rows with their scales, which the next
+linear multiplies as they are. Activations are rounded to e4m3 there (2^-4 relative at most);
+the residual stream, attention, norms and lm_head keep the precision they have otherwise.
 """
 from __future__ import annotations
 
@@ -24,7 +30,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from . import _lib
+from . import _lib, fp8
 from .linear import packed_linear, packed_linear_allreduce
 from .packed import PackedWeight, concat_rows
 
@@ -48,7 +54,7 @@ class DecoderShape:
 @dataclass
 class DecodeLayer:
     """One decoder layer's weights: OABF PackedWeights (or, for the uncompressed baseline,
-    dense bf16 [N, K] tensors in their place)."""
+    dense bf16 [N, K] tensors in their place, or block-scaled 8-bit Fp8Rows [N, K])."""
     qkv: PackedWeight                     # q | k | v rows
     o: PackedWeight
     gate_up: PackedWeight                 # gate | up rows
@@ -62,8 +68,8 @@ class DecodeLayer:
 
 
 def _dims(w) -> tuple:
-    """(rows, columns) of a layer weight: a PackedWeight, or a dense bf16 [N, K] tensor (the
-    uncompressed baseline decoder)."""
+    """(rows, columns) of a layer weight: a PackedWeight, a dense bf16 [N, K] tensor (the
+    uncompressed baseline decoder) or 8-bit rows."""
     if isinstance(w, PackedWeight):
         return w.n_out, w.k_in
     return int(w.shape[0]), int(w.shape[1])
@@ -121,6 +127,12 @@ class GemmaDecoder:
                                  f"{2 * self.inter_l}, o in {ko}, down in {kd})")
         if self.world == 1 and self.inter_l != s.inter:
             raise ValueError(f"gate|up holds {2 * self.inter_l} rows, not {2 * s.inter}")
+        eight = [isinstance(w, fp8.Fp8Rows) for ly in layers for w in (ly.qkv, ly.o, ly.gate_up, ly.down)]
+        self.fp8 = any(eight)
+        if self.fp8 and not all(eight):
+            raise ValueError("8-bit linears are all or none: some layer weights are Fp8Rows, others are not")
+        if self.fp8 and reducer is not None:
+            raise ValueError("8-bit linears run on one GPU (no reducer)")
         self.max_ctx = int(max_ctx)
         bf = dict(dtype=torch.bfloat16, device=dev)
         self.embed = embed.to(**bf).contiguous()
@@ -151,6 +163,11 @@ class GemmaDecoder:
         self.o = torch.zeros(R, s.hidden, **bf)
         self.gu = torch.zeros(R, 2 * self.inter_l, **bf)
         self.act = torch.zeros(R, self.inter_l, **bf)
+        if self.fp8:                                          # the linears' inputs as 8-bit rows
+            with torch.cuda.device(dev):
+                self.x8 = fp8.empty_rows(R, s.hidden, dev)
+                self.attn8 = fp8.empty_rows(R, self.hq * s.head_dim, dev)
+                self.act8 = fp8.empty_rows(R, self.inter_l, dev)
         self.down = torch.zeros(R, s.hidden, **bf)
         self.logits = torch.zeros(B, self.vocab_l, **bf)     # per sequence: this rank's vocabulary rows
         if reducer is not None:
@@ -175,10 +192,15 @@ class GemmaDecoder:
     # -- construction from a Hugging Face Gemma-3 model after compress_gemma_model -----------
     @classmethod
     def from_hf(cls, model, max_ctx: int, device=None, max_prefill: int = 128,
-                reducer=None, batch: int = 1) -> "GemmaDecoder":
+                reducer=None, batch: int = 1, weights: str = "oabf") -> "GemmaDecoder":
         """The decoder of a Gemma-3 causal LM after ``compress_gemma_model``; with ``reducer``,
         of a model compressed with ``compress_gemma_model(..., rank=r, world=reducer.world)``
-        on every rank (this rank's shards; lm_head rows split here)."""
+        on every rank (this rank's shards; lm_head rows split here). ``weights="fp8"``: of an
+        uncompressed model, its attention and MLP linears quantised to block-scaled 8 bits here."""
+        if weights not in ("oabf", "fp8"):
+            raise ValueError(f"weights must be 'oabf' or 'fp8', not {weights!r}")
+        if weights == "fp8" and reducer is not None:
+            raise ValueError("8-bit linears run on one GPU (no reducer)")
         cfg = model.config
         if getattr(cfg, "final_logit_softcapping", None) or getattr(cfg, "attn_logit_softcapping", None):
             raise NotImplementedError("logit soft-capping is not supported")
@@ -195,18 +217,29 @@ class GemmaDecoder:
         for i, lyr in enumerate(inner.layers):
             mods = (lyr.self_attn.q_proj, lyr.self_attn.k_proj, lyr.self_attn.v_proj, lyr.self_attn.o_proj,
                     lyr.mlp.gate_proj, lyr.mlp.up_proj, lyr.mlp.down_proj)
-            if not all(isinstance(m, OABFLinear) and m.compressed for m in mods):
+            if weights == "fp8":
+                if not all(isinstance(m, torch.nn.Linear) and m.bias is None for m in mods):
+                    raise TypeError(f"layer {i}: weights='fp8' takes plain linears without bias (an "
+                                    "uncompressed model)")
+            elif not all(isinstance(m, OABFLinear) and m.compressed for m in mods):
                 raise TypeError(f"layer {i} is not compressed: run compress_gemma_model first")
         dev = torch.device(device) if device is not None else inner.embed_tokens.weight.device
         layers = []
+
+        def joined(*mods):
+            """The linears' rows back to back, as one weight."""
+            if weights == "fp8":
+                return fp8.quantize_fp8(torch.cat([m.weight.data.to(dev) for m in mods]))
+            return mods[0].packed if len(mods) == 1 else concat_rows([m.packed for m in mods])
+
         with torch.cuda.device(dev):
             for lyr in inner.layers:
                 at, mlp = lyr.self_attn, lyr.mlp
                 layers.append(DecodeLayer(
-                    qkv=concat_rows([at.q_proj.packed, at.k_proj.packed, at.v_proj.packed]),
-                    o=at.o_proj.packed,
-                    gate_up=concat_rows([mlp.gate_proj.packed, mlp.up_proj.packed]),
-                    down=mlp.down_proj.packed,
+                    qkv=joined(at.q_proj, at.k_proj, at.v_proj),
+                    o=joined(at.o_proj),
+                    gate_up=joined(mlp.gate_proj, mlp.up_proj),
+                    down=joined(mlp.down_proj),
                     input_ln=lyr.input_layernorm.weight.data, post_attn_ln=lyr.post_attention_layernorm.weight.data,
                     pre_ffn_ln=lyr.pre_feedforward_layernorm.weight.data,
                     post_ffn_ln=lyr.post_feedforward_layernorm.weight.data,
@@ -231,8 +264,10 @@ class GemmaDecoder:
                    lm_head, max_ctx, dev, max_prefill, reducer=reducer, vocab_offset=v0, batch=batch)
 
     # -- one token ---------------------------------------------------------------------------
-    def _linear(self, x: torch.Tensor, pw, out: torch.Tensor) -> None:
-        if isinstance(pw, PackedWeight):
+    def _linear(self, x, pw, out: torch.Tensor) -> None:
+        if isinstance(pw, fp8.Fp8Rows):                       # x: 8-bit rows too
+            fp8.fp8_linear(x, pw, out=out)
+        elif isinstance(pw, PackedWeight):
             packed_linear(x, pw, None, torch.bfloat16, out=out)
         else:                                                 # a dense bf16 weight (baseline)
             torch.matmul(x, pw.t(), out=out)
@@ -265,6 +300,11 @@ class GemmaDecoder:
         self.reducer(slots)
         tok.copy_(argmax_pick(slots, self.world))
 
+    @staticmethod
+    def _rows8(r: fp8.Fp8Rows, m: int) -> fp8.Fp8Rows:
+        """The first m rows of a buffer of 8-bit rows."""
+        return fp8.Fp8Rows(r.values[:m], r.scales[:-(-m // 128)])
+
     def _layers(self, m: int, chunk_seq: Optional[int]) -> None:
         """Every layer over rows 0..m-1 of the activation buffers: with chunk_seq = b, a prompt
         chunk of sequence b at positions pos[b] .. pos[b] + m - 1 (causal over the chunk);
@@ -274,11 +314,13 @@ class GemmaDecoder:
         eps = float(s.rms_norm_eps)
         h, x, qkv, q, attn = self.h[:m], self.x[:m], self.qkv[:m], self.q[:m], self.attn[:m]
         o, gu, act, down = self.o[:m], self.gu[:m], self.act[:m], self.down[:m]
+        if self.fp8:
+            x8, attn8, act8 = (self._rows8(r, m) for r in (self.x8, self.attn8, self.act8))
         for li, ly in enumerate(self.layers):
             kind = s.layer_types[li]
             cos_t, sin_t = self.rope[kind]
             window = s.sliding_window if kind == "sliding_attention" else 0
-            self._linear(x, ly.qkv, qkv)
+            self._linear(x8 if self.fp8 else x, ly.qkv, qkv)
             if chunk_seq is None:
                 _lib.check(L.fbfp_decode_attention_step(
                     P(qkv), m, self.hq, self.hkv, s.head_dim, P(ly.q_norm), P(ly.k_norm), eps, P(cos_t),
@@ -294,13 +336,22 @@ class GemmaDecoder:
                 _lib.check(L.fbfp_decode_attention(P(q), m, P(kc), P(vc), self.hq, self.hkv, s.head_dim,
                                                    self.max_ctx, P(pos), window, self.scaling, P(attn), st),
                            "fbfp_decode_attention")
-            self._row_linear(attn, ly.o, o)
-            _lib.check(L.fbfp_post_residual_norm(P(o), m, P(ly.post_attn_ln), P(h), P(ly.pre_ffn_ln), eps,
-                                                 s.hidden, P(x), st), "fbfp_post_residual_norm")
-            self._linear(x, ly.gate_up, gu)
-            _lib.check(L.fbfp_geglu(P(gu), m, self.inter_l, P(act), st), "fbfp_geglu")
-            self._row_linear(act, ly.down, down)
             nxt = self.layers[li + 1].input_ln if li + 1 < len(self.layers) else self.final_norm
+            if self.fp8:
+                self._linear(fp8.quantize_fp8(attn, out=attn8), ly.o, o)
+                fp8.rmsnorm_fp8(o, ly.pre_ffn_ln, eps, residual=h, post_weight=ly.post_attn_ln, out=x8)
+                self._linear(x8, ly.gate_up, gu)
+                self._linear(fp8.geglu_fp8(gu, out=act8), ly.down, down)
+                if li + 1 < len(self.layers):
+                    fp8.rmsnorm_fp8(down, nxt, eps, residual=h, post_weight=ly.post_ffn_ln, out=x8)
+                    continue                                  # after the last layer: bf16, for lm_head
+            else:
+                self._row_linear(attn, ly.o, o)
+                _lib.check(L.fbfp_post_residual_norm(P(o), m, P(ly.post_attn_ln), P(h), P(ly.pre_ffn_ln), eps,
+                                                     s.hidden, P(x), st), "fbfp_post_residual_norm")
+                self._linear(x, ly.gate_up, gu)
+                _lib.check(L.fbfp_geglu(P(gu), m, self.inter_l, P(act), st), "fbfp_geglu")
+                self._row_linear(act, ly.down, down)
             _lib.check(L.fbfp_post_residual_norm(P(down), m, P(ly.post_ffn_ln), P(h), P(nxt), eps,
                                                  s.hidden, P(x), st), "fbfp_post_residual_norm")
 
@@ -309,6 +360,9 @@ class GemmaDecoder:
         P = _lib.ptr
         _lib.check(L.fbfp_embed(P(ids), m, P(self.embed), s.vocab, s.hidden, self.embed_scale, P(self.h),
                                 P(self.err), st), "fbfp_embed")
+        if self.fp8:
+            fp8.rmsnorm_fp8(self.h[:m], self.layers[0].input_ln, float(s.rms_norm_eps), out=self._rows8(self.x8, m))
+            return
         _lib.check(L.fbfp_rmsnorm(P(self.h), m, P(self.layers[0].input_ln), float(s.rms_norm_eps), s.hidden,
                                   P(self.x), st), "fbfp_rmsnorm")
 
@@ -383,6 +437,8 @@ class GemmaDecoder:
     def check(self) -> None:
         """Raise if a kernel met an out-of-range token (1) or position (2)."""
         self.stream.synchronize()
+        if self.fp8:
+            fp8.check_device_errors(self.device)
         e = int(self.err.item())
         if e:
             self.reset(self.pos.tolist())          # clears the error word on the decoder's stream

@@ -102,3 +102,11 @@ def test_rows_on_the_cpu():
     s = r.scale_matrix()
     for row in (0, 31, 32, 127, 128, 129):
         assert torch.equal(s[row].double(), torch.exp2(codes[row].double() - 127))
+
+
+def test_decoder_weight_kinds():
+    from flashbfp_b200.decode import GemmaDecoder
+    with pytest.raises(ValueError, match="'oabf' or 'fp8'"):
+        GemmaDecoder.from_hf(None, max_ctx=8, weights="int4")
+    with pytest.raises(ValueError, match="one GPU"):
+        GemmaDecoder.from_hf(None, max_ctx=8, weights="fp8", reducer=object())
