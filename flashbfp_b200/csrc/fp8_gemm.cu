@@ -14,7 +14,7 @@ using namespace sm100;
 
 struct Fp8Args {
   int64_t m, n;
-  int nkb;                 // ceil(k / 128): K blocks
+  uint32_t nkb;            // ceil(k / 128): K blocks
   int kgroups;             // ceil(k / 512): scale tiles of a row group
   const uint8_t *x_scales, *w_scales;
   const void* bias;
@@ -22,7 +22,8 @@ struct Fp8Args {
   void* y;
   int64_t ldy;
   int32_t* err;
-  int64_t n_tt;            // token tiles
+  uint32_t n_tt;           // token tiles (more than 64 tokens)
+  uint32_t tiles;
   int stages;              // depth of the operand ring
 };
 
@@ -82,8 +83,8 @@ __device__ __forceinline__ void store4(T* p, int n, const float4& v, bool vec) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Few tokens (up to 64). A CTA takes 128 output features (the MMA's M side: 128 weight rows) x BN
-// tokens (its N side) and a contiguous range of the K blocks; the CTAs of a cluster (up to 8) share
+// Few tokens (up to 64). A CTA takes 128 output features (the MMA's M side: 128 weight rows) x the
+// tokens (its N side, BN of them, zeros past the last) and a contiguous range of the K blocks; the CTAs of a cluster (up to 8) share
 // a tile and split its K blocks. Per K block one stage: 128 x 128 weight bytes, BN x 128 token
 // bytes (128-byte swizzle) and both scale tiles. Warp 0 loads, warp 1 copies the scales to tensor
 // memory and issues four MMAs, warps 2-5 read the sums back (a feature per lane) into shared
@@ -124,10 +125,9 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
   const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const int64_t tile = blockIdx.x / splits;
-  const int64_t n0 = tile / a.n_tt * 128, m0 = tile % a.n_tt * BN;
-  const int kb0 = (int)((int64_t)a.nkb * rank / splits), kb1 = (int)((int64_t)a.nkb * (rank + 1) / splits);
-  const int ntok = (int)(a.m - m0 < BN ? a.m - m0 : BN);
+  const int64_t n0 = (int64_t)(blockIdx.x / splits) * 128;
+  const int kb0 = (int)(a.nkb * rank / splits), kb1 = (int)(a.nkb * (rank + 1) / splits);   // nkb < 2^24
+  const int ntok = (int)a.m;                             // <= BN
   const int own = (int)((ntok + splits - 1) / splits);   // tokens a CTA of the cluster owns
   const int t1 = min(own, ntok - (int)rank * own);       // this one (none: <= 0)
 
@@ -163,10 +163,9 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
         uint8_t* st = smem + (size_t)s * C::kStage;
         mbar_arrive_expect_tx(&full[s], C::kStage);
         tma_2d_g2s(st, &M.w, kb * 128, (int)n0, &full[s]);
-        tma_2d_g2s(st + C::kA, &M.x, kb * 128, (int)m0, &full[s]);
+        tma_2d_g2s(st + C::kA, &M.x, kb * 128, 0, &full[s]);
         bulk_g2s(st + C::kA + C::kB, a.w_scales + (n0 / 128 * a.kgroups + kb / 4) * C::kSf, C::kSf, &full[s]);
-        bulk_g2s(st + C::kA + C::kB + C::kSf, a.x_scales + (m0 / 128 * a.kgroups + kb / 4) * C::kSf, C::kSf,
-                 &full[s]);
+        bulk_g2s(st + C::kA + C::kB + C::kSf, a.x_scales + (int64_t)(kb / 4) * C::kSf, C::kSf, &full[s]);
         ++issued;
         if (++s == stages) { s = 0; ph ^= 1; }
       }
@@ -242,7 +241,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < nf) bias[i] = load_as_float(a.bias, a.bias_dtype, n0 + f + i);
-  T* y = reinterpret_cast<T*>(a.y) + (m0 + (int)rank * own) * a.ldy + n0 + f;
+  T* y = reinterpret_cast<T*>(a.y) + (int64_t)((int)rank * own) * a.ldy + n0 + f;
 #pragma unroll 1
   for (int t = warp; t < t1; t += C::kThreads / 32) {
     float4 p = make_float4(bias[0], bias[1], bias[2], bias[3]);
@@ -274,11 +273,12 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 // completed. A tile starts on a whole scale tile (features in steps of 128), which keeps the
 // scales' tensor-memory addresses on multiples of 4 columns.
 //
-// Epilogue: eight warps, each a unit of 32 tokens (a lane quarter; a token per lane) x BN / 2
-// features. The sums go to registers first, so that the accumulator is free again after the
-// loads. With a split every unit has an owner among the cluster's CTAs: the others store their
-// sums into its shared memory (rows padded to 17 x 16 bytes, free of bank conflicts), and it adds
-// them to its own in rank order.
+// Epilogue: eight warps, each with 32 tokens (a lane quarter; a token per lane) x BN / 2 features. The
+// sums go to registers first, so that the accumulator is free again after the loads. With a split
+// every block of 32 tokens x 32 features has an owner among the cluster's CTAs: the others store
+// their sums into its shared memory (a warp's store is 512 bytes in a row: 16 bytes a lane), and it
+// adds them to its own in rank order. Owners are spread so that four warps of every CTA have a block
+// (split four ways) or two.
 template <int CG, int BN>
 struct Many {
   static constexpr int kRowsB = BN / CG;
@@ -293,12 +293,11 @@ struct Many {
   static constexpr int kCols = BN / 2;                           // columns of a unit
   static constexpr int kTurn = 32 * 17 * 4;                      // a warp's 32 x 16 words, rows 17 apart
   static constexpr int kTurns = kEpiWarps * kTurn;
-  static constexpr int kSumRow = kCols + 4;                      // floats
-  static constexpr int kUnit = 32 * kSumRow * 4;
-  static constexpr int kSums = 7 * kUnit;                        // at most 7 units from other CTAs
+  static constexpr int kBlock = 32 * 32 * 4;                     // [feature / 4][token][4]
+  static constexpr int kSums = 12 * kBlock;                      // 16 / S blocks from S - 1 CTAs, S 2 or 4
   static constexpr int kBars = (2 * kMaxStages + 2 + 2 + 2) * 8 + 16;
   static constexpr int kFixed = kBars + 1024;                    // stages start on 1 KB
-  static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kUnit % 16 == 0, "alignment");
+  static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kBlock % 16 == 0, "alignment");
   static_assert(kSfCol0 + kSfSlots * kSfCols <= kTmemCols, "tensor memory budget");
 };
 
@@ -311,6 +310,7 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
                                           uint32_t* turn) {
   const int lane = threadIdx.x & 31;
   const int64_t row = tok0 + lane;
+  const int rows = a.m - tok0 < 32 ? (int)(a.m - tok0) : 32;
   T* y = reinterpret_cast<T*>(a.y);
   if constexpr (sizeof(T) == 4) {
     if (vec && f0 + 32 <= a.n) {
@@ -336,9 +336,10 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
       for (int i = 0; i < 16; ++i) turn[lane * 17 + i] = __float_as_uint(v[16 * h + i]);
       __syncwarp();
       const int64_t f = f0 + 16 * h + (lane & 15);
+      const int r1 = f < a.n ? rows : 0;
+      T* p = y + (tok0 + (lane >> 4)) * a.ldy + f;
 #pragma unroll 4
-      for (int r = lane >> 4; r < 32; r += 2)
-        if (tok0 + r < a.m && f < a.n) y[(tok0 + r) * a.ldy + f] = __uint_as_float(turn[r * 17 + (lane & 15)]);
+      for (int r = lane >> 4; r < r1; r += 2, p += 2 * a.ldy) *p = __uint_as_float(turn[r * 17 + (lane & 15)]);
     }
   } else {
     uint32_t w[16];
@@ -364,11 +365,20 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
 #pragma unroll
     for (int i = 0; i < 16; ++i) turn[lane * 17 + i] = w[i];
     __syncwarp();
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r)
-      if (tok0 + r < a.m && f0 + lane < a.n)
-        y[(tok0 + r) * a.ldy + f0 + lane] = reinterpret_cast<const T*>(turn + r * 17)[lane];
+    const int r1 = f0 + lane < a.n ? rows : 0;
+    T* p = y + tok0 * a.ldy + f0 + lane;
+#pragma unroll 8
+    for (int r = 0; r < r1; ++r, p += a.ldy) *p = reinterpret_cast<const T*>(turn + r * 17)[lane];
   }
+}
+
+// The split whose CTA owns block (lane quarter q, 32-feature column c) of a split two or four ways,
+// and its place among that CTA's blocks.
+__device__ __forceinline__ int block_owner(int q, int c, int splits) {
+  return splits == 2 ? c >> 1 : c;
+}
+__device__ __forceinline__ int block_slot(int q, int c, int splits) {
+  return splits == 2 ? q * 2 + (c & 1) : q;
 }
 
 template <int CG>
@@ -405,10 +415,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   const uint32_t rank = cluster_rank(), pr = rank % CG, lead = rank - pr;
   const int sp = (int)(rank / CG);                                  // which split of the K blocks
   const uint16_t pair_mask = (uint16_t)(3u << lead);
-  const int64_t team = blockIdx.x / (CG * splits), teams = gridDim.x / (CG * splits);
-  const int64_t tiles = (a.n + BN - 1) / BN * a.n_tt;
-  const int kb0 = (int)((int64_t)a.nkb * sp / splits), kb1 = (int)((int64_t)a.nkb * (sp + 1) / splits);
-  const int per = 8 / splits;                                       // units a CTA owns
+  const uint32_t team = blockIdx.x / (CG * splits), teams = gridDim.x / (CG * splits);
+  const int kb0 = (int)(a.nkb * sp / splits), kb1 = (int)(a.nkb * (sp + 1) / splits);   // nkb < 2^24
   if (warp == 0 && elect_one_sync()) {
     // the first weights on their way to L2 while the previous kernel of the stream ends
     prefetch_tmap(&M.w); prefetch_tmap(&M.x); prefetch_tmap(&M.ws); prefetch_tmap(&M.xs);
@@ -422,11 +430,12 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     mbar_init(landed, 1);
     *A.flag = 0;
     fence_mbar_init();
-    if (splits > 1) {                                    // units of this CTA that have tokens
+    if (splits > 1) {                                    // this CTA's blocks that have tokens
       int live = 0;
-      for (int u = sp * per; u < (sp + 1) * per; ++u)
-        live += team % a.n_tt * (128 * CG) + 128 * pr + (u >> 1) * 32 < a.m;
-      if (live) mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * C::kCols * 4));
+      for (int b = 0; b < 16; ++b)
+        live += block_owner(b >> 2, b & 3, splits) == sp &&
+                (int64_t)(team % a.n_tt) * (128 * CG) + 128 * pr + (b >> 2) * 32 < a.m;
+      if (live) mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * 32 * 4));
     }
   }
   if (warp == 2) {
@@ -448,8 +457,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
       uint32_t ph = 0;
       int64_t issued = 0;
       bool ok = true;
-      for (int64_t t = team; t < tiles && ok; t += teams) {
-        const int64_t m0 = t % a.n_tt * (128 * CG) + 128 * pr, n0 = t / a.n_tt * BN;
+      for (uint32_t t = team; t < a.tiles && ok; t += teams) {
+        const int64_t n0 = (int64_t)(t / a.n_tt) * BN, m0 = (int64_t)(t % a.n_tt) * (128 * CG) + 128 * pr;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = fp8_wait<CG == 2>(&empty[s], ph ^ 1, A, 23))) break;
           const uint32_t st = sbase + (uint32_t)s * C::kStage;
@@ -482,13 +491,12 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     if (elect_one_sync()) {
       constexpr uint32_t kIdesc = idesc_mxf8(128 * CG, BN);
       const uint32_t sbase = smem_u32(smem);
-      const int64_t mine = team < tiles ? (tiles - team + teams - 1) / teams : 0;
-      const int64_t total = mine * (kb1 - kb0);
+      const int64_t total = (int64_t)((a.tiles - team + teams - 1) / teams) * (kb1 - kb0);   // team < tiles
       int64_t it = 0;
       int s = 0, buf = 0, slot = C::kSfSlots - 1;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
-      for (int64_t t = team; t < tiles && ok; t += teams) {
+      for (uint32_t t = team; t < a.tiles && ok; t += teams) {
         if (!(ok = fp8_wait<CG == 2>(&acc_empty[buf], aph ^ 1, A, 24))) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
@@ -527,15 +535,15 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     __syncwarp();
   } else if (warp >= 4) {
     const int q4 = warp & 3, half = (warp - 4) >> 2, col0 = half * C::kCols;
-    const int unit = 2 * q4 + half, owner = unit / per;
     uint32_t* turn = reinterpret_cast<uint32_t*>(turns + (warp - 4) * C::kTurn);
     const uint64_t bits = (uint64_t)(uintptr_t)a.y | (uint64_t)a.ldy * sizeof(T);
     const int vec = (bits & 31) == 0 ? 32 : (bits & 15) == 0 ? 16 : 0;
     int buf = 0;
     uint32_t ph = 0;
 #pragma unroll 1
-    for (int64_t t = team; t < tiles; t += teams) {
-      const int64_t tok0 = t % a.n_tt * (128 * CG) + 128 * pr + q4 * 32, n0 = t / a.n_tt * BN + col0;
+    for (uint32_t t = team; t < a.tiles; t += teams) {
+      const int64_t tok0 = (int64_t)(t % a.n_tt) * (128 * CG) + 128 * pr + q4 * 32;
+      const int64_t n0 = (int64_t)(t / a.n_tt) * BN + col0;
       if (!__all_sync(0xffffffffu, fp8_wait<CG == 2>(&acc_full[buf], ph, A, 26))) break;
       tc_fence_after();
       const uint32_t taddr = tmem + buf * BN + col0 + ((uint32_t)(q4 * 32) << 16);
@@ -551,29 +559,18 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
       }
       if constexpr (BN == 128) {
         if (splits > 1 && tok0 < a.m) {
-          if (owner != sp) {
-            // into the owner's room for this unit and split
-            const int from = sp < owner ? sp : sp - 1, to = owner * CG + pr;
-            const uint32_t dst = map_shared(smem_u32(sums) + (unit % per * (splits - 1) + from) * C::kUnit +
-                                                lane * C::kSumRow * 4, to);
+          // into the owner's room for this block and split
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int owner = block_owner(q4, 2 * half + c, splits);
+            if (owner == sp) continue;
+            const int to = owner * CG + pr, from = sp < owner ? sp : sp - 1;
+            const int room = block_slot(q4, 2 * half + c, splits) * (splits - 1) + from;
+            const uint32_t dst = map_shared(smem_u32(sums) + room * C::kBlock + lane * 16, to);
             const uint32_t bar = map_shared(smem_u32(landed), to);
 #pragma unroll
-            for (int c = 0; c < C::kCols; c += 4)
-              st_async_v4(dst + c * 4, v[c / 32][c % 32], v[c / 32][c % 32 + 1], v[c / 32][c % 32 + 2],
-                          v[c / 32][c % 32 + 3], bar);
-            continue;
-          }
-          if (!__all_sync(0xffffffffu, fp8_wait<true>(landed, 0, A, 27))) break;
-#pragma unroll 1
-          for (int r = 0; r < splits - 1; ++r) {
-            const float* p = reinterpret_cast<const float*>(sums + (unit % per * (splits - 1) + r) * C::kUnit) +
-                             lane * C::kSumRow;
-#pragma unroll
-            for (int c = 0; c < C::kCols; c += 4) {
-              const float4 q = *reinterpret_cast<const float4*>(p + c);
-              v[c / 32][c % 32] += q.x; v[c / 32][c % 32 + 1] += q.y;
-              v[c / 32][c % 32 + 2] += q.z; v[c / 32][c % 32 + 3] += q.w;
-            }
+            for (int i = 0; i < 32; i += 4)
+              st_async_v4(dst + i * 128, v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3], bar);
           }
         }
       }
@@ -581,6 +578,21 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
       for (int c = 0; c < C::kCols / 32; ++c) {
         const int64_t f0 = n0 + 32 * c;
         if (f0 >= a.n || tok0 >= a.m) break;             // whole warps
+        if constexpr (BN == 128) {
+          if (splits > 1) {
+            if (block_owner(q4, 2 * half + c, splits) != sp) continue;
+            if (!__all_sync(0xffffffffu, fp8_wait<true>(landed, 0, A, 27))) break;
+            const uint8_t* p = sums + block_slot(q4, 2 * half + c, splits) * (splits - 1) * C::kBlock + lane * 16;
+#pragma unroll 1
+            for (int r = 0; r < splits - 1; ++r, p += C::kBlock) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(p + i * 128);
+                v[c][i] += q.x; v[c][i + 1] += q.y; v[c][i + 2] += q.z; v[c][i + 3] += q.w;
+              }
+            }
+          }
+        }
         if (a.bias) {
           const float b = f0 + lane < a.n ? load_as_float(a.bias, a.bias_dtype, f0 + lane) : 0.f;
 #pragma unroll
@@ -630,17 +642,45 @@ int launch_cluster(void (*kernel)(KArgs...), int dev, bool (&attr_set)[64], int6
   return FBFP_OK;
 }
 
-// K is split over a cluster while that fills idle CTA slots (two per SM) and leaves every CTA at
-// least 4 K blocks.
+// How many clusters of `cluster` CTAs run at a time (clusters do not span the SM groups of the chip,
+// so the largest leave SMs idle: on 148 SMs, one CTA each, 74 of 2, 33 of 4, 15 of 8).
+template <typename... KArgs>
+int clusters_at_a_time(void (*kernel)(KArgs...), int dev, int (&known)[64][9], int cluster, int threads, size_t smem) {
+  if (dev >= 0 && dev < 64 && known[dev][cluster] > 0) return known[dev][cluster];
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOne);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+  cudaGetLastError();
+  if (dev >= 0 && dev < 64) known[dev][cluster] = n;
+  return n;
+}
+
+// K is split over as large a cluster (up to 8) as leaves every CTA at least 4 K blocks and all
+// tiles running at a time, two CTAs per SM.
 template <int BN, typename T>
-int launch_few(Fp8Args a, const Fp8Maps& M, int dev, int nsm, cudaStream_t st) {
+int launch_few(Fp8Args a, const Fp8Maps& M, int dev, cudaStream_t st) {
   using C = Few<BN>;
   static bool attr_set[64] = {false};
-  const int64_t tiles = (a.n + 127) / 128 * a.n_tt;
-  int splits = (int)(2 * nsm / tiles < 8 ? 2 * nsm / tiles : 8);
-  if (splits > a.nkb / 4) splits = a.nkb / 4;
-  if (splits < 1) splits = 1;
-  const int extra = splits > 1 ? C::kSums : 0;
+  static int known[64][9];
+  const int64_t tiles = (a.n + 127) / 128;
+  int splits = 1, extra = 0;
+  for (int c = 8; c > 1; --c)
+    if ((int)a.nkb >= 4 * c &&
+        tiles <= clusters_at_a_time(fp8_few_kernel<BN, T>, dev, known, c, C::kThreads, kSmemTwo)) {
+      splits = c;
+      extra = C::kSums;
+      break;
+    }
   const int fit = (kSmemTwo - C::kFixed - extra) / C::kStage;
   a.stages = fit < kMaxStages ? fit : kMaxStages;
   return launch_cluster(fp8_few_kernel<BN, T>, dev, attr_set, tiles * splits, splits, C::kThreads,
@@ -675,52 +715,57 @@ int encode_scales(CUtensorMap* map, const void* base, int64_t tiles) {
 }
 
 // Which tile and split: the least of an estimate in SM cycles, rounds of tiles x (K blocks x
-// cycles per block + 2500 for a tile's fill and drain) + 6000 for a split's exchange of partial
-// sums. Cycles per K block: 128 x BN x 128 multiply-adds take 2 BN, and the operand rows come
-// in at about 64 bytes a cycle: measured 512 (one CTA, 128 features; bound by the loads), 768 (256
-// features), 400 and 560 (a pair; loads and MMAs nearly even). Measured against the alternatives: 512
-// tokens x 8192 x 3840 16.5 us on 256-wide pair tiles and 18.7 on 128-wide ones, 512 x 3840 x
-// 15360 the other way around (41.0 and 31.5 us: 30 and 60 tiles for 74 pairs), 128 x 3840 x 15360
-// 19.7 us split four ways, 22.0 in two pairs, 29.1 unsplit.
+// cycles per block + 2500 for a tile's fill and drain) + 5000 for a split's exchange of partial
+// sums. Cycles per K block: 128 x BN x 128 multiply-adds take 2 BN, and the operand rows come in
+// at about 60 bytes a cycle: measured 520 (one CTA, 128 features; bound by the loads), 768 (256
+// features), 500 and 580 (a pair). Measured against the alternatives: 512 tokens x 8192 x 3840
+// 16.3 us on 256-wide pair tiles and 18.4 on 128-wide ones, 512 x 3840 x 15360 the other way
+// around (40.2 and 31.0 us: 30 and 60 tiles for 74 pairs), 128 x 3840 x 15360 16.1 us split four
+// ways, 21.7 two ways, 256 x 3840 x 4096 10.6 split and 11.0 not. Clusters of 8 lose: 100 x
+// 2000 x 16000 14.1 us split four ways, 21.2 eight ways.
 struct ManyPlan {
   int cg, bn, splits, teams;
-  int64_t token_tiles;
+  int64_t token_tiles, tiles;
 };
-ManyPlan plan_many(int64_t m, int64_t n, int nkb, int nsm) {
+ManyPlan plan_many(int64_t m, int64_t n, int nkb, int dev) {
+  static int known[64][9];
+  const auto kernel = fp8_many_kernel<1, 128, float>;    // one CTA per SM, as all of them
+  const int threads = Many<1, 128>::kThreads;
   ManyPlan best{};
   double least = 0;
   for (int cg = m <= 128 ? 1 : 2; cg <= 2; ++cg)
     for (int bn = 128; bn <= 256; bn += 128)
-      for (int splits = 1; splits * cg <= 8 && (splits == 1 || (bn == 128 && nkb >= 4 * splits)); splits *= 2) {
+      for (int splits = 1; splits * cg <= 4 && (splits == 1 || (bn == 128 && nkb >= 4 * splits)); splits *= 2) {
         const int64_t tt = (m + 128 * cg - 1) / (128 * cg), tiles = (n + bn - 1) / bn * tt;
-        const int64_t slots = nsm / (cg * splits);       // teams that run at a time
+        const int64_t slots = clusters_at_a_time(kernel, dev, known, cg * splits, threads, kSmemOne);
         if (splits > 1 && tiles > slots) continue;
         const int64_t rounds = (tiles + slots - 1) / slots;
-        const double per_kb = cg == 1 ? (bn == 128 ? 512 : 768) : (bn == 128 ? 400 : 560);
-        const double cost = (double)rounds * ((nkb + splits - 1) / splits * per_kb + 2500) + (splits > 1 ? 6000 : 0);
+        const double per_kb = cg == 1 ? (bn == 128 ? 520 : 768) : (bn == 128 ? 500 : 580);
+        const double cost = (double)rounds * ((nkb + splits - 1) / splits * per_kb + 2500) + (splits > 1 ? 5000 : 0);
         if (best.cg == 0 || cost < least) {
           least = cost;
-          best = ManyPlan{cg, bn, splits, (int)(tiles < slots ? tiles : slots), tt};
+          best = ManyPlan{cg, bn, splits, (int)(tiles < slots ? tiles : slots), tt, tiles};
         }
       }
   return best;
 }
 
 template <typename T>
-int fp8_dispatch(Fp8Args& a, const Fp8Operands& o, int dev, int nsm, cudaStream_t st) {
+int fp8_dispatch(Fp8Args& a, const Fp8Operands& o, int dev, cudaStream_t st) {
   Fp8Maps M;
   int rc;
   if (a.m <= 64) {
     const int bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : 64;
-    a.n_tt = 1;
     if ((rc = encode_rows(&M.x, o.x, a.m, o.k, o.ldx, bn)) != FBFP_OK) return rc;
     if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, 128)) != FBFP_OK) return rc;
-    return bn == 16   ? launch_few<16, T>(a, M, dev, nsm, st)
-           : bn == 32 ? launch_few<32, T>(a, M, dev, nsm, st)
-                      : launch_few<64, T>(a, M, dev, nsm, st);
+    return bn == 16   ? launch_few<16, T>(a, M, dev, st)
+           : bn == 32 ? launch_few<32, T>(a, M, dev, st)
+                      : launch_few<64, T>(a, M, dev, st);
   }
-  const ManyPlan p = plan_many(a.m, a.n, a.nkb, nsm);
-  a.n_tt = p.token_tiles;
+  const ManyPlan p = plan_many(a.m, a.n, (int)a.nkb, dev);
+  FBFP_CHECK_ARG(p.tiles < ((int64_t)1 << 31), "too many output tiles");
+  a.n_tt = (uint32_t)p.token_tiles;
+  a.tiles = (uint32_t)p.tiles;
   if ((rc = encode_rows(&M.x, o.x, a.m, o.k, o.ldx, 128)) != FBFP_OK) return rc;
   if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, p.bn / p.cg)) != FBFP_OK) return rc;
   if ((rc = encode_scales(&M.xs, a.x_scales, (a.m + 127) / 128 * a.kgroups)) != FBFP_OK) return rc;
@@ -752,7 +797,7 @@ extern "C" int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx,
   FBFP_CHECK_ARG(dtype_ok(y_dtype) && (!bias || dtype_ok(bias_dtype)), "bad y or bias dtype");
   Fp8Args a;
   a.m = m; a.n = n;
-  a.nkb = (int)((k + 127) / 128);
+  a.nkb = (uint32_t)((k + 127) / 128);
   a.kgroups = (int)((k + 511) / 512);
   FBFP_CHECK_ARG((m + 127) / 128 * a.kgroups < ((int64_t)1 << 31) && (n + 127) / 128 * a.kgroups < ((int64_t)1 << 31),
                  "too many scale tiles");
@@ -764,9 +809,8 @@ extern "C" int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx,
   const Fp8Operands o{x, w, k, ldx, ldw};
   int dev = 0;
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
-  const int nsm = sm_count(dev);
   const cudaStream_t st = as_stream(stream);
-  return y_dtype == FBFP_BF16  ? fp8_dispatch<__nv_bfloat16>(a, o, dev, nsm, st)
-         : y_dtype == FBFP_F16 ? fp8_dispatch<__half>(a, o, dev, nsm, st)
-                               : fp8_dispatch<float>(a, o, dev, nsm, st);
+  return y_dtype == FBFP_BF16  ? fp8_dispatch<__nv_bfloat16>(a, o, dev, st)
+         : y_dtype == FBFP_F16 ? fp8_dispatch<__half>(a, o, dev, st)
+                               : fp8_dispatch<float>(a, o, dev, st);
 }
