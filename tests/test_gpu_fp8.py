@@ -131,7 +131,7 @@ def check_quantised(r, y, d):
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("mode", ["plain", "add", "post"])
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 3840), (2, 16), (3, 77), (5, 513), (130, 256), (17, 4090), (4, 8192),
-                                 (3, 16384), (2, 16400), (2, 32768)])
+                                 (3, 16384), (2, 16400), (2, 32768), (3, 8199), (2, 20001), (1500, 48), (700, 1040)])
 def test_rmsnorm(m, k, mode, dtype):
     """Relative error of the fp32 part: a mean of k squares (each thread sums 16 or 32, then a tree
     and at most 32 warp sums: at most 96 roundings, halved by the root), rsqrt (2 ulp), at most
@@ -198,6 +198,21 @@ def test_rmsnorm_strided_rows_and_residual():
         assert torch.equal(a.values.float(), b.values.float()) and torch.equal(ref.codes_of(a), ref.codes_of(b))
         assert torch.equal(res, rc)
         assert torch.equal(r0[:, :4], resw[:, :4]) and torch.equal(r0[:, 904:], resw[:, 904:])
+
+
+def test_rmsnorm_of_the_residual_itself():
+    """x may be the residual: h = 2 x, in place; and one row given for all rows."""
+    from flashbfp_b200 import fp8
+    g = gen(4)
+    w = torch.zeros(1024, device=DEV)
+    x = torch.randn(600, 1024, device=DEV, generator=g)
+    a, b = x.clone(), x.clone()
+    r = fp8.rmsnorm_fp8(a, w, 1e-6, residual=a)
+    q = fp8.rmsnorm_fp8(x, w, 1e-6, residual=b)
+    assert torch.equal(a, 2 * x) and torch.equal(a, b)
+    assert torch.equal(r.values.float(), q.values.float()) and torch.equal(ref.codes_of(r), ref.codes_of(q))
+    one = fp8.rmsnorm_fp8(x[:1].expand(500, -1), w, 1e-6)
+    assert torch.equal(one.dequantize(), fp8.rmsnorm_fp8(x[:1], w, 1e-6).dequantize().expand(500, -1))
 
 
 # ---------------------------------------------------------------------------- GeGLU
@@ -299,7 +314,7 @@ def test_linear_of_real_values(m, n, k):
 
 def test_linear_nan_rows_stay_in_their_rows():
     from flashbfp_b200 import fp8
-    for m in (5, 300):
+    for m in (5, 100, 300):
         x, xd = integer_rows(m, 640, 1)
         w, wd = integer_rows(200, 640, 2)
         codes = ref.codes_of(x).clone()
@@ -329,6 +344,80 @@ def test_linear_strides_and_empty():
     assert torch.equal(fp8.fp8_linear(fp8.Fp8Rows(big[:, 32:732], x.scales), w, out_dtype=torch.float32).double(), want)
     none = fp8.Fp8Rows(x.values[:0], fp8.empty_rows(0, 700, DEV).scales)
     assert fp8.fp8_linear(none, w).shape == (0, 150)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values in and out: the last rows, and the rows on either side of 2^31."""
+    from flashbfp_b200 import fp8
+    m, k = 33000, 65540                               # k: not a multiple of 16
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+    rows = [0, 2 ** 31 // k - 1, 2 ** 31 // k, 2 ** 31 // k + 1, m - 1]
+    x[rows] = torch.randn(len(rows), k, device=DEV, generator=gen(1)).bfloat16()
+    r = fp8.quantize_fp8(x)
+    q, codes = ref.quantise(x[rows])
+    assert torch.equal(r.values[rows].double(), q)
+    t = r.scales.view(torch.uint8)
+    for i, row in enumerate(rows):
+        got = t[row // 128, :, row % 32, row % 128 // 32].reshape(-1)[:codes.shape[1]].int()
+        assert torch.equal(got, codes[i])
+    assert not r.values[1:100].view(torch.uint8).any()
+    del x, r, t
+    n = 1_000_003
+    xi, xd = integer_rows(2200, 128, 7)
+    wi, wd = integer_rows(n, 128, 8)
+    y = fp8.fp8_linear(xi, wi)
+    for sl in (slice(0, 3), slice(2140, 2150), slice(2197, 2200)):
+        assert torch.equal(y[sl], (xd[sl] @ wd.t()).to(torch.bfloat16))
+    fp8.check_device_errors(DEV)
+
+
+def test_first_calls_inside_a_capture():
+    """Kernels whose first launch is captured (another output type and tile than any warm call's)."""
+    from flashbfp_b200 import fp8
+    x, xd = integer_rows(70, 4100, 1)
+    w, wd = integer_rows(300, 4100, 2)
+    fp8.fp8_linear(fp8.Fp8Rows(x.values[:1], x.scales), w)          # the error word exists
+    y, z = torch.zeros(70, 300, device=DEV, dtype=torch.float16), torch.zeros(20, 300, device=DEV, dtype=torch.float16)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        fp8.fp8_linear(x, w, out=y)
+        fp8.fp8_linear(fp8.Fp8Rows(x.values[:20], x.scales), w, out=z)
+    graph.replay()
+    want = (xd @ wd.t()).to(torch.float16)
+    assert torch.equal(y, want) and torch.equal(z, want[:20])
+
+
+def test_two_graphs_and_a_third_stream():
+    """Two captured chains replayed at the same time as eager calls: nothing is shared between them."""
+    from flashbfp_b200 import fp8
+    g = gen(6)
+    w = fp8.quantize_fp8(0.02 * torch.randn(640, 3000, generator=g, device=DEV))
+    lnw = torch.zeros(3000, device=DEV, dtype=torch.bfloat16)
+    xs = [torch.randn(m, 3000, generator=g, device=DEV).bfloat16() for m in (1, 90, 300)]
+
+    def chain(x, out):
+        return fp8.fp8_linear(fp8.rmsnorm_fp8(x, lnw, 1e-6), w, out=out)
+
+    want = [chain(x, None) for x in xs]
+    outs = [torch.zeros_like(y) for y in want]
+    streams = [torch.cuda.Stream(DEV) for _ in xs]
+    graphs = []
+    torch.cuda.synchronize()
+    for x, o in zip(xs[:2], outs):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            chain(x, o)
+        graphs.append(gr)
+    for _ in range(20):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        with torch.cuda.stream(streams[2]):
+            chain(xs[2], outs[2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    fp8.check_device_errors(DEV)
 
 
 def test_stream_and_graph():
