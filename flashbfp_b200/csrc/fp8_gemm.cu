@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 // every block of 32 tokens x 32 features has an owner among the cluster's CTAs: the others store
 // their sums into its shared memory (a warp's store is 512 bytes in a row: 16 bytes a lane), and it
 // adds them to its own in rank order. Owners are spread so that four warps of every CTA have a block
-// (split four ways) or two.
+// (split four ways) or two (eight ways: two warps with one).
 template <int CG, int BN>
 struct Many {
   static constexpr int kRowsB = BN / CG;
@@ -294,7 +294,7 @@ struct Many {
   static constexpr int kTurn = 32 * 17 * 4;                      // a warp's 32 x 16 words, rows 17 apart
   static constexpr int kTurns = kEpiWarps * kTurn;
   static constexpr int kBlock = 32 * 32 * 4;                     // [feature / 4][token][4]
-  static constexpr int kSums = 12 * kBlock;                      // 16 / S blocks from S - 1 CTAs, S 2 or 4
+  static constexpr int kSums = 14 * kBlock;                      // 16 / S blocks from S - 1 CTAs, S 2, 4 or 8
   static constexpr int kBars = (2 * kMaxStages + 2 + 2 + 2) * 8 + 16;
   static constexpr int kFixed = kBars + 1024;                    // stages start on 1 KB
   static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kBlock % 16 == 0, "alignment");
@@ -338,8 +338,12 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
       const int64_t f = f0 + 16 * h + (lane & 15);
       const int r1 = f < a.n ? rows : 0;
       T* p = y + (tok0 + (lane >> 4)) * a.ldy + f;
-#pragma unroll 4
-      for (int r = lane >> 4; r < r1; r += 2, p += 2 * a.ldy) *p = __uint_as_float(turn[r * 17 + (lane & 15)]);
+      T q[16];                                           // all loads, then all stores: twice as fast as in turn
+#pragma unroll
+      for (int r = 0; r < 16; ++r) q[r] = __uint_as_float(turn[(2 * r + (lane >> 4)) * 17 + (lane & 15)]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r, p += 2 * a.ldy)
+        if (2 * r + (lane >> 4) < r1) *p = q[r];
     }
   } else {
     uint32_t w[16];
@@ -367,18 +371,22 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
     __syncwarp();
     const int r1 = f0 + lane < a.n ? rows : 0;
     T* p = y + tok0 * a.ldy + f0 + lane;
-#pragma unroll 8
-    for (int r = 0; r < r1; ++r, p += a.ldy) *p = reinterpret_cast<const T*>(turn + r * 17)[lane];
+    T q[32];
+#pragma unroll
+    for (int r = 0; r < 32; ++r) q[r] = reinterpret_cast<const T*>(turn + r * 17)[lane];
+#pragma unroll
+    for (int r = 0; r < 32; ++r, p += a.ldy)
+      if (r < r1) *p = q[r];
   }
 }
 
-// The split whose CTA owns block (lane quarter q, 32-feature column c) of a split two or four ways,
+// The split whose CTA owns block (lane quarter q, 32-feature column c) of a split two, four or eight ways,
 // and its place among that CTA's blocks.
 __device__ __forceinline__ int block_owner(int q, int c, int splits) {
-  return splits == 2 ? c >> 1 : c;
+  return splits == 2 ? c >> 1 : splits == 4 ? c : 2 * c + (q >> 1);
 }
 __device__ __forceinline__ int block_slot(int q, int c, int splits) {
-  return splits == 2 ? q * 2 + (c & 1) : q;
+  return splits == 2 ? q * 2 + (c & 1) : splits == 4 ? q : q & 1;
 }
 
 template <int CG>
@@ -444,8 +452,13 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   }
   __syncwarp();
   tc_fence_before();
-  cluster_arrive();
-  cluster_wait();                                        // every CTA of the cluster runs, its barriers are ready
+  if constexpr (CG == 2) {                               // every CTA of the cluster runs, its barriers are ready
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+    if (splits > 1) cluster_arrive();                    // waited for where the others are needed
+  }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_prologue();
@@ -535,6 +548,7 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     __syncwarp();
   } else if (warp >= 4) {
     const int q4 = warp & 3, half = (warp - 4) >> 2, col0 = half * C::kCols;
+    if (CG == 1 && splits > 1) cluster_wait();           // the owners' barriers are ready
     uint32_t* turn = reinterpret_cast<uint32_t*>(turns + (warp - 4) * C::kTurn);
     const uint64_t bits = (uint64_t)(uintptr_t)a.y | (uint64_t)a.ldy * sizeof(T);
     const int vec = (bits & 31) == 0 ? 32 : (bits & 15) == 0 ? 16 : 0;
@@ -604,9 +618,14 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     }
   }
   __syncwarp();
+  if (CG == 1 && splits > 1 && warp < 4) cluster_wait();
   tc_fence_before();
-  cluster_arrive_relaxed();
-  cluster_wait();                                        // no CTA leaves while another may still reach it
+  if (CG == 2 || splits > 1) {                           // no CTA leaves while another may still reach it
+    cluster_arrive_relaxed();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   if (warp == 2) {
     tc_fence_after();
     if constexpr (CG == 1) tmem_dealloc(tmem, C::kTmemCols);
@@ -715,7 +734,7 @@ int encode_scales(CUtensorMap* map, const void* base, int64_t tiles) {
 }
 
 // Which tile and split: the least of an estimate in SM cycles, rounds of tiles x (K blocks x
-// cycles per block + 2500 for a tile's fill and drain) + 5000 for a split's exchange of partial
+// cycles per block + 2000 for a tile's fill and drain, 3500 for a pair's) + 5000 for a split's exchange of partial
 // sums. Cycles per K block: 128 x BN x 128 multiply-adds take 2 BN, and the operand rows come in
 // at about 60 bytes a cycle: measured 520 (one CTA, 128 features; bound by the loads), 768 (256
 // features), 500 and 580 (a pair). Measured against the alternatives: 512 tokens x 8192 x 3840
@@ -733,15 +752,16 @@ ManyPlan plan_many(int64_t m, int64_t n, int nkb, int dev) {
   const int threads = Many<1, 128>::kThreads;
   ManyPlan best{};
   double least = 0;
-  for (int cg = m <= 128 ? 1 : 2; cg <= 2; ++cg)
+  for (int cg = 1; cg <= 2; ++cg)
     for (int bn = 128; bn <= 256; bn += 128)
-      for (int splits = 1; splits * cg <= 4 && (splits == 1 || (bn == 128 && nkb >= 4 * splits)); splits *= 2) {
+      for (int splits = 1; splits * cg <= 8 && (splits == 1 || (bn == 128 && nkb >= 4 * splits)); splits *= 2) {
         const int64_t tt = (m + 128 * cg - 1) / (128 * cg), tiles = (n + bn - 1) / bn * tt;
         const int64_t slots = clusters_at_a_time(kernel, dev, known, cg * splits, threads, kSmemOne);
         if (splits > 1 && tiles > slots) continue;
         const int64_t rounds = (tiles + slots - 1) / slots;
         const double per_kb = cg == 1 ? (bn == 128 ? 520 : 768) : (bn == 128 ? 500 : 580);
-        const double cost = (double)rounds * ((nkb + splits - 1) / splits * per_kb + 2500) + (splits > 1 ? 5000 : 0);
+        const double cost = (double)rounds * ((nkb + splits - 1) / splits * per_kb + (cg == 1 ? 2000 : 3500)) +
+                            (splits > 1 ? 5000 : 0);
         if (best.cg == 0 || cost < least) {
           least = cost;
           best = ManyPlan{cg, bn, splits, (int)(tiles < slots ? tiles : slots), tt, tiles};

@@ -63,56 +63,108 @@ __device__ __forceinline__ void st32(void* p, const uint32_t* w) {
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-// A lane's 16 values of a segment as they lie in memory: loaded early, unpacked where they are
-// needed. VEC: values 16 lane .. 16 lane + 15, in whole 32-byte sectors, for rows that start on 32
-// bytes and hold a multiple of 16 values. Not VEC: values lane + 32 i, so that rows of any
-// alignment and length are read and written along the lanes. (One kernel for both would run a
-// third slower: its branches cost instruction fetches that short rows cannot hide.)
-template <typename T>
-struct Raw16 {
-  uint32_t w[kLane * sizeof(T) / 4];
+// The bytes of a tensor, from its first value to its last.
+struct Span {
+  const char *lo, *hi;
 };
 
-template <bool VEC>
-__device__ __forceinline__ int place(int i) {
-  const int lane = threadIdx.x & 31;
-  return VEC ? lane * kLane + i : lane + 32 * i;
+// Two kinds of rows. VEC: rows that start on 32 bytes and hold a multiple of 16 values, moved in whole
+// 32-byte sectors. Not VEC: any other, moved in the aligned 16-byte vectors that hold them and
+// shifted into place (by the same number of bytes in all lanes of a warp). They are separate
+// kernels: branches between the two would cost instruction fetches that short rows cannot hide.
+
+// Words out[0..N) = the bytes of in[0..N + 4) from byte s (0..14, even) on.
+template <int N>
+__device__ __forceinline__ void shift_words(uint32_t (&in)[N + 4], int s, uint32_t (&out)[N]) {
+  if (s & 8) {
+#pragma unroll
+    for (int i = 0; i < N + 2; ++i) in[i] = in[i + 2];
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) in[i] = in[i + 1];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(in[i], in[i + 1], 8 * (s & 2));
 }
+
+// A lane's 16 consecutive values of a segment as they lie in memory: loaded early, unpacked where
+// they are needed. Not VEC: the vectors that hold them, `shift` the bytes before the first value,
+// `mine` how many of the values exist.
+template <bool VEC, typename T>
+struct Raw16 {
+  static constexpr int kWords = kLane * sizeof(T) / 4;
+  uint32_t w[kWords + (VEC ? 0 : 4)];
+  int shift, mine;
+};
 
 // p: the segment's first value; n of the segment's values exist (the others read as zero).
 template <bool VEC, typename T>
-__device__ __forceinline__ Raw16<T> load16(const T* p, int n) {
-  Raw16<T> r;
-  constexpr int words = kLane * sizeof(T) / 4;
+__device__ __forceinline__ Raw16<VEC, T> load16(const T* p, int n, Span t) {
+  Raw16<VEC, T> r;
+  constexpr int words = Raw16<VEC, T>::kWords;
+  const int lane = threadIdx.x & 31;
+  const char* q = reinterpret_cast<const char*>(p + lane * kLane);
+  r.mine = n - lane * kLane;
+  r.shift = 0;
 #pragma unroll
-  for (int i = 0; i < words; ++i) r.w[i] = 0;
+  for (int i = 0; i < words + (VEC ? 0 : 4); ++i) r.w[i] = 0;
   if constexpr (VEC) {
-    if (place<VEC>(0) < n) {
+    if (r.mine > 0) {
 #pragma unroll
-      for (int h = 0; h < words; h += 8) ld32(reinterpret_cast<const uint32_t*>(p + place<VEC>(0)) + h, r.w + h);
+      for (int h = 0; h < words; h += 8) ld32(q + 4 * h, r.w + h);
     }
   } else {
+    const int s = (int)((uintptr_t)q & 15);
+    const int bytes = s + (r.mine < kLane ? r.mine : kLane) * (int)sizeof(T);   // up to the last existing value
+    const char* base = q - s;
+    if (r.mine > 0 && base >= t.lo && base + ((bytes + 15) & ~15) <= t.hi) {
+      r.shift = s;
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      if (place<VEC>(i) < n) {
-        if constexpr (sizeof(T) == 4)
-          r.w[i] = __float_as_uint(p[place<VEC>(i)]);
-        else
-          r.w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[place<VEC>(i)] << (16 * (i & 1));
+      for (int h = 0; h < words + 4; h += 4)
+        if (4 * h < bytes) {
+          const uint4 u = *reinterpret_cast<const uint4*>(base + 4 * h);
+          r.w[h] = u.x; r.w[h + 1] = u.y; r.w[h + 2] = u.z; r.w[h + 3] = u.w;
+        }
+    } else {                                             // a vector would reach past the tensor: value by value
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) {
+        if (i < r.mine) {
+          if constexpr (sizeof(T) == 4) r.w[i] = reinterpret_cast<const uint32_t*>(q)[i];
+          else r.w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[i] << (16 * (i & 1));
+        }
       }
     }
   }
   return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const Raw16<T>& r, float2 (&v)[kPairs]) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void unpack16(const Raw16<VEC, T>& r, float2 (&v)[kPairs]) {
+  constexpr int words = Raw16<VEC, T>::kWords;
+  uint32_t w[words];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < words; ++i) w[i] = r.w[i];
+  } else {
+    uint32_t in[words + 4];
+#pragma unroll
+    for (int i = 0; i < words + 4; ++i) in[i] = r.w[i];
+    shift_words<words>(in, r.shift, w);
+    if (r.mine < kLane) {                                // behind the row's end
+#pragma unroll
+      for (int i = 0; i < words; ++i) {
+        const int left = r.mine * (int)sizeof(T) - 4 * i;
+        w[i] &= left >= 4 ? 0xFFFFFFFFu : left > 0 ? 0xFFFFu : 0u;
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
     if constexpr (sizeof(T) == 4)
-      v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+      v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     else
-      v[i] = unpack2(r.w[i], (const T*)nullptr);
+      v[i] = unpack2(w[i], (const T*)nullptr);
   }
 }
 
@@ -129,18 +181,36 @@ __device__ __forceinline__ void store16(T* p, int n, const float2 (&v)[kPairs]) 
       w[i] = pack2(v[i], (const T*)nullptr);
     }
   }
+  const int lane = threadIdx.x & 31;
+  T* q = p + lane * kLane;
   if constexpr (VEC) {
-    if (place<VEC>(0) < n) {
+    if (lane * kLane < n) {
 #pragma unroll
-      for (int h = 0; h < words; h += 8) st32(reinterpret_cast<uint32_t*>(p + place<VEC>(0)) + h, w + h);
+      for (int h = 0; h < words; h += 8) st32(reinterpret_cast<uint32_t*>(q) + h, w + h);
     }
   } else {
+    // aligned vectors of this lane's values and the next lane's first, as far as the segment's
+    // values fill them; what is left at either end value by value
+    constexpr int G = 16 / sizeof(T);                    // values of a vector
+    const int s = (int)((uintptr_t)q & 15), lead = s ? (16 - s) / (int)sizeof(T) : 0;
+    const int end = n >= lead ? lead + (n - lead) / G * G : 0, v0 = lane * kLane;
+    uint32_t in[words + 4], out[words];
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      if (place<VEC>(i) < n) {
-        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[place<VEC>(i)] = w[i];
-        else reinterpret_cast<uint16_t*>(p)[place<VEC>(i)] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-      }
+    for (int i = 0; i < words; ++i) in[i] = w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[words + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+    shift_words<words>(in, (16 - s) & 15, out);
+#pragma unroll
+    for (int h = 0; h < kLane / G; ++h)
+      if (v0 + lead + (h + 1) * G <= end)
+        reinterpret_cast<uint4*>(q + lead)[h] = make_uint4(out[4 * h], out[4 * h + 1], out[4 * h + 2], out[4 * h + 3]);
+    if (v0 < lead || v0 + kLane > end) {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i)
+        if ((v0 + i < lead || v0 + i >= end) && v0 + i < n) {
+          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(q)[i] = w[i];
+          else reinterpret_cast<uint16_t*>(q)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        }
     }
   }
 }
@@ -168,45 +238,34 @@ __device__ __forceinline__ float scale_inverse(int c) {
 template <bool VEC>
 __device__ __forceinline__ void quantise_segment(const float2 (&v)[kPairs], int64_t row, int seg, const RowsOut& o) {
   const int lane = threadIdx.x & 31;
-  uint8_t* q = o.q + row * o.ldq + (int64_t)seg * kSeg;
-  const int n = (int)(o.k - (int64_t)seg * kSeg < kSeg ? o.k - (int64_t)seg * kSeg : kSeg);
-  uint32_t word;
-  if constexpr (VEC) {                                   // a block lies in 8 lanes
-    float top = 0.f;
+  uint8_t* q = o.q + row * o.ldq + (int64_t)seg * kSeg + lane * kLane;
+  const int64_t left = o.k - (int64_t)seg * kSeg - lane * kLane;
+  const int mine = left < kLane ? (int)left : kLane;     // of this lane's values exist
+  float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) top = amax3(top, v[i].x, v[i].y);
-    uint32_t amax = __float_as_uint(top);
+  for (int i = 0; i < kPairs; ++i) top = amax3(top, v[i].x, v[i].y);
+  uint32_t amax = __float_as_uint(top);
 #pragma unroll
-    for (int s = 4; s > 0; s >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, s));
-    const int c = scale_byte(amax);
-    const float2 inv = make_float2(scale_inverse(c), scale_inverse(c));
-    uint32_t w[4];
+  for (int s = 4; s > 0; s >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+  const int c = scale_byte(amax);
+  const float2 inv = make_float2(scale_inverse(c), scale_inverse(c));
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i], inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i + 1], inv), __NV_SATFINITE, __NV_E4M3);
-      w[i] = lo | (hi << 16);
-    }
-    if (place<VEC>(0) < n) *reinterpret_cast<uint4*>(q + place<VEC>(0)) = make_uint4(w[0], w[1], w[2], w[3]);
-    word = (uint32_t)c;
-#pragma unroll
-    for (int b = 1; b < 4; ++b) word |= (uint32_t)__shfl_sync(0xffffffffu, c, 8 * b) << (8 * b);
-  } else {                                               // a block is four values of every lane
-    word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const float top = amax3(amax3(0.f, v[2 * b].x, v[2 * b].y), v[2 * b + 1].x, v[2 * b + 1].y);
-      const int c = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-      const float2 inv = make_float2(scale_inverse(c), scale_inverse(c));
-      word |= (uint32_t)c << (8 * b);
-#pragma unroll
-      for (int i = 2 * b; i < 2 * b + 2; ++i) {
-        const uint32_t e = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[i], inv), __NV_SATFINITE, __NV_E4M3);
-        if (place<VEC>(2 * i) < n) q[place<VEC>(2 * i)] = (uint8_t)e;
-        if (place<VEC>(2 * i + 1) < n) q[place<VEC>(2 * i + 1)] = (uint8_t)(e >> 8);
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i], inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * i + 1], inv), __NV_SATFINITE, __NV_E4M3);
+    w[i] = lo | (hi << 16);
   }
+  if (VEC ? mine > 0 : mine >= kLane) {
+    *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (!VEC) {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i)
+      if (i < mine) q[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+  }
+  uint32_t word = (uint32_t)c;
+#pragma unroll
+  for (int b = 1; b < 4; ++b) word |= (uint32_t)__shfl_sync(0xffffffffu, c, 8 * b) << (8 * b);
   // lane 0's word is right; past the row's last block the values are zero and so are the bytes
   if (lane == 0) o.sc[scale_word(row, seg, o.segs)] = word;
   // the last row also zeroes the tile's rows behind it, so that every scale byte is defined
@@ -240,7 +299,7 @@ __device__ __forceinline__ float2 gelu_tanh(float2 g) {
 
 // One warp per (row, segment). GEGLU: the row holds gate | up, `k` values each.
 template <typename T, bool GEGLU, bool VEC>
-__global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int64_t ldx, const RowsOut o) {
+__global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int64_t ldx, const Span t, const RowsOut o) {
   pdl_prologue();
   const int64_t unit = (int64_t)blockIdx.x * (kFlatThreads / 32) + (threadIdx.x >> 5);
   const int64_t row = unit / o.segs;
@@ -249,14 +308,14 @@ __global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int6
   const T* p = x + row * ldx + (int64_t)seg * kSeg;
   float2 v[kPairs];
   if constexpr (GEGLU) {
-    const Raw16<T> gr = load16<VEC>(p, n), ur = load16<VEC>(p + o.k, n);
+    const Raw16<VEC, T> gr = load16<VEC>(p, n, t), ur = load16<VEC>(p + o.k, n, t);
     float2 u[kPairs];
     unpack16(gr, v);
     unpack16(ur, u);
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(gelu_tanh(v[i]), u[i]);
   } else {
-    unpack16(load16<VEC>(p, n), v);
+    unpack16(load16<VEC>(p, n, t), v);
   }
   quantise_segment<VEC>(v, row, seg, o);
 }
@@ -271,6 +330,7 @@ __global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int6
 struct NormArgs {
   int64_t ldx, ldr;
   float eps, inv_k;
+  Span xs, rs, ws, ps;                                   // of x, resid, w, w_post
   int team;                                              // warps per row
 };
 
@@ -297,7 +357,7 @@ template <typename T, int NV, int MODE, int THREADS, int MINB, bool VEC>
 __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, const T* w, const T* w_post, T* resid,
                                                                     const NormArgs a, const RowsOut o) {
   pdl_prologue();
-  constexpr bool kEarly = THREADS < 1024 && (sizeof(T) == 2 || NV == 1);
+  constexpr bool kEarly = NV == 1 ? THREADS < 1024 || sizeof(T) == 2 : THREADS < 1024 && sizeof(T) == 2;
   constexpr int kWarps = THREADS / 32, kTeams = THREADS <= 256 ? kWarps : 1;   // at most, a CTA
   __shared__ __align__(16) float reds[2][kTeams * kWarps];
   for (int i = threadIdx.x; i < 2 * kTeams * kWarps; i += blockDim.x) (&reds[0][0])[i] = 0.f;
@@ -308,13 +368,13 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
   const int64_t step = (int64_t)gridDim.x * teams;
   int64_t row = (int64_t)blockIdx.x * teams + warp / a.team;
   const T *xp = x + row * a.ldx, *rp = resid + row * a.ldr;
-  Raw16<T> xr[NV], rr[NV];
+  Raw16<VEC, T> xr[NV], rr[NV];
   if constexpr (kEarly) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int seg = seg0 + i * a.team, n = row < o.m ? left_of(o.k, seg) : 0;
-      xr[i] = load16<VEC>(xp + seg * kSeg, n);
-      if constexpr (MODE > 0) rr[i] = load16<VEC>(rp + seg * kSeg, n);
+      xr[i] = load16<VEC>(xp + seg * kSeg, n, a.xs);
+      if constexpr (MODE > 0) rr[i] = load16<VEC>(rp + seg * kSeg, n, a.rs);
     }
   }
   int turn = 0;
@@ -328,14 +388,14 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int seg = seg0 + i * a.team, all = left_of(o.k, seg), n = live ? all : 0;
-      if constexpr (!kEarly) xr[i] = load16<VEC>(x + row * a.ldx + seg * kSeg, n);
+      if constexpr (!kEarly) xr[i] = load16<VEC>(x + row * a.ldx + seg * kSeg, n, a.xs);
       unpack16(xr[i], v[i]);
-      if constexpr (kEarly) xr[i] = load16<VEC>(xp + seg * kSeg, more ? all : 0);
+      if constexpr (kEarly) xr[i] = load16<VEC>(xp + seg * kSeg, more ? all : 0, a.xs);
       if constexpr (MODE == 1) {
-        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n);
+        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n, a.rs);
         float2 r[kPairs];
         unpack16(rr[i], r);
-        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0);
+        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0, a.rs);
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) v[i][e] = __fadd2_rn(v[i][e], r[e]);
         store16<VEC>(now + seg * kSeg, n, v[i]);
@@ -350,16 +410,16 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int seg = seg0 + i * a.team, all = left_of(o.k, seg), n = live ? all : 0;
-        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n);
+        if constexpr (!kEarly) rr[i] = load16<VEC>((const T*)now + seg * kSeg, n, a.rs);
         float2 wv[kPairs];
-        unpack16(load16<VEC>(w_post + seg * kSeg, n), wv);
+        unpack16(load16<VEC>(w_post + seg * kSeg, n, a.ps), wv);
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {               // y = v rs, y + y w
           v[i][e] = __fmul2_rn(v[i][e], both(rs));
           v[i][e] = __ffma2_rn(v[i][e], wv[e], v[i][e]);
         }
         unpack16(rr[i], wv);
-        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0);
+        if constexpr (kEarly) rr[i] = load16<VEC>((const T*)now + step * a.ldr + seg * kSeg, more ? all : 0, a.rs);
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {
           v[i][e] = __fadd2_rn(v[i][e], wv[e]);
@@ -376,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
         const int seg = seg0 + i * a.team;
         if (seg >= o.segs) break;                        // whole warps
         float2 wv[kPairs];
-        unpack16(load16<VEC>(w + seg * kSeg, left_of(o.k, seg)), wv);
+        unpack16(load16<VEC>(w + seg * kSeg, left_of(o.k, seg), a.ws), wv);
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {
           v[i][e] = __fmul2_rn(v[i][e], both(rs));
@@ -412,13 +472,19 @@ int rows_out(int64_t m, int64_t k, void* values, int64_t ldv, void* scales, Rows
   return FBFP_OK;
 }
 
+template <typename T>
+Span span(const void* p, int64_t rows, int64_t ld, int64_t len) {
+  const char* c = reinterpret_cast<const char*>(p);
+  return Span{c, c ? c + ((rows - 1) * ld + len) * (int64_t)sizeof(T) : c};
+}
+
 template <typename T, bool GEGLU>
 cudaError_t launch_flat(const void* x, int64_t ldx, const RowsOut& o, cudaStream_t st) {
   const bool vec = whole_sectors(bits_of(x) | (uint64_t)ldx * sizeof(T), o.k);
   const int64_t units = o.m * o.segs, per = kFlatThreads / 32;
   return launch_pdl(vec ? fp8_rows_kernel<T, GEGLU, true> : fp8_rows_kernel<T, GEGLU, false>,
                     dim3((unsigned)((units + per - 1) / per)), dim3(kFlatThreads), 0, st,
-                    reinterpret_cast<const T*>(x), ldx, o);
+                    reinterpret_cast<const T*>(x), ldx, span<T>(x, o.m, ldx, GEGLU ? 2 * o.k : o.k), o);
 }
 
 struct NormPtrs {
@@ -429,6 +495,10 @@ struct NormPtrs {
 template <typename T, int NV, int MODE, int THREADS, int MINB, bool VEC>
 cudaError_t launch_norm(const NormPtrs& p, NormArgs a, const RowsOut& o, int nsm, cudaStream_t st) {
   a.team = (o.segs + NV - 1) / NV;
+  a.xs = span<T>(p.x, o.m, a.ldx, o.k);
+  a.rs = span<T>(p.resid, o.m, a.ldr, o.k);
+  a.ws = span<T>(p.w, 1, 0, o.k);
+  a.ps = span<T>(p.w_post, 1, 0, o.k);
   const int teams = THREADS <= 256 ? THREADS / 32 / a.team : 1;   // rows of a CTA at a time
   const int64_t want = (o.m + teams - 1) / teams;
   const int64_t room = (int64_t)nsm * MINB;
@@ -446,8 +516,10 @@ cudaError_t norm_by_size(const NormPtrs& p, NormArgs a, const RowsOut& o, int ns
   // CTAs per SM by the registers of a row's 16 values a thread (twice as many words in fp32)
   constexpr int kThree = sizeof(T) == 2 ? 3 : 2, kTwo = sizeof(T) == 2 ? 2 : 1;
   if (!vec)
-    return o.segs <= 8 ? launch_norm<T, 1, MODE, 256, kThree, false>(p, a, o, nsm, st)
-                       : launch_norm<T, 2, MODE, 1024, 1, false>(p, a, o, nsm, st);
+    return o.segs <= 8    ? launch_norm<T, 1, MODE, 256, 2, false>(p, a, o, nsm, st)
+           : o.segs <= 16 ? launch_norm<T, 1, MODE, 512, 1, false>(p, a, o, nsm, st)
+           : o.segs <= 32 ? launch_norm<T, 2, MODE, 512, 1, false>(p, a, o, nsm, st)
+                          : launch_norm<T, 2, MODE, 1024, 1, false>(p, a, o, nsm, st);
   return o.segs <= 8    ? launch_norm<T, 1, MODE, 256, kThree, true>(p, a, o, nsm, st)
          : o.segs <= 16 ? launch_norm<T, 1, MODE, 512, kTwo, true>(p, a, o, nsm, st)
          : o.segs <= 32 ? launch_norm<T, 2, MODE, 512, 1, true>(p, a, o, nsm, st)
@@ -515,7 +587,7 @@ extern "C" int fbfp_fp8_rmsnorm(const void* x, int dtype, int64_t m, int64_t k, 
   int dev = 0;
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
   const NormPtrs p{x, w, w_post, resid};
-  const NormArgs a{ldx, ldr, eps, 1.f / (float)k, 0};
+  const NormArgs a{ldx, ldr, eps, 1.f / (float)k, {}, {}, {}, {}, 0};
   const int nsm = sm_count(dev);
   const cudaStream_t st = as_stream(stream);
   FBFP_CUDA_TRY(dtype == FBFP_BF16  ? norm_by_mode<__nv_bfloat16>(p, a, o, nsm, st)

@@ -186,18 +186,22 @@ def test_rmsnorm_zero_infinite_and_nan_rows():
 def test_rmsnorm_strided_rows_and_residual():
     from flashbfp_b200 import fp8
     g = gen(9)
-    wide = torch.randn(6, 1500, device=DEV, generator=g).bfloat16()
-    resw = torch.randn(6, 1304, device=DEV, generator=g).bfloat16()
+    wide = torch.randn(6, 1501, device=DEV, generator=g).bfloat16()
+    resw = torch.randn(6, 1303, device=DEV, generator=g).bfloat16()
     w = torch.randn(900, device=DEV, generator=g).bfloat16()
-    for c0 in (0, 1, 8):
-        x, r0 = wide[:, c0:c0 + 900], resw.clone()
-        res = r0[:, 4:904]
-        a = fp8.rmsnorm_fp8(x, w, 1e-5, residual=res)
-        rc = resw[:, 4:904].contiguous()
-        b = fp8.rmsnorm_fp8(x.contiguous(), w, 1e-5, residual=rc)
-        assert torch.equal(a.values.float(), b.values.float()) and torch.equal(ref.codes_of(a), ref.codes_of(b))
-        assert torch.equal(res, rc)
-        assert torch.equal(r0[:, :4], resw[:, :4]) and torch.equal(r0[:, 904:], resw[:, 904:])
+    for dt in (torch.bfloat16, torch.float32):
+        wide, resw, w = wide.to(dt), resw.to(dt), w.to(dt)
+        for c0, c1 in ((0, 4), (1, 4), (8, 16), (3, 7), (5, 2), (0, 13)):      # every start within 16 bytes
+            for k in (900, 512, 511, 896, 5):
+                x, r0 = wide[:, c0:c0 + k], resw.clone()
+                res = r0[:, c1:c1 + k]
+                a = fp8.rmsnorm_fp8(x, w[:k], 1e-5, residual=res)
+                rc = resw[:, c1:c1 + k].contiguous()
+                b = fp8.rmsnorm_fp8(x.contiguous(), w[:k].contiguous(), 1e-5, residual=rc)
+                # the sums of squares have the same order: rows of any alignment have the same lanes
+                assert torch.equal(a.values.float(), b.values.float()) and torch.equal(ref.codes_of(a), ref.codes_of(b))
+                assert torch.equal(res, rc)
+                assert torch.equal(r0[:, :c1], resw[:, :c1]) and torch.equal(r0[:, c1 + k:], resw[:, c1 + k:])
 
 
 def test_rmsnorm_of_the_residual_itself():
