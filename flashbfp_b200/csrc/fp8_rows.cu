@@ -282,8 +282,11 @@ __device__ __forceinline__ int left_of(int64_t k, int seg) {   // values of the 
 constexpr int kFlatThreads = 256;
 
 // gelu_tanh(g) = g (1 + tanh t) / 2 = g / (1 + exp(-2 t)), t = sqrt(2 / pi) (g + 0.044715 g^3): no
-// cancellation for negative g. The exponent is taken to base 2, log2(e) in its constants; where the
-// power overflows the quotient is 0, as it should be.
+// cancellation for negative g. The exponent is taken to base 2, log2(e) in its constants. EXACT: the
+// approximate reciprocal's quotient is corrected from its residual, for fp32 inputs. (16-bit ones
+// round to the same 8-bit values without, in every case compared with fp64 and with the divided
+// form; it costs them 7%.)
+template <bool EXACT>
 __device__ __forceinline__ float2 gelu_tanh(float2 g) {
   const float c1 = 2.302208198144325f, c2 = 0.1029432395800235f;   // 2 log2(e) sqrt(2 / pi) (1, 0.044715)
   const float2 t = __fmul2_rn(g, __ffma2_rn(make_float2(-c2, -c2), __fmul2_rn(g, g), make_float2(-c1, -c1)));
@@ -291,10 +294,13 @@ __device__ __forceinline__ float2 gelu_tanh(float2 g) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
   e = __fadd2_rn(e, make_float2(1.f, 1.f));
+  if constexpr (EXACT) e = make_float2(fminf(e.x, 8e37f), fminf(e.y, 8e37f));   // normal reciprocals
   float2 r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
-  return __fmul2_rn(g, r);
+  const float2 q = __fmul2_rn(g, r);
+  if constexpr (!EXACT) return q;
+  return __ffma2_rn(__ffma2_rn(make_float2(-q.x, -q.y), e, g), r, q);
 }
 
 // One warp per (row, segment). GEGLU: the row holds gate | up, `k` values each.
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kFlatThreads) fp8_rows_kernel(const T* x, int6
     unpack16(gr, v);
     unpack16(ur, u);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(gelu_tanh(v[i]), u[i]);
+    for (int i = 0; i < kPairs; ++i) v[i] = __fmul2_rn(gelu_tanh<sizeof(T) == 4>(v[i]), u[i]);
   } else {
     unpack16(load16<VEC>(p, n, t), v);
   }
@@ -333,6 +339,16 @@ struct NormArgs {
   Span xs, rs, ws, ps;                                   // of x, resid, w, w_post
   int team;                                              // warps per row
 };
+
+// 1 / sqrt(ss / k + eps). A relative error here moves a whole row, and with it the share of its
+// values that round to the other side in 8 bits: so the quotient (a product with inv_k = 1 / k) and
+// the approximate root (2 units in the last place) each get a correction from their residual.
+__device__ __forceinline__ float row_scale(float ss, float k, float inv_k, float eps) {
+  float q = ss * inv_k;
+  q = q < 3.4e38f ? fmaf(fmaf(-q, k, ss), inv_k, q) : q;
+  const float a = q + eps, y = rsqrtf(a);
+  return y > 0.f && a > 0.f ? fmaf(0.5f * y, fmaf(-a * y, y, 1.f), y) : y;   // not for a = 0 or infinity
+}
 
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
@@ -367,6 +383,7 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
   float* red = reds[0] + warp / a.team * kWarps;         // this team's sums, two rooms in turn
   const int64_t step = (int64_t)gridDim.x * teams;
   int64_t row = (int64_t)blockIdx.x * teams + warp / a.team;
+  const float rk = (float)o.k;
   const T *xp = x + row * a.ldx, *rp = resid + row * a.ldr;
   Raw16<VEC, T> xr[NV], rr[NV];
   if constexpr (kEarly) {
@@ -403,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) ss = __ffma2_rn(v[i][e], v[i][e], ss);
     }
-    float rs = rsqrtf(team_sum<kWarps>(ss, red + turn, seg0) * a.inv_k + a.eps);
+    float rs = row_scale(team_sum<kWarps>(ss, red + turn, seg0), rk, a.inv_k, a.eps);
     turn ^= kTeams * kWarps;
     if constexpr (MODE == 2) {
       ss = make_float2(0.f, 0.f);
@@ -427,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, MINB) fp8_rmsnorm_kernel(const T* x, 
         }
         store16<VEC>(now + seg * kSeg, n, v[i]);
       }
-      rs = rsqrtf(team_sum<kWarps>(ss, red + turn, seg0) * a.inv_k + a.eps);
+      rs = row_scale(team_sum<kWarps>(ss, red + turn, seg0), rk, a.inv_k, a.eps);
       turn ^= kTeams * kWarps;
     }
     if (live) {
