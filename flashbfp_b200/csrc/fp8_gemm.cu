@@ -266,36 +266,39 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 // 128 + BN / 2 rows of 128 bytes per K block for 128 x BN x 128 multiply-adds. Persistent, or with a
 // split: the CTAs (pairs) of a cluster share a tile and split its K blocks.
 //
+// A tile's features are one or two halves of 128, an MMA and an accumulator each; the accumulators
+// are a ring of two (BN = 128) or three (BN = 256). So the next tile's first half starts at once
+// where the last tile's MMAs end, and its second half follows, up to four K blocks behind, when
+// the epilogue has drained the last tile's first half: with one 256-wide accumulator the tensor
+// core waited about 2100 of 19700 cycles per tile of 3840 deep.
+//
 // Scale tiles are loaded once per 512 values of K, with the stage of the group's first K block, and
 // copied to one of four slots of tensor memory in turn. A slot is written again 10 or more K
 // blocks later where a tile has more than 8 (more than the stages in flight), else at least two
-// tiles later (whose accumulator had to be drained first): either way the MMAs that read it have
-// completed. A tile starts on a whole scale tile (features in steps of 128), which keeps the
+// tiles later (whose accumulators had to be drained first): either way the MMAs that read it
+// have completed. A tile starts on a whole scale tile (features in steps of 128), which keeps the
 // scales' tensor-memory addresses on multiples of 4 columns.
 //
-// Epilogue: eight warps, each with 32 tokens (a lane quarter; a token per lane) x BN / 2 features. The
-// sums go to registers first, so that the accumulator is free again after the loads. With a split
-// every block of 32 tokens x 32 features has an owner among the cluster's CTAs: the others store
-// their sums into its shared memory (a warp's store is 512 bytes in a row: 16 bytes a lane), and it
-// adds them to its own in rank order. Owners are spread so that four warps of every CTA have a block
-// (split four ways) or two (eight ways: two warps with one).
+// Epilogue: eight warps, each with 32 tokens (a lane quarter; a token per lane) x 64 features of a
+// half. The sums go to registers first, so that the accumulator is free again after the
+// loads. With a split every block of 32 tokens x 32 features has an owner among the cluster's CTAs:
+// the others store their sums into its shared memory (a warp's store is 512 bytes in a row: 16
+// bytes a lane), and it adds them to its own in rank order. Owners are spread so that four warps
+// of every CTA have a block (split four ways) or two (eight ways: two warps with one).
 template <int CG, int BN>
 struct Many {
-  static constexpr int kRowsB = BN / CG;
-  static constexpr int kChunks = BN / 128;                       // scale tiles of the features
-  static constexpr int kA = 128 * 128, kB = kRowsB * 128, kSf = 512 * (1 + kChunks);
+  static constexpr int kHalves = BN / 128, kRing = kHalves + 1;
+  static constexpr int kRowsB = 128 / CG;                        // weight rows of a half in this CTA
+  static constexpr int kA = 128 * 128, kHalfB = kRowsB * 128, kB = kHalves * kHalfB, kSf = 512 * (1 + kHalves);
   static constexpr int kStage = kA + kB + (kSf + 1023) / 1024 * 1024;
-  static constexpr int kBufs = CG == 2 && BN == 128 ? 2 : 1;     // accumulators
-  static constexpr int kSfCols = 4 * (1 + kChunks), kSfSlots = 4;
-  static constexpr uint32_t kSfCol0 = kBufs * BN;
-  static constexpr uint32_t kTmemCols = kSfCol0 + kSfSlots * kSfCols <= 256 ? 256 : 512;
+  static constexpr int kSfCols = 4 * (1 + kHalves), kSfSlots = 4;
+  static constexpr uint32_t kSfCol0 = kRing * 128, kTmemCols = 512;
   static constexpr int kEpiWarps = 8, kThreads = 32 * (4 + kEpiWarps);
-  static constexpr int kCols = BN / 2;                           // columns of a unit
   static constexpr int kTurn = 32 * 17 * 4;                      // a warp's 32 x 16 words, rows 17 apart
   static constexpr int kTurns = kEpiWarps * kTurn;
   static constexpr int kBlock = 32 * 32 * 4;                     // [feature / 4][token][4]
   static constexpr int kSums = 14 * kBlock;                      // 16 / S blocks from S - 1 CTAs, S 2, 4 or 8
-  static constexpr int kBars = (2 * kMaxStages + 2 + 2 + 2) * 8 + 16;
+  static constexpr int kBars = (2 * kMaxStages + 2 * kRing + 2) * 8 + 16;
   static constexpr int kFixed = kBars + 1024;                    // stages start on 1 KB
   static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kBlock % 16 == 0, "alignment");
   static_assert(kSfCol0 + kSfSlots * kSfCols <= kTmemCols, "tensor memory budget");
@@ -414,8 +417,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   uint64_t* full = reinterpret_cast<uint64_t*>(sums + (splits > 1 ? C::kSums : C::kTurns));   // used in a pair's CTA 0
   uint64_t* empty = full + kMaxStages;
   uint64_t* acc_full = empty + kMaxStages;
-  uint64_t* acc_empty = acc_full + 2;                               // used in a pair's CTA 0
-  uint64_t* tail = acc_empty + 2;
+  uint64_t* acc_empty = acc_full + C::kRing;                        // used in a pair's CTA 0
+  uint64_t* tail = acc_empty + C::kRing;
   uint64_t* landed = tail + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 1);
   const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
@@ -429,11 +432,12 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     // the first weights on their way to L2 while the previous kernel of the stream ends
     prefetch_tmap(&M.w); prefetch_tmap(&M.x); prefetch_tmap(&M.ws); prefetch_tmap(&M.xs);
     for (int kb = kb0; kb < kb1 && kb < kb0 + stages; ++kb)
-      tma_2d_prefetch(&M.w, kb * 128, (int)(team / a.n_tt * BN + pr * C::kRowsB));
+      for (int h = 0; h < C::kHalves; ++h)
+        tma_2d_prefetch(&M.w, kb * 128, (int)(team / a.n_tt * BN + 128 * h + pr * C::kRowsB));
   }
   if (threadIdx.x == 32) {
     for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], CG * C::kEpiWarps); }
+    for (int b = 0; b < C::kRing; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], CG * C::kEpiWarps); }
     mbar_init(tail, 1);
     mbar_init(landed, 1);
     *A.flag = 0;
@@ -480,11 +484,13 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
           // a pair's CTA 0 expects both CTAs' bytes
           if (pr == 0) mbar_arrive_expect_tx(&full[s], CG * (C::kA + C::kB + (sf ? C::kSf : 0)));
           load_tile<CG>(st, &M.x, kb * 128, (int)m0, bar);
-          load_tile<CG>(st + C::kA, &M.w, kb * 128, (int)(n0 + pr * C::kRowsB), bar);
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h)
+            load_tile<CG>(st + C::kA + h * C::kHalfB, &M.w, kb * 128, (int)(n0 + 128 * h + pr * C::kRowsB), bar);
           if (sf) {                                      // tiles past the last one read as zero
             load_tile<CG>(st + C::kA + C::kB, &M.xs, 0, (int)(m0 / 128 * a.kgroups + kb / 4), bar);
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c)
+            for (int c = 0; c < C::kHalves; ++c)
               load_tile<CG>(st + C::kA + C::kB + 512 * (1 + c), &M.ws, 0,
                             (int)((n0 / 128 + c) * a.kgroups + kb / 4), bar);
           }
@@ -502,43 +508,74 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     __syncwarp();
   } else if (warp == 1 && pr == 0) {
     if (elect_one_sync()) {
-      constexpr uint32_t kIdesc = idesc_mxf8(128 * CG, BN);
+      constexpr uint32_t kIdesc = idesc_mxf8(128 * CG, 128);
+      constexpr int kAhead = 4;                          // K blocks of a first half before its second
       const uint32_t sbase = smem_u32(smem);
       const int64_t total = (int64_t)((a.tiles - team + teams - 1) / teams) * (kb1 - kb0);   // team < tiles
       int64_t it = 0;
-      int s = 0, buf = 0, slot = C::kSfSlots - 1;
-      uint32_t ph = 0, aph = 0;
+      int s = 0, slot = C::kSfSlots - 1, ring = 0;
+      uint32_t ph = 0, rph = 0, sfa = 0;
       bool ok = true;
+      // a half's four MMAs of K block kb (32 values = 32 bytes per step), in stage `stage`
+      auto issue = [&](int half, uint32_t acc_slot, int stage, int kb) {
+        const uint32_t st = sbase + (uint32_t)stage * C::kStage;
+        const uint64_t da = smem_desc_sw128(st, 1024), db = smem_desc_sw128(st + C::kA + half * C::kHalfB, 1024);
+        const uint32_t id = idesc_mxf8_id(kIdesc, kb & 3);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_mxf8<CG>(tmem + acc_slot * 128, da + 2 * k, db + 2 * k, id, sfa, sfa + 4 + 4 * half, kb > kb0 || k > 0);
+      };
+      auto release = [&](int stage) {                    // only where the producers wait for it
+        if (it + stages < total) commit<CG>(&empty[stage], pair_mask);
+        ++it;
+      };
       for (uint32_t t = team; t < a.tiles && ok; t += teams) {
-        if (!(ok = fp8_wait<CG == 2>(&acc_empty[buf], aph ^ 1, A, 24))) break;
+        const uint32_t first = ring, fph = rph;
+        if (++ring == C::kRing) { ring = 0; rph ^= 1; }
+        const uint32_t second = ring, sph = rph;         // (two halves)
+        if (C::kHalves == 2 && ++ring == C::kRing) { ring = 0; rph ^= 1; }
+        if (!(ok = fp8_wait<CG == 2>(&acc_empty[first], fph ^ 1, A, 24))) break;
         tc_fence_after();
-        const uint32_t d = tmem + buf * BN;
-        uint32_t acc = 0, sfa = 0;
+        bool open = false;                               // the second half's accumulator is free
+        int s0 = s;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = fp8_wait<CG == 2>(&full[s], ph, A, 25))) break;
           tc_fence_after();
-          const uint32_t st = sbase + (uint32_t)s * C::kStage;
           if ((kb & 3) == 0 || kb == kb0) {
+            const uint32_t st = sbase + (uint32_t)s * C::kStage;
             slot = slot == C::kSfSlots - 1 ? 0 : slot + 1;
             sfa = tmem + C::kSfCol0 + slot * C::kSfCols;
 #pragma unroll
-            for (int c = 0; c < 1 + C::kChunks; ++c)
+            for (int c = 0; c < 1 + C::kHalves; ++c)
               scales_to_tmem<CG>(sfa + 4 * c, smem_desc_scales(st + C::kA + C::kB + 512 * c));
           }
-          const uint64_t da = smem_desc_sw128(st, 1024), db = smem_desc_sw128(st + C::kA, 1024);
-          const uint32_t id = idesc_mxf8_id(kIdesc, kb & 3);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {                  // 32 values = 32 bytes per step
-            mma_mxf8<CG>(d, da + 2 * k, db + 2 * k, id, sfa, sfa + 4, acc);
-            acc = 1;
+          issue(0, first, s, kb);
+          if constexpr (C::kHalves == 1) {
+            release(s);
+          } else if (open) {
+            issue(1, second, s, kb);
+            release(s);
+          } else {
+            // a tile's first blocks share one scale group: kb0 = 0 with two halves, kAhead <= 4
+            open = mbar_test(&acc_empty[second], sph ^ 1);
+            if (!open && (kb + 1 == kb1 || kb + 1 == kb0 + kAhead)) {
+              if (!(ok = fp8_wait<CG == 2>(&acc_empty[second], sph ^ 1, A, 24))) break;
+              open = true;
+            }
+            if (open) {
+              tc_fence_after();
+              for (int j = kb0; j <= kb; ++j) {
+                issue(1, second, s0, j);
+                release(s0);
+                if (++s0 == stages) s0 = 0;
+              }
+            }
           }
-          if (it + stages < total) commit<CG>(&empty[s], pair_mask);   // only where the producers wait for it
-          ++it;
           if (++s == stages) { s = 0; ph ^= 1; }
         }
         if (!ok) break;
-        commit<CG>(&acc_full[buf], pair_mask);
-        if (++buf == C::kBufs) { buf = 0; aph ^= 1; }
+        commit<CG>(&acc_full[first], pair_mask);
+        if constexpr (C::kHalves == 2) commit<CG>(&acc_full[second], pair_mask);
       }
       if (!ok) {                                         // MMAs in flight end before the memory goes
         commit<CG>(tail, pair_mask);
@@ -547,39 +584,42 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int q4 = warp & 3, half = (warp - 4) >> 2, col0 = half * C::kCols;
+    const int q4 = warp & 3, side = (warp - 4) >> 2;
     if (CG == 1 && splits > 1) cluster_wait();           // the owners' barriers are ready
     uint32_t* turn = reinterpret_cast<uint32_t*>(turns + (warp - 4) * C::kTurn);
     const uint64_t bits = (uint64_t)(uintptr_t)a.y | (uint64_t)a.ldy * sizeof(T);
     const int vec = (bits & 31) == 0 ? 32 : (bits & 15) == 0 ? 16 : 0;
-    int buf = 0;
+    int ring = 0;
     uint32_t ph = 0;
+    uint32_t t = team;
+    int half = 0;
 #pragma unroll 1
-    for (uint32_t t = team; t < a.tiles; t += teams) {
+    for (; t < a.tiles; half == C::kHalves - 1 ? (half = 0, t += teams) : ++half) {
       const int64_t tok0 = (int64_t)(t % a.n_tt) * (128 * CG) + 128 * pr + q4 * 32;
-      const int64_t n0 = (int64_t)(t / a.n_tt) * BN + col0;
-      if (!__all_sync(0xffffffffu, fp8_wait<CG == 2>(&acc_full[buf], ph, A, 26))) break;
+      const int64_t n0 = (int64_t)(t / a.n_tt) * BN + 128 * half + 64 * side;
+      if (!__all_sync(0xffffffffu, fp8_wait<CG == 2>(&acc_full[ring], ph, A, 26))) break;
       tc_fence_after();
-      const uint32_t taddr = tmem + buf * BN + col0 + ((uint32_t)(q4 * 32) << 16);
-      float v[C::kCols / 32][32];
+      const uint32_t taddr = tmem + ring * 128 + 64 * side + ((uint32_t)(q4 * 32) << 16);
+      float v[2][32];
 #pragma unroll
-      for (int c = 0; c < C::kCols / 32; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, v[c]);
+      for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(taddr + 32 * c, v[c]);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 1) mbar_arrive(&acc_empty[buf]);
-        else mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[buf]), lead));
+        if constexpr (CG == 1) mbar_arrive(&acc_empty[ring]);
+        else mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[ring]), lead));
       }
+      if (++ring == C::kRing) { ring = 0; ph ^= 1; }
       if constexpr (BN == 128) {
         if (splits > 1 && tok0 < a.m) {
           // into the owner's room for this block and split
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int owner = block_owner(q4, 2 * half + c, splits);
+            const int owner = block_owner(q4, 2 * side + c, splits);
             if (owner == sp) continue;
             const int to = owner * CG + pr, from = sp < owner ? sp : sp - 1;
-            const int room = block_slot(q4, 2 * half + c, splits) * (splits - 1) + from;
+            const int room = block_slot(q4, 2 * side + c, splits) * (splits - 1) + from;
             const uint32_t dst = map_shared(smem_u32(sums) + room * C::kBlock + lane * 16, to);
             const uint32_t bar = map_shared(smem_u32(landed), to);
 #pragma unroll
@@ -589,14 +629,14 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
         }
       }
 #pragma unroll
-      for (int c = 0; c < C::kCols / 32; ++c) {
+      for (int c = 0; c < 2; ++c) {
         const int64_t f0 = n0 + 32 * c;
         if (f0 >= a.n || tok0 >= a.m) break;             // whole warps
         if constexpr (BN == 128) {
           if (splits > 1) {
-            if (block_owner(q4, 2 * half + c, splits) != sp) continue;
+            if (block_owner(q4, 2 * side + c, splits) != sp) continue;
             if (!__all_sync(0xffffffffu, fp8_wait<true>(landed, 0, A, 27))) break;
-            const uint8_t* p = sums + block_slot(q4, 2 * half + c, splits) * (splits - 1) * C::kBlock + lane * 16;
+            const uint8_t* p = sums + block_slot(q4, 2 * side + c, splits) * (splits - 1) * C::kBlock + lane * 16;
 #pragma unroll 1
             for (int r = 0; r < splits - 1; ++r, p += C::kBlock) {
 #pragma unroll
@@ -614,7 +654,6 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
         }
         store_y32<T>(a, tok0, f0, v[c], vec, turn);
       }
-      if (++buf == C::kBufs) { buf = 0; ph ^= 1; }
     }
   }
   __syncwarp();
@@ -787,7 +826,7 @@ int fp8_dispatch(Fp8Args& a, const Fp8Operands& o, int dev, cudaStream_t st) {
   a.n_tt = (uint32_t)p.token_tiles;
   a.tiles = (uint32_t)p.tiles;
   if ((rc = encode_rows(&M.x, o.x, a.m, o.k, o.ldx, 128)) != FBFP_OK) return rc;
-  if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, p.bn / p.cg)) != FBFP_OK) return rc;
+  if ((rc = encode_rows(&M.w, o.w, a.n, o.k, o.ldw, 128 / p.cg)) != FBFP_OK) return rc;
   if ((rc = encode_scales(&M.xs, a.x_scales, (a.m + 127) / 128 * a.kgroups)) != FBFP_OK) return rc;
   if ((rc = encode_scales(&M.ws, a.w_scales, (a.n + 127) / 128 * a.kgroups)) != FBFP_OK) return rc;
   if (p.cg == 1)
