@@ -45,6 +45,8 @@ def test_row_entries_refuse(L):
         refused(L, fn(P, 1, 1, 16, 32, odd, 16, P, None), "aligned")
         refused(L, fn(P, 1, 1, 16, 32, P, 16, odd, None), "aligned")
         refused(L, fn(P, 1, 4, 16, -1, P, 16, P, None), "stride")
+        refused(L, fn(ctypes.c_void_p(4097), 1, 1, 16, 32, P, 16, P, None), "aligned to their type")
+        refused(L, fn(ctypes.c_void_p(4098), 0, 1, 16, 32, P, 16, P, None), "aligned to their type")
 
     def norm(x=P, dt=1, m=2, k=16, ldx=16, w=P, wp=None, r=None, ldr=0, v=P, ldv=16, s=P):
         return L.fbfp_fp8_rmsnorm(x, dt, m, k, ldx, w, wp, r, ldr, 1e-6, v, ldv, s, None)
@@ -55,6 +57,8 @@ def test_row_entries_refuse(L):
     refused(L, norm(r=P, ldr=8), "stride")
     refused(L, norm(k=32769, ldx=40000, ldv=32784), "at most 32768")
     refused(L, norm(dt=3), "dtype")
+    refused(L, norm(w=ctypes.c_void_p(4097)), "aligned to their type")
+    refused(L, norm(r=ctypes.c_void_p(4097), ldr=16), "aligned to their type")
 
 
 def test_linear_refuses(L):
@@ -74,6 +78,8 @@ def test_linear_refuses(L):
     refused(L, lin(ldy=7), "ldy")
     refused(L, lin(yd=5), "dtype")
     refused(L, lin(b=P, bd=9), "dtype")
+    refused(L, lin(y=ctypes.c_void_p(4097)), "aligned to their types")
+    refused(L, lin(b=ctypes.c_void_p(4098), bd=0), "aligned to their types")
 
 
 def test_cpu_tensors_are_refused():
