@@ -85,14 +85,15 @@ __device__ __forceinline__ void store4(T* p, int n, const float4& v, bool vec) {
 // ---------------------------------------------------------------------------------------
 // Few tokens (up to 64). A CTA takes 128 output features (the MMA's M side: 128 weight rows) x the
 // tokens (its N side, BN of them, zeros past the last) and a contiguous range of the K blocks; the
-// CTAs of a cluster (up to 8) share a tile and split its K blocks. Per K block one stage: 128 x 128 weight bytes, BN x 128 token
-// bytes (128-byte swizzle) and both scale tiles. Warp 0 loads, warp 1 copies the scales to tensor
-// memory and issues four MMAs, warps 2-5 read the sums back (a feature per lane) into shared
-// memory. With a split each CTA owns some of the tile's tokens: the others store their fp32
+// CTAs of a cluster (up to 8) share a tile and split its K blocks. Per K block one stage: 128 x 128
+// weight bytes, BN x 128 token bytes (128-byte swizzle) and both scale tiles. Warp 0 loads, warp 1
+// copies the scales to tensor memory and issues four MMAs, warps 2-5 read the sums back (a feature
+// per lane) into shared memory. With a split each CTA owns some of the tile's tokens: the others store their fp32
 // partial sums straight into its shared memory, and it adds them in rank order (a fixed order: same
 // bits every time). Bound by the weights' bytes, and by some 3.4 us of launch, first bytes and
-// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.2 us
-// (5.6 TB/s), 64 x 30720 x 3840 23.7 us (5.2 TB/s), 1 x 8192 x 3840 8.7 us, 1 x 3840 x 4096 6.0 us.
+// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.0 us
+// (5.7 TB/s), 64 x 30720 x 3840 23.2 us (5.3 TB/s), 64 x 8192 x 28672 42.3 us (5.6 TB/s), 1 x 8192
+// x 3840 8.1 us, 1 x 3840 x 4096 5.9 us.
 template <int BN>
 struct Few {
   static constexpr int kA = 128 * 128, kB = BN * 128, kSf = 512;
@@ -731,26 +732,40 @@ int clusters_at_a_time(void (*kernel)(KArgs...), int dev, int (&known)[64][9], i
   return n;
 }
 
-// K is split over as large a cluster (up to 8) as leaves every CTA at least 4 K blocks and all
-// tiles running at a time, two CTAs per SM.
+// K is split over as large a cluster (up to 8) as leaves every CTA at least 4 K blocks and all tiles
+// running at a time, one CTA per SM where these fill 75% of the SMs or two per SM would split no
+// further: a deeper ring, fewer partial sums to exchange. A ring has no more stages than a CTA has
+// K blocks, so that the next kernel's CTAs start beside it. Measured, one / two per SM: 64 x 8192 x
+// 28672 42.6 / 52.4 us, 64 x 3840 x 15360 13.9 / 16.8, 1 x 8192 x 3840 8.1 / 8.7, 16 x 18944 x 3840
+// 13.9 / 15.1; the other way around 16 x 30720 x 3840 24.9 / 21.2, 32 x 10240 x 3840 11.8 / 10.1, 1 x
+// 4096 x 2048 (rings of 8 and of 5 stages) 4.7 / 3.7. Timings of every split of 172 shapes put the
+// choice 1.1% behind the best on average, 15% at worst. Occupancy counted one CTA per SM for this
+// kernel at 80 to 113 KB of shared memory too, where two do run (296 tiles take one round): twice
+// the count is taken for two.
 template <int BN, typename T>
 int launch_few(Fp8Args a, const Fp8Maps& M, int dev, cudaStream_t st) {
   using C = Few<BN>;
   static bool attr_set[64] = {false};
   static int known[64][9];
+  const auto kernel = fp8_few_kernel<BN, T>;
   const int64_t tiles = (a.n + 127) / 128;
-  int splits = 1, extra = 0;
-  for (int c = 8; c > 1; --c)
-    if ((int)a.nkb >= 4 * c &&
-        tiles <= clusters_at_a_time(fp8_few_kernel<BN, T>, dev, known, c, C::kThreads, kSmemTwo)) {
-      splits = c;
-      extra = C::kSums;
-      break;
-    }
-  const int fit = (kSmemTwo - C::kFixed - extra) / C::kStage;
-  a.stages = fit < kMaxStages ? fit : kMaxStages;
-  return launch_cluster(fp8_few_kernel<BN, T>, dev, attr_set, tiles * splits, splits, C::kThreads,
-                        (size_t)a.stages * C::kStage + extra + C::kFixed, st, a, M);
+  auto clusters = [&](int c) { return (int64_t)clusters_at_a_time(kernel, dev, known, c, C::kThreads, kSmemOne); };
+  auto split = [&](int per_sm) {
+    for (int c = 8; c > 1; --c)
+      if ((int)a.nkb >= 4 * c && tiles <= per_sm * clusters(c)) return c;
+    return 1;
+  };
+  const int64_t sms = clusters(1);
+  const int one = split(1), two = split(2);
+  const bool alone = tiles <= sms && (tiles * one * 4 >= sms * 3 || one == two);
+  const int splits = alone ? one : two, extra = splits > 1 ? C::kSums : 0;
+  int stages = ((alone ? kSmemOne : kSmemTwo) - C::kFixed - extra) / C::kStage;
+  const int blocks = (int)((a.nkb + splits - 1) / splits);
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (stages > blocks) stages = blocks < 3 ? 3 : blocks;   // at least 3: the sums' place without a split
+  a.stages = stages;
+  return launch_cluster(kernel, dev, attr_set, tiles * splits, splits, C::kThreads,
+                        (size_t)stages * C::kStage + extra + C::kFixed, st, a, M);
 }
 
 template <int CG, int BN, typename T>
