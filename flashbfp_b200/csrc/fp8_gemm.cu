@@ -91,9 +91,9 @@ __device__ __forceinline__ void store4(T* p, int n, const float4& v, bool vec) {
 // per lane) into shared memory. With a split each CTA owns some of the tile's tokens: the others store their fp32
 // partial sums straight into its shared memory, and it adds them in rank order (a fixed order: same
 // bits every time). Bound by the weights' bytes, and by some 3.4 us of launch, first bytes and
-// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.0 us
-// (5.7 TB/s), 64 x 30720 x 3840 23.2 us (5.3 TB/s), 64 x 8192 x 28672 42.3 us (5.6 TB/s), 1 x 8192
-// x 3840 8.1 us, 1 x 3840 x 4096 5.9 us.
+// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.3 us
+// (5.6 TB/s), 64 x 30720 x 3840 23.2 us (5.3 TB/s), 64 x 8192 x 28672 43.0 us (5.6 TB/s), 1 x 8192
+// x 3840 8.1 us, 1 x 3840 x 4096 6.0 us.
 template <int BN>
 struct Few {
   static constexpr int kA = 128 * 128, kB = BN * 128, kSf = 512;
@@ -733,15 +733,16 @@ int clusters_at_a_time(void (*kernel)(KArgs...), int dev, int (&known)[64][9], i
 }
 
 // K is split over as large a cluster (up to 8) as leaves every CTA at least 4 K blocks and all tiles
-// running at a time, one CTA per SM where these fill 75% of the SMs or two per SM would split no
-// further: a deeper ring, fewer partial sums to exchange. A ring has no more stages than a CTA has
-// K blocks, so that the next kernel's CTAs start beside it. Measured, one / two per SM: 64 x 8192 x
-// 28672 42.6 / 52.4 us, 64 x 3840 x 15360 13.9 / 16.8, 1 x 8192 x 3840 8.1 / 8.7, 16 x 18944 x 3840
-// 13.9 / 15.1; the other way around 16 x 30720 x 3840 24.9 / 21.2, 32 x 10240 x 3840 11.8 / 10.1, 1 x
-// 4096 x 2048 (rings of 8 and of 5 stages) 4.7 / 3.7. Timings of every split of 172 shapes put the
-// choice 1.1% behind the best on average, 15% at worst. Occupancy counted one CTA per SM for this
-// kernel at 80 to 113 KB of shared memory too, where two do run (296 tiles take one round): twice
-// the count is taken for two.
+// running at a time: one CTA per SM where these fill 70% of the SMs, else two per SM. A CTA that has
+// an SM to itself and more than twice the K blocks of the ring that two leave room for takes the
+// larger ring; the others keep the small one, beside which the next kernel's CTAs start. No ring has
+// more stages than its CTA has K blocks. Measured, larger / small ring, weights read from HBM: 64 x
+// 8192 x 28672 42.6 / 52.4 us, 64 x 3840 x 15360 13.9 / 16.8; read from L2: 1 x 3840 x 4096 5.5 /
+// 4.5. One / two per SM: 16 x 18944 x 3840 13.8 / 14.6, 16 x 30720 x 3840 24.9 / 21.2, 32 x 10240 x
+// 3840 11.8 / 10.1. In timings of every split of 172 shapes the choice is 1.6% behind the best
+// with weights from HBM (11% at worst) and 2.9% with weights from L2 (19%). Occupancy counted one
+// CTA per SM for this kernel at 80 to 113 KB of shared memory too, where two do run (296 tiles take
+// one round): twice the count is taken for two.
 template <int BN, typename T>
 int launch_few(Fp8Args a, const Fp8Maps& M, int dev, cudaStream_t st) {
   using C = Few<BN>;
@@ -756,11 +757,12 @@ int launch_few(Fp8Args a, const Fp8Maps& M, int dev, cudaStream_t st) {
     return 1;
   };
   const int64_t sms = clusters(1);
-  const int one = split(1), two = split(2);
-  const bool alone = tiles <= sms && (tiles * one * 4 >= sms * 3 || one == two);
-  const int splits = alone ? one : two, extra = splits > 1 ? C::kSums : 0;
-  int stages = ((alone ? kSmemOne : kSmemTwo) - C::kFixed - extra) / C::kStage;
+  const int one = split(1);
+  const int splits = tiles <= sms && tiles * one * 10 >= sms * 7 ? one : split(2);
+  const int extra = splits > 1 ? C::kSums : 0;
   const int blocks = (int)((a.nkb + splits - 1) / splits);
+  int stages = (kSmemTwo - C::kFixed - extra) / C::kStage;
+  if (tiles <= sms && splits == one && blocks > 2 * stages) stages = (kSmemOne - C::kFixed - extra) / C::kStage;
   if (stages > kMaxStages) stages = kMaxStages;
   if (stages > blocks) stages = blocks < 3 ? 3 : blocks;   // at least 3: the sums' place without a split
   a.stages = stages;
