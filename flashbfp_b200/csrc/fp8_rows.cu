@@ -287,25 +287,35 @@ __device__ __forceinline__ int left_of(int64_t k, int seg) {   // values of the 
 constexpr int kFlatThreads = 256;
 
 // gelu_tanh(g) = g (1 + tanh t) / 2 = g / (1 + exp(-2 t)), t = sqrt(2 / pi) (g + 0.044715 g^3): no
-// cancellation for negative g. The exponent is taken to base 2, log2(e) in its constants. EXACT: the
-// approximate reciprocal's quotient is corrected from its residual, for fp32 inputs. (16-bit ones
-// round to the same 8-bit values without, in every case compared with fp64 and with the divided
-// form; it costs them 7%.)
+// cancellation for negative g. The exponent e is taken to base 2, log2(e) in its constants.
+// EXACT, for fp32 inputs: with s = 2^-|e|, g (s or 1) / (1 + s), whose denominator lies in [1, 2]
+// for every gate and whose reciprocal's quotient is corrected from its residual. Else g / (1 + 2^e)
+// as it is. Either way a very negative gate (a mask of the lowest value, say) gives 0: s flushes to
+// 0 below 2^-126, as does the reciprocal of a denominator above 2^126, off by at most 10.1 * 2^-126
+// (gates between -10.0 and -10.3). (16-bit inputs round to the same 8-bit values without the
+// correction, in every case compared with fp64 and with the divided form; it costs them 7%.)
 template <bool EXACT>
 __device__ __forceinline__ float2 gelu_tanh(float2 g) {
   const float c1 = 2.302208198144325f, c2 = 0.1029432395800235f;   // 2 log2(e) sqrt(2 / pi) (1, 0.044715)
   const float2 t = __fmul2_rn(g, __ffma2_rn(make_float2(-c2, -c2), __fmul2_rn(g, g), make_float2(-c1, -c1)));
-  float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-  e = __fadd2_rn(e, make_float2(1.f, 1.f));
-  if constexpr (EXACT) e = make_float2(fminf(e.x, 8e37f), fminf(e.y, 8e37f));   // normal reciprocals
-  float2 r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
-  const float2 q = __fmul2_rn(g, r);
-  if constexpr (!EXACT) return q;
-  return __ffma2_rn(__ffma2_rn(make_float2(-q.x, -q.y), e, g), r, q);
+  float2 e, r;
+  if constexpr (EXACT) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(-fabsf(t.x)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(-fabsf(t.y)));
+    const float2 n = __fmul2_rn(g, make_float2(t.x > 0.f ? e.x : 1.f, t.y > 0.f ? e.y : 1.f));
+    e = __fadd2_rn(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    const float2 q = __fmul2_rn(n, r);
+    return __ffma2_rn(__ffma2_rn(make_float2(-q.x, -q.y), e, n), r, q);
+  } else {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = __fadd2_rn(e, make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return __fmul2_rn(g, r);
+  }
 }
 
 // One warp per (row, segment). GEGLU: the row holds gate | up, `k` values each.
