@@ -5,6 +5,7 @@
 
 #include "common.cuh"
 #include "fp8_mma.cuh"
+#include "fp8_split.h"
 #include "pdl.cuh"
 #include "tc_host.h"
 
@@ -292,8 +293,9 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 // half. The sums go to registers first, so that the accumulator is free again after the
 // loads. With a split every block of 32 tokens x 32 features has an owner among the cluster's CTAs:
 // the others store their sums into its shared memory (a warp's store is 512 bytes in a row: 16
-// bytes a lane), and it adds them to its own in rank order. Owners are spread so that four warps
-// of every CTA have a block (split four ways) or two (eight ways: two warps with one).
+// bytes a lane), and it adds them to its own in rank order, once all of them have landed (fp8_split.h).
+// Owners are spread so that four warps of every CTA have a block (split four ways) or two (eight
+// ways: two warps with one).
 template <int CG, int BN>
 struct Many {
   static constexpr int kHalves = BN / 128, kRing = kHalves + 1;
@@ -392,15 +394,6 @@ __device__ __forceinline__ void store_y32(const Fp8Args& a, int64_t tok0, int64_
   }
 }
 
-// The split whose CTA owns block (lane quarter q, 32-feature column c) of a split two, four or eight ways,
-// and its place among that CTA's blocks.
-__device__ __forceinline__ int block_owner(int q, int c, int splits) {
-  return splits == 2 ? c >> 1 : splits == 4 ? c : 2 * c + (q >> 1);
-}
-__device__ __forceinline__ int block_slot(int q, int c, int splits) {
-  return splits == 2 ? q * 2 + (c & 1) : splits == 4 ? q : q & 1;
-}
-
 template <int CG>
 __device__ __forceinline__ void commit(uint64_t* bar, uint16_t pair_mask) {
   if constexpr (CG == 1) mma_commit(bar);
@@ -451,11 +444,9 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     mbar_init(landed, 1);
     *A.flag = 0;
     fence_mbar_init();
-    if (splits > 1) {                                    // this CTA's blocks that have tokens
-      int live = 0;
-      for (int b = 0; b < 16; ++b)
-        live += block_owner(b >> 2, b & 3, splits) == sp &&
-                (int64_t)(team % a.n_tt) * (128 * CG) + 128 * pr + (b >> 2) * 32 < a.m;
+    if (splits > 1) {
+      const int live = owned_blocks(sp, splits, (int64_t)(team % a.n_tt) * (128 * CG) + 128 * pr,
+                                    (int64_t)(team / a.n_tt) * BN, a.m, a.n);
       if (live) mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * 32 * 4));
     }
   }
@@ -621,12 +612,12 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
       }
       if (++ring == C::kRing) { ring = 0; ph ^= 1; }
       if constexpr (BN == 128) {
-        if (splits > 1 && tok0 < a.m) {
+        if (splits > 1) {
           // into the owner's room for this block and split
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int owner = block_owner(q4, 2 * side + c, splits);
-            if (owner == sp) continue;
+            if (owner == sp || !block_live(tok0, n0 + 32 * c, a.m, a.n)) continue;
             const int to = owner * CG + pr, from = sp < owner ? sp : sp - 1;
             const int room = block_slot(q4, 2 * side + c, splits) * (splits - 1) + from;
             const uint32_t dst = map_shared(smem_u32(sums) + room * C::kBlock + lane * 16, to);
@@ -640,7 +631,7 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int64_t f0 = n0 + 32 * c;
-        if (f0 >= a.n || tok0 >= a.m) break;             // whole warps
+        if (!block_live(tok0, f0, a.m, a.n)) break;      // whole warps
         if constexpr (BN == 128) {
           if (splits > 1) {
             if (block_owner(q4, 2 * side + c, splits) != sp) continue;
