@@ -593,6 +593,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     uint32_t ph = 0;
     uint32_t t = team;
     int half = 0;
+    int64_t drained = 0;                                 // halves so far, of all
+    const int64_t halves = (int64_t)((a.tiles - team + teams - 1) / teams) * C::kHalves;   // team < tiles
 #pragma unroll 1
     for (; t < a.tiles; half == C::kHalves - 1 ? (half = 0, t += teams) : ++half) {
       const int64_t tok0 = (int64_t)(t % a.n_tt) * (128 * CG) + 128 * pr + q4 * 32;
@@ -606,7 +608,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
+      // only where an MMA waits for it: a pair's CTA 0 is gone otherwise when the arrival comes
+      if (lane == 0 && arrival_awaited(drained++, C::kRing, halves)) {
         if constexpr (CG == 1) mbar_arrive(&acc_empty[ring]);
         else mbar_arrive_cluster(map_shared(smem_u32(&acc_empty[ring]), lead));
       }

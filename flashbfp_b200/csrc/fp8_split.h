@@ -1,5 +1,6 @@
-// fp8_split.h — who adds what where CTAs share a tile of the block-scaled product and split its K
-// blocks. Plain C++ beside the kernel (fp8_gemm.cu), so that the rule can be run on the host.
+// fp8_split.h — what the CTAs of a cluster send each other in the block-scaled product: who adds what
+// where they share a tile and split its K blocks, and which arrivals are waited for. Plain C++
+// beside the kernel (fp8_gemm.cu), so that the rules can be run on the host.
 //
 // A CTA's 128 tokens x 128 features of sums are 16 blocks of 32 x 32: lane quarter q (tokens), column
 // c (features). Each has an owner among the splits: the others store their sums into its shared
@@ -34,5 +35,10 @@ FBFP_HD int owned_blocks(int sp, int splits, int64_t tok, int64_t f, int64_t m, 
     live += block_owner(b >> 2, b & 3, splits) == sp && block_live(tok + (b >> 2) * 32, f + (b & 3) * 32, m, n);
   return live;
 }
+
+// Whether the MMAs wait for half h (of `halves` that a CTA or pair computes in turn) to be drained: the
+// half `ring` later takes its accumulator. An arrival that nobody waits for must not be sent to
+// another CTA, which may have left.
+FBFP_HD bool arrival_awaited(int64_t h, int ring, int64_t halves) { return h + ring < halves; }
 
 }  // namespace fbfp

@@ -46,18 +46,47 @@ extern "C" int tile(int cg, int splits, int64_t tok, int64_t f0, int64_t m, int6
   }
   return bad;
 }
+// The accumulators' ring: the MMAs take halves in turn and wait, from the second use of a slot on,
+// for its last drain; the epilogue drains in turn. all: every drain arrives (the control). Returns
+// the arrivals that nobody waited for, or -1 if a wait would never end.
+extern "C" int64_t ring(int64_t halves, int ring, int all) {
+  int64_t arrived[8] = {0}, waited[8] = {0};
+  for (int64_t h = 0; h < halves; ++h) {
+    const int slot = (int)(h % ring);
+    if (h >= ring && arrived[slot] < ++waited[slot]) return -1;
+    arrived[slot] += all || arrival_awaited(h, ring, halves);
+  }
+  int64_t rest = 0;
+  for (int i = 0; i < ring; ++i) rest += arrived[i] - waited[i];
+  return rest;
+}
 """
 
 
 @pytest.fixture(scope="module")
-def tile(tmp_path_factory):
+def rules(tmp_path_factory):
     d = tmp_path_factory.mktemp("split")
     (d / "h.cpp").write_text(HARNESS)
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, str(d / "h.cpp"), "-o",
                     str(d / "h.so")], check=True)
-    f = ctypes.CDLL(str(d / "h.so")).tile
-    f.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 4 + [ctypes.c_int]
-    return f
+    lib = ctypes.CDLL(str(d / "h.so"))
+    lib.tile.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 4 + [ctypes.c_int]
+    lib.ring.argtypes, lib.ring.restype = [ctypes.c_int64, ctypes.c_int, ctypes.c_int], ctypes.c_int64
+    return lib
+
+
+@pytest.fixture(scope="module")
+def tile(rules):
+    return rules.tile
+
+
+@pytest.mark.parametrize("halves_per_tile", [1, 2])
+def test_no_arrival_is_left_over(rules, halves_per_tile):
+    """Drained accumulators are reported to a pair's first CTA exactly as often as its MMAs wait."""
+    ring = halves_per_tile + 1
+    for tiles in list(range(1, 40)) + [1000]:
+        assert rules.ring(tiles * halves_per_tile, ring, 0) == 0
+        assert rules.ring(tiles * halves_per_tile, ring, 1) == min(ring, tiles * halves_per_tile)     # the control
 
 
 def tiles(m, n, cg):

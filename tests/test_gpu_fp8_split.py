@@ -34,3 +34,27 @@ def test_chains_of_split_products(dtype):
     for i, y in enumerate(want):
         for o in outs[i]:
             assert torch.equal(o, y), SHAPES[i]
+
+
+def test_chains_of_products_on_cta_pairs():
+    """One tile a pair and many, queued behind one another in turn."""
+    from flashbfp_b200 import fp8
+    shapes = [(257, 1100, 900), (512, 768, 2048), (1024, 2048, 1280), (2100, 1240, 700), (2048, 4096, 512),
+              (3000, 5000, 256)]
+    ops, want, outs = [], [], []
+    for m, n, k in shapes:
+        x, xd = integer_rows(m, k, m + n)
+        w, wd = integer_rows(n, k, n + k)
+        ops.append((x, w))
+        want.append((xd @ wd.t()).float())
+        outs.append([torch.zeros(m, n, device=DEV) for _ in range(2)])
+    torch.cuda.synchronize()
+    for rep in range(10):
+        for i in range(len(shapes)):
+            fp8.fp8_linear(*ops[i], out=outs[i][rep % 2])
+            j = (i * 5 + rep) % len(shapes)
+            fp8.fp8_linear(*ops[j], out=outs[j][rep % 2])
+    fp8.check_device_errors(DEV)
+    for i, y in enumerate(want):
+        for o in outs[i]:
+            assert torch.equal(o, y), shapes[i]
