@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import threading
 from typing import Dict, NamedTuple, Optional
 
 import torch
@@ -64,21 +65,26 @@ def empty_rows(m: int, k: int, device) -> Fp8Rows:
 # per device: the word in which a kernel records a bounded wait that gave up (never reallocated,
 # so captured graphs may hold its address)
 _ERROR_WORDS: Dict[int, torch.Tensor] = {}
+_ERROR_WORDS_LOCK = threading.Lock()
 
 
 def _error_word(index: int) -> int:
-    """The address of a device's error word (asked for once per device)."""
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("the first fp8_linear on a device must run outside a CUDA graph capture")
-    w = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
-    torch.cuda.synchronize(index)                  # zero before any stream uses it
-    _ERROR_WORDS[index] = w
+    """The address of a device's error word (made at the first call)."""
+    with _ERROR_WORDS_LOCK:                        # synchronising lets other threads in: they wait here
+        w = _ERROR_WORDS.get(index)
+        if w is None:
+            with torch.cuda.device(index):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first fp8_linear on a device must run outside a CUDA graph capture")
+                w = torch.zeros(64, dtype=torch.int32, device=torch.device("cuda", index))
+                torch.cuda.synchronize(index)      # zero before any stream uses it
+            _ERROR_WORDS[index] = w
     return w.data_ptr()
 
 
 def check_device_errors(device=None) -> None:
     """Synchronise and raise if an ``fp8_linear`` on `device` gave up a bounded device-side wait."""
-    for idx, w in _ERROR_WORDS.items():
+    for idx, w in list(_ERROR_WORDS.items()):
         if device is not None and torch.device(device).index not in (None, idx):
             continue
         with torch.cuda.device(idx):
