@@ -25,6 +25,17 @@ static inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// The encoder's call. Where it is a host thread's first CUDA call the driver has no current context
+// yet: selecting the device again makes the runtime's current on the thread.
+template <typename... Args>
+static inline CUresult encode_tiled(EncodeTiledFn fn, Args... args) {
+  CUresult r = fn(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = fn(args...);
+  return r;
+}
+
 // 2-D tensor map over a row-major [rows][inner] array with the given row pitch (bytes);
 // out-of-range elements of a box read as zero.
 static inline int encode_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner,
@@ -37,8 +48,8 @@ static inline int encode_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* 
   const cuuint64_t strides[1] = {row_bytes};
   const cuuint32_t box[2] = {box_inner, box_rows};
   const cuuint32_t es[2] = {1, 1};
-  CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, es,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swz, prom, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, m, dt, 2u, const_cast<void*>(base), dims, strides, box, es,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swz, prom, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(FBFP_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return FBFP_OK;
 }
