@@ -329,4 +329,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp8_bind", "checks and calls of f
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fp8_bind(void) { return PyModule_Create(&module); }
+// `built_for` names the torch and the Python whose headers this was compiled with.
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fp8_bind(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", FBFP_BUILT_FOR) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -103,8 +103,14 @@ def _module():
         if not os.path.exists(build.BIND):
             raise _lib.FlashBFPError(f"{build.BIND} is missing: build it with `python -m flashbfp_b200.build`")
         spec = importlib.util.spec_from_file_location("flashbfp_b200._fp8_bind", build.BIND)
-        m = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(m)
+        again = "build it again with `python -m flashbfp_b200.build`"
+        try:
+            m = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(m)
+        except ImportError as e:                   # another torch's symbols
+            raise _lib.FlashBFPError(f"{build.BIND} does not load ({e}): {again}") from e
+        if m.built_for != build.bind_for():
+            raise _lib.FlashBFPError(f"{build.BIND} is built for {m.built_for}, this is {build.bind_for()}: {again}")
         m.setup(Fp8Rows, _error_word)
         _bind = m
     return _bind
