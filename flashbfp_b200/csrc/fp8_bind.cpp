@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -139,6 +140,23 @@ void call(int index, const char* what, F f) {
   refuse(type, "%s: %s: %s", what, fbfp_status_string(status), fbfp_last_error());
 }
 
+// A tensor that a call writes in place. There are no gradients, so one that requires a gradient is
+// refused while they are recorded; afterwards its autograd version goes up, so that a backward pass
+// which needs the old values says so.
+void check_written(const at::Tensor& t, const char* what) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse(PyExc_RuntimeError,
+           "%s is written in place and requires a gradient, which the 8-bit operators do not give: detach it or "
+           "call under torch.no_grad()", what);
+}
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const Rows& r) {
+  written(*r.v);
+  written(*r.s);
+}
+
 // A reference that is given up unless it is taken.
 struct Ref {
   PyObject* o;
@@ -187,6 +205,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return fbfp_fp8_quantize(x.t->const_data_ptr(), x.code, x.m, x.k, x.ld, r.v->data_ptr(), r.ld,
                                  r.s->data_ptr(), st);
       });
+    written(r);
     return out.take();
   });
 }
@@ -205,6 +224,7 @@ PyObject* geglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return fbfp_fp8_geglu(x.t->const_data_ptr(), x.code, x.m, x.k / 2, x.ld, r.v->data_ptr(), r.ld,
                               r.s->data_ptr(), st);
       });
+    written(r);
     return out.take();
   });
 }
@@ -236,6 +256,7 @@ PyObject* rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse(PyExc_ValueError, "residual must be %s of shape (%lld, %lld) on cuda:%d",
                c10::toString(x.t->scalar_type()), (long long)x.m, (long long)x.k, x.index);
       if (r.ld < r.k) refuse(PyExc_ValueError, "residual rows overlap: each is updated in place");
+      check_written(*r.t, "residual");
       resid = r.t->data_ptr();
       ldr = r.ld;
       if (a[4] != Py_None) post = norm_weight(a[4], "post_weight", x);
@@ -249,6 +270,8 @@ PyObject* rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return fbfp_fp8_rmsnorm(x.t->const_data_ptr(), x.code, x.m, x.k, x.ld, w, post, resid, ldr, (float)eps,
                                 q.v->data_ptr(), q.ld, q.s->data_ptr(), st);
       });
+    written(q);
+    if (resid) written(THPVariable_Unpack(a[3]));
     return out.take();
   });
 }
@@ -300,6 +323,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse(PyExc_ValueError, "out must have shape (%lld, %lld) on cuda:%d%s%s", (long long)x.m, (long long)w.m,
              index, typed ? " and dtype " : "", typed ? c10::toString(want) : "");
     if (y.ld < y.k) refuse(PyExc_ValueError, "out's rows overlap");
+    check_written(*y.t, "out");
     if (x.m && w.m) {
       void* const word = error_word(index);
       call(index, "fbfp_fp8_linear", [&](void* st) {
@@ -307,6 +331,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                w.m, w.ld, w.s->const_data_ptr(), bias, bias_code, y.t->data_ptr(), y.code, y.ld,
                                word, st);
       });
+      written(*y.t);
     }
     return out.take();
   });

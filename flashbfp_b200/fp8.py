@@ -14,6 +14,11 @@ the smallest power of two (at least 2^-127) that brings its block into e4m3's ra
 block with an infinity or a NaN becomes NaN, scale and values, and so does the output row (or
 column) of a product that reads it. Everything runs on the GPU; the results of a call follow its
 inputs' stream order on the current stream.
+
+Forward only: results carry no gradient, whatever their inputs. What a call writes in place (the
+residual, ``out``) must not require one while gradients are recorded, and counts as modified for
+autograd. ``out`` must not overlap the inputs, nor the residual the other inputs, unless x is the
+residual itself.
 """
 from __future__ import annotations
 
