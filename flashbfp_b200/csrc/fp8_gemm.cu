@@ -55,6 +55,19 @@ __device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, const A
   return false;
 }
 
+// After a wait gave up: what is in flight lands before its memory is given up. Each wait has a bound
+// of its own again, some 0.3 s times `bounds`.
+__device__ __forceinline__ bool settle(uint64_t* bar, uint32_t parity, uint32_t bounds = 1) {
+  for (uint32_t it = 0; it < (bounds << 14); ++it)
+    if (mbar_try_wait_cluster(bar, parity, 20000u)) return true;
+  return false;
+}
+// The last loads into the stages, of `issued`.
+__device__ __forceinline__ void settle_loads(uint64_t* full, int64_t issued, int stages) {
+  for (int64_t j = issued > stages ? issued - stages : 0; j < issued; ++j)
+    settle(&full[j % stages], (uint32_t)(j / stages) & 1);
+}
+
 __device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
   const __nv_bfloat162 h = __float22bfloat162_rn(make_float2(a, b));
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -103,12 +116,18 @@ struct Few {
   static constexpr int kThreads = 192;
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
   static constexpr uint32_t kTmemCols = 128;
-  static constexpr int kBars = (2 * kMaxStages + 1) * 8 + 16;
+  static constexpr int kBars = (2 * kMaxStages + 2) * 8 + 16;
   static constexpr int kFixed = kBars + 1024;           // stages start on 1 KB
   static_assert(kStage % 1024 == 0, "swizzled stages start on 1 KB");
   static_assert(kSums <= 3 * kStage, "unsplit, the sums take the place of the stages (at least 3)");
   static_assert(kAccCols + 8 * kMaxStages <= (int)kTmemCols, "tensor memory budget");
 };
+
+// After a wait gave up, once every role has ended. (Out of line: inlined, it costs a one-token call 0.1 us.)
+__device__ __noinline__ void settle_few(uint64_t* full, uint64_t* done, int64_t issued, int stages) {
+  settle_loads(full, issued, stages);
+  settle(done, 0);                                       // the MMAs
+}
 
 template <int BN, typename T>
 __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Args a,
@@ -125,7 +144,8 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * C::kStage + (splits > 1 ? C::kSums : 0));
   uint64_t* empty = full + kMaxStages;
   uint64_t* done = empty + kMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int64_t* issued_loads = reinterpret_cast<int64_t*>(done + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(issued_loads + 1);
   const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -159,23 +179,19 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 
   if (warp == 0) {
     if (elect_one_sync()) {
-      int s = 0, issued = 0;
+      int s = 0, kb = kb0;
       uint32_t ph = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = fp8_wait<false>(&empty[s], ph ^ 1, A, 20))) break;
+      for (; kb < kb1; ++kb) {
+        if (!fp8_wait<false>(&empty[s], ph ^ 1, A, 20)) break;
         uint8_t* st = smem + (size_t)s * C::kStage;
         mbar_arrive_expect_tx(&full[s], C::kStage);
         tma_2d_g2s(st, &M.w, kb * 128, (int)n0, &full[s]);
         tma_2d_g2s(st + C::kA, &M.x, kb * 128, 0, &full[s]);
         bulk_g2s(st + C::kA + C::kB, a.w_scales + (n0 / 128 * a.kgroups + kb / 4) * C::kSf, C::kSf, &full[s]);
         bulk_g2s(st + C::kA + C::kB + C::kSf, a.x_scales + (int64_t)(kb / 4) * C::kSf, C::kSf, &full[s]);
-        ++issued;
         if (++s == stages) { s = 0; ph ^= 1; }
       }
-      if (!ok)                                           // copies in flight land before the CTA exits
-        for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
-          mbar_wait(&full[j % stages], (uint32_t)(j / stages) & 1, 1u << 20);
+      *issued_loads = kb - kb0;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -184,9 +200,8 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
       const uint32_t sbase = smem_u32(smem);
       int s = 0;
       uint32_t ph = 0, acc = 0;
-      bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = fp8_wait<false>(&full[s], ph, A, 21))) break;
+        if (!fp8_wait<false>(&full[s], ph, A, 21)) break;
         tc_fence_after();
         const uint32_t st = sbase + s * C::kStage;
         const uint32_t sfa = tmem + C::kAccCols + s * 8, sfb = sfa + 4;
@@ -203,7 +218,6 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
         if (++s == stages) { s = 0; ph ^= 1; }
       }
       mma_commit(done);
-      if (!ok) mbar_wait(done, 0, 1u << 22);             // MMAs in flight end before their memory goes
     }
     __syncwarp();
   }
@@ -258,6 +272,10 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
     store4(y + t * a.ldy, nf, p, vec);
   }
   if (warp == 2) {
+    if (*A.flag) {
+      settle_few(full, done, *issued_loads, stages);
+      __syncwarp();
+    }
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
   }
@@ -309,7 +327,7 @@ struct Many {
   static constexpr int kTurns = kEpiWarps * kTurn;
   static constexpr int kBlock = 32 * 32 * 4;                     // [feature / 4][token][4]
   static constexpr int kSums = 14 * kBlock;                      // 16 / S blocks from S - 1 CTAs, S 2, 4 or 8
-  static constexpr int kBars = (2 * kMaxStages + 2 * kRing + 2) * 8 + 16;
+  static constexpr int kBars = (2 * kMaxStages + 2 * kRing + 6) * 8 + 16;
   static constexpr int kFixed = kBars + 1024;                    // stages start on 1 KB
   static_assert(BN % 128 == 0 && kStage % 1024 == 0 && kTurn % 16 == 0 && kBlock % 16 == 0, "alignment");
   static_assert(kSfCol0 + kSfSlots * kSfCols <= kTmemCols, "tensor memory budget");
@@ -405,6 +423,40 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const void* map, int x, 
   else tma_2d_g2s_pair(dst, map, x, y, bar);
 }
 
+// After a wait gave up, one thread of the CTA, once every role has ended: the loads, the MMAs and the
+// other CTAs' sums in flight are waited for. A pair's loads complete on its first CTA's barriers,
+// which expect both CTAs' bytes from the first CTA's own load on: the second says how many loads it
+// issued, the first makes up the difference where one got further (loads_owed) and lets the second
+// go in the end. No barrier of the cluster: every wait is bounded.
+template <int CG, int BN>
+__device__ __noinline__ void settle_many(uint64_t* full, uint64_t* rest, volatile int64_t* issued, int stages, int kb0,
+                                         int kb1, int64_t tiles) {
+  using C = Many<CG, BN>;
+  uint64_t *told = rest + 1, *landed = rest + 2, *acc_full = full + 2 * kMaxStages;
+  const uint32_t rank = cluster_rank(), pr = rank % CG;
+  settle(landed, 0);
+  if (pr == 1) {
+    st_shared_cluster(map_shared(smem_u32((const void*)(issued + 1)), rank - 1), issued[0]);
+    mbar_arrive_cluster(map_shared(smem_u32(told), rank - 1));
+    settle(rest, 0, kMaxStages + 4);
+    return;
+  }
+  const int64_t mine = issued[0], other = CG == 2 && settle(told, 0, 2) ? issued[1] : mine;
+  const int64_t most = mine > other ? mine : other;
+  for (int64_t j = mine < other ? mine : other; j < most; ++j) {
+    const int kb = kb0 + (int)(j % (kb1 - kb0));
+    const uint32_t bytes = C::kA + C::kB + ((kb & 3) == 0 || kb == kb0 ? C::kSf : 0);   // of one CTA
+    if (loads_owed(j, mine, other) > 0) mbar_arrive_expect_tx(&full[j % stages], bytes);
+    else mbar_complete_tx(&full[j % stages], bytes);
+  }
+  settle_loads(full, most, stages);
+  // the MMAs of whole tiles (a role that gave up has waited for its own)
+  const int64_t halves = tiles * C::kHalves;
+  for (int64_t h = halves > C::kRing ? halves - C::kRing : 0; h < halves; ++h)
+    settle(&acc_full[h % C::kRing], (uint32_t)(h / C::kRing) & 1);
+  if constexpr (CG == 2) mbar_arrive_cluster(map_shared(smem_u32(rest), rank + 1));
+}
+
 template <int CG, int BN, typename T>
 __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(const Fp8Args a, const int splits,
                                                                               const __grid_constant__ Fp8Maps M) {
@@ -421,8 +473,10 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   uint64_t* acc_full = empty + kMaxStages;
   uint64_t* acc_empty = acc_full + C::kRing;                        // used in a pair's CTA 0
   uint64_t* tail = acc_empty + C::kRing;
-  uint64_t* landed = tail + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 1);
+  uint64_t* rest = tail + 1;
+  uint64_t* landed = rest + 2;                                       // told between them (settle_many)
+  volatile int64_t* issued_loads = reinterpret_cast<volatile int64_t*>(landed + 1);   // this CTA's, a pair's other's
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(landed + 3);
   const Abort A{reinterpret_cast<volatile int*>(tmem_slot + 1), a.err};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank(), pr = rank % CG, lead = rank - pr;
@@ -441,13 +495,17 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < C::kRing; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], CG * C::kEpiWarps); }
     mbar_init(tail, 1);
+    mbar_init(rest, 1);
+    mbar_init(rest + 1, 1);
     mbar_init(landed, 1);
     *A.flag = 0;
     fence_mbar_init();
-    if (splits > 1) {
+    if (splits == 1) {
+      mbar_arrive(landed);
+    } else {
       const int live = owned_blocks(sp, splits, (int64_t)(team % a.n_tt) * (128 * CG) + 128 * pr,
                                     (int64_t)(team / a.n_tt) * BN, a.m, a.n);
-      if (live) mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * 32 * 4));
+      mbar_arrive_expect_tx(landed, (uint32_t)(live * (splits - 1) * 32 * 32 * 4));
     }
   }
   if (warp == 2) {
@@ -498,12 +556,8 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
           if (++s == stages) { s = 0; ph ^= 1; }
         }
       }
-      if (!ok) {                                         // copies in flight land before the CTA exits
-        if (pr == 0)
-          for (int64_t j = issued > stages ? issued - stages : 0; j < issued; ++j)
-            mbar_wait(&full[j % stages], (uint32_t)(j / stages) & 1, 1u << 16);
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-      }
+      issued_loads[0] = issued;
+      __threadfence_block();                             // the closing barrier may order nothing
     }
     __syncwarp();
   } else if (warp == 1 && pr == 0) {
@@ -661,6 +715,11 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   }
   __syncwarp();
   if (CG == 1 && splits > 1 && warp < 4) cluster_wait();
+  if (*A.flag) {                                         // a wait gave up: the other CTA of a pair is told
+    if constexpr (CG == 2) st_shared_cluster(map_shared(smem_u32((const void*)A.flag), rank ^ 1), 1u);
+    fence_cluster();                                     // the closing barrier orders nothing by itself
+  }
+  __syncwarp();
   tc_fence_before();
   if (CG == 2 || splits > 1) {                           // no CTA leaves while another may still reach it
     cluster_arrive_relaxed();
@@ -669,6 +728,11 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
     __syncthreads();
   }
   if (warp == 2) {
+    if (*A.flag) {                                       // the same in a pair's CTAs from here on
+      if (lane == 0)
+        settle_many<CG, BN>(full, rest, issued_loads, stages, kb0, kb1, (int64_t)((a.tiles - team + teams - 1) / teams));
+      __syncwarp();
+    }
     tc_fence_after();
     if constexpr (CG == 1) tmem_dealloc(tmem, C::kTmemCols);
     else tmem_dealloc_pair(tmem, C::kTmemCols);

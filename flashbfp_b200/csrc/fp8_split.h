@@ -41,4 +41,12 @@ FBFP_HD int owned_blocks(int sp, int splits, int64_t tok, int64_t f, int64_t m, 
 // another CTA, which may have left.
 FBFP_HD bool arrival_awaited(int64_t h, int ring, int64_t halves) { return h + ring < halves; }
 
+// Loads of a pair complete on its first CTA's barriers: that CTA's own load arrives there and expects
+// both CTAs' bytes. After a failure, `mine` loads of the first CTA and `other` of the second having
+// been issued, its barrier of load j (j at least the smaller of the two) lacks: an arrival that
+// expects the second CTA's bytes (1), or the bytes that the second CTA never sends (-1).
+FBFP_HD int loads_owed(int64_t j, int64_t mine, int64_t other) {
+  return j >= mine && j < other ? 1 : j < mine && j >= other ? -1 : 0;
+}
+
 }  // namespace fbfp

@@ -60,6 +60,23 @@ extern "C" int64_t ring(int64_t halves, int ring, int all) {
   for (int i = 0; i < ring; ++i) rest += arrived[i] - waited[i];
   return rest;
 }
+// A pair's stages after a failure: each stage's barrier counts one arrival and the bytes of both CTAs.
+// `mine` and `other` loads were issued; fix: whether the first CTA makes up the difference. Returns how
+// many of the last `stages` loads' phases never complete, whatever the order of the copies.
+extern "C" int pair_loads(int64_t mine, int64_t other, int stages, int fix) {
+  const int64_t most = mine > other ? mine : other;
+  int open = 0;
+  for (int64_t j = most > stages ? most - stages : 0; j < most; ++j) {
+    const int64_t bytes = 1000 + j % 5;                     // of one CTA; they differ from load to load
+    int64_t pending = 1, tx = 0;
+    if (j < mine) { --pending; tx += 2 * bytes; tx -= bytes; }
+    if (j < other) tx -= bytes;
+    if (fix && loads_owed(j, mine, other) > 0) { --pending; tx += bytes; }
+    if (fix && loads_owed(j, mine, other) < 0) tx -= bytes;
+    open += pending != 0 || tx != 0;
+  }
+  return open;
+}
 """
 
 
@@ -71,6 +88,7 @@ def rules(tmp_path_factory):
                     str(d / "h.so")], check=True)
     lib = ctypes.CDLL(str(d / "h.so"))
     lib.tile.argtypes = [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 4 + [ctypes.c_int]
+    lib.pair_loads.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int]
     lib.ring.argtypes, lib.ring.restype = [ctypes.c_int64, ctypes.c_int, ctypes.c_int], ctypes.c_int64
     return lib
 
@@ -106,3 +124,12 @@ def test_blocks_without_features_would_be_sent_to_nobody(tile):
     for m, n, cg, splits in ((90, 200, 1, 8), (100, 2000, 1, 4), (128, 4160, 1, 4), (333, 1999, 2, 4)):
         assert any(tile(cg, splits, t, f, m, n, 0) & 4 for t, f in tiles(m, n, cg)), (m, n)
         assert all(tile(cg, splits, t, f, m, n, 1) == 0 for t, f in tiles(m, n, cg))
+
+
+@pytest.mark.parametrize("stages", [4, 6, 8])
+def test_copies_of_a_pair_that_gave_up_all_land(rules, stages):
+    """Whichever CTA of a pair got further (by at most the ring), every load's phase completes."""
+    for mine in range(0, 30):
+        for other in range(max(0, mine - stages), mine + stages + 1):
+            assert rules.pair_loads(mine, other, stages, 1) == 0, (mine, other)
+            assert (rules.pair_loads(mine, other, stages, 0) > 0) == (mine != other)       # the control
