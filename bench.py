@@ -678,8 +678,15 @@ def _decoder(layers, device, reducer, rank, world, batch, prompt, gen):
                         max_prefill=prompt, reducer=reducer, vocab_offset=v0, batch=batch)
 
 
+def _weight_bytes(w):
+    """Bytes of one linear's weight: a PackedWeight, a bf16 tensor, or 8-bit rows with their scales."""
+    if isinstance(w, tuple):
+        return sum(t.numel() * t.element_size() for t in w)
+    return w.numel() * w.element_size() if isinstance(w, torch.Tensor) else w.packed_bytes()
+
+
 def run_model_decode(layers, device, reducer=None, rank=0, world=1, batch=1, prompt=128, gen=256,
-                     dense=False):
+                     linears="OABF linears"):
     """Whole decode tokens of the random-init 12B-class Gemma-3: every sequence's ``prompt``
     tokens as one prefill chunk (timed on its own), then ``gen`` greedy tokens for all ``batch``
     sequences together, timed as back-to-back replays of the one-step CUDA graph (max over
@@ -713,10 +720,7 @@ def run_model_decode(layers, device, reducer=None, rank=0, world=1, batch=1, pro
     if world > 1:
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
     ms, prefill_ms = float(t[0]), float(t[1])
-    if dense:
-        lin = sum(2 * Ly[kk].numel() for Ly in layers for kk in KINDS)      # bf16 tensors
-    else:
-        lin = sum(Ly[kk].packed_bytes() for Ly in layers for kk in KINDS)
+    lin = sum(_weight_bytes(Ly[kk]) for Ly in layers for kk in KINDS)
     H = 3840
     per_rank = lin + 2 * dec.vocab_l * H + 2 * batch * H      # linears, lm_head rows, embedding rows
     dec.release()
@@ -726,7 +730,7 @@ def run_model_decode(layers, device, reducer=None, rank=0, world=1, batch=1, pro
                          "layers of 1024 per global one), 16 q / 8 kv heads x 256, vocab 262144, "
                          f"{prompt} prompt tokens then {gen} greedy tokens, batch {batch}, "
                          f"{'tp%d' % world if world > 1 else '1 GPU'}"
-                         + (", uncompressed bf16 linears (cuBLAS)" if dense else ", OABF linears")),
+                         + ", " + linears),
             "batch": batch, "ms_per_step": round(ms, 4),
             "tokens_per_s": round(batch * 1000.0 / ms, 1),
             "prefill_ms": round(prefill_ms, 3),
@@ -739,7 +743,8 @@ def run_model_decode(layers, device, reducer=None, rank=0, world=1, batch=1, pro
 
 def run_models(layers, device, rank, world):
     """Whole-model decode at batch 1 and 8 (tensor-parallel over the ranks), and at one GPU the
-    same decoder on uncompressed bf16 linears, with the speed-up over it."""
+    same decoder on uncompressed bf16 linears, with the speed-up over it, and on block-scaled 8-bit
+    linears made from those."""
     out = {}
     dred = None
     if world > 1:
@@ -756,17 +761,24 @@ def run_models(layers, device, rank, world):
     if world == 1:
         try:
             dl = dense_layers(len(layers), device)
-            out["bf16_batch1"] = run_model_decode(dl, device, dense=True)
-            del dl
-            torch.cuda.empty_cache()
+            out["bf16_batch1"] = run_model_decode(dl, device, linears="uncompressed bf16 linears (cuBLAS)")
             if "tokens_per_s" in out.get("batch1", {}):
                 r = out["batch1"]["tokens_per_s"] / out["bf16_batch1"]["tokens_per_s"]
                 out["speedup_vs_bf16"] = round(r, 3)
                 out["speedup_note"] = ("whole-token tokens/s of the OABF decoder over the same decoder on "
                                        "uncompressed bf16 linears (cuBLAS), both one CUDA graph per token; "
                                        "target 3x, weight-byte ceiling of the linears 2.55x")
+            from flashbfp_b200 import fp8
+            for Ly in dl:                               # in place of the bf16 weights, layer by layer
+                for kk in KINDS:
+                    Ly[kk] = fp8.quantize_fp8(Ly[kk])
+            for key, batch in (("fp8_batch1", 1), ("fp8_batch8", 8)):
+                out[key] = run_model_decode(dl, device, batch=batch, linears="block-scaled 8-bit linears")
+            del dl
+            torch.cuda.empty_cache()
         except Exception as e:
-            out["bf16_batch1"] = {"error": f"{type(e).__name__}: {e}"[:300]}
+            key = "fp8_batch1" if "bf16_batch1" in out else "bf16_batch1"
+            out[key] = {"error": f"{type(e).__name__}: {e}"[:300]}
     if dred is not None:
         torch.cuda.synchronize(device)
         dred.close()
