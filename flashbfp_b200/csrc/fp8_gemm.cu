@@ -105,9 +105,9 @@ __device__ __forceinline__ void store4(T* p, int n, const float4& v, bool vec) {
 // per lane) into shared memory. With a split each CTA owns some of the tile's tokens: the others store their fp32
 // partial sums straight into its shared memory, and it adds them in rank order (a fixed order: same
 // bits every time). Bound by the weights' bytes, and by some 3.4 us of launch, first bytes and
-// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.3 us
-// (5.6 TB/s), 64 x 30720 x 3840 23.2 us (5.3 TB/s), 64 x 8192 x 28672 43.0 us (5.6 TB/s), 1 x 8192
-// x 3840 8.1 us, 1 x 3840 x 4096 6.0 us.
+// drain. Measured, in a graph over more weights than L2 holds: 16 x 30720 x 3840 21.9 us
+// (5.5 TB/s), 64 x 30720 x 3840 24.2 us (5.1 TB/s), 64 x 8192 x 28672 41.9 us (5.6 TB/s), 1 x 8192
+// x 3840 8.4 us, 1 x 3840 x 4096 6.1 us.
 template <int BN>
 struct Few {
   static constexpr int kA = 128 * 128, kB = BN * 128, kSf = 512;
@@ -288,9 +288,9 @@ __global__ void __launch_bounds__(Few<BN>::kThreads) fp8_few_kernel(const Fp8Arg
 // 128 + BN / 2 rows of 128 bytes per K block for 128 x BN x 128 multiply-adds. Persistent, or with a
 // split: the CTAs (pairs) of a cluster share a tile and split its K blocks.
 //
-// Measured, in a graph over more weights than L2 holds: 2048 x 30720 x 3840 174 us in bursts
-// (2.77 PFLOP/s; 202 us at the power limit), 4096 x 8192 x 28672 664 us (2.90 PFLOP/s), 512 x 8192
-// x 3840 17.4 us, 128 x 30720 x 3840 25.7 us, 128 x 3840 x 15360 16.4 us (3.8 TB/s). Bound by the
+// Measured, in a graph over more weights than L2 holds: 2048 x 30720 x 3840 169 to 176
+// us in bursts (2.75 to 2.86 PFLOP/s; 202 us at the power limit), 4096 x 8192 x 28672 664 us (2.90
+// PFLOP/s), 512 x 8192 x 3840 16.4 us, 128 x 30720 x 3840 26.4 us, 128 x 3840 x 15360 16.5 us (3.8 TB/s). Bound by the
 // operand rows an SM can take in, about 60 bytes a cycle: 585 cycles for the 512 of a pair's
 // 256-wide K block.
 //
@@ -721,7 +721,9 @@ __global__ void __launch_bounds__((Many<CG, BN>::kThreads), 1) fp8_many_kernel(c
   }
   __syncwarp();
   tc_fence_before();
-  if (CG == 2 || splits > 1) {                           // no CTA leaves while another may still reach it
+  // every role of the cluster has ended; no memory is ordered by this: what CTAs send each other is
+  // waited for on barriers of its own
+  if (CG == 2 || splits > 1) {
     cluster_arrive_relaxed();
     cluster_wait();
   } else {
@@ -862,8 +864,12 @@ int encode_scales(CUtensorMap* map, const void* base, int64_t tiles) {
 // features), 500 and 580 (a pair). Measured against the alternatives: 512 tokens x 8192 x 3840
 // 16.3 us on 256-wide pair tiles and 18.4 on 128-wide ones, 512 x 3840 x 15360 the other way
 // around (40.2 and 31.0 us: 30 and 60 tiles for 74 pairs), 128 x 3840 x 15360 16.1 us split four
-// ways, 21.7 two ways, 256 x 3840 x 4096 10.6 split and 11.0 not. Clusters of 8 lose: 100 x
-// 2000 x 16000 14.1 us split four ways, 21.2 eight ways.
+// ways, 21.7 two ways, 256 x 3840 x 4096 10.6 split and 11.0 not. Clusters of 8 are for products
+// of at most 15 tiles, all that run at a time: 128 x 1920 x 15360 12.2 us, 14.3 split four ways, 100 x
+// 1000 x 16000 11.1 and 13.6, 100 x 512 x 8192 7.7 and 9.0; at 4096 deep they are even (0.93 to 1.01
+// of the time in 22 shapes of up to 8 tiles) and lose where 12 to 15 tiles leave few SMs idle
+// anyway (128 x 1920 x 4096 8.4 and 7.7). One tile more takes a second round: 100 x 2000 x 16000
+// (16 tiles) 14.5 us split four ways, 21.2 eight ways.
 struct ManyPlan {
   int cg, bn, splits, teams;
   int64_t token_tiles, tiles;

@@ -13,10 +13,10 @@
 // 128-row x 4-block tiles that the tensor core's scale copies take as they are. All of it is
 // bound by memory: every input is read once and every output written once. Measured (in a graph
 // over more data than L2 holds): quantise 3840 x 15360 fp32 44.4 us (6.65 TB/s), 8192 x 8192 bf16
-// 33.5 us (6.0 TB/s); GeGLU 2048 x 15360 bf16 27.3 us (5.8 TB/s), 2047 x 15001, whose rows start
-// anywhere, 35.7 us; residual addition and norm of 8192 x 8192 bf16 81.5 us (5.8 TB/s); post-norm,
-// addition and norm of 2048 x 3840 bf16 13.2 us (4.2 TB/s: 4.6 rounds of rows), 2048 x 3841 25.4 us,
-// one row 2.5 us.
+// 33.5 us (6.0 TB/s); GeGLU 2048 x 15360 bf16 26.7 us (5.9 TB/s), fp32 45.9 us (6.2 TB/s), 2047 x
+// 15001, whose rows start anywhere, 35.1 and 47.7 us; residual addition and norm of 8192 x 8192
+// bf16 81.5 us (5.8 TB/s); post-norm, addition and norm of 2048 x 3840 bf16 13.2 us (4.2 TB/s: a team
+// of warps is in one row at a time and stopped twice in it), 2048 x 3841 25.4 us, one row 2.5 us.
 #include <cuda_fp8.h>
 
 #include "common.cuh"

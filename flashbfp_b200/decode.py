@@ -18,9 +18,10 @@ prefill GEMM once M > 16), and logits for the last row only.
 model).
 
 With ``from_hf(..., weights="fp8")`` (an uncompressed model) or layers that hold ``fp8.Fp8Rows`` the
-linears run as block-scaled 8-bit products (``fp8.py``): the norms between a layer's halves, the
-GeGLU activation and the attention output leave as e4m3 rows with their scales, which the next
-linear multiplies as they are. Activations are rounded to e4m3 there (2^-4 relative at most);
+linears run as block-scaled 8-bit products (``fp8.py``): the norms between a layer's halves and the
+GeGLU activation leave as e4m3 rows with their scales, which the next linear multiplies as they
+are; the attention output is rounded to bf16 and quantised by a launch of its own. Activations
+are rounded to e4m3 there (2^-4 relative at most);
 the residual stream, attention, norms and lm_head keep the precision they have otherwise.
 """
 from __future__ import annotations

@@ -51,7 +51,8 @@ class Fp8Rows(NamedTuple):
         return torch.where(codes == 255, torch.full_like(s, float("nan")), s)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The rows the operand stands for: values * scale (exact in fp32 and in bf16)."""
+        """The rows the operand stands for: values * scale, rounded to `dtype` (exact in fp32, and in
+        bf16 where the scale is at least 2^-124)."""
         k = self.values.shape[1]
         s = self.scale_matrix().repeat_interleave(128, dim=1)[:, :k]
         return (self.values.float() * s).to(dtype)
