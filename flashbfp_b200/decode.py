@@ -189,6 +189,7 @@ class GemmaDecoder:
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(dev)
+        self.stream.wait_stream(torch.cuda.current_stream(dev))     # weights and buffers made above, and before
 
     # -- construction from a Hugging Face Gemma-3 model after compress_gemma_model -----------
     @classmethod
@@ -470,6 +471,7 @@ class GemmaDecoder:
         return out[0] if single else out
 
     def release(self) -> None:
+        self.stream.synchronize()                  # its buffers may go to other streams' tensors next
         if self.graph is not None:
             self.graph.reset()
             self.graph = None
