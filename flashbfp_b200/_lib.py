@@ -86,6 +86,16 @@ _PROTOS = {
     "fbfp_fp8_geglu": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
     "fbfp_fp8_linear": (_c_int, [_vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _vp,
                                  _c_int, _c_i64, _vp, _vp]),
+    "fbfp_kv4_write": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "fbfp_kv4_read": (_c_int, [_vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp, _vp]),
+    "fbfp_kv4_append": (_c_int, [_vp, _vp, _c_i64, _c_i64, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                 _vp]),
+    "fbfp_kv4_attention_workspace_bytes": (_c_i64, [_vp, _c_i64, _c_i64]),
+    "fbfp_kv4_attention": (_c_int, [_vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64,
+                                    ctypes.c_float, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
+    "fbfp_prompt_attention_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "fbfp_prompt_attention": (_c_int, [_vp, _vp, _vp, _c_int, *[_c_i64] * 12, _vp, _vp, _c_i64, ctypes.c_float, _vp,
+                                       _c_i64, _c_i64, _vp, _c_i64, _vp, _vp]),
     "fbfp_compress_scratch_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "fbfp_compress_threshold": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _vp]),
     "fbfp_compress_pack": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp,
@@ -93,6 +103,12 @@ _PROTOS = {
     "fbfp_compress_outliers": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp,
                                         _vp, _vp, _vp, _vp, _vp]),
 }
+
+class KV4CacheStruct(ctypes.Structure):
+    """fbfp_kv4_cache."""
+    _fields_ = [(n, _vp) for n in ("k_values", "k_scales", "v_values", "v_scales")] + \
+               [(n, _c_i64) for n in ("seqs", "kv_heads", "positions", "head_dim")]
+
 
 _lib = None
 

@@ -19,6 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libflashbfp.so")
 BIND = os.path.join(HERE, "_fp8_bind.so")
+BIND_SOURCES = [os.path.join(CSRC, f) for f in ("fp8_bind.cpp", "attn_bind.cpp")]
 BIND_STAMP = os.path.join(HERE, "_build", "fp8_bind.stamp")      # what BIND was built for
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -63,7 +64,7 @@ def _bind_missing() -> str | None:
 def _bind_stale() -> bool:
     if not os.path.exists(BIND) or not os.path.exists(BIND_STAMP):
         return True
-    deps = (os.path.join(CSRC, "fp8_bind.cpp"), os.path.join(os.path.dirname(HERE), "include", "flashbfp.h"))
+    deps = (*BIND_SOURCES, os.path.join(CSRC, "bind.h"), os.path.join(os.path.dirname(HERE), "include", "flashbfp.h"))
     if any(os.path.getmtime(p) > os.path.getmtime(BIND) for p in deps):
         return True
     with open(BIND_STAMP) as f:
@@ -73,12 +74,12 @@ def _bind_stale() -> bool:
 def _build_bind(force: bool, verbose: bool) -> None:
     """_fp8_bind.so: the Python entry points that check their tensors and call the library. The
     library alone (the C ABI) needs none of what this one needs, so a machine without it gets the
-    library and a note; flashbfp_b200.fp8 then says that the module is missing."""
+    library and a note; flashbfp_b200.fp8, .attention and .kv4 then say that the module is missing."""
     missing = _bind_missing()
     if not force and (missing is None or "torch" not in missing) and not _bind_stale():
         return
     if missing:
-        print(f"{os.path.basename(BIND)} (the 8-bit linears' Python entry points) is not built: {missing}",
+        print(f"{os.path.basename(BIND)} (the Python entry points of the 8-bit linears, the prompts' attention and the 4-bit cache) is not built: {missing}",
               file=sys.stderr, flush=True)
         return
     root = os.path.dirname(importlib.util.find_spec("torch").origin)
@@ -88,7 +89,7 @@ def _build_bind(force: bool, verbose: bool) -> None:
     tmp = BIND + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DFBFP_BUILT_FOR="{bind_for()}"',
-           *[a for i in inc for a in ("-isystem", i)], os.path.join(CSRC, "fp8_bind.cpp"), "-o", tmp, "-L" + HERE,
+           *[a for i in inc for a in ("-isystem", i)], *BIND_SOURCES, "-o", tmp, "-L" + HERE,
            "-l:libflashbfp.so", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
            "-lc10_cuda", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(root, "lib")]
     if verbose:

@@ -2,57 +2,14 @@
 // and the call into libflashbfp.so, without Python code in between. A small call's time is its host
 // side (the launch itself takes about 2 us): checked in Python and called through ctypes, a
 // quantisation took 6.9 us, of which this leaves the launch and less than a microsecond.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
+#include "bind.h"
 
-#include <ATen/ATen.h>
-#include <ATen/core/grad_mode.h>
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <cstdarg>
-#include <cstdio>
-#include <string>
-
-#include "../../include/flashbfp.h"
+extern PyMethodDef attn_methods[];       // attn_bind.cpp
 
 namespace {
 
 PyObject* g_rows_type = nullptr;        // Fp8Rows
-PyObject* g_error_word = nullptr;       // callable(device index) -> address, for a device's first product
-void* g_error_words[64] = {nullptr};
-bool g_has_word[64] = {false};
-
-struct Refusal {
-  PyObject* type;
-  std::string text;
-};
-[[noreturn]] __attribute__((format(printf, 2, 3))) void refuse(PyObject* type, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  throw Refusal{type, buf};
-}
-
-const at::Tensor& tensor(PyObject* o, const char* what) {
-  if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda())
-    refuse(PyExc_RuntimeError, "%s must be a CUDA tensor: FlashBFP-B200 runs only on the GPU (no CPU fallback)", what);
-  return THPVariable_Unpack(o);
-}
-
-int dtype_code(at::ScalarType t, const char* what) {
-  switch (t) {
-    case at::kFloat: return FBFP_F32;
-    case at::kBFloat16: return FBFP_BF16;
-    case at::kHalf: return FBFP_F16;
-    default: refuse(PyExc_NotImplementedError, "%s: unsupported dtype %s", what, c10::toString(t));
-  }
-}
+ErrorWords g_words;                     // where products record a wait that gave up
 
 struct Plain {                          // a 2-D tensor of plain values
   const at::Tensor* t;
@@ -122,75 +79,16 @@ PyObject* new_rows(int64_t m, int64_t k, int index) {
   return r;
 }
 
-// Runs f(stream) on device `index` and its current stream; raises what a status stands for.
-template <typename F>
-void call(int index, const char* what, F f) {
-  const int before = c10::cuda::current_device();
-  if (before != index) c10::cuda::set_device((c10::DeviceIndex)index);
-  void* const stream = (void*)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
-  int status;
-  Py_BEGIN_ALLOW_THREADS                // a launch waits while the device's queue is full
-  status = f(stream);
-  Py_END_ALLOW_THREADS
-  if (before != index) c10::cuda::set_device((c10::DeviceIndex)before);
-  if (status == FBFP_OK) return;
-  PyObject* type = status == FBFP_ERR_ARG || status == FBFP_ERR_ALIGN ? PyExc_ValueError
-                   : status == FBFP_ERR_UNSUPPORTED                   ? PyExc_NotImplementedError
-                                                                      : PyExc_RuntimeError;
-  refuse(type, "%s: %s: %s", what, fbfp_status_string(status), fbfp_last_error());
-}
-
-// A tensor that a call writes in place. There are no gradients, so one that requires a gradient is
-// refused while they are recorded; afterwards its autograd version goes up, so that a backward pass
-// which needs the old values says so.
-void check_written(const at::Tensor& t, const char* what) {
-  if (t.requires_grad() && at::GradMode::is_enabled())
-    refuse(PyExc_RuntimeError,
-           "%s is written in place and requires a gradient, which the 8-bit operators do not give: detach it or "
-           "call under torch.no_grad()", what);
-}
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 void written(const Rows& r) {
   written(*r.v);
   written(*r.s);
 }
 
-// A reference that is given up unless it is taken.
-struct Ref {
-  PyObject* o;
-  explicit Ref(PyObject* p) : o(p) {}
-  Ref(const Ref&) = delete;
-  ~Ref() { Py_XDECREF(o); }
-  PyObject* take() {
-    PyObject* p = o;
-    o = nullptr;
-    return p;
-  }
-};
 // `given`, or new rows where it is None (a new reference either way).
 PyObject* rows_or_new(PyObject* given, int64_t m, int64_t k, int index) {
   if (given == Py_None) return new_rows(m, k, index);
   Py_INCREF(given);
   return given;
-}
-
-template <typename F>
-PyObject* guarded(F f) {
-  HANDLE_TH_ERRORS
-  try {
-    return f();
-  } catch (const Refusal& r) {
-    PyErr_SetString(r.type, r.text.c_str());
-    return nullptr;
-  }
-  END_HANDLE_TH_ERRORS
-}
-
-bool arity(Py_ssize_t n, Py_ssize_t want) {
-  if (n != want) PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", want, n);
-  return n == want;
 }
 
 // quantize(x, out)
@@ -276,19 +174,6 @@ PyObject* rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-void* error_word(int index) {
-  if (index >= 64) refuse(PyExc_RuntimeError, "device index %d", index);
-  if (!g_has_word[index]) {
-    PyObject* r = PyObject_CallFunction(g_error_word, "i", index);
-    if (!r) throw python_error();
-    g_error_words[index] = PyLong_AsVoidPtr(r);
-    Py_DECREF(r);
-    if (PyErr_Occurred()) throw python_error();
-    g_has_word[index] = true;
-  }
-  return g_error_words[index];
-}
-
 // linear(x, w, bias, out_dtype, out)
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 5)) return nullptr;
@@ -325,7 +210,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (y.ld < y.k) refuse(PyExc_ValueError, "out's rows overlap");
     check_written(*y.t, "out");
     if (x.m && w.m) {
-      void* const word = error_word(index);
+      void* const word = g_words.of(index);
       call(index, "fbfp_fp8_linear", [&](void* st) {
         return fbfp_fp8_linear(x.v->const_data_ptr(), x.m, x.k, x.ld, x.s->const_data_ptr(), w.v->const_data_ptr(),
                                w.m, w.ld, w.s->const_data_ptr(), bias, bias_code, y.t->data_ptr(), y.code, y.ld,
@@ -342,14 +227,13 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 2)) return nullptr;
   for (int i = 0; i < 2; ++i) Py_INCREF(a[i]);
   g_rows_type = a[0];
-  g_error_word = a[1];
+  g_words.make = a[1];
   Py_RETURN_NONE;
 }
 
-#define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(quantize), FAST(geglu), FAST(rmsnorm), FAST(linear), FAST(setup),
                          {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp8_bind", "checks and calls of flashbfp_b200.fp8", -1, methods,
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp8_bind", "checks and calls of flashbfp_b200.fp8, .attention and .kv4", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -357,7 +241,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp8_bind", "checks and calls of f
 // `built_for` names the torch and the Python whose headers this was compiled with.
 extern "C" __attribute__((visibility("default"))) PyObject* PyInit__fp8_bind(void) {
   PyObject* m = PyModule_Create(&module);
-  if (m && PyModule_AddStringConstant(m, "built_for", FBFP_BUILT_FOR) < 0) {
+  if (m && (PyModule_AddStringConstant(m, "built_for", FBFP_BUILT_FOR) < 0 ||
+            PyModule_AddFunctions(m, attn_methods) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }

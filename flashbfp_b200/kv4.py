@@ -1,0 +1,94 @@
+"""The key/value cache in 4 bits: rows are quantised as they are written, read back as plain rows,
+or attended to as they are held.
+
+A cached head of D values is cut into groups of 32 (the last may be shorter). A group's scale is the
+bf16 nearest to max|x| / 7, and a value is held as x / scale rounded to a whole number in -7..7 (nearest
+even), plus 8, in 4 bits: 4.5 bits a value with the scales. A group with an infinity or a NaN reads
+back as NaN. Rows that enter are plain rows of any float type; what is already rounded stays what it
+is, so a row that is read back and written again is held as it was.
+
+``KV4Cache`` holds keys and values [sequences, kv_heads, positions, ...]. Positions are int32 tensors on
+the device, and so are lengths: calls read nothing back and can be captured. A position outside the
+cache is skipped and recorded (``check_device_errors`` raises it). Forward only, as ``attention``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import device_errors
+from .device_errors import check as check_device_errors
+
+__all__ = ["KV4Cache", "empty_cache", "kv4_write", "kv4_read", "kv4_attention", "check_device_errors"]
+
+
+class KV4Cache(NamedTuple):
+    k_values: torch.Tensor                # uint8 [sequences, kv_heads, positions, 16 ceil(D / 32)]
+    k_scales: torch.Tensor                # bfloat16 [sequences, kv_heads, positions, ceil(D / 32)]
+    v_values: torch.Tensor
+    v_scales: torch.Tensor
+    head_dim: int
+
+    @property
+    def positions(self) -> int:
+        return self.k_values.shape[2]
+
+    def sequence(self, b: int) -> "KV4Cache":
+        """Sequence b alone (a view)."""
+        return KV4Cache(*(t[b:b + 1] for t in self[:4]), self.head_dim)
+
+
+def empty_cache(sequences: int, kv_heads: int, positions: int, head_dim: int, device) -> KV4Cache:
+    """A cache of zeros; ``positions`` is rounded up to a multiple of 32."""
+    if head_dim < 8 or head_dim > 256 or head_dim % 8:
+        raise ValueError(f"head_dim {head_dim} is not a multiple of 8 up to 256")
+    if min(sequences, kv_heads, positions) < 1:
+        raise ValueError("a cache holds at least one sequence, head and position")
+    g = -(-head_dim // 32)
+    shape = (sequences, kv_heads, -(-positions // 32) * 32)
+    made = [torch.zeros(*shape, n, dtype=t, device=device)
+            for n, t in ((16 * g, torch.uint8), (g, torch.bfloat16)) * 2]
+    return KV4Cache(*made, head_dim)
+
+
+def _module():
+    return device_errors._bind or device_errors.module()
+
+
+def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor,
+              starts: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> None:
+    """Quantise rows k, v [T, kv_heads, D] (bf16, fp16 or fp32) into the cache: row r of sequence b goes
+    to position pos[b] + r - starts[b]. ``starts`` (int32 [sequences + 1]) packs the rows of several
+    sequences; without it there is one row per sequence. Rows from starts[-1] on are not written."""
+    _module().kv4_write(cache, k, v, pos, starts, err)
+
+
+def kv4_read(cache: KV4Cache, first: torch.Tensor, starts: torch.Tensor, rows: Optional[int] = None,
+             dtype: torch.dtype = torch.bfloat16, out: Optional[Sequence[torch.Tensor]] = None,
+             err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows k, v [rows, kv_heads, D] of ``dtype`` from the cache: row r of sequence b comes from position
+    first[b] + r - starts[b]. ``out`` gives both tensors (any strides between rows and heads), else
+    ``rows`` and ``dtype`` make them; rows from starts[-1] on are left as they were."""
+    if out is None:
+        if rows is None:
+            raise ValueError("kv4_read needs the number of rows, or out")
+        shape = (rows, cache.k_values.shape[1], cache.head_dim)
+        out = [torch.empty(shape, dtype=dtype, device=cache.k_values.device) for _ in range(2)]
+    k, v = out
+    _module().kv4_read(cache, first, starts, k, v, err)
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, cache: KV4Cache, pos: torch.Tensor, window: int = 0,
+                  scaling: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                  err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the newest rows of each sequence over its cache. q is [sequences, heads, D] (one row
+    each) or [sequences, rows, heads, D], bf16 or fp16; row i of sequence b stands at position pos[b] + i
+    (its keys and values are in the cache already) and sees the positions up to its own, with ``window``
+    > 0 the last ``window`` of them; query head h reads key/value head h // (heads // kv_heads). A row
+    whose position is outside the cache gives 0. The result has q's shape and type.
+
+    The cached whole numbers enter the products as they are; scales, scores, softmax statistics and sums
+    are fp32."""
+    return _module().kv4_attention(q, cache, pos, window, scaling, out, err)

@@ -411,6 +411,68 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
                     const void* w, int64_t n, int64_t ldw, const void* w_scales, const void* bias,
                     int bias_dtype, void* y, int y_dtype, int64_t ldy, void* workspace, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Attention of packed prompts, and the key/value cache held in 4 bits (no counterpart in the
+ * reference). Packed rows: `starts` holds seqs + 1 ascending int32; rows starts[b] ..
+ * starts[b + 1] - 1 are sequence b's, rows from starts[seqs] on nobody's: they are neither read
+ * nor written. A null `starts`: row r is sequence r. Heads of head_dim values, a multiple of 8 up to
+ * 256; query head h reads key/value head h / (heads / kv_heads). Strides in elements.
+ *
+ * The cache: for keys and for values, `values` [seqs][kv_heads][positions][16 g] bytes and `scales`
+ * [seqs][kv_heads][positions][g] bf16, g = ceil(head_dim / 32) groups of 32 values. A group's scale s
+ * is the bf16 nearest to max|x| / 7 and a value is held as n + 8, n = x / s rounded to nearest
+ * even (0 where s is 0), in 4 bits: value 2 i in the low half of byte i, value 2 i + 1 in the high
+ * half. A group with an infinity or NaN has a NaN scale. All four 16-byte aligned, positions a
+ * multiple of 32 below 2^30.
+ *
+ * fbfp_kv4_write: row r of k and v (any fbfp_dtype) to position pos[b] + r - starts[b] of its sequence.
+ * fbfp_kv4_read: row r of k and v from position first[b] + r - starts[b].
+ * fbfp_kv4_append: fused q|k|v rows (bf16, heads + 2 kv_heads heads, contiguous): RMSNorm (1 + w) of
+ *   every q and k head, the rotary embedding with the bf16 cos/sin rows [positions][head_dim] at the
+ *   row's position (roundings as fbfp_qk_rope_cache), q to q_out [rows][heads][head_dim], k and v to
+ *   the cache as fbfp_kv4_write does. head_dim a multiple of 16.
+ * A position outside the cache sets *err = 2, and nothing is written for that row.
+ * fbfp_kv4_attention: q [seqs][rows][heads][head_dim]; row i of sequence b, at position pos[b] + i,
+ *   attends to positions up to its own (with window > 0 only to the last `window` of those):
+ *   softmax(q k^T scaling) v, rounded once to the output's type (q's; bf16 or fp16). A row whose
+ *   position is outside the cache gives 0 and sets *err = 2. `workspace`:
+ *   fbfp_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, its contents of no account; not
+ *   shared by calls that run at the same time.
+ * fbfp_prompt_attention: q [rows] packed by `starts`, k and v [kv_rows] packed by `kv_starts` (null:
+ *   by `starts`), all bf16 or all fp16, out of the same type. Of a sequence with n rows and c >= n
+ *   keys, row i stands at place c - n + i and attends to keys up to its place (the last `window` of
+ *   those); rows that see no key give 0. Pointers 16-byte aligned, strides multiples of 8.
+ *   `workspace`: fbfp_prompt_attention_workspace_bytes(...) bytes as above.
+ * ---------------------------------------------------------------------------------- */
+typedef struct fbfp_kv4_cache {
+  void *k_values, *k_scales, *v_values, *v_scales;
+  int64_t seqs, kv_heads, positions, head_dim;
+} fbfp_kv4_cache;
+
+int fbfp_kv4_write(const fbfp_kv4_cache* cache, const void* k, const void* v, int dtype, int64_t rows,
+                   int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, const int32_t* pos,
+                   const int32_t* starts, int32_t* err, void* stream);
+int fbfp_kv4_read(const fbfp_kv4_cache* cache, void* k, void* v, int dtype, int64_t rows, int64_t k_row,
+                  int64_t k_head, int64_t v_row, int64_t v_head, const int32_t* first,
+                  const int32_t* starts, int32_t* err, void* stream);
+int fbfp_kv4_append(const fbfp_kv4_cache* cache, const void* qkv, int64_t rows, int64_t heads,
+                    const void* q_norm_w, const void* k_norm_w, float eps, const void* cos_table,
+                    const void* sin_table, const int32_t* pos, const int32_t* starts, void* q_out,
+                    int32_t* err, void* stream);
+int64_t fbfp_kv4_attention_workspace_bytes(const fbfp_kv4_cache* cache, int64_t rows, int64_t heads);
+int fbfp_kv4_attention(const fbfp_kv4_cache* cache, const void* q, int dtype, int64_t rows, int64_t heads,
+                       int64_t q_seq, int64_t q_row, int64_t q_head, const int32_t* pos, int64_t window,
+                       float scaling, void* out, int64_t o_seq, int64_t o_row, int64_t o_head,
+                       void* workspace, int64_t workspace_bytes, int32_t* err, void* stream);
+int64_t fbfp_prompt_attention_workspace_bytes(int64_t rows, int64_t kv_rows, int64_t seqs, int64_t heads,
+                                              int64_t kv_heads, int64_t head_dim, int64_t window);
+int fbfp_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t rows,
+                          int64_t kv_rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                          int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
+                          int64_t v_head, const int32_t* starts, const int32_t* kv_starts, int64_t window,
+                          float scaling, void* out, int64_t o_row, int64_t o_head, void* workspace,
+                          int64_t workspace_bytes, int32_t* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
