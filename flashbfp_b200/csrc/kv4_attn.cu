@@ -1,5 +1,5 @@
-// attention.cu — attention of packed prompts, and of the newest tokens over the 4-bit cache: one CTA per
-// (row, query head), a warp per key in turn, an online softmax per warp, merged at the end.
+// kv4_attn.cu — attention of the newest tokens over the 4-bit cache: one CTA per (row, query head), a
+// warp per key in turn, an online softmax per warp, merged at the end.
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -7,20 +7,6 @@ namespace fbfp {
 namespace {
 
 constexpr int kWarps = 8;
-
-// A row's keys: those of places lo .. hi - 1, of which `load` gives a lane's 8 values.
-template <typename T>
-struct PlainKeys {
-  const T *k, *v;
-  int64_t k_row, v_row;
-  int hd;
-  __device__ __forceinline__ void load(const T* base, int64_t row, int64_t j, int lane, float (&x)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = lane * 8 < hd ? load_as_float(base + j * row + lane * 8, sizeof(T) == 4 ? FBFP_F32 : std::is_same<T, __half>::value ? FBFP_F16 : FBFP_BF16, i) : 0.f;
-  }
-  __device__ __forceinline__ void key(int64_t j, int lane, float (&x)[8]) const { load(k, k_row, j, lane, x); }
-  __device__ __forceinline__ void value(int64_t j, int lane, float (&x)[8]) const { load(v, v_row, j, lane, x); }
-};
 
 struct CachedKeys {
   Kv4 c;
@@ -79,33 +65,6 @@ __device__ void attend_row(const T* q, T* out, int hd, const Keys& keys, int64_t
   }
 }
 
-struct PromptArgs {
-  const void *q, *k, *v;
-  void* out;
-  int64_t rows, kv_rows, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, window;
-  int seqs, heads, kv_heads, hd;
-  const int32_t *starts, *kv_starts;
-  float scaling;
-};
-
-template <typename T>
-__global__ void prompt_rows_kernel(PromptArgs a) {
-  pdl_prologue();
-  const int64_t row = blockIdx.x / a.heads;
-  const int h = (int)(blockIdx.x % a.heads), kvh = h / (a.heads / a.kv_heads);
-  int64_t i;
-  const int b = packed_seq(row, a.starts, a.seqs, i);
-  if (b < 0) return;
-  const int64_t n = a.starts[b + 1] - (int64_t)a.starts[b];
-  const int64_t k0 = max((int64_t)a.kv_starts[b], (int64_t)0), k1 = min((int64_t)a.kv_starts[b + 1], a.kv_rows);
-  const int64_t at = k1 - k0 - n + i;
-  const int64_t hi = min(k1 - k0, at + 1), lo = a.window > 0 ? max(at - a.window + 1, (int64_t)0) : 0;
-  PlainKeys<T> keys{(const T*)a.k + k0 * a.k_row + kvh * a.k_head, (const T*)a.v + k0 * a.v_row + kvh * a.v_head,
-                    a.k_row, a.v_row, a.hd};
-  attend_row((const T*)a.q + row * a.q_row + h * a.q_head, (T*)a.out + row * a.o_row + h * a.o_head, a.hd, keys, lo, hi,
-             a.scaling);
-}
-
 struct Kv4Args {
   const void* q;
   void* out;
@@ -136,41 +95,6 @@ __global__ void kv4_rows_kernel(Kv4 c, Kv4Args a) {
 }  // namespace fbfp
 
 using namespace fbfp;
-
-extern "C" int64_t fbfp_prompt_attention_workspace_bytes(int64_t rows, int64_t kv_rows, int64_t seqs, int64_t heads,
-                                                         int64_t kv_heads, int64_t head_dim, int64_t window) {
-  return 0;
-}
-
-extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t rows,
-                                     int64_t kv_rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                     int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
-                                     int64_t v_head, const int32_t* starts, const int32_t* kv_starts, int64_t window,
-                                     float scaling, void* out, int64_t o_row, int64_t o_head, void* workspace,
-                                     int64_t workspace_bytes, int32_t* err, void* stream) {
-  FBFP_CHECK_ARG(q && k && v && starts && out && err, "null pointer");
-  FBFP_CHECK_ARG(dtype == FBFP_BF16 || dtype == FBFP_F16, "bad dtype %d (bf16 or fp16)", dtype);
-  FBFP_CHECK_ARG(rows >= 1 && rows < (1 << 30) && kv_rows >= 1 && kv_rows < (1 << 30) && seqs >= 1 && seqs <= 65535,
-                 "bad sizes (%lld rows, %lld key rows, %lld sequences)", (long long)rows, (long long)kv_rows,
-                 (long long)seqs);
-  FBFP_CHECK_ARG(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && heads <= 65535, "%lld heads over %lld",
-                 (long long)heads, (long long)kv_heads);
-  FBFP_CHECK_ARG(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, "head_dim %lld is not a multiple of 8 up to 256",
-                 (long long)head_dim);
-  FBFP_CHECK_ARG(q_row >= 0 && q_head >= 0 && k_row >= 0 && k_head >= 0 && v_row >= 0 && v_head >= 0 && o_row >= 0 &&
-                     o_head >= 0 && ((q_row | q_head | k_row | k_head | v_row | v_head | o_row | o_head) & 7) == 0,
-                 "strides must be multiples of 8");
-  FBFP_CHECK_ARG(window >= 0, "negative window");
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
-    return set_error(FBFP_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
-  PromptArgs a{q, k, v, out, rows, kv_rows, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, window,
-               (int)seqs, (int)heads, (int)kv_heads, (int)head_dim, starts, kv_starts ? kv_starts : starts, scaling};
-  FBFP_CHECK_ARG(rows * heads <= 0x7FFFFFFF, "too many rows");
-  auto kernel = dtype == FBFP_BF16 ? prompt_rows_kernel<__nv_bfloat16> : prompt_rows_kernel<__half>;
-  FBFP_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)(rows * heads)), dim3(kWarps * 32), 0, as_stream(stream), a));
-  FBFP_LAUNCH_CHECK("prompt_rows_kernel");
-  return FBFP_OK;
-}
 
 extern "C" int64_t fbfp_kv4_attention_workspace_bytes(const fbfp_kv4_cache* cache, int64_t rows, int64_t heads) {
   return 0;
