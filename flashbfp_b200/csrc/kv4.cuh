@@ -59,13 +59,15 @@ __device__ __forceinline__ float kv4_scale(float top) {
   return __bfloat162float(__float2bfloat16_rn(q));
 }
 
-// A group's 32 values spread over 4 neighbouring lanes, 8 each: the lane's 8 nibbles and the
-// group's scale. All lanes of the warp take part. x / s is rounded exactly: the rest x - n s is a
-// multiple of the finer of the two's last places and at most s / 2, so fp32 holds it.
-__device__ __forceinline__ void kv4_quantise(const float (&x)[8], uint32_t& word, float& s) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+// A group's 32 values spread over 4 neighbouring lanes, 8 each, `top` the bits of the lane's largest
+// magnitude: the lane's 8 nibbles and the group's scale. All lanes of the warp take part.
+// WIDE: values of more than 16 bits. A quotient x / s is refined once, y + (x - y s) / s, which leaves it
+// exact where fp32 holds it, halves among that. Of values of 16 bits no other quotient comes near a half
+// (2 x - (2 n + 1) s is a multiple of both's last places: 2^-13 of s at least), so y rounds as x / s does.
+// Wider values decide by the rest x - n s, which fp32 holds: a multiple of the finer of both's last
+// places and at most s / 2.
+template <bool WIDE>
+__device__ __forceinline__ void kv4_quantise(const float (&x)[8], uint32_t top, uint32_t& word, float& s) {
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   word = 0x88888888u;
@@ -75,23 +77,39 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[8], uint32_t& word
   }
   s = kv4_scale(__uint_as_float(top));
   if (s == 0.f) return;
-  const float inv = __fdiv_rn(1.f, s);
-  const bool slow = !(s > 1e-37f);                   // 1 / s overflows
-  word = 0;
+  const float up = s < 1e-30f ? 0x1p100f : 1.f;      // where 1 / s could overflow and x - n s be subnormal: exact
+  const float t = s * up, inv = __frcp_rn(t);
+  // n + 8 comes out in the low bits of 1.5 2^23 + 8, rounded to even; the sum of those words times 16^i is the
+  // nibbles' word and what the upper bits add to it
+  word = 0u - (uint32_t)(0x4B400000ull * 0x11111111ull);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float n = rintf(slow ? __fdiv_rn(x[i], s) : x[i] * inv);
-    const float rest = fmaf(-n, s, x[i]);
-    const float twice = 2.f * fabsf(rest);
-    if (twice > s || (twice == s && ((int)n & 1))) n += rest > 0.f ? 1.f : -1.f;
-    word |= (uint32_t)((int)n + 8) << (4 * i);
+    const float z = x[i] * up;
+    float y = z * inv;
+    if constexpr (WIDE) {
+      y = rintf(y);
+      const float rest = fmaf(-y, t, z);
+      const float twice = 2.f * fabsf(rest);
+      if (twice > t || (twice == t && ((int)y & 1))) y += rest > 0.f ? 1.f : -1.f;
+    } else {
+      y = fmaf(fmaf(-y, t, z), inv, y);
+    }
+    word += __float_as_uint(y + 12582920.f) << (4 * i);
   }
+}
+template <bool WIDE>
+__device__ __forceinline__ void kv4_quantise(const float (&x)[8], uint32_t& word, float& s) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  kv4_quantise<WIDE>(x, top, word, s);
 }
 
 // The 8 values of a word of a group with scale s.
 __device__ __forceinline__ void kv4_values(uint32_t word, float s, float (&x)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)((int)((word >> (4 * i)) & 15) - 8) * s;
+  for (int i = 0; i < 8; ++i)                        // n in the low bits of 2^23, minus 2^23 + 8: exact
+    x[i] = (__uint_as_float(0x4B000000u | ((word >> (4 * i)) & 15u)) - 8388616.f) * s;
 }
 
 }  // namespace fbfp

@@ -12,11 +12,11 @@
 // mma.sync and not tcgen05: its operands come from registers, where the unpacked values are; for
 // tcgen05 each would have to be written to shared memory once more for at most 16 columns.
 //
-// Work: pieces of a (sequence, key/value head, block of columns), cut where a sequence is long, so that
-// the SMs fill whatever the lengths are, which only the device knows. A warp of a piece takes every
-// sixth tile of 32 positions through a ring of its own (TMA: values swizzled so that fragments
-// read without bank conflicts), with a running maximum and sum; the warps join in shared memory, the
-// pieces of a sequence in a second launch.
+// Work: all tiles of 32 positions in one list, of which each CTA takes an even share, so that the SMs fill
+// and end together whatever the lengths are, which only the device knows. A warp takes every sixth tile
+// through a ring of its own (TMA: values swizzled so that fragments read without bank conflicts),
+// with a running maximum and sum; the warps join in shared memory, parts of a sequence in a second
+// launch.
 #include <cuda.h>
 
 #include "kv4.cuh"
@@ -27,11 +27,10 @@ namespace fbfp {
 namespace {
 using namespace sm100;
 
-constexpr int kWarps = 6, kThreads = kWarps * 32;
 constexpr int kTok = 32;                 // positions of a tile
-constexpr int kLeast = 2 * kWarps;       // tiles of a piece, where its sequence has as many
-constexpr int kSlots = 2 * 148;          // pieces at a time
-constexpr int kMost = 3 * kSlots;        // pieces of about even length that all work is cut into
+constexpr int kLeast = 16;               // tiles that are worth a CTA
+constexpr int kSms = 148;
+constexpr int kAccumulators = 8;         // 32 dims x 8 columns each, of a warp at most: 64 registers of a thread
 
 struct Args {
   Kv4 c;
@@ -41,8 +40,9 @@ struct Args {
   int window, rows, heads, group, columns, blocks;    // columns = rows x group, in `blocks` blocks
   const int32_t* pos;
   int32_t* err;
+  int slots;                             // CTAs at a time
   float scale;                           // scaling log2(e)
-  float *part, *ml;                      // pieces: unnormalised results [piece][column][hd]; maximum and sum
+  float *part, *ml;                      // segments: unnormalised results [segment][column][hd]; maximum and sum
 };
 
 struct Maps {
@@ -61,73 +61,86 @@ __device__ __forceinline__ Reach reach_of(const Args& a, int b) {
   return {(int)(lo / kTok), (int)((hi + kTok - 1) / kTok - lo / kTok)};
 }
 
-// All pieces: sequence by sequence, each cut into the same number of parts for all its heads and blocks.
-struct Cut {
-  int parts, first_piece;
+// All work is a list of items, (sequence, key/value head, block of columns), sequence by sequence, of
+// so many tiles each (at least one, so that each item has a CTA). Where every item, cut into parts of kLeast
+// tiles, fits the SMs at once, a CTA takes one part (the list is padded to whole parts); else each CTA takes the
+// same length of the list, as many items or parts of items as that is. What a CTA does of one item
+// is a segment; segment number = CTA + item, each its own.
+struct Schedule {
+  bool parts;
+  int64_t share, total;                  // tiles a CTA, of all (padded)
 };
-__device__ __forceinline__ int parts_of(int tiles, int chunk) { return tiles <= chunk ? 1 : (tiles + chunk - 1) / chunk; }
-
-// The tiles of a piece at most, by this warp.
-__device__ __forceinline__ int chunk_of(const Args& a) {
-  const int lane = threadIdx.x & 31;
-  int64_t total = 0;
-  for (int b = lane; b < a.c.seqs; b += 32) total += reach_of(a, b).tiles;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  total *= a.c.nkv * a.blocks;
-  const int64_t even = (total + kMost - 1) / kMost;
-  return (int)max(even, (int64_t)kLeast);
+__device__ __forceinline__ int64_t padded(int tiles, const Schedule& s) {
+  const int n = max(tiles, 1);
+  return s.parts ? (n + kLeast - 1) / kLeast * kLeast : n;
 }
-
-// The piece `index`: its sequence, head, block of columns and part; false past the last.
-struct Piece {
-  int b, head, block, part, parts;
-};
-__device__ __forceinline__ bool find_piece(const Args& a, int chunk, int index, Piece& r) {
+// By this warp.
+__device__ __forceinline__ Schedule schedule_of(const Args& a) {
+  int64_t total = 0, parts = 0;
+  for (int b = threadIdx.x & 31; b < a.c.seqs; b += 32) {
+    const int n = max(reach_of(a, b).tiles, 1);
+    total += n;
+    parts += (n + kLeast - 1) / kLeast;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    parts += __shfl_xor_sync(0xffffffffu, parts, o);
+  }
+  const int64_t per = (int64_t)a.c.nkv * a.blocks;
+  total *= per, parts *= per;
+  if (parts <= a.slots) return {true, kLeast, parts * kLeast};
+  return {false, max((total + a.slots - 1) / a.slots, (int64_t)kLeast), total};
+}
+// The sequence that place `at` (below the total) of the list is in, and where its first item begins.
+__device__ __forceinline__ void find_sequence(const Args& a, const Schedule& s, int64_t at, int& seq, int64_t& begin) {
   const int lane = threadIdx.x & 31;
-  const int per = a.c.nkv * a.blocks;
+  const int64_t per = (int64_t)a.c.nkv * a.blocks;
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.seqs; b0 += 32) {
     const int b = b0 + lane;
-    const int parts = b < a.c.seqs ? parts_of(reach_of(a, b).tiles, chunk) : 0;
-    int sum = parts;
+    const int64_t n = b < a.c.seqs ? padded(reach_of(a, b).tiles, s) * per : 0;
+    int64_t sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    const int64_t from = before + (int64_t)(sum - parts) * per;
-    const uint32_t who = __ballot_sync(0xffffffffu, index >= from && index < from + (int64_t)parts * per);
+    const uint32_t who = __ballot_sync(0xffffffffu, at >= before + sum - n && at < before + sum);
     if (who) {
       const int src = __ffs(who) - 1;
-      const int rest = __shfl_sync(0xffffffffu, (int)(index - from), src);
-      r.parts = __shfl_sync(0xffffffffu, parts, src);
-      r.b = b0 + src;
-      r.part = rest % r.parts;
-      r.block = rest / r.parts % a.blocks;
-      r.head = rest / r.parts / a.blocks;
-      return true;
+      seq = b0 + src;
+      begin = before + __shfl_sync(0xffffffffu, sum - n, src);
+      return;
     }
-    before += (int64_t)__shfl_sync(0xffffffffu, sum, 31) * per;
+    before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  return false;
+  seq = 0, begin = 0;                                 // not reached
 }
 
-template <int NG, int NT, typename T>
+struct Piece {
+  int b, head, block;
+};
+
+template <int NG, int NT>
 struct Cfg {
+  // Two CTAs of six warps an SM: 168 registers a thread.
+  static constexpr int kCtas = 2, kWarps = 6, kThreads = kWarps * 32;
   static constexpr int kValues = kTok * 16 * NG, kScales = kTok * 2 * NG;       // bytes of a tile, keys or values
+  static constexpr int kMostDepth = NG > 6 ? 4 : 8;
   static constexpr int kEntry = kValues + kScales;          // keys and values of a tile are entries of their own
   static constexpr int kFrag = NT * NG * 32 * 16;                               // queries as fragments
-  static constexpr int kInit = std::is_same<T, __half>::value ? 0 : NT * NG * 4 * 16;
-  // two CTAs an SM (227 KB of shared memory, 1 KB of it a CTA's own)
-  static constexpr int kRoom = 115712 - 1024 - kFrag - kInit - 256;
+  static constexpr int kColumns = 8 * NT * 4;
+  // of 228 KB shared memory an SM, 1 KB of it each CTA's own
+  static constexpr int kMore = kFrag + kColumns + kWarps * 8 * kMostDepth + 16;  // barriers, the word that says that a wait gave up
+  static constexpr int kRoom = 115712 - kMore;
   static constexpr int kFit = kRoom / (kWarps * kEntry);
-  static constexpr int kDepth = kFit > 8 ? 8 : kFit;
+  static constexpr int kDepth = kFit > kMostDepth ? kMostDepth : kFit;
   static constexpr int kRing = kWarps * kDepth * kEntry;
   static constexpr int kJoin = (kWarps * 8 * NT * (32 * NG + 4) + kWarps * 8 * NT * 2) * 4;      // where the warps join
-  static constexpr int kSmem = 1024 + (kRing > kJoin ? kRing : kJoin) + kFrag + kInit;
+  static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kMore;
   static_assert(kDepth >= 3, "keys, values and the next keys");
-  static_assert(kSmem <= 232448 - 512, "shared memory of a CTA");
+  static_assert(kSmem <= 115712, "shared memory of a CTA");
   static constexpr int kMask = NG == 8 ? 7 : NG == 4 ? 3 : NG == 2 ? 1 : 0;     // swizzle: 16-byte piece ^ 128-byte line
 };
 
@@ -140,20 +153,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   atomicExch(err, 48);
   return false;
 }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
   for (uint32_t it = 0; it < (1u << 14); ++it)
     if (mbar_try_wait_sleep(bar, parity, 20000u)) return;
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4],
-                                    const __nv_bfloat16*) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-}
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4],
-                                    const __half*) {
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -174,46 +180,46 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// a & mask | bits in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+// a & mask | 1024 in each half, in one instruction.
+__device__ __forceinline__ uint32_t in_1024(uint32_t a, uint32_t mask) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(r) : "r"(a), "r"(mask));
   return r;
 }
-__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t m, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(m), "r"(c));
+  return r;
 }
-// Nibbles (i, i + 4) of a word, i = 0..3, as bf16 pairs 128 + nibble: the nibble in the mantissa of 128.
-__device__ __forceinline__ void pairs_128(uint32_t w, uint32_t (&x)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+__device__ __forceinline__ uint32_t half2_add(uint32_t a, uint32_t c) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(c));
+  return r;
 }
-// The same as whole numbers nibble - 8 (exact differences), in bf16 or fp16. fp16's mantissa takes a
-// nibble in its first four bits (1024 + n) and in the next four (1024 + 16 n).
-__device__ __forceinline__ void pairs(uint32_t w, uint32_t (&x)[4], const __nv_bfloat16*) {
-  pairs_128(w, x);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = sub_bf2(x[i], 0x43084308u);        // 136
-}
-__device__ __forceinline__ void pairs(uint32_t w, uint32_t (&x)[4], const __half*) {
+// Nibbles n = 0..3 of each half of a word as fp16 pairs n - 8: in the first four bits of 1024's mantissa a
+// nibble makes it 1024 + n, in the next four 1024 + 16 n; - 1032, or / 16 - 72, is exact.
+__device__ __forceinline__ void pairs(uint32_t w, uint32_t (&x)[4]) {
   const uint32_t h = w >> 8;
-  const uint32_t lo[2] = {and_or(w, 0x000F000Fu, 0x64006400u), and_or(h, 0x000F000Fu, 0x64006400u)};
-  const uint32_t hi[2] = {and_or(w, 0x00F000F0u, 0x64006400u), and_or(h, 0x00F000F0u, 0x64006400u)};
-  const __half2 b = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));          // 1032
-  const __half2 m = __halves2half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00));          // 1 / 16
-  const __half2 c = __halves2half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480));          // -72
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const __half2 l = __hsub2(*reinterpret_cast<const __half2*>(&lo[i]), b);
-    const __half2 u = __hfma2(*reinterpret_cast<const __half2*>(&hi[i]), m, c);
-    x[2 * i] = *reinterpret_cast<const uint32_t*>(&l);
-    x[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&u);
-  }
+  x[0] = half2_add(in_1024(w, 0x000F000Fu), 0xE408E408u);
+  x[1] = half2_fma(in_1024(w, 0x00F000F0u), 0x2C002C00u, 0xD480D480u);
+  x[2] = half2_add(in_1024(h, 0x000F000Fu), 0xE408E408u);
+  x[3] = half2_fma(in_1024(h, 0x00F000F0u), 0x2C002C00u, 0xD480D480u);
 }
-__device__ __forceinline__ uint32_t pack_bf(float a, float b) {
-  const __nv_bfloat162 h = __float22bfloat162_rn(make_float2(a, b));
+__device__ __forceinline__ uint32_t pack_h(float a, float b) {
+  const __half2 h = __float22half2_rn(make_float2(a, b));
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float lo_h(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)w)); }
+__device__ __forceinline__ float hi_h(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)(w >> 16))); }
+__device__ __forceinline__ void fma2(float& a0, float& a1, float x0, float x1, float y) {
+  asm("{\n\t.reg .b64 a, x, y;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, x, y, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1) : "f"(x0), "f"(x1), "f"(y));
+}
+__device__ __forceinline__ void mul2(float& r0, float& r1, float x0, float x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r0), "=f"(r1) : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
 __device__ __forceinline__ float lo_bf(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -238,16 +244,87 @@ __device__ __forceinline__ void load_scales(uint32_t at, uint32_t (&w)[(NG + 1) 
   }
 }
 
+// The bits of the largest finite scale of 32 positions' values, of those that some column of the block sees:
+// a position per lane.
+template <int NG>
+__device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts) {
+  uint32_t w[(NG + 1) / 2], high = 0;                 // in halves
+  load_scales<NG>(vss + (threadIdx.x & 31) * 2 * NG, w);
+#pragma unroll
+  for (int i = 0; i < (NG + 1) / 2; ++i) high = __vmaxu2(high, w[i]);
+  high = counts ? max(high & 0xFFFFu, high >> 16) : 0;
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (high < 0x7F80u) return high;
+  high = 0;                                           // infinite and NaN scales make their own dims NaN: the rest counts
+#pragma unroll
+  for (int i = 0; i < (NG + 1) / 2; ++i) {
+    const uint32_t w0 = w[i] & 0x7FFFu, w1 = (w[i] >> 16) & 0x7FFFu;
+    high = max(high, max(w0 >= 0x7F80u ? 0u : w0, w1 >= 0x7F80u ? 0u : w1));
+  }
+  return __reduce_max_sync(0xffffffffu, counts ? high : 0u);
+}
+
+// O += (p s) n of 32 positions. The weights p carry a power of two that brings (p s) into fp16's range.
+// CUT: some column does not see some position, whose scale may be anything.
+template <int NG, int NT, bool CUT>
+__device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float (&p)[2][NT][4],
+                                           uint32_t vss, uint32_t vb, uint32_t half, int p0,
+                                           const int (&at_c)[NT], const int (&low_c)[NT]) {
+  using C = Cfg<NG, NT>;
+  const int t = threadIdx.x & 3;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t sc[4][(NG + 1) / 2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load_scales<NG>(vss + (16 * h + t + 4 * e) * 2 * NG, sc[e]);
+    // k index 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of 16 positions are t, t + 4, t + 8, t + 12
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      uint32_t x[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        constexpr uint32_t turn = C::kMask ? ((4 * 16 * NG >> 7) & C::kMask) << 4 : 0;   // rows 4 further
+        const uint32_t w0 = lds32((C::kMask ? vb ^ (j << 4) : vb + (j << 4)) + (16 * h + 8 * i) * 16 * NG);
+        const uint32_t w1 = lds32((C::kMask ? vb ^ ((j << 4) ^ turn) : vb + (j << 4)) + (16 * h + 8 * i + 4) * 16 * NG);
+        pairs(__byte_perm(w0, w1, half), x[i]);
+      }
+      const uint32_t a0[4] = {x[0][0], x[0][1], x[1][0], x[1][1]};
+      const uint32_t a1[4] = {x[0][2], x[0][3], x[1][2], x[1][3]};
+      float s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = j & 1 ? hi_bf(sc[e][j / 2]) : lo_bf(sc[e][j / 2]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+        if constexpr (CUT) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = p0 + 16 * h + t + 4 * e;
+            w[e] = at <= at_c[n] && at >= low_c[n] ? p[h][n][e] * s[e] : 0.f;
+          }
+        } else {
+          mul2(w[0], w[1], p[h][n][0], p[h][n][1], s[0], s[1]);
+          mul2(w[2], w[3], p[h][n][2], p[h][n][3], s[2], s[3]);
+        }
+        const uint32_t b0 = pack_h(w[0], w[1]), b1 = pack_h(w[2], w[3]);
+        mma(o[j][0][n], a0, b0, b1, o[j][0][n]);
+        mma(o[j][1][n], a1, b0, b1, o[j][1][n]);
+      }
+    }
+  }
+}
+
 template <int NG, int NT, typename T>
-__global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
-  using C = Cfg<NG, NT, T>;
+__global__ void __launch_bounds__((Cfg<NG, NT>::kThreads), (Cfg<NG, NT>::kCtas))
+kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
+  using C = Cfg<NG, NT>;
+  constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[kWarps * C::kDepth];
-  __shared__ int abort_flag;
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];   // (no other shared memory in front of it)
   uint8_t* frag = smem + (C::kRing > C::kJoin ? C::kRing : C::kJoin);
-  uint8_t* init = frag + C::kFrag;
+  float* column_scale = reinterpret_cast<float*>(frag + C::kFrag);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(frag + C::kFrag + C::kColumns);
+  volatile int& abort_flag = *reinterpret_cast<volatile int*>(bars + kWarps * C::kMostDepth);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int hd = a.c.hd;
   if (threadIdx.x == 0) {
@@ -256,24 +333,43 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
     fence_mbar_init();
   }
   pdl_prologue();
-  const int chunk = chunk_of(a);
-  Piece pc;
-  if (!find_piece(a, chunk, blockIdx.x, pc)) return;
-  const Reach reach = reach_of(a, pc.b);
-  const int64_t pos = __ldg(a.pos + pc.b);
-  const int t0 = reach.first + (int)((int64_t)reach.tiles * pc.part / pc.parts);
-  const int t1 = reach.first + (int)((int64_t)reach.tiles * (pc.part + 1) / pc.parts);
-  const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;       // this warp's tiles
-  __syncthreads();                                    // the barriers are there
-
-  // a warp's ring: the values of all entries first (swizzled rows), then their scales; entry 2 i holds the
-  // keys of the warp's tile i, entry 2 i + 1 its values
+  const Schedule sch = schedule_of(a);
+  // a warp's ring: the values of all entries first (swizzled rows), then their scales; the keys and
+  // the values of a tile are entries that follow each other
   uint64_t* bar = bars + warp * C::kDepth;
   uint8_t* const ring = smem + warp * C::kDepth * C::kValues;
   uint8_t* const ring_s = smem + kWarps * C::kDepth * C::kValues + warp * C::kDepth * C::kScales;
+  int base = 0;                                       // entries of the segments before
+  const int64_t end = min((int64_t)(blockIdx.x + 1) * sch.share, sch.total);
+#pragma unroll 1
+  for (int64_t at = (int64_t)blockIdx.x * sch.share; at < end;) {
+  Piece pc;
+  int64_t begin;
+  find_sequence(a, sch, at, pc.b, begin);
+  const Reach reach = reach_of(a, pc.b);
+  const int64_t pos = __ldg(a.pos + pc.b);
+  const int64_t n_item = padded(reach.tiles, sch);
+  const int64_t nth = (at - begin) / n_item, in_item = (at - begin) - nth * n_item;
+  const int64_t item = (int64_t)pc.b * a.c.nkv * a.blocks + nth;
+  pc.head = (int)(nth / a.blocks);
+  pc.block = (int)(nth - (int64_t)pc.head * a.blocks);
+  const int64_t length = min(n_item - in_item, end - at);
+  at += length;
+  const bool whole = length == n_item;
+  int t0, t1;                                         // tiles of the sequence
+  if (sch.parts) {                                    // parts of even length
+    const int64_t parts = n_item / kLeast, part = in_item / kLeast;
+    t0 = reach.first + (int)(reach.tiles * part / parts);
+    t1 = reach.first + (int)(reach.tiles * (part + 1) / parts);
+  } else {
+    t0 = reach.first + (int)in_item;
+    t1 = reach.first + min((int)(in_item + length), reach.tiles);
+  }
+  const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;       // this warp's tiles
+  __syncthreads();                                    // the barriers are there; the last segment's join is read
   const int64_t row0 = a.c.at(pc.b, pc.head, 0);
-  const auto load = [&](int e) {                      // lane 0
-    const int slot = e % C::kDepth;
+  const auto load = [&](int e) {                      // lane 0: entry e of the segment
+    const int slot = (base + e) % C::kDepth;
     const int64_t row = row0 + (int64_t)(t0 + warp + (e >> 1) * kWarps) * kTok;
     mbar_arrive_expect_tx(&bar[slot], C::kEntry);
     tma_2d_g2s(ring + slot * C::kValues, e & 1 ? &M.v : &M.k, 0, (int)row, &bar[slot]);
@@ -283,27 +379,39 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
     for (int e = 0; e < min(2 * mine, C::kDepth); ++e) load(e);
 
   // the queries as the MMA's column operand: of group j, lane (g, t) holds column g's values 8 t + (0, 4),
-  // (1, 5), (2, 6), (3, 7); bf16 also what 128 + nibble - n adds to a group's sum, -136 sum q
+  // (1, 5), (2, 6), (3, 7). A power of two per column brings its largest value to 2^12: bf16 values down to 2^-29
+  // of the largest are exact in fp16.
   for (int i = warp; i < NT * NG; i += kWarps) {
-    const int j = i % NG, col = pc.block * 8 * NT + i / NG * 8 + g, d = 32 * j + 8 * t;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (col < a.columns && d < hd)
-      x = *reinterpret_cast<const uint4*>((const T*)a.q + pc.b * a.q_seq + col / a.group * a.q_row +
-                                          (pc.head * a.group + col % a.group) * a.q_head + d);
-    reinterpret_cast<uint4*>(frag)[i * 32 + lane] =
-        make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
-                   __byte_perm(x.y, x.w, 0x7632));
-    if constexpr (!kHalf) {
-      float s = lo_bf(x.x) + hi_bf(x.x) + lo_bf(x.y) + hi_bf(x.y) + lo_bf(x.z) + hi_bf(x.z) + lo_bf(x.w) + hi_bf(x.w);
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if ((t & 1) == 0) reinterpret_cast<float*>(init)[(i * 4 + g / 2) * 4 + (g & 1) + t] = -136.f * s;   // twice
+    const int j = i % NG, col = pc.block * 8 * NT + i / NG * 8 + g;
+    const T* row = (const T*)a.q + pc.b * a.q_seq + col / a.group * a.q_row + (pc.head * a.group + col % a.group) * a.q_head;
+    float x[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const int d = 32 * k + 8 * t;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (col < a.columns && d < hd) u = *reinterpret_cast<const uint4*>(row + d);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y0 = kHalf ? lo_h(w[e]) : lo_bf(w[e]), y1 = kHalf ? hi_h(w[e]) : hi_bf(w[e]);
+        top = max(top, max(__float_as_uint(y0) & 0x7FFFFFFFu, __float_as_uint(y1) & 0x7FFFFFFFu));
+        if (k == j) x[2 * e] = y0, x[2 * e + 1] = y1;
+      }
     }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+    const float up = __uint_as_float((uint32_t)(127 + 12 - ex) << 23);
+    if (j == 0 && t == 0) column_scale[i / NG * 8 + g] = a.scale * __uint_as_float((uint32_t)(ex - 12 + 127) << 23);
+    reinterpret_cast<uint4*>(frag)[i * 32 + lane] = make_uint4(pack_h(x[0] * up, x[4] * up), pack_h(x[1] * up, x[5] * up),
+                                                               pack_h(x[2] * up, x[6] * up), pack_h(x[3] * up, x[7] * up));
   }
   __syncthreads();
 
   // this lane's columns (of the values' product): 8 nt + g
   int at_c[NT], low_c[NT];
+  float scale[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int col = pc.block * 8 * NT + 8 * n + g;
@@ -311,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
     const bool in = col < a.columns && p >= 0 && p < a.c.positions;
     at_c[n] = in ? (int)p : -1;
     low_c[n] = in && a.window > 0 ? (int)max(p + 1 - a.window, (int64_t)0) : 0;
+    scale[n] = column_scale[8 * n + g];
   }
   // every column of a row sees all of positions all_low .. all_high
   const int all_high = (int)min(max(pos, (int64_t)-1), (int64_t)a.c.positions);
@@ -319,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
 
   float o[NG][2][NT][4];
   float m[NT], l[NT];
+  int ev = -1000;                                     // weights are 2^(score - m + 8 - ev), ev near the scales' exponent
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = -INFINITY, l[n] = 0.f;
@@ -337,9 +447,9 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
   int done = 0;                                       // entries
 #pragma unroll 1
   for (; done < 2 * mine; ++done) {
-    const int slot_k = done % C::kDepth, slot_v = (done + 1) % C::kDepth;
-    if (!__all_sync(0xffffffffu, wait(&bar[slot_k], (uint32_t)(done / C::kDepth) & 1, &abort_flag, a.err))) break;
-    const uint32_t ks = smem_u32(ring) + slot_k * C::kValues, vs = smem_u32(ring) + slot_v * C::kValues;
+    const int slot_k = (base + done) % C::kDepth, slot_v = (base + done + 1) % C::kDepth;
+    if (!__all_sync(0xffffffffu, wait(&bar[slot_k], (uint32_t)((base + done) / C::kDepth) & 1, &abort_flag, a.err))) break;
+    const uint32_t kb = smem_u32(ring) + slot_k * C::kValues + at_k, vb = smem_u32(ring) + slot_v * C::kValues + at_v;
     const uint32_t kss = smem_u32(ring_s) + slot_k * C::kScales, vss = smem_u32(ring_s) + slot_v * C::kScales;
     const int p0 = (t0 + warp + (done >> 1) * kWarps) * kTok;
 
@@ -359,34 +469,28 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
       for (int j = 0; j < NG; ++j) {
         uint32_t x[4][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // 8 rows are whole turns of the swizzle where there is one
-          const uint32_t w = lds32(ks + (C::kMask ? at_k ^ (j << 4) : at_k + (j << 4)) + r * 128 * NG);
-          if constexpr (kHalf) pairs(w, x[r], (const T*)nullptr);
-          else pairs_128(w, x[r]);
-        }
+        for (int r = 0; r < 4; ++r)                   // 8 rows are whole turns of the swizzle where there is one
+          pairs(lds32((C::kMask ? kb ^ (j << 4) : kb + (j << 4)) + r * 128 * NG), x[r]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 q = lds128(smem_u32(frag) + ((n * NG + j) * 32 + lane) * 16);
-          float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (!kHalf) {
-            const uint4 c = lds128(smem_u32(init) + ((n * NG + j) * 4 + t) * 16);
-            zero[0] = __uint_as_float(c.x), zero[1] = __uint_as_float(c.y);
-            zero[2] = __uint_as_float(c.z), zero[3] = __uint_as_float(c.w);
-          }
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float d[4];
             const uint32_t a0[4] = {x[2 * h][0], x[2 * h + 1][0], x[2 * h][1], x[2 * h + 1][1]};
             const uint32_t a1[4] = {x[2 * h][2], x[2 * h + 1][2], x[2 * h][3], x[2 * h + 1][3]};
-            mma(d, a0, q.x, q.y, zero, (const T*)nullptr);
-            mma(d, a1, q.z, q.w, d, (const T*)nullptr);
+            mma(d, a0, q.x, q.y, zero);
+            mma(d, a1, q.z, q.w, d);
             const float s0 = j & 1 ? hi_bf(sc[2 * h][j / 2]) : lo_bf(sc[2 * h][j / 2]);
             const float s1 = j & 1 ? hi_bf(sc[2 * h + 1][j / 2]) : lo_bf(sc[2 * h + 1][j / 2]);
-            s[h][n][0] = fmaf(s0, d[0], s[h][n][0]);
-            s[h][n][1] = fmaf(s0, d[1], s[h][n][1]);
-            s[h][n][2] = fmaf(s1, d[2], s[h][n][2]);
-            s[h][n][3] = fmaf(s1, d[3], s[h][n][3]);
+            if constexpr (NT == 1) {                  // a pair needs its scale twice: not worth it for one
+              s[h][n][0] = fmaf(s0, d[0], s[h][n][0]), s[h][n][1] = fmaf(s0, d[1], s[h][n][1]);
+              s[h][n][2] = fmaf(s1, d[2], s[h][n][2]), s[h][n][3] = fmaf(s1, d[3], s[h][n][3]);
+            } else {
+              fma2(s[h][n][0], s[h][n][1], d[0], d[1], s0);
+              fma2(s[h][n][2], s[h][n][3], d[2], d[3], s1);
+            }
           }
         }
       }
@@ -404,36 +508,46 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
         for (int e = 0; e < 4; ++e) {                 // position t + 4 e: row t + 4 (e & 1) of half e / 2
           const float even = __shfl_sync(0xffffffffu, s[h][n][2 * (e >> 1)], src + 16 * (e & 1));
           const float odd = __shfl_sync(0xffffffffu, s[h][n][2 * (e >> 1) + 1], src + 16 * (e & 1));
-          p[h][n][e] = (g & 1 ? odd : even) * a.scale;
+          p[h][n][e] = (g & 1 ? odd : even) * scale[n];
         }
+    ++done;
+    if (!__all_sync(0xffffffffu, wait(&bar[slot_v], (uint32_t)((base + done) / C::kDepth) & 1, &abort_flag, a.err))) break;
     const bool cut = p0 + kTok - 1 > all_high || p0 < all_low;
+    bool counts = true;                               // some column of the block sees position p0 + lane
     if (cut) {
+      counts = p0 + lane <= newest && p0 + lane >= (a.window > 0 ? pos + 1 - a.window : 0);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int at = p0 + 16 * h + t + 4 * e;
-            if (at > at_c[n] || at < low_c[n]) p[h][n][e] = -INFINITY;
+            const int at_p = p0 + 16 * h + t + 4 * e;
+            if (at_p > at_c[n] || at_p < low_c[n]) p[h][n][e] = -INFINITY;
           }
     }
-    bool moved = false;
+    const uint32_t high = largest_scale<NG>(vss, counts);
+    const int ex = min(max((int)(high >> 7) - 127, -90), 120);
+    const bool grown = ex > ev + 3;                   // the references move when weights could pass 2^14 in fp16
+    const float turn = grown ? (ev < -90 ? 0.f : ex2((float)(ev - ex))) : 1.f;
+    if (grown) ev = ex;
+    bool moved = grown;
     float f[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top = m[n];
+      float top = p[0][n][0];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, p[h][n][e]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      moved |= top != m[n];
-      f[n] = m[n] == -INFINITY ? 0.f : ex2(m[n] - top);
-      m[n] = top;
+      const bool raise = top > m[n] + 3.f;
+      f[n] = raise ? ex2(m[n] - top) * turn : turn;   // 0 where nothing was seen yet
+      if (raise) m[n] = top;
+      moved |= raise;
     }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, moved) && done > 1) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         l[n] *= f[n];
@@ -446,70 +560,29 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float less = m[n] == -INFINITY ? 0.f : m[n];
+      const float add = (m[n] == -INFINITY ? 0.f : -m[n]) + (float)(8 - ev);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[h][n][e] = ex2(p[h][n][e] - less);
+          p[h][n][e] = ex2(p[h][n][e] + add);
           l[n] += p[h][n][e];
         }
     }
-
-    ++done;
-    if (!__all_sync(0xffffffffu, wait(&bar[slot_v], (uint32_t)(done / C::kDepth) & 1, &abort_flag, a.err))) break;
-    // O += (p s) n, 16 positions at a time: k index 2 t, 2 t + 1, 2 t + 8, 2 t + 9 are positions t, t + 4, t + 8, t + 12
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t sc[4][(NG + 1) / 2];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) load_scales<NG>(vss + (16 * h + t + 4 * e) * 2 * NG, sc[e]);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        uint32_t u[2], x[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // rows 4 further: half a turn of the swizzle
-          const uint32_t turn = C::kMask ? ((4 * 16 * NG >> 7) & C::kMask) << 4 : 0;
-          const uint32_t w0 = lds32(vs + (C::kMask ? at_v ^ (j << 4) : at_v + (j << 4)) + (16 * h + 8 * i) * 16 * NG);
-          const uint32_t w1 = lds32(vs + (C::kMask ? at_v ^ (j << 4) ^ turn : at_v + (j << 4)) + (16 * h + 8 * i + 4) * 16 * NG);
-          u[i] = __byte_perm(w0, w1, half);
-          pairs(u[i], x[i], (const __nv_bfloat16*)nullptr);
-        }
-        const uint32_t a0[4] = {x[0][0], x[0][1], x[1][0], x[1][1]};
-        const uint32_t a1[4] = {x[0][2], x[0][3], x[1][2], x[1][3]};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float sv = j & 1 ? hi_bf(sc[e][j / 2]) : lo_bf(sc[e][j / 2]);
-            if (cut) {                                // a position that this column does not see may have any scale
-              const int at = p0 + 16 * h + t + 4 * e;
-              if (at > at_c[n] || at < low_c[n]) sv = 0.f;
-            }
-            w[e] = p[h][n][e] * sv;
-          }
-          const uint32_t b0 = pack_bf(w[0], w[1]), b1 = pack_bf(w[2], w[3]);
-          mma(o[j][0][n], a0, b0, b1, o[j][0][n], (const __nv_bfloat16*)nullptr);
-          mma(o[j][1][n], a1, b0, b1, o[j][1][n], (const __nv_bfloat16*)nullptr);
-          if constexpr (kHalf) {                      // what the rounding of the weights left
-            const uint32_t r0 = pack_bf(w[0] - lo_bf(b0), w[1] - hi_bf(b0)), r1 = pack_bf(w[2] - lo_bf(b1), w[3] - hi_bf(b1));
-            mma(o[j][0][n], a0, r0, r1, o[j][0][n], (const __nv_bfloat16*)nullptr);
-            mma(o[j][1][n], a1, r0, r1, o[j][1][n], (const __nv_bfloat16*)nullptr);
-          }
-        }
-      }
-    }
+    if (cut) add_values<NG, NT, true>(o, p, vss, vb, half, p0, at_c, low_c);
+    else add_values<NG, NT, false>(o, p, vss, vb, half, p0, at_c, low_c);
     __syncwarp();
     if (lane == 0 && done + C::kDepth < 2 * mine) load(done + C::kDepth);
   }
   if (done < 2 * mine && lane == 0)                   // a wait gave up: the loads in flight land first
-    for (int e = done; e < min(done + C::kDepth, 2 * mine); ++e) settle(&bar[e % C::kDepth], (uint32_t)(e / C::kDepth) & 1);
+    for (int e = done; e < min(done + C::kDepth, 2 * mine); ++e) settle(&bar[(base + e) % C::kDepth], (uint32_t)((base + e) / C::kDepth) & 1);
+  base += 2 * mine;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
     l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+    // sums and results are 2^(8 - ev) as large as the weights 2^(score - m) make them
+    if (m[n] != -INFINITY) m[n] += (float)(ev - 8);
   }
   __syncthreads();                                    // all tiles are read: their place is free
 
@@ -553,16 +626,15 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
       L += lw * fw;
       r.x += x.x * fw, r.y += x.y * fw, r.z += x.z * fw, r.w += x.w * fw;
     }
-    if (pc.parts > 1) {
-      const int64_t to = (int64_t)blockIdx.x * (8 * NT) + c;
+    if (!whole) {
+      const int64_t to = (blockIdx.x + item) * (8 * NT) + c;
       *reinterpret_cast<float4*>(a.part + to * hd + d) = r;
       if (d == 0) a.ml[to * 2] = M, a.ml[to * 2 + 1] = L;
     } else {
       const float inv = L == 0.f ? 0.f : 1.f / L;
       const int64_t row = col / a.group;
       T* to = (T*)a.out + pc.b * a.o_seq + row * a.o_row + (pc.head * a.group + col % a.group) * a.o_head + d;
-      const int64_t at = pos + row;
-      if (at < 0 || at >= a.c.positions) {
+      if (pos + row < 0 || pos + row >= a.c.positions) {
         r = make_float4(0.f, 0.f, 0.f, 0.f);
         atomicExch(a.err, 2);
       }
@@ -572,9 +644,12 @@ __global__ void __launch_bounds__(kThreads, NG * NT > 8 ? 1 : 2) kv4_attn_kernel
       store_from_float(to, kHalf ? FBFP_F16 : FBFP_BF16, 3, r.w * inv);
     }
   }
+  fence_async_proxy();                                // the next segment's loads land where this one joined
+  if (abort_flag) break;
+  }
 }
 
-// Joins the parts of sequences that were cut; a warp per column.
+// Joins the segments of items that were cut; a warp per column.
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const Args a, int block_columns) {
   pdl_prologue();
@@ -583,15 +658,19 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Args a, int block_c
   const int64_t per_seq = (int64_t)a.c.nkv * a.columns;
   if (w >= per_seq * a.c.seqs) return;
   const int b = (int)(w / per_seq), rest = (int)(w - b * per_seq), head = rest / a.columns, col = rest % a.columns;
-  const int chunk = chunk_of(a);
-  const int parts = parts_of(reach_of(a, b).tiles, chunk);
-  if (parts == 1) return;
+  const Schedule sch = schedule_of(a);
+  const int64_t n_item = padded(reach_of(a, b).tiles, sch);
   int64_t before = 0;
-  for (int i = lane; i < b; i += 32) before += parts_of(reach_of(a, i).tiles, chunk);
+  for (int i = lane; i < b; i += 32) before += padded(reach_of(a, i).tiles, sch);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  const int64_t piece = before * a.c.nkv * a.blocks + ((int64_t)head * a.blocks + col / block_columns) * parts;
-  const int64_t from = piece * block_columns + col % block_columns;
+  const int64_t nth = (int64_t)head * a.blocks + col / block_columns;
+  const int64_t begin = before * a.c.nkv * a.blocks + nth * n_item;
+  const int64_t first = begin / sch.share;
+  const int parts = (int)((begin + n_item - 1) / sch.share - first) + 1;
+  if (parts == 1) return;
+  const int64_t item = (int64_t)b * a.c.nkv * a.blocks + nth;
+  const int64_t from = (first + item) * block_columns + col % block_columns;
   float M = -INFINITY, L = 0.f, r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < parts; ++i) M = fmaxf(M, a.ml[(from + (int64_t)i * block_columns) * 2]);
   for (int i = 0; i < parts; ++i) {
@@ -619,16 +698,16 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Args a, int block_c
 }
 
 // Columns that a block holds: more let one unpacking serve more columns, as far as the accumulators
-// (32 registers for each 8 columns of 128 dims) leave two CTAs an SM.
+// leave two CTAs an SM.
 int column_tiles(int64_t columns, int groups) {
-  if (columns <= 8) return 1;
-  if (columns <= 16 || groups > 4) return 2;
+  if (columns <= 8 || 2 * groups > kAccumulators) return 1;
+  if (columns <= 16 || 4 * groups > kAccumulators) return 2;
   return 4;
 }
 
 struct Plan {
-  int nt, blocks;
-  int64_t pieces;
+  int nt, blocks, slots;
+  int64_t ctas, segments;
   bool joins;
 };
 Plan plan_of(const Kv4& c, int64_t rows, int64_t heads, int64_t window) {
@@ -636,12 +715,14 @@ Plan plan_of(const Kv4& c, int64_t rows, int64_t heads, int64_t window) {
   const int64_t columns = rows * (heads / c.nkv);
   p.nt = column_tiles(columns, c.groups);
   p.blocks = (int)((columns + 8 * p.nt - 1) / (8 * p.nt));
+  p.slots = kSms * 2;                                // Cfg::kCtas
   const int64_t items = (int64_t)c.seqs * c.nkv * p.blocks;
   int64_t tiles = c.positions / kTok;                     // of a sequence at most
   if (window > 0 && (window + rows + kTok - 2) / kTok + 1 < tiles) tiles = (window + rows + kTok - 2) / kTok + 1;
-  p.joins = tiles > kLeast;
-  // parts_of adds at most one part to tiles / chunk, and all tiles / chunk are kMost at most
-  p.pieces = items + (p.joins ? (items * tiles < kMost * (int64_t)kLeast ? items * tiles / kLeast : kMost) : 0);
+  const int64_t parts = (tiles + kLeast - 1) / kLeast * items;
+  p.ctas = parts < p.slots ? parts : p.slots;
+  p.joins = parts > items || parts > p.slots;
+  p.segments = p.ctas + items;
   return p;
 }
 
@@ -652,10 +733,10 @@ int launch(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
   int dev = 0;
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !set[dev]) {
-    FBFP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NG, NT, T>::kSmem));
+    FBFP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NG, NT>::kSmem));
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  FBFP_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)p.pieces), dim3(kThreads), (size_t)Cfg<NG, NT, T>::kSmem, st, a, m));
+  FBFP_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(Cfg<NG, NT>::kThreads), (size_t)Cfg<NG, NT>::kSmem, st, a, m));
   FBFP_LAUNCH_CHECK("kv4_attn_kernel");
   if (p.joins) {
     const int64_t warps = (int64_t)a.c.seqs * a.c.nkv * a.columns;
@@ -666,9 +747,11 @@ int launch(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
 }
 template <int NG, typename T>
 int launch_nt(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
-  if constexpr (NG <= 4)
+  if constexpr (4 * NG <= kAccumulators)
     if (p.nt == 4) return launch<NG, 4, T>(a, m, p, st);
-  return p.nt == 1 ? launch<NG, 1, T>(a, m, p, st) : launch<NG, 2, T>(a, m, p, st);
+  if constexpr (2 * NG <= kAccumulators)
+    if (p.nt == 2) return launch<NG, 2, T>(a, m, p, st);
+  return launch<NG, 1, T>(a, m, p, st);
 }
 template <typename T>
 int launch_ng(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
@@ -693,7 +776,7 @@ extern "C" int64_t fbfp_kv4_attention_workspace_bytes(const fbfp_kv4_cache* cach
   Kv4 c;
   if (kv4_check(cache, c) || rows < 1 || heads < 1 || heads % c.nkv) return -1;
   const Plan p = plan_of(c, rows, heads, 0);
-  return p.joins ? p.pieces * 8 * p.nt * (c.hd + 2) * 4 : 0;
+  return p.joins ? p.segments * 8 * p.nt * (c.hd + 2) * 4 : 0;
 }
 
 extern "C" int fbfp_kv4_attention(const fbfp_kv4_cache* cache, const void* q, int dtype, int64_t rows, int64_t heads,
@@ -715,14 +798,14 @@ extern "C" int fbfp_kv4_attention(const fbfp_kv4_cache* cache, const void* q, in
   FBFP_CHECK_ARG((int64_t)c.seqs * c.nkv * c.positions < ((int64_t)1 << 31), "the cache has 2^31 rows or more");
   if (window > c.positions + rows) window = 0;              // sees everything
   const Plan p = plan_of(c, rows, heads, window);
-  FBFP_CHECK_ARG(p.pieces <= 0x7FFFFFFF && (int64_t)c.seqs * heads * rows < ((int64_t)1 << 31), "too many rows");
-  const int64_t need = p.joins ? p.pieces * 8 * p.nt * (c.hd + 2) * 4 : 0;
+  FBFP_CHECK_ARG((int64_t)c.seqs * heads * rows < ((int64_t)1 << 31), "too many rows");
+  const int64_t need = p.joins ? p.segments * 8 * p.nt * (c.hd + 2) * 4 : 0;
   FBFP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                  "the workspace must be %lld bytes, 16-byte aligned", (long long)need);
   const int group = (int)(heads / c.nkv);
   Args a{c, q, out, q_seq, q_row, q_head, o_seq, o_row, o_head, (int)window, (int)rows, (int)heads, group,
-         (int)rows * group, p.blocks, pos, err, scaling * 1.4426950408889634f, (float*)workspace,
-         (float*)workspace + p.pieces * 8 * p.nt * c.hd};
+         (int)rows * group, p.blocks, pos, err, p.slots, scaling * 1.4426950408889634f, (float*)workspace,
+         (float*)workspace + p.segments * 8 * p.nt * c.hd};
   Maps m;
   const uint64_t cells = (uint64_t)c.seqs * c.nkv * c.positions;
   const CUtensorMapSwizzle swz = c.groups == 8   ? CU_TENSOR_MAP_SWIZZLE_128B

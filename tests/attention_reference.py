@@ -40,8 +40,10 @@ def stored(x):
     return c[..., 0::2] + 16 * c[..., 1::2], s, vals
 
 
-def attend(q, k, v, seen, scaling, out_dtype, weight_u):
-    """q [heads, rows, D], k and v [heads, keys, D] in fp64, seen [rows, keys] -> (o, bound)."""
+def attend(q, k, v, seen, scaling, out_dtype, weight_u, step=0.0):
+    """q [heads, rows, D], k and v [heads, keys, D] in fp64, seen [rows, keys] -> (o, bound). ``step``: half the
+    smallest step of a weight times the largest value that it meets, relative to the row's largest weight
+    (the sum that results are divided by is at least that): small weights are off by that much each."""
     s = q @ k.transpose(1, 2) * scaling
     e_s = float(((q.abs() @ k.abs().transpose(1, 2)) * abs(scaling) * seen).max()) * (q.shape[-1] + 4) * 2.0 ** -24 \
         if seen.any() else 0.0
@@ -54,8 +56,9 @@ def attend(q, k, v, seen, scaling, out_dtype, weight_u):
     u = torch.finfo(out_dtype).eps / 2
     w = weight_u + 2 * e_s + 2.0 ** -19
     bound = u * o.abs() + (1 + u) * w * (p @ v.abs())
+    bound = bound + step * seen.sum(-1)[None, :, None]
     if out_dtype == torch.float16:
-        bound = bound + 2.0 ** -25                                                # half a subnormal step
+        bound = bound + 2.0 ** -25                                                # half a subnormal step of the result
     return o, bound + 1e-30
 
 
@@ -82,7 +85,9 @@ def packed(q, k, v, starts, kv_starts, window, scaling, weight_u):
             continue
         qq = q[q0:q1].double().transpose(0, 1)
         kk, vv = (x[k0:k1].double().transpose(0, 1).repeat_interleave(grp, 0) for x in (k, v))
-        oo, bb = attend(qq, kk, vv, seen, scaling, q.dtype, weight_u)
+        # fp16 weights are 2^6 times as large as the row's largest makes them: half a step is 2^-25 / 2^6
+        step = 2.0 ** -31 * float(vv.abs().max()) if q.dtype == torch.float16 and torch.isfinite(vv).all() else 0.0
+        oo, bb = attend(qq, kk, vv, seen, scaling, q.dtype, weight_u, step)
         o[q0:q1], bound[q0:q1] = oo.transpose(0, 1).cpu(), bb.transpose(0, 1).cpu()
     return o, bound
 
@@ -113,7 +118,11 @@ def cached(q, cache, pos, window, scaling, weight_u):
         seen = j <= at
         if window:
             seen = seen & (j > at - window)
-        oo, bb = attend(q[b, inside].double().transpose(0, 1), k, v, seen, scaling, q.dtype, weight_u)
+        # weights times scales are fp16, 2^8 times as large as the largest scale's power of two makes them:
+        # half a step is 2^-25 / 2^8 of it, times |n| <= 7
+        sc = cache.v_scales[b, :, lo:n].float()
+        step = 7 * 2.0 ** -33 * float(torch.where(torch.isfinite(sc), sc, torch.zeros_like(sc)).max())
+        oo, bb = attend(q[b, inside].double().transpose(0, 1), k, v, seen, scaling, q.dtype, weight_u, step)
         o[b, inside], bound[b, inside] = oo.transpose(0, 1).cpu(), bb.transpose(0, 1).cpu()
     return o, bound
 

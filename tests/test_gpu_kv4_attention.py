@@ -1,7 +1,6 @@
 """Attention over the 4-bit cache against its definition in 64 bits, with the bounds that
-attention_reference derives: cached whole numbers are exact in the products; the weight that meets v
-(softmax weight times the value's scale) is rounded to bf16 for bf16 results (u = 2^-8), and kept to
-2^-16 (bf16 in two parts, 2^-8 of 2^-8) for fp16 results."""
+attention_reference derives: cached whole numbers are exact in the products; the weight that meets them
+(softmax weight times the value's scale) is rounded to fp16, u = 2^-11."""
 import pytest
 import torch
 
@@ -10,7 +9,7 @@ from test_gpu_kv4_store import garbage, ints, rows
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-WEIGHT_U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16}
+WEIGHT_U = {torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -11}
 
 
 def filled(seqs, heads, positions, dim, seed):
