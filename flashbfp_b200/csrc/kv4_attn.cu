@@ -145,10 +145,7 @@ struct Cfg {
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
-  for (uint32_t it = 0; it < (1u << 16); ++it) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if ((it & 15) == 15 && *abort) return false;
-  }
+  if (mbar_wait_second(bar, parity, abort)) return true;
   *abort = 1;
   atomicExch(err, 48);
   return false;

@@ -2,12 +2,12 @@
 // softmax weights back into it as 16-bit operand, O += P V in tensor memory.
 //
 // A tile is 128 rows: `ntok` tokens of one sequence x the `hp` query heads that share a key/value head,
-// so that grouped heads read keys and values once and a few tokens fill a tile. Its keys are taken in
-// blocks of 128. Roles: a warp loads (TMA), a thread issues the MMAs, four warps per tile hold one row
-// a thread: scores from tensor memory, running maximum and sum, weights back. Heads of up to 128
-// values: a CTA takes two tiles, one's softmax runs under the other's MMAs. Heads of up to 256: one
-// tile (its O fills half of tensor memory) with two score buffers, the next block's scores being made
-// under this block's softmax.
+// so that grouped heads read keys and values once and a few tokens fill a tile. Keys and values are
+// loaded in blocks of 128 keys. Roles: a warp loads (TMA), a thread issues the MMAs, four warps per tile
+// hold one row a thread: scores from tensor memory, running maximum and sum, weights back. Each tile has
+// two score buffers, so that its next scores are made under its softmax. Heads of up to 128 values: a CTA
+// takes two tiles, of 64 keys a step. Heads of up to 256: one tile (its O fills half of tensor memory), 128 keys
+// a step.
 //
 // softmax: weights are 2^(s c - r), c = scaling log2(e), r the row's reference: its first block's
 // maximum, raised (and O and the sum rescaled) only when a score comes out 2^8 above it, which leaves
@@ -25,6 +25,7 @@ using namespace sm100;
 struct PromptArgs {
   int64_t rows, kv_rows, o_row, o_head, v_row, v_head, window;
   const int32_t *starts, *kv_starts;
+  int wide;                    // out may be stored 32 bytes at a time
   int seqs, heads, hd, hp, ntok, head_blocks, group, splits;
   float c;                     // |scaling| log2(e)
   uint32_t negate;             // scaling < 0
@@ -44,7 +45,10 @@ constexpr int kTile = 128;     // keys of a block, rows of a tile
 template <int HDP>
 struct Cfg {
   static constexpr int kTiles = HDP <= 128 ? 2 : 1;
-  static constexpr int kAhead = HDP <= 128 ? 1 : 2;       // blocks whose scores are made ahead
+  // Scores are made in steps of kKeys keys, two steps ahead of their softmax: each tile has two score buffers.
+  static constexpr int kKeys = HDP <= 128 ? 64 : 128;
+  static constexpr int kSub = kTile / kKeys;              // steps of a block
+  static constexpr int kAhead = 2 / kSub;                 // blocks whose keys are loaded before the first values
   static constexpr int kCols = HDP < 128 ? HDP : 128;     // values of a unit
   static constexpr int kUnit = kTile * kCols * 2;        // a block's keys or values come in units
   static constexpr int kPer = HDP / kCols;                // units per block
@@ -52,21 +56,28 @@ struct Cfg {
   static constexpr int kQ = kTile * HDP * 2;
   static constexpr int kSmem = kTiles * kQ + kUnits * kUnit + 1024;
   static constexpr int kSoft = 128 * kTiles;              // softmax threads
-  static constexpr int kThreads = kSoft + 64;
+  static constexpr int kThreads = kSoft + 32 + 32 * kTiles;
   static constexpr uint32_t kO = 256;                     // first column of O; scores at 0 and 128
 };
 
+// What a CTA works on.
+struct Work {
+  int q0, len, k0, klen, tok0;  // the sequence's rows and keys, the first token
+  int hb, split;                // block of heads, share of the keys
+  int any;
+};
+
 struct Ctl {
-  uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2], v_here[2], o_done[2], voted[2], drain;
+  uint64_t q_full[2], q_empty, full[8], empty[8], s_full[2][2], p_full[2][2], v_here[2], o_done[2][2], voted[2], drain;
+  uint64_t info_full[2], info_empty[2], next_full;
+  uint4 next;                   // the answer to a request for another CTA's work
+  Work info[2];                 // this tile's and the next one's, any = 0 behind the last
   uint32_t tmem;
-  int abort, skip[2], vote[2][4];
+  int abort, skip[2][2], vote[2][4];
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl& ctl, int32_t* err, int site) {
-  for (uint32_t it = 0; it < (1u << 16); ++it) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if ((it & 15) == 15 && *(volatile int*)&ctl.abort) return false;
-  }
+  if (mbar_wait_second(bar, parity, &ctl.abort)) return true;
   *(volatile int*)&ctl.abort = 1;
   atomicExch(err, site);
   return false;
@@ -82,13 +93,31 @@ __device__ __forceinline__ void tma_3d_g2s(uint32_t dst, const void* tmap, int x
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n"
       ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
+// The tensor core's instructions for a warp that goes the same way as a whole: one lane (`one`) issues, by a
+// predicate and not a branch, so that descriptors are computed in uniform registers.
 // D[tmem] (+)= A[smem] B[smem].
-__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc) : "memory");
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem].
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(acc), "r"(one) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
+      ::"r"(smem_u32(bar)), "r"(one) : "memory");
 }
 // Values [128 keys][64] in 128-byte swizzled rows as the N-major operand: 8-key groups 1 KB apart,
 // 64-value parts 16 KB apart.
@@ -189,17 +218,21 @@ __device__ __forceinline__ bool any_of_tile(bool x, int t, uint32_t& k, Ctl& ctl
   return r;
 }
 
-// O += P V over keys l .. h of a block, for this thread's row: the weights come from tensor memory, the
-// values from global memory. (Out of line: only where a value is infinite or NaN.)
+// O += P V over keys l .. h of a step, for this thread's row: the weights come from tensor memory, the
+// values from global memory. `fresh`: O holds nothing yet. (Out of line: only where a value is infinite or NaN.)
 template <int HDP, typename T>
-__device__ __noinline__ void add_seen(uint32_t o_at, uint32_t p_at, const T* v, int64_t v_row, int hd, int l, int h) {
+__device__ __noinline__ void add_seen(uint32_t o_at, uint32_t p_at, const T* v, int64_t v_row, int hd, int l, int h,
+                                      bool fresh) {
 #pragma unroll 1
   for (int d = 0; d < HDP; d += 32) {
     float o[32];
     tmem_load32(o_at + d, o);
     tmem_arrived<32>(o);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (fresh) o[i] = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < kTile / 2; ++i) {
+    for (int i = 0; i < Cfg<HDP>::kKeys / 2; ++i) {
       uint32_t w;
       asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(w) : "r"(p_at + i) : "memory");
       tmem_wait_ld();
@@ -221,18 +254,12 @@ __device__ __noinline__ void add_seen(uint32_t o_at, uint32_t p_at, const T* v, 
   tmem_wait_st();
 }
 
-// What a CTA works on.
-struct Work {
-  int q0, len, k0, klen, tok0;  // the sequence's rows and keys, the first token
-  bool any;
-};
-
 // CTA `index` of all tiles: the sequences' tiles from last to first, so that a prompt's longest tiles
 // start first. Every warp finds it by itself.
 __device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int toks) {
   const int lane = threadIdx.x & 31;
   int total = 0;
-  Work w{0, 0, 0, 0, 0, false};
+  Work w{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     int before = 0;
@@ -263,7 +290,7 @@ __device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int to
           const int bb = b0 + src;
           w.k0 = min((int64_t)max(__ldg(a.kv_starts + bb), 0), a.kv_rows);
           w.klen = (int)min((int64_t)max(__ldg(a.kv_starts + bb + 1), w.k0), a.kv_rows) - w.k0;
-          w.any = true;
+          w.any = 1;
           return w;
         }
       }
@@ -273,6 +300,24 @@ __device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int to
     if (index >= total) return w;
   }
   return w;
+}
+
+// Asks for the work of a CTA that has not been launched yet; the answer arrives on `bar`.
+__device__ __forceinline__ void ask_next(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+// Whether there was such a CTA, and its block index.
+__device__ __forceinline__ bool read_next(const uint4* answer, uint32_t& x, uint32_t& y) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, _, _}, r;\n\t}"
+      : "=r"(ok), "=r"(x), "=r"(y) : "r"(smem_u32(answer)) : "memory");
+  return ok != 0;
 }
 
 // Blocks of keys that tokens tok .. tok + n - 1 (those below len) see, cut to this split's share.
@@ -288,6 +333,32 @@ __device__ __forceinline__ Span blocks_of(const Work& w, const PromptArgs& a, in
   const int lo = a.window > 0 ? (int)max((int64_t)first - a.window + 1, (int64_t)0) : 0;
   return {lo / kTile, (hi + kTile - 1) / kTile};
 }
+// The blocks of each tile of a CTA and of the CTA as a whole, lo .. hi - 1.
+template <int TILES>
+__device__ __forceinline__ void spans_of(const Work& w, const PromptArgs& a, Span (&span)[TILES], int& lo, int& hi) {
+  lo = 1 << 30, hi = 0;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    span[t] = blocks_of(w, a, w.tok0 + t * a.ntok, a.ntok);
+    if (span[t].hi > span[t].lo) lo = min(lo, span[t].lo), hi = max(hi, span[t].hi);
+  }
+  if (hi <= lo) lo = hi = 0;
+  if (a.splits > 1) {
+    const int n = hi - lo;
+    const int from = lo + (int)((int64_t)n * w.split / a.splits), to = lo + (int)((int64_t)n * (w.split + 1) / a.splits);
+    lo = from, hi = to;
+  }
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    span[t].lo = max(span[t].lo, lo), span[t].hi = min(span[t].hi, hi);
+    if (span[t].hi <= span[t].lo) span[t] = {lo, lo};
+  }
+}
+// 32 bytes at p, 32-byte aligned.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 
 template <int HDP, typename T>
 __global__ void __launch_bounds__(Cfg<HDP>::kThreads, 1)
@@ -297,55 +368,35 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
   __shared__ Ctl ctl;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t sq = smem_u32(smem), sring = sq + C::kTiles * C::kQ;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_dependency_wait();
-  const int hb = blockIdx.x % a.head_blocks;
-  const Work w = find_work(a, blockIdx.x / a.head_blocks, a.ntok * C::kTiles);
-  if (!w.any) {
-    grid_launch_dependents();
-    return;
-  }
-  const int kvh = hb / (a.group / a.hp), head0 = hb * a.hp;
-  // the blocks of each tile, and of the CTA
-  Span span[C::kTiles];
-  int lo = 1 << 30, hi = 0;
-#pragma unroll
-  for (int t = 0; t < C::kTiles; ++t) {
-    span[t] = blocks_of(w, a, w.tok0 + t * a.ntok, a.ntok);
-    if (span[t].hi > span[t].lo) lo = min(lo, span[t].lo), hi = max(hi, span[t].hi);
-  }
-  if (hi <= lo) lo = hi = 0;
-  if (a.splits > 1) {
-    const int n = hi - lo, s = blockIdx.y;
-    const int from = lo + (int)((int64_t)n * s / a.splits), to = lo + (int)((int64_t)n * (s + 1) / a.splits);
-    lo = from, hi = to;
-  }
-#pragma unroll
-  for (int t = 0; t < C::kTiles; ++t) {
-    span[t].lo = max(span[t].lo, lo), span[t].hi = min(span[t].hi, hi);
-    if (span[t].hi <= span[t].lo) span[t] = {0, 0};
-  }
-
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kLoad = C::kSoft / 32, kMma = kLoad + 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.q_full[i], 1);
-      mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.p_full[i], 4);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&ctl.s_full[i][k], 1);
+        mbar_init(&ctl.p_full[i][k], 4);
+        mbar_init(&ctl.o_done[i][k], 1);
+        ctl.skip[i][k] = 0;
+      }
       mbar_init(&ctl.v_here[i], 1);
       mbar_init(&ctl.voted[i], 4);
       for (int k = 0; k < 4; ++k) ctl.vote[i][k] = 0;
-      mbar_init(&ctl.o_done[i], 1);
-      ctl.skip[i] = 0;
+      mbar_init(&ctl.info_full[i], 1);
+      mbar_init(&ctl.info_empty[i], kLoad + C::kTiles);
     }
     for (int i = 0; i < 8; ++i) {
       mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], 1);
+      mbar_init(&ctl.empty[i], C::kTiles);
     }
-    mbar_init(&ctl.drain, 1);
+    mbar_init(&ctl.q_empty, C::kTiles);
+    mbar_init(&ctl.next_full, 1);
+    mbar_init(&ctl.drain, C::kTiles);
     ctl.abort = 0;
     fence_mbar_init();
   }
-  if (warp == C::kSoft / 32) {                       // the loading warp: 512 columns, one CTA per SM
+  grid_dependency_wait();                            // before tensor memory is taken: the kernel before may hold some
+  if (warp == kLoad) {                               // 512 columns, one CTA per SM
     tmem_alloc(&ctl.tmem, 512);
     tmem_relinquish();
   }
@@ -355,126 +406,185 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
   grid_launch_dependents();                          // not before tensor memory is ours: a dependent may want some
   const uint32_t tmem = ctl.tmem;
 
-  int issued = 0;                                    // loading: units issued
-  if (warp == C::kSoft / 32) {
-    if (lane == 0 && hi > lo) {
+  // The CTA goes on with the work of CTAs that have not started, tile after tile: the loads of the next tile and
+  // its first scores come under the end of this one.
+  const auto next_work = [&](int m, bool& ok) {      // tile m of this CTA, as the loading warp found it
+    ok = __all_sync(0xffffffffu, wait(&ctl.info_full[m & 1], (uint32_t)(m >> 1) & 1, ctl, a.err, 43));
+    Work w;                                          // (broadcast: the same in all lanes, for the compiler too)
+    const int* from = reinterpret_cast<const int*>(&ctl.info[m & 1]);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Work) / 4); ++i)
+      reinterpret_cast<int*>(&w)[i] = __shfl_sync(0xffffffffu, *(volatile const int*)(from + i), 0);
+    if (lane == 0) mbar_arrive(&ctl.info_empty[m & 1]);
+    return w;
+  };
+
+  int issued = 0, q_loads = 0;                       // loading: units and queries issued
+  if (warp == kLoad) {
+    if (lane == 0) {
       prefetch_tmap(&M.q);
       prefetch_tmap(&M.k);
       prefetch_tmap(&M.v);
-      const uint32_t q_bytes = (uint32_t)a.ntok * a.hp * 128 * (HDP / 64);
-      const auto load_q = [&](int t) {
-        mbar_arrive_expect_tx(&ctl.q_full[t], q_bytes);
-        for (int c = 0; c < HDP / 64; ++c)
-          tma_3d_g2s(sq + t * C::kQ + c * 16384, &M.q, c * 64, head0, w.q0 + w.tok0 + t * a.ntok, smem_u32(&ctl.q_full[t]));
-      };
-      bool ok = true;
-      const auto load = [&](const CUtensorMap* map, int j) {        // the units of block j
-        for (int p = 0; p < C::kPer && ok; ++p) {
-          const int slot = issued % C::kUnits;
-          if (issued >= C::kUnits) ok = wait(&ctl.empty[slot], (uint32_t)(issued / C::kUnits - 1) & 1, ctl, a.err, 32);
-          if (!ok) return;
-          mbar_arrive_expect_tx(&ctl.full[slot], C::kUnit);
-          for (int c = 0; c < C::kCols / 64; ++c)
-            tma_3d_g2s(sring + slot * C::kUnit + c * 16384, map, p * C::kCols + c * 64, kvh, w.k0 + j * kTile,
-                       smem_u32(&ctl.full[slot]));
-          ++issued;
-        }
-      };
-      load_q(0);
-      load(&M.k, lo);
-      if (C::kTiles == 2) load_q(1);
-      for (int j = lo + 1; j < min(lo + C::kAhead, hi); ++j) load(&M.k, j);
-      for (int j = lo; j < hi && ok; ++j) {
-        load(&M.v, j);
-        if (j + C::kAhead < hi) load(&M.k, j + C::kAhead);
-      }
     }
-  } else if (warp == C::kSoft / 32 + 1) {
-    if (lane == 0 && hi > lo) {
-      const uint32_t id_s = idesc<T>(kTile, false) | (a.negate << 13), id_o = idesc<T>(C::kCols, true);
-      int used = 0;                                  // units taken, in the order of their loading
-      bool ok = true;
-      const auto arrived = [&]() {                   // the next block's units: the first's number
-        const int u = used;
-        for (int p = 0; p < C::kPer && ok; ++p, ++used)
-          ok = wait(&ctl.full[used % C::kUnits], (uint32_t)(used / C::kUnits) & 1, ctl, a.err, 33);
-        return u;
-      };
-      const auto release = [&](int u) {
-        for (int p = 0; p < C::kPer; ++p) mma_commit(&ctl.empty[(u + p) % C::kUnits]);
-      };
-      const auto scores = [&](int t, int buf, int u) {
-        for (int p = 0; p < C::kPer; ++p) {
-          const uint32_t kb = sring + ((u + p) % C::kUnits) * C::kUnit;
-          for (int s = 0; s < C::kCols / 16; ++s) {
-            const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
-            mma_ss(tmem + buf * 128, smem_desc_sw128(sq + t * C::kQ + p * 32768 + at, 1024), smem_desc_sw128(kb + at, 1024),
-                   id_s, p + s > 0);
-          }
-        }
-        mma_commit(&ctl.s_full[buf]);
-      };
-      const auto values = [&](int t, int buf, int u, bool skip) {
-        if (!skip)
-          for (int p = 0; p < C::kPer; ++p) {
-            const uint32_t vb = sring + ((u + p) % C::kUnits) * C::kUnit;
-            for (int s = 0; s < kTile / 16; ++s)
-              mma_ts(tmem + C::kO + t * HDP + p * C::kCols, tmem + buf * 128 + s * 8, desc_values(vb + s * 2048), id_o, 1);
-          }
-        mma_commit(&ctl.o_done[t]);
-      };
-      uint32_t p_seen[2] = {0, 0};
-      if constexpr (C::kTiles == 2) {
-        ok = wait(&ctl.q_full[0], 0, ctl, a.err, 34);
-        const int u0 = ok ? arrived() : 0;
-        if (ok && span[0].lo == lo && span[0].hi > lo) scores(0, 0, u0);
-        if (ok) ok = wait(&ctl.q_full[1], 0, ctl, a.err, 34);
-        if (ok && span[1].lo == lo && span[1].hi > lo) scores(1, 1, u0);
-        if (ok) release(u0);
-        for (int j = lo; j < hi && ok; ++j) {
-          const int uv = arrived();
-          if (!ok) break;
-          for (int t = 0; t < 2; ++t)
-            if (j >= span[t].lo && j < span[t].hi) mbar_arrive(&ctl.v_here[t]);
-          const int uk = j + 1 < hi ? arrived() : 0;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (ok && j >= span[t].lo && j < span[t].hi) {
-              ok = wait(&ctl.p_full[t], p_seen[t]++ & 1, ctl, a.err, 35);
-              if (!ok) break;
-              tc_fence_after();
-              values(t, t, uv, *(volatile int*)&ctl.skip[t]);
+    const uint32_t q_bytes = (uint32_t)a.ntok * a.hp * 128 * (HDP / 64);
+    uint32_t x = blockIdx.x, y = blockIdx.y;
+    bool ok = true, more = true;
+    int m = 0;                                       // tiles made known
+    const auto tell = [&](const Work& w) {
+      if (m >= 2) ok = __all_sync(0xffffffffu, wait(&ctl.info_empty[m & 1], (uint32_t)((m >> 1) - 1) & 1, ctl, a.err, 44));
+      if (lane == 0 && ok) {
+        ctl.info[m & 1] = w;
+        mbar_arrive(&ctl.info_full[m & 1]);
+      }
+      ++m;
+    };
+#pragma unroll 1
+    for (uint32_t asked = 0; more && ok; ++asked) {
+      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles);
+      w.hb = x % a.head_blocks, w.split = y;
+      if (w.any) {
+        tell(w);
+        const int kvh = w.hb / (a.group / a.hp), head0 = w.hb * a.hp;
+        Span span[C::kTiles];
+        int lo, hi;
+        spans_of(w, a, span, lo, hi);
+        if (lane == 0 && hi > lo && ok) {
+          const auto load_q = [&](int t) {
+            mbar_arrive_expect_tx(&ctl.q_full[t], q_bytes);
+            for (int c = 0; c < HDP / 64; ++c)
+              tma_3d_g2s(sq + t * C::kQ + c * 16384, &M.q, c * 64, head0, w.q0 + w.tok0 + t * a.ntok, smem_u32(&ctl.q_full[t]));
+          };
+          const auto load = [&](const CUtensorMap* map, int j) {        // the units of block j
+            for (int p = 0; p < C::kPer && ok; ++p) {
+              const int slot = issued % C::kUnits;
+              if (issued >= C::kUnits) ok = wait(&ctl.empty[slot], (uint32_t)(issued / C::kUnits - 1) & 1, ctl, a.err, 32);
+              if (!ok) return;
+              mbar_arrive_expect_tx(&ctl.full[slot], C::kUnit);
+              for (int c = 0; c < C::kCols / 64; ++c)
+                tma_3d_g2s(sring + slot * C::kUnit + c * 16384, map, p * C::kCols + c * 64, kvh, w.k0 + j * kTile,
+                           smem_u32(&ctl.full[slot]));
+              ++issued;
             }
-            if (t == 1 && ok) release(uv);
-            if (ok && j + 1 >= span[t].lo && j + 1 < span[t].hi) scores(t, t, uk);
+          };
+          if (q_loads > 0) ok = wait(&ctl.q_empty, (uint32_t)(q_loads - 1) & 1, ctl, a.err, 45);
+          if (ok) {
+            for (int t = 0; t < C::kTiles; ++t) load_q(t);
+            ++q_loads;
           }
-          if (ok && j + 1 < hi) release(uk);
-        }
-      } else {
-        ok = wait(&ctl.q_full[0], 0, ctl, a.err, 34);
-        for (int j = lo; j < min(lo + 2, hi) && ok; ++j) {
-          const int u = arrived();
-          if (!ok) break;
-          scores(0, (j - lo) & 1, u);
-          release(u);
-        }
-        for (int j = lo; j < hi && ok; ++j) {
-          const int buf = (j - lo) & 1;
-          const int uv = arrived();
-          if (!ok) break;
-          mbar_arrive(&ctl.v_here[0]);
-          ok = wait(&ctl.p_full[buf], p_seen[buf]++ & 1, ctl, a.err, 35);
-          if (!ok) break;
-          tc_fence_after();
-          values(0, buf, uv, *(volatile int*)&ctl.skip[buf]);
-          release(uv);
-          if (j + 2 < hi) {
-            const int u = arrived();
-            if (!ok) break;
-            scores(0, buf, u);
-            release(u);
+          for (int j = lo; j < min(lo + C::kAhead, hi) && ok; ++j) load(&M.k, j);
+          for (int j = lo; j < hi && ok; ++j) {
+            load(&M.v, j);
+            if (j + C::kAhead < hi) load(&M.k, j + C::kAhead);
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      // asked for when this tile's loads are under way, no sooner: whoever is done first takes the next
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&ctl.next_full, 16);
+        ask_next(&ctl.next, &ctl.next_full);
+      }
+      if (!__all_sync(0xffffffffu, wait(&ctl.next_full, asked & 1, ctl, a.err, 46))) ok = false;
+      if (ok) more = read_next(&ctl.next, x, y);
+      fence_async_proxy();                           // read before the next answer lands
+      __syncwarp();
+    }
+    if (ok) tell(Work{0, 0, 0, 0, 0, 0, 0, 0});
+  } else if (warp >= kMma) {
+    const int t = warp - kMma;                       // this warp's tile
+    // The whole warp goes the same way, one elected lane issues: descriptors stay in uniform registers.
+    const uint32_t one = elect_one_sync();
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), ring = __shfl_sync(0xffffffffu, sring, 0);
+    const uint32_t id_s = idesc<T>(C::kKeys, false) | (a.negate << 13), id_o = idesc<T>(C::kCols, true);
+    const uint64_t q_desc = smem_desc_sw128(__shfl_sync(0xffffffffu, sq, 0), 1024);
+    const uint64_t k_desc = smem_desc_sw128(ring, 1024), v_desc = desc_values(ring);     // of slot 0
+    // The ring: the next unit's slot, and the parity of its phase.
+    uint32_t slot = 0, parity = 0;
+    uint32_t made = 0, met = 0;                      // steps: scores made, values met (buffer: the lowest bit)
+    int q_used = 0;
+    bool ok = true;
+    const auto arrived = [&]() {                     // the next block's units: the first's slot
+      const uint32_t u = slot;
+#pragma unroll
+      for (int p = 0; p < C::kPer; ++p) {
+        if (ok) ok = __all_sync(0xffffffffu, wait(&ctl.full[slot], parity, ctl, a.err, 33));
+        if (++slot == C::kUnits) slot = 0, parity ^= 1;
+      }
+      return u;
+    };
+    const auto after = [&](uint32_t u, int p) { return u + p >= C::kUnits ? u + p - C::kUnits : u + p; };
+    const auto release = [&](uint32_t u) {
+#pragma unroll
+      for (int p = 0; p < C::kPer; ++p) commit(one, &ctl.empty[after(u, p)]);
+    };
+    // A step's scores, later the product of its weights and values; `sub`: which keys of the block. Descriptors
+    // count 16 bytes.
+    const auto scores = [&](int sub, uint32_t u) {
+      const uint32_t buf = made++ & 1;
+      const uint32_t d = base + t * 128 + buf * C::kKeys;
+#pragma unroll
+      for (int p = 0; p < C::kPer; ++p) {
+        const uint64_t qd = q_desc + (uint32_t)((t * C::kQ + p * 32768) / 16);
+        const uint64_t kd = k_desc + after(u, p) * (C::kUnit / 16) + (uint32_t)(sub * (C::kKeys * 128) / 16);
+#pragma unroll
+        for (int s = 0; s < C::kCols / 16; ++s) {
+          const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) / 16;
+          mma_ss(one, d, qd + at, kd + at, id_s, p + s > 0);
+        }
+      }
+      commit(one, &ctl.s_full[t][buf]);
+    };
+    const auto values = [&](int sub, uint32_t u, bool first) {
+      const uint32_t buf = met & 1;
+      ok = __all_sync(0xffffffffu, wait(&ctl.p_full[t][buf], (met++ >> 1) & 1, ctl, a.err, 35));
+      if (!ok) return;
+      tc_fence_after();
+      const bool skip = __any_sync(0xffffffffu, *(volatile int*)&ctl.skip[t][buf]);
+      if (!skip)
+#pragma unroll
+        for (int p = 0; p < C::kPer; ++p) {
+          const uint64_t vd = v_desc + after(u, p) * (C::kUnit / 16) + (uint32_t)(sub * (C::kKeys * 128) / 16);
+#pragma unroll
+          for (int s = 0; s < C::kKeys / 16; ++s)
+            mma_ts(one, base + C::kO + t * HDP + p * C::kCols, base + t * 128 + buf * C::kKeys + s * 8, vd + s * 128, id_o,
+                   !first || s > 0);
+        }
+      commit(one, &ctl.o_done[t][buf]);
+    };
+#pragma unroll 1
+    for (int m = 0; ok; ++m) {
+      const Work w = next_work(m, ok);
+      if (!ok || !w.any) break;
+      Span span[C::kTiles];
+      int lo, hi;
+      spans_of(w, a, span, lo, hi);
+      const int steps = (hi - lo) * C::kSub;
+      if (steps == 0) continue;
+      const Span mine = t == 0 ? span[0] : span[C::kTiles - 1];
+      const int from = (mine.lo - lo) * C::kSub, to = (mine.hi - lo) * C::kSub;      // this tile's steps
+      uint32_t uk = 0, uv = 0;
+      if (ok) ok = __all_sync(0xffffffffu, wait(&ctl.q_full[t], q_used & 1, ctl, a.err, 34));
+      ++q_used;
+      for (int i = 0; i < min(2, steps) && ok; ++i) {
+        if (i % C::kSub == 0) uk = arrived();
+        if (ok && i >= from && i < to) scores(i % C::kSub, uk);
+        if (ok && i % C::kSub == C::kSub - 1) release(uk);
+      }
+      if (steps <= 2 && ok) commit(one, &ctl.q_empty);
+      for (int i = 0; i < steps && ok; ++i) {
+        const bool in = i >= from && i < to;
+        if (i % C::kSub == 0) {
+          uv = arrived();
+          if (!ok) break;
+          if (one && in) mbar_arrive(&ctl.v_here[t]);
+        }
+        if (i + 2 < steps && (i + 2) % C::kSub == 0) uk = arrived();
+        if (ok && in) values(i % C::kSub, uv, i == from);
+        if (!ok) break;
+        if (i % C::kSub == C::kSub - 1) release(uv);
+        if (i + 2 >= from && i + 2 < to) scores(i % C::kSub, uk);       // (two steps on: the same part)
+        if (i + 2 < steps && (i + 2) % C::kSub == C::kSub - 1) release(uk);
+        if (i + 3 == steps) commit(one, &ctl.q_empty);
       }
     }
   } else {
@@ -482,6 +592,18 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const int r = threadIdx.x & 127;                 // this thread's row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t o_at = tmem + C::kO + t * HDP + lanes;
+    const float shift = kType<T> ? 0.f : 6.f;        // fp16 weights are 2^6 times as large
+    uint32_t votes = 0, blocks_seen = 0, g = 0;      // votes, blocks and steps so far
+    int units = 0;                                   // units of the tiles so far
+    bool ok = true;
+#pragma unroll 1
+    for (int m = 0; ok; ++m) {
+    const Work w = next_work(m, ok);
+    if (!ok || !w.any) break;
+    Span span[C::kTiles];
+    int lo, hi;
+    spans_of(w, a, span, lo, hi);
+    const int kvh = w.hb / (a.group / a.hp), head0 = w.hb * a.hp;
     const int tok = w.tok0 + t * a.ntok + r / a.hp, head = head0 + r % a.hp;
     const bool mine = r < a.ntok * a.hp && tok < w.len;
     const int place = mine ? w.klen - w.len + tok : -1;
@@ -490,51 +612,44 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const int tile0 = w.tok0 + t * a.ntok, tile1 = min(tile0 + a.ntok, w.len) - 1;
     const int all_high = w.klen - w.len + tile0;
     const int all_low = a.window > 0 ? (int)((int64_t)(w.klen - w.len + tile1) - a.window + 1) : 0;
-    const float shift = kType<T> ? 0.f : 6.f;        // fp16 weights are 2^6 times as large
     float ref = -INFINITY, sum0 = 0.f, sum1 = 0.f;   // reference (times c), sum of weights
-    uint32_t votes = 0;
-    bool ok = true;
-    const int j0 = t == 0 ? span[0].lo : span[C::kTiles - 1].lo, j1 = t == 0 ? span[0].hi : span[C::kTiles - 1].hi;
-    if (j1 > j0) {
-      float z[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) z[i] = 0.f;
+    const int j0 = t == 0 ? span[0].lo : span[C::kTiles - 1].lo;
+    const int i0 = j0 * C::kSub, steps = (t == 0 ? span[0].hi : span[C::kTiles - 1].hi) * C::kSub - i0;
 #pragma unroll 1
-      for (int d = 0; d < HDP; d += 32) tmem_store32(o_at + d, z);
-    }
-#pragma unroll 1
-    for (int j = j0; j < j1; ++j) {
-      const int n = j - j0;                          // blocks before
-      const int buf = C::kTiles == 2 ? t : n & 1;
-      const uint32_t phase = C::kTiles == 2 ? n & 1 : (n >> 1) & 1;
-      ok = __all_sync(0xffffffffu, wait(&ctl.s_full[buf], phase, ctl, a.err, 36));
+    for (int n = 0; n < steps; ++n, ++g) {
+      const int buf = g & 1;
+      ok = __all_sync(0xffffffffu, wait(&ctl.s_full[t][buf], (g >> 1) & 1, ctl, a.err, 36));
       if (!ok) break;
       tc_fence_after();
-      float s[128];
-      const uint32_t s_at = tmem + buf * 128 + lanes;
+      float s[C::kKeys];
+      const uint32_t s_at = tmem + t * 128 + buf * C::kKeys + lanes;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_load32(s_at + 32 * i, s + 32 * i);
-      tmem_arrived<128>(s);
-      const int key0 = j * kTile;
-      const bool cut = key0 + kTile - 1 > all_high || key0 < all_low;        // the same in the whole tile
-      const int h = place - key0, l = low - key0;     // the row sees keys l .. h of the block
+      for (int i = 0; i < C::kKeys / 32; ++i) tmem_load32(s_at + 32 * i, s + 32 * i);
+      tmem_arrived<C::kKeys>(s);
+      const int key0 = (i0 + n) * C::kKeys;
+      const bool cut = key0 + C::kKeys - 1 > all_high || key0 < all_low;      // the same in the whole tile
+      const int h = place - key0, l = low - key0;     // the row sees keys l .. h of the step
       bool skip = false;
       if (cut) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
+        for (int i = 0; i < C::kKeys; ++i)
           if (i > h || i < l) s[i] = -INFINITY;
       }
-      float top = s[0];
+      float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 1; i < 128; ++i) top = fmaxf(top, s[i]);
-      top *= a.c;
+      for (int i = 4; i < C::kKeys; ++i) tops[i & 3] = fmaxf(tops[i & 3], s[i]);
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.c;
+      // the step before: its product
+      const auto done_before = [&](int site) {
+        return __all_sync(0xffffffffu, wait(&ctl.o_done[t][buf ^ 1], ((g - 1) >> 1) & 1, ctl, a.err, site));
+      };
       if (n == 0) {
         ref = top;
       } else {
         const bool raise = top > ref + 8.f;
         if (__any_sync(0xffffffffu, raise)) {
           // O and the sum to the new reference, once the MMAs before have added to O
-          ok = __all_sync(0xffffffffu, wait(&ctl.o_done[t], (uint32_t)(n - 1) & 1, ctl, a.err, 37));
+          ok = done_before(37);
           if (!ok) break;
           tc_fence_after();
           const float f = raise ? ex2(ref - top) : 1.f;              // 0 where there was none
@@ -554,41 +669,44 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       }
       const float less = ref == -INFINITY ? 0.f : shift - ref;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t p[16];
+      for (int i = 0; i < C::kKeys / 16; ++i) {
+        uint32_t p[8];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x = s[32 * i + e], y = s[32 * i + e + 1];
+        for (int e = 0; e < 16; e += 2) {
+          float x = s[16 * i + e], y = s[16 * i + e + 1];
           fma2(x, y, a.c, less);
           x = ex2(x);
           y = ex2(y);
           add2(sum0, sum1, x, y);
           p[e / 2] = pack2(x, y, (const T*)nullptr);
         }
-        uint32_t p0[8], p1[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p0[e] = p[e], p1[e] = p[8 + e];
-        tmem_st_32x32b_x8(s_at + 16 * i, p0);
-        tmem_st_32x32b_x8(s_at + 16 * i + 8, p1);
+        tmem_st_32x32b_x8(s_at + 8 * i, p);
       }
       tmem_wait_st();
       if (cut) {
         // A weight of 0 does not silence an infinity or NaN in a value that its row does not see. Such
-        // values of keys past the sequence's end, which no row sees, become 0; for others this block's
+        // values of keys past the sequence's end, which no row sees, become 0; for others this step's
         // product is made here, over what each row sees.
-        const int block = j - lo, blocks = hi - lo;
-        const int unit = min(C::kAhead + 2 * block, blocks + block) * C::kPer;   // as they are loaded
-        ok = wait(&ctl.v_here[t], n & 1, ctl, a.err, 39);
+        const int block = (i0 + n) / C::kSub - lo, blocks = hi - lo;
+        const int unit = units + min(C::kAhead + 2 * block, blocks + block) * C::kPer;   // as they are loaded
+        ok = wait(&ctl.v_here[t], (blocks_seen + n / C::kSub) & 1, ctl, a.err, 39);
         for (int p = 0; p < C::kPer && ok; ++p)
           ok = wait(&ctl.full[(unit + p) % C::kUnits], (uint32_t)((unit + p) / C::kUnits) & 1, ctl, a.err, 40);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint32_t most = 0;                           // of the bits of key r's values, in halves
+        // the tile's threads share the keys: this one's 16-byte pieces of key k's values, in an order free of
+        // bank conflicts
+        constexpr int kMine = HDP / 8 * C::kKeys / 128, kTurn = kMine < 8 ? kMine : 8;
+        const int k = r % C::kKeys, first = r / C::kKeys * kMine;
+        uint8_t* const rows = smem + C::kTiles * C::kQ + ((i0 + n) % C::kSub * C::kKeys + k) * 128;
+        const auto piece = [&](int i) {
+          const int x = first + (i & ~(kTurn - 1)) + ((i + k) & (kTurn - 1));     // of HDP / 8
+          return reinterpret_cast<uint4*>(rows + (unit + (x >> 4)) % C::kUnits * C::kUnit + ((x >> 3) & 1) * 16384 + ((x & 7) << 4));
+        };
+        uint32_t most = 0;                           // the largest bits, in halves
 #pragma unroll
-        for (int i = 0; i < HDP / 8; ++i) {
-          const int part = i >> 3;                   // 64 values; their 16-byte pieces in an order free of conflicts
-          const uint4 x = *reinterpret_cast<const uint4*>(smem + C::kTiles * C::kQ + (unit + part / 2) % C::kUnits * C::kUnit +
-                                                          (part & 1) * 16384 + r * 128 + (((i + r) & 7) << 4));
+        for (int i = 0; i < kMine; ++i) {
+          const uint4 x = *piece(i);
           most = __vmaxu2(most, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu),
                                          __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
         }
@@ -597,85 +715,99 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         const bool found = any_of_tile(odd, t, votes, ctl, a.err, ok);
         if (!ok) break;
         if (found) {
-          const bool past = key0 + r >= w.klen;
+          const bool past = key0 + k >= w.klen;
           if (odd && past)
-            for (int i = 0; i < HDP / 8; ++i)
-              *reinterpret_cast<uint4*>(smem + C::kTiles * C::kQ + (unit + (i >> 4)) % C::kUnits * C::kUnit +
-                                        ((i >> 3) & 1) * 16384 + r * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kMine; ++i) *piece(i) = make_uint4(0, 0, 0, 0);
           fence_async_proxy();
           skip = any_of_tile(odd && !past, t, votes, ctl, a.err, ok);
           if (!ok) break;
           if (skip) {
-            if (n > 0) ok = __all_sync(0xffffffffu, wait(&ctl.o_done[t], (uint32_t)(n - 1) & 1, ctl, a.err, 41));
+            if (n > 0) ok = done_before(41);
             if (!ok) break;
             tc_fence_after();
-            add_seen<HDP, T>(o_at, s_at, (const T*)a.v + (w.k0 + (int64_t)key0) * a.v_row + kvh * a.v_head, a.v_row, a.hd, l, h);
+            add_seen<HDP, T>(o_at, s_at, (const T*)a.v + (w.k0 + (int64_t)key0) * a.v_row + kvh * a.v_head, a.v_row, a.hd, l, h,
+                             n == 0);
           }
         }
       }
       tc_fence_before();
-      if (r == 0) *(volatile int*)&ctl.skip[buf] = skip;
+      if (r == 0) *(volatile int*)&ctl.skip[t][buf] = skip;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.p_full[buf]);
+      if (lane == 0) mbar_arrive(&ctl.p_full[t][buf]);
     }
-    // the last block's product; with two score buffers the one before it may be on its way too
-    for (int n = max(j1 - j0 - C::kAhead, 0); n < j1 - j0 && ok; ++n)
-      ok = __all_sync(0xffffffffu, wait(&ctl.o_done[t], (uint32_t)n & 1, ctl, a.err, 38));
-    if (ok) {
+    if (!ok) break;
+    units += 2 * (hi - lo) * C::kPer;
+    blocks_seen += steps / C::kSub;
+    if (steps > 0) {                                 // the last step's product, and all before it
+      ok = __all_sync(0xffffffffu, wait(&ctl.o_done[t][(g - 1) & 1], ((g - 1) >> 1) & 1, ctl, a.err, 38));
+      if (!ok) break;
       tc_fence_after();
-      const float sum = sum0 + sum1;
-      const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);      // NaN stays
-      const int64_t row = w.q0 + tok;
-      if (a.splits > 1 && mine)
-        a.lse[((int64_t)blockIdx.y * a.rows + row) * a.heads + head] = sum > 0.f ? lg2(sum) + ref - shift : (sum == 0.f ? -INFINITY : sum);
+    }
+    const float sum = sum0 + sum1;
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // NaN stays
+    const int64_t row = w.q0 + tok;
+    if (a.splits > 1 && mine)
+      a.lse[((int64_t)w.split * a.rows + row) * a.heads + head] = sum > 0.f ? lg2(sum) + ref - shift : (sum == 0.f ? -INFINITY : sum);
 #pragma unroll 1
-      for (int d = 0; d < HDP; d += 32) {
-        float o[32];
-        if (j1 > j0) {
-          tmem_load32(o_at + d, o);
-          tmem_arrived<32>(o);
+    for (int d = 0; d < HDP; d += 32) {
+      float o[32];
+      if (steps > 0) {
+        tmem_load32(o_at + d, o);
+        tmem_arrived<32>(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] *= inv;
+      if (mine) {
+        if (a.splits > 1) {
+          float* p = a.part + (((int64_t)w.split * a.rows + row) * a.heads + head) * a.hd + d;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (d + i < a.hd) {
+              uint32_t x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(o[i + e]);
+              store32(p + i, x);
+            }
         } else {
+          T* p = (T*)a.out + row * a.o_row + head * a.o_head + d;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
+          for (int i = 0; i < 32; i += 16) {
+            uint32_t x[8];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= inv;
-        if (mine) {
-          if (a.splits > 1) {
-            float* p = a.part + (((int64_t)blockIdx.y * a.rows + row) * a.heads + head) * a.hd + d;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (d + i < a.hd) *reinterpret_cast<float4*>(p + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          } else {
-            T* p = (T*)a.out + row * a.o_row + head * a.o_head + d;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              if (d + i < a.hd)
-                *reinterpret_cast<uint4*>(p + i) =
-                    make_uint4(pack2(o[i], o[i + 1], p), pack2(o[i + 2], o[i + 3], p), pack2(o[i + 4], o[i + 5], p),
-                               pack2(o[i + 6], o[i + 7], p));
+            for (int e = 0; e < 8; ++e) x[e] = pack2(o[i + 2 * e], o[i + 2 * e + 1], p);
+            if (a.wide) {                            // (values come in sixteens then)
+              if (d + i < a.hd) store32(p + i, x);
+            } else {
+              if (d + i < a.hd) *reinterpret_cast<uint4*>(p + i) = make_uint4(x[0], x[1], x[2], x[3]);
+              if (d + i + 8 < a.hd) *reinterpret_cast<uint4*>(p + i + 8) = make_uint4(x[4], x[5], x[6], x[7]);
+            }
           }
         }
       }
+    }
+    tc_fence_before();                               // O is read before the next tile's products overwrite it
     }
     tc_fence_before();
   }
   __syncwarp();
   __syncthreads();                                   // every role has ended
   if (*(volatile int*)&ctl.abort) {                  // a wait gave up: loads and MMAs in flight land first
-    if (warp == C::kSoft / 32 && lane == 0) {
+    if (warp == kLoad && lane == 0) {
       for (int u = issued > C::kUnits ? issued - C::kUnits : 0; u < issued; ++u)
         settle(&ctl.full[u % C::kUnits], (uint32_t)(u / C::kUnits) & 1);
-      if (hi > lo)
-        for (int t = 0; t < C::kTiles; ++t) settle(&ctl.q_full[t], 0);
+      if (q_loads > 0)
+        for (int t = 0; t < C::kTiles; ++t) settle(&ctl.q_full[t], (uint32_t)(q_loads - 1) & 1);
     }
-    if (warp == C::kSoft / 32 + 1 && lane == 0) {
+    if (warp >= kMma && elect_one_sync()) {          // the lane that issued
       mma_commit(&ctl.drain);
       settle(&ctl.drain, 0);
     }
     __syncthreads();
   }
-  if (warp == C::kSoft / 32) {
+  if (warp == kLoad) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -821,11 +953,12 @@ extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v
   const Plan p = plan_of(rows, kv_rows, seqs, heads, kv_heads, head_dim, window);
   FBFP_CHECK_ARG(p.ctas <= 0x7FFFFFFF, "too many rows");
   const int64_t need = fbfp_prompt_attention_workspace_bytes(rows, kv_rows, seqs, heads, kv_heads, head_dim, window);
-  FBFP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
-                 "the workspace must be %lld bytes, 16-byte aligned", (long long)need);
+  FBFP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 31) == 0),
+                 "the workspace must be %lld bytes, 32-byte aligned", (long long)need);
   const int group = (int)(heads / kv_heads);
   if (window > (1 << 30)) window = 1 << 30;          // no longer than any sequence
-  PromptArgs a{rows, kv_rows, o_row, o_head, v_row, v_head, window, starts, kv_starts ? kv_starts : starts, (int)seqs, (int)heads,
+  PromptArgs a{rows, kv_rows, o_row, o_head, v_row, v_head, window, starts, kv_starts ? kv_starts : starts,
+               head_dim % 16 == 0 && ((uintptr_t)out & 31) == 0 && ((o_row | o_head) & 15) == 0, (int)seqs, (int)heads,
                (int)head_dim, p.hp, p.ntok, p.head_blocks, group, p.splits,
                fmaxf(fabsf(scaling) * 1.4426950408889634f, 1e-30f), scaling < 0.f ? 1u : 0u, v, out, (float*)workspace,
                (float*)workspace + p.splits * rows * heads * head_dim, err};

@@ -34,6 +34,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
+// Whether the phase with the given parity is complete, at once.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 // Same, but the thread may be suspended in hardware for up to `hint_ns` nanoseconds while the
 // phase is incomplete (it resumes when the phase completes), so waiting warps do not take issue
 // slots from working warps.
@@ -52,6 +62,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
   for (uint32_t i = 0; i < limit; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return false;
+}
+
+__device__ __forceinline__ uint64_t globaltimer_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+  return t;
+}
+// Wait for a phase for about a second, giving up early once `*gave_up` is set. No suspension hint: a
+// hinted wait sleeps in steps that cost a short wait some hundred cycles. The clock, slow to read, is
+// looked at only after many polls.
+__device__ __forceinline__ bool mbar_wait_second(uint64_t* bar, uint32_t parity, const volatile int* gave_up) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*gave_up || globaltimer_ns() - t0 > 1000000000ull) return false;
+  }
 }
 
 // ---------------------------------------------------------------- bulk copies

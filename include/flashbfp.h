@@ -442,7 +442,7 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
  *   by `starts`), all bf16 or all fp16, out of the same type. Of a sequence with n rows and c >= n
  *   keys, row i stands at place c - n + i and attends to keys up to its place (the last `window` of
  *   those); rows that see no key give 0. Pointers 16-byte aligned, strides multiples of 8.
- *   `workspace`: fbfp_prompt_attention_workspace_bytes(...) bytes as above.
+ *   `workspace`: fbfp_prompt_attention_workspace_bytes(...) bytes as above, 32-byte aligned.
  * ---------------------------------------------------------------------------------- */
 typedef struct fbfp_kv4_cache {
   void *k_values, *k_scales, *v_values, *v_scales;
