@@ -23,15 +23,21 @@ GeGLU activation leave as e4m3 rows with their scales, which the next linear mul
 are; the attention output is rounded to bf16 and quantised by a launch of its own. Activations
 are rounded to e4m3 there (2^-4 relative at most);
 the residual stream, attention, norms and lm_head keep the precision they have otherwise.
+
+With ``kv_cache="int4"`` keys and values are held in 4 bits (``kv4.py``), and a context may be as long as
+memory allows (the bf16 cache's attention holds a row's scores in shared memory: max_ctx + 8 head_dim <=
+10000). A token step appends and attends in 4 bits; prompt chunks, of several sequences at once, are
+written, the context that they see is read back, and ``attention.prompt_attention`` runs over it: every
+row attends to what the cache holds, whichever way it went in.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
-from . import _lib, fp8
+from . import _lib, attention, fp8, kv4
 from .linear import packed_linear, packed_linear_allreduce
 from .packed import PackedWeight, concat_rows
 
@@ -98,7 +104,11 @@ class GemmaDecoder:
 
     def __init__(self, shape: DecoderShape, layers: List[DecodeLayer], embed: torch.Tensor,
                  final_norm: torch.Tensor, lm_head: torch.Tensor, max_ctx: int, device=None,
-                 max_prefill: int = 128, reducer=None, vocab_offset: int = 0, batch: int = 1):
+                 max_prefill: int = 128, reducer=None, vocab_offset: int = 0, batch: int = 1,
+                 kv_cache: str = "bf16"):
+        if kv_cache not in ("bf16", "int4"):
+            raise ValueError(f"kv_cache must be 'bf16' or 'int4', not {kv_cache!r}")
+        self.int4 = kv_cache == "int4"
         self.L = _lib.lib()
         self.shape, self.layers = shape, layers
         dev = torch.device(device) if device is not None else embed.device
@@ -109,7 +119,9 @@ class GemmaDecoder:
         self.rank = reducer.rank if reducer is not None else 0
         if len(layers) != len(s.layer_types):
             raise ValueError(f"{len(layers)} layers but {len(s.layer_types)} layer types")
-        if s.head_dim % 16 or s.head_dim > 256 or max_ctx + 8 * s.head_dim > 10000:
+        if self.int4 and (s.head_dim % 16 or s.head_dim > 256 or max_ctx < 1):
+            raise ValueError("head_dim must be a multiple of 16 up to 256, and max_ctx at least 1")
+        if not self.int4 and (s.head_dim % 16 or s.head_dim > 256 or max_ctx + 8 * s.head_dim > 10000):
             raise ValueError("head_dim must be a multiple of 16 up to 256, and max_ctx + 8 * head_dim "
                              "at most 10000")
         if s.n_heads % self.world or s.n_kv_heads % self.world:
@@ -150,9 +162,17 @@ class GemmaDecoder:
         B = self.batch = int(batch)
         if not 1 <= B <= 64:
             raise ValueError(f"batch {B} outside [1, 64]")
-        cache = (len(layers), B, self.hkv, self.max_ctx, s.head_dim)      # per layer and sequence
-        self.k_cache = torch.zeros(cache, **bf)
-        self.v_cache = torch.zeros(cache, **bf)
+        if self.int4:
+            self.cache4 = [kv4.empty_cache(B, self.hkv, self.max_ctx, s.head_dim, dev) for _ in layers]
+            if self.cache4 and self.cache4[0].positions > self.max_ctx:   # the cache rounds up; angles for all of it
+                for kind, theta in (("sliding_attention", s.rope_theta_local), ("full_attention", s.rope_theta_global)):
+                    self.rope[kind] = rope_tables(theta, s.head_dim, self.cache4[0].positions, dev)
+            self.back: List[Optional[torch.Tensor]] = [None, None]        # keys and values read back for a chunk
+            self.reach = [0] * B                                 # positions of each sequence, as the host counts them
+        else:
+            cache = (len(layers), B, self.hkv, self.max_ctx, s.head_dim)  # per layer and sequence
+            self.k_cache = torch.zeros(cache, **bf)
+            self.v_cache = torch.zeros(cache, **bf)
         self.seq_stride = self.hkv * self.max_ctx * s.head_dim
         self.max_rows = max(1, int(max_prefill))             # rows of a prompt chunk
         R = max(self.max_rows, B)
@@ -183,9 +203,10 @@ class GemmaDecoder:
         self.ids = torch.zeros(R, dtype=torch.int64, device=dev)    # a prompt chunk's ids
         self.tok = torch.zeros(B, dtype=torch.int64, device=dev)    # per sequence: current / next token
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)    # per sequence: its position
-        self.attn_scratch = torch.zeros(
-            self.L.fbfp_decode_attention_step_scratch_bytes(B, self.hq, s.head_dim, self.max_ctx),
-            dtype=torch.uint8, device=dev)
+        if not self.int4:
+            self.attn_scratch = torch.zeros(
+                self.L.fbfp_decode_attention_step_scratch_bytes(B, self.hq, s.head_dim, self.max_ctx),
+                dtype=torch.uint8, device=dev)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(dev)
@@ -194,11 +215,12 @@ class GemmaDecoder:
     # -- construction from a Hugging Face Gemma-3 model after compress_gemma_model -----------
     @classmethod
     def from_hf(cls, model, max_ctx: int, device=None, max_prefill: int = 128,
-                reducer=None, batch: int = 1, weights: str = "oabf") -> "GemmaDecoder":
+                reducer=None, batch: int = 1, weights: str = "oabf", kv_cache: str = "bf16") -> "GemmaDecoder":
         """The decoder of a Gemma-3 causal LM after ``compress_gemma_model``; with ``reducer``,
         of a model compressed with ``compress_gemma_model(..., rank=r, world=reducer.world)``
         on every rank (this rank's shards; lm_head rows split here). ``weights="fp8"``: of an
-        uncompressed model, its attention and MLP linears quantised to block-scaled 8 bits here."""
+        uncompressed model, its attention and MLP linears quantised to block-scaled 8 bits here.
+        ``kv_cache="int4"``: keys and values held in 4 bits."""
         if weights not in ("oabf", "fp8"):
             raise ValueError(f"weights must be 'oabf' or 'fp8', not {weights!r}")
         if weights == "fp8" and reducer is not None:
@@ -263,7 +285,8 @@ class GemmaDecoder:
         elif any(hasattr(m, "tp_mode") for m in model.modules()):
             raise ValueError("the model holds tensor-parallel shards: pass the reducer")
         return cls(shape, layers, inner.embed_tokens.weight.data, inner.norm.weight.data,
-                   lm_head, max_ctx, dev, max_prefill, reducer=reducer, vocab_offset=v0, batch=batch)
+                   lm_head, max_ctx, dev, max_prefill, reducer=reducer, vocab_offset=v0, batch=batch,
+                   kv_cache=kv_cache)
 
     # -- one token ---------------------------------------------------------------------------
     def _linear(self, x, pw, out: torch.Tensor) -> None:
@@ -307,10 +330,54 @@ class GemmaDecoder:
         """The first m rows of a buffer of 8-bit rows."""
         return fp8.Fp8Rows(r.values[:m], r.scales[:-(-m // 128)])
 
-    def _layers(self, m: int, chunk_seq: Optional[int]) -> None:
+    def _chunk4(self, lens: Sequence[int]) -> Dict[str, Tuple[torch.Tensor, torch.Tensor, int]]:
+        """What the layers of a packed prompt chunk need (lens: rows of each sequence): where its rows begin, and
+        per kind of layer the first cached position that they see of each sequence, where those rows begin
+        when they are read back, and a bound of how many there are."""
+        s, dev = self.shape, self.device
+        n = torch.tensor(list(lens), dtype=torch.int32).to(dev)
+        zero = torch.zeros(1, dtype=torch.int32, device=dev)
+
+        def starts(x):
+            return torch.cat((zero, x.cumsum(0, dtype=torch.int32)))
+
+        plan = {"starts": (starts(n), n, sum(lens))}
+        for kind in set(s.layer_types):
+            window = s.sliding_window if kind == "sliding_attention" else 0
+            first = (self.pos + (1 - window)).clamp_min(0) if window else torch.zeros_like(self.pos)
+            seen = torch.where(n > 0, self.pos + n - first, torch.zeros_like(n))
+            rows = sum(min(r, window - 1) + m if window else r + m for r, m in zip(self.reach, lens) if m)
+            plan[kind] = (first, starts(seen), rows)
+            self.err.masked_fill_(seen.sum() > rows, 2)      # positions that were not set through reset()
+        most = max(plan[kind][2] for kind in set(s.layer_types)) if s.layer_types else 0
+        if most and (self.back[0] is None or self.back[0].shape[0] < most):
+            room = min(self.batch * self.cache4[0].positions, -(-most // 1024) * 1024)
+            self.back = [torch.empty(max(room, most), self.hkv, s.head_dim, dtype=torch.bfloat16, device=dev)
+                         for _ in range(2)]
+        return plan
+
+    def _attend4(self, li: int, ly: DecodeLayer, qkv, q, attn, m: int, plan) -> None:
+        """Attention of layer li over the 4-bit cache: plan None for a token step, else _chunk4's."""
+        s = self.shape
+        kind = s.layer_types[li]
+        cos_t, sin_t = self.rope[kind]
+        window = s.sliding_window if kind == "sliding_attention" else 0
+        cache, eps = self.cache4[li], float(s.rms_norm_eps)
+        q3, o3 = q.view(m, self.hq, s.head_dim), attn.view(m, self.hq, s.head_dim)
+        starts = None if plan is None else plan["starts"][0]
+        kv4.kv4_append(cache, qkv, ly.q_norm, ly.k_norm, eps, cos_t, sin_t, self.pos, q3, starts=starts, err=self.err)
+        if plan is None:
+            kv4.kv4_attention(q3, cache, self.pos, window=window, scaling=self.scaling, out=o3, err=self.err)
+            return
+        first, back_starts, rows = plan[kind]
+        k, v = kv4.kv4_read(cache, first, back_starts, out=[t[:rows] for t in self.back], err=self.err)
+        attention.prompt_attention(q3, k, v, starts, kv_starts=back_starts, window=window, scaling=self.scaling, out=o3,
+                                   err=self.err)
+
+    def _layers(self, m: int, chunk_seq: Optional[int], plan=None) -> None:
         """Every layer over rows 0..m-1 of the activation buffers: with chunk_seq = b, a prompt
         chunk of sequence b at positions pos[b] .. pos[b] + m - 1 (causal over the chunk);
-        with chunk_seq = None, one new token per sequence (m = batch)."""
+        with chunk_seq = None, one new token per sequence (m = batch), or the packed rows of ``plan``."""
         L, s, st = self.L, self.shape, _lib.stream_ptr(self.device)
         P = _lib.ptr
         eps = float(s.rms_norm_eps)
@@ -323,7 +390,9 @@ class GemmaDecoder:
             cos_t, sin_t = self.rope[kind]
             window = s.sliding_window if kind == "sliding_attention" else 0
             self._linear(x8 if self.fp8 else x, ly.qkv, qkv)
-            if chunk_seq is None:
+            if self.int4:
+                self._attend4(li, ly, qkv, q, attn, m, plan)
+            elif chunk_seq is None:
                 _lib.check(L.fbfp_decode_attention_step(
                     P(qkv), m, self.hq, self.hkv, s.head_dim, P(ly.q_norm), P(ly.k_norm), eps, P(cos_t),
                     P(sin_t), P(self.pos), self.max_ctx, P(self.k_cache[li]), P(self.v_cache[li]),
@@ -371,6 +440,9 @@ class GemmaDecoder:
     def _enqueue(self, m: int, seq: int = 0) -> None:
         """A prompt chunk of m tokens (self.ids[:m]) of sequence seq: every layer, then the logits
         of the last row into self.logits[seq], the greedy pick into self.tok[seq] and pos[seq] += m."""
+        if self.int4:
+            self._enqueue_packed([m if b == seq else 0 for b in range(self.batch)])
+            return
         self._embed(self.ids, m)
         self._layers(m, seq)
         torch.matmul(self.x[m - 1:m], self.lm_head.t(), out=self.logits[seq:seq + 1])   # bf16 lm_head
@@ -378,6 +450,31 @@ class GemmaDecoder:
                    self.pick[seq:seq + 1] if self.reducer is not None else None)
         _lib.check(self.L.fbfp_advance_position(_lib.ptr(self.pos[seq:seq + 1]), m, _lib.stream_ptr(self.device)),
                    "fbfp_advance_position")
+
+    def _enqueue_packed(self, lens: Sequence[int]) -> None:
+        """A packed prompt chunk (4-bit cache): self.ids holds lens[b] tokens of each sequence b back to back;
+        logits, picks and positions of the sequences that have some."""
+        m = sum(lens)
+        self._embed(self.ids, m)
+        plan = self._chunk4(lens)
+        self._layers(m, None, plan)
+        some = [b for b, n in enumerate(lens) if n]
+        ends, at = [], 0
+        for n in lens:
+            at += n
+            if n:
+                ends.append(at - 1)
+        seqs = torch.tensor(some, dtype=torch.int64).to(self.device)
+        rows = self.x[torch.tensor(ends, dtype=torch.int64).to(self.device)]
+        logits = torch.matmul(rows, self.lm_head.t())                        # bf16 lm_head
+        self.logits[seqs] = logits
+        tok = self.tok[seqs]
+        slots = torch.empty_like(self.pick[:len(some)]) if self.reducer is not None else None
+        self._pick(logits, tok, slots)
+        self.tok[seqs] = tok
+        self.pos += plan["starts"][1]
+        for b, n in enumerate(lens):
+            self.reach[b] += n
 
     def _enqueue_step(self) -> None:
         """One new token for every sequence: tokens self.tok at positions self.pos; leaves the
@@ -403,6 +500,21 @@ class GemmaDecoder:
             self.ids[:m].copy_(torch.as_tensor(list(ids), dtype=torch.int64), non_blocking=False)
             self._enqueue(m, seq)
 
+    def prefill_packed(self, chunks: Sequence[Sequence[int]]) -> None:
+        """Run prompt chunks of several sequences in one pass (4-bit cache): ``chunks`` holds one list of ids per
+        sequence, some of them empty, at most max_prefill in all; sequence b's go to positions pos[b] on, as
+        ``prefill`` does for one."""
+        if not self.int4:
+            raise ValueError("packed prompts need kv_cache='int4'")
+        lens = [len(c) for c in chunks]
+        if len(lens) != self.batch or not 1 <= sum(lens) <= self.max_rows:
+            raise ValueError(f"one chunk per sequence ({self.batch}), 1..{self.max_rows} tokens in all "
+                             f"(got {len(lens)} with {sum(lens)})")
+        with torch.cuda.device(self.device), torch.cuda.stream(self.stream):
+            ids = [int(t) for c in chunks for t in c]
+            self.ids[:len(ids)].copy_(torch.as_tensor(ids, dtype=torch.int64), non_blocking=False)
+            self._enqueue_packed(lens)
+
     def reset(self, pos=0) -> None:
         """Set the positions (an int for every sequence, or one per sequence) and clear the error
         word, in order with the decoder's stream."""
@@ -412,6 +524,8 @@ class GemmaDecoder:
             else:
                 self.pos.copy_(torch.as_tensor(list(pos), dtype=torch.int32), non_blocking=False)
             self.err.zero_()
+        if self.int4:
+            self.reach = [pos] * self.batch if isinstance(pos, int) else [int(p) for p in pos]
 
     def capture(self) -> None:
         """Record one token step as a CUDA graph (after one eager step that sets the kernels up;
@@ -435,6 +549,8 @@ class GemmaDecoder:
                 self.graph.replay()
             else:
                 self._enqueue_step()
+        if self.int4:
+            self.reach = [r + 1 for r in self.reach]
 
     def check(self) -> None:
         """Raise if a kernel met an out-of-range token (1) or position (2)."""
@@ -458,9 +574,19 @@ class GemmaDecoder:
         if max(len(p) for p in prompts) + n_new > self.max_ctx or min(len(p) for p in prompts) < 1:
             raise ValueError("prompt + new tokens exceed the KV cache (or a prompt is empty)")
         self.reset(0)
-        for b, p in enumerate(prompts):
-            for i in range(0, len(p), self.max_rows):
-                self.prefill(p[i:i + self.max_rows], seq=b)
+        if self.int4:                              # several sequences' rows in one pass
+            left = [list(p) for p in prompts]
+            while any(left):
+                room, chunks = self.max_rows, []
+                for p in left:
+                    chunks.append(p[:room])
+                    room -= len(chunks[-1])
+                self.prefill_packed(chunks)
+                left = [p[len(c):] for p, c in zip(left, chunks)]
+        else:
+            for b, p in enumerate(prompts):
+                for i in range(0, len(p), self.max_rows):
+                    self.prefill(p[i:i + self.max_rows], seq=b)
         out = [[] for _ in prompts]
         for _ in range(n_new):
             self.stream.synchronize()

@@ -13,14 +13,15 @@ cache is skipped and recorded (``check_device_errors`` raises it). Forward only,
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
-from . import device_errors
+from . import _lib, device_errors
 from .device_errors import check as check_device_errors
 
-__all__ = ["KV4Cache", "empty_cache", "kv4_write", "kv4_read", "kv4_attention", "check_device_errors"]
+__all__ = ["KV4Cache", "empty_cache", "kv4_write", "kv4_append", "kv4_read", "kv4_attention", "check_device_errors"]
 
 
 class KV4Cache(NamedTuple):
@@ -62,6 +63,46 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tens
     to position pos[b] + r - starts[b]. ``starts`` (int32 [sequences + 1]) packs the rows of several
     sequences; without it there is one row per sequence. Rows from starts[-1] on are not written."""
     _module().kv4_write(cache, k, v, pos, starts, err)
+
+
+def kv4_append(cache: KV4Cache, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
+               cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, q_out: torch.Tensor,
+               starts: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> None:
+    """A decoder layer's step to the cache in one launch: of fused bf16 rows q | k | v [T, (heads + 2 kv_heads) D],
+    RMSNorm (weights 1 + w) of every q and k head, the rotary embedding with the bf16 rows cos, sin
+    [positions, D] at the row's position, q to q_out [T, heads, D], k and v into the cache as ``kv4_write``
+    puts them. D is a multiple of 16."""
+    values, d = cache.k_values, cache.head_dim
+    kvh = values.shape[1]
+    what = {"qkv": qkv, "q_norm": q_norm, "k_norm": k_norm, "cos": cos, "sin": sin, "q_out": q_out}
+    for name, t in what.items():
+        _lib.require_cuda(t, name)
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != values.device:
+            raise ValueError(f"{name} must be contiguous bfloat16 on {values.device}")
+    rows, heads = qkv.shape[0], qkv.shape[1] // d - 2 * kvh
+    if qkv.dim() != 2 or heads < 1 or qkv.shape[1] != (heads + 2 * kvh) * d or q_out.numel() != rows * heads * d:
+        raise ValueError(f"qkv {tuple(qkv.shape)} and q_out {tuple(q_out.shape)} do not hold heads of {d} beside "
+                         f"2 x {kvh}")
+    if q_norm.numel() != d or k_norm.numel() != d or cos.shape != sin.shape or cos.shape[1] != d:
+        raise ValueError("norm weights and cos / sin rows must have one value per value of a head")
+    if cos.shape[0] < cache.positions:
+        raise ValueError(f"cos and sin hold {cos.shape[0]} positions, the cache {cache.positions}")
+    for name, t, n in (("pos", pos, values.shape[0]), ("starts", starts, values.shape[0] + 1), ("err", err, 1)):
+        if t is not None and (t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != values.device):
+            raise ValueError(f"{name} must be {n} contiguous int32 on {values.device}")
+    if starts is None and rows != values.shape[0]:
+        raise ValueError(f"{rows} rows for {values.shape[0]} sequences: pass starts")
+    if rows == 0:
+        return
+    c = _lib.KV4CacheStruct(*(t.data_ptr() for t in cache[:4]), *values.shape[:3], d)
+    P = _lib.ptr
+    with torch.cuda.device(values.device):
+        word = P(err) if err is not None else device_errors.word(values.device.index)
+        _lib.check(_lib.lib().fbfp_kv4_append(ctypes.byref(c), P(qkv), rows, heads, P(q_norm), P(k_norm), float(eps),
+                                              P(cos), P(sin), P(pos), P(starts), P(q_out), word,
+                                              _lib.stream_ptr(values.device)), "fbfp_kv4_append")
+    for t in (*cache[:4], q_out):
+        torch.autograd.graph.increment_version(t)
 
 
 def kv4_read(cache: KV4Cache, first: torch.Tensor, starts: torch.Tensor, rows: Optional[int] = None,
