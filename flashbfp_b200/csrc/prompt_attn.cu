@@ -49,14 +49,19 @@ struct Cfg {
   static constexpr int kKeys = HDP <= 128 ? 64 : 128;
   static constexpr int kSub = kTile / kKeys;              // steps of a block
   static constexpr int kAhead = 2 / kSub;                 // blocks whose keys are loaded before the first values
-  static constexpr int kCols = HDP < 128 ? HDP : 128;     // values of a unit
-  static constexpr int kUnit = kTile * kCols * 2;        // a block's keys or values come in units
-  static constexpr int kPer = HDP / kCols;                // units per block
-  static constexpr int kUnits = HDP == 64 ? 8 : 5;        // depth of the ring
+  // A block's keys or values come in units. Up to 128 values a head: one unit. Up to 256: four units, of 64 of the
+  // keys' values, or of 64 keys and 128 values, each given back as soon as it is used: the ring holds little
+  // more than a block, and loads take as long as a block's products.
+  static constexpr bool kFine = HDP == 256;
+  static constexpr int kCols = HDP < 128 ? HDP : 128;     // values of a product's accumulator columns
+  static constexpr int kUnit = kFine ? 16384 : kTile * HDP * 2;
+  static constexpr int kPer = kFine ? 4 : 1;              // units per block
+  static constexpr int kUnits = HDP == 64 ? 8 : kFine ? 10 : 5;           // depth of the ring
+  static constexpr int kValueRows = kFine ? 64 : 128;     // keys of a unit of values
   static constexpr int kQ = kTile * HDP * 2;
   static constexpr int kSmem = kTiles * kQ + kUnits * kUnit + 1024;
   static constexpr int kSoft = 128 * kTiles;              // softmax threads
-  static constexpr int kThreads = kSoft + 32 + 32 * kTiles;
+  static constexpr int kThreads = kSoft + 96;
   static constexpr uint32_t kO = 256;                     // first column of O; scores at 0 and 128
 };
 
@@ -68,7 +73,7 @@ struct Work {
 };
 
 struct Ctl {
-  uint64_t q_full[2], q_empty, full[8], empty[8], s_full[2][2], p_full[2][2], v_here[2], o_done[2][2], voted[2], drain;
+  uint64_t q_full[2], q_empty, full[10], empty[10], s_full[2][2], p_full[2][2], v_here[2], o_done[2][2], voted[2], drain;
   uint64_t info_full[2], info_empty[2], next_full;
   uint4 next;                   // the answer to a request for another CTA's work
   Work info[2];                 // this tile's and the next one's, any = 0 behind the last
@@ -76,11 +81,27 @@ struct Ctl {
   int abort, skip[2][2], vote[2][4];
 };
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl& ctl, int32_t* err, int site) {
+// Out of line: the wait that does not end within some thousand polls.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, Ctl& ctl, int32_t* err, int site) {
   if (mbar_wait_second(bar, parity, &ctl.abort)) return true;
   *(volatile int*)&ctl.abort = 1;
   atomicExch(err, site);
   return false;
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl& ctl, int32_t* err, int site) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+      "LOOP_%=:\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE_%=;\n\t"
+      "add.u32 n, n, 1;\n\t"
+      "setp.lt.u32 q, n, 1024;\n\t"
+      "@q bra LOOP_%=;\n"
+      "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  if (__builtin_expect(ok != 0, 1)) return true;
+  return wait_long(bar, parity, ctl, err, site);
 }
 // After a wait gave up: what is in flight lands first (a bound of its own again, some 0.3 s).
 __device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
@@ -119,12 +140,12 @@ __device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
       ::"r"(smem_u32(bar)), "r"(one) : "memory");
 }
-// Values [128 keys][64] in 128-byte swizzled rows as the N-major operand: 8-key groups 1 KB apart,
-// 64-value parts 16 KB apart.
-__device__ __forceinline__ uint64_t desc_values(uint32_t saddr) {
+// Values [keys][64] in 128-byte swizzled rows as the N-major operand: 8-key groups 1 KB apart, 64-value parts
+// `part` bytes apart.
+__device__ __forceinline__ uint64_t desc_values(uint32_t saddr, uint32_t part) {
   uint64_t d = 0;
   d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(16384 >> 4) << 16;
+  d |= (uint64_t)(part >> 4) << 16;
   d |= (uint64_t)(1024 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
@@ -383,15 +404,15 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       mbar_init(&ctl.voted[i], 4);
       for (int k = 0; k < 4; ++k) ctl.vote[i][k] = 0;
       mbar_init(&ctl.info_full[i], 1);
-      mbar_init(&ctl.info_empty[i], kLoad + C::kTiles);
+      mbar_init(&ctl.info_empty[i], kLoad + 2);
     }
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 10; ++i) {
       mbar_init(&ctl.full[i], 1);
-      mbar_init(&ctl.empty[i], C::kTiles);
+      mbar_init(&ctl.empty[i], C::kTiles);           // (fine units are one warp's alone)
     }
     mbar_init(&ctl.q_empty, C::kTiles);
     mbar_init(&ctl.next_full, 1);
-    mbar_init(&ctl.drain, C::kTiles);
+    mbar_init(&ctl.drain, 2);
     ctl.abort = 0;
     fence_mbar_init();
   }
@@ -419,7 +440,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     return w;
   };
 
-  int issued = 0, q_loads = 0;                       // loading: units and queries issued
+  int issued = 0, q_loads = 0, last = -1;            // loading: units and queries issued; this lane's last unit
   if (warp == kLoad) {
     if (lane == 0) {
       prefetch_tmap(&M.q);
@@ -448,36 +469,47 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         Span span[C::kTiles];
         int lo, hi;
         spans_of(w, a, span, lo, hi);
-        if (lane == 0 && hi > lo && ok) {
-          const auto load_q = [&](int t) {
-            mbar_arrive_expect_tx(&ctl.q_full[t], q_bytes);
-            for (int c = 0; c < HDP / 64; ++c)
-              tma_3d_g2s(sq + t * C::kQ + c * 16384, &M.q, c * 64, head0, w.q0 + w.tok0 + t * a.ntok, smem_u32(&ctl.q_full[t]));
-          };
-          const auto load = [&](const CUtensorMap* map, int j) {        // the units of block j
-            for (int p = 0; p < C::kPer && ok; ++p) {
-              const int slot = issued % C::kUnits;
-              if (issued >= C::kUnits) ok = wait(&ctl.empty[slot], (uint32_t)(issued / C::kUnits - 1) & 1, ctl, a.err, 32);
-              if (!ok) return;
-              mbar_arrive_expect_tx(&ctl.full[slot], C::kUnit);
-              for (int c = 0; c < C::kCols / 64; ++c)
-                tma_3d_g2s(sring + slot * C::kUnit + c * 16384, map, p * C::kCols + c * 64, kvh, w.k0 + j * kTile,
-                           smem_u32(&ctl.full[slot]));
-              ++issued;
+        if (hi > lo && ok) {
+          // the units of block j, a lane each: one lane's waits and copies in a row would take as long as the
+          // products that they feed
+          const auto load = [&](const CUtensorMap* map, int j) {
+            bool here = true;
+            if (lane < C::kPer) {
+              const int u = issued + lane, slot = u % C::kUnits;
+              if (u >= C::kUnits) here = wait(&ctl.empty[slot], (uint32_t)(u / C::kUnits - 1) & 1, ctl, a.err, 32);
+              if (here) {
+                mbar_arrive_expect_tx(&ctl.full[slot], C::kUnit);
+                const uint32_t to = sring + slot * C::kUnit, bar = smem_u32(&ctl.full[slot]);
+                if constexpr (!C::kFine) {
+                  for (int c = 0; c < HDP / 64; ++c) tma_3d_g2s(to + c * 16384, map, c * 64, kvh, w.k0 + j * kTile, bar);
+                } else if (map == &M.k) {
+                  tma_3d_g2s(to, map, lane * 64, kvh, w.k0 + j * kTile, bar);
+                } else {
+                  for (int c = 0; c < 2; ++c)
+                    tma_3d_g2s(to + c * 8192, map, (lane & 1) * 128 + c * 64, kvh, w.k0 + j * kTile + (lane >> 1) * 64, bar);
+                }
+                last = u;
+              }
             }
+            ok = __all_sync(0xffffffffu, here);
+            issued += C::kPer;
           };
-          if (q_loads > 0) ok = wait(&ctl.q_empty, (uint32_t)(q_loads - 1) & 1, ctl, a.err, 45);
+          if (q_loads > 0) ok = __all_sync(0xffffffffu, wait(&ctl.q_empty, (uint32_t)(q_loads - 1) & 1, ctl, a.err, 45));
           if (ok) {
-            for (int t = 0; t < C::kTiles; ++t) load_q(t);
+            if (lane == 0)
+              for (int t = 0; t < C::kTiles; ++t) {
+                mbar_arrive_expect_tx(&ctl.q_full[t], q_bytes);
+                for (int c = 0; c < HDP / 64; ++c)
+                  tma_3d_g2s(sq + t * C::kQ + c * 16384, &M.q, c * 64, head0, w.q0 + w.tok0 + t * a.ntok, smem_u32(&ctl.q_full[t]));
+              }
             ++q_loads;
           }
           for (int j = lo; j < min(lo + C::kAhead, hi) && ok; ++j) load(&M.k, j);
           for (int j = lo; j < hi && ok; ++j) {
             load(&M.v, j);
-            if (j + C::kAhead < hi) load(&M.k, j + C::kAhead);
+            if (ok && j + C::kAhead < hi) load(&M.k, j + C::kAhead);
           }
         }
-        ok = __all_sync(0xffffffffu, ok);
       }
       // asked for when this tile's loads are under way, no sooner: whoever is done first takes the next
       if (lane == 0) {
@@ -490,6 +522,79 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       __syncwarp();
     }
     if (ok) tell(Work{0, 0, 0, 0, 0, 0, 0, 0});
+  } else if (warp >= kMma && C::kFine) {
+    // Two warps issue, one the scores, one the products with the values: waits for units in between would keep
+    // one from being ahead of the tensor cores. Each goes its way as a whole, one elected lane issues.
+    const bool of_scores = warp == kMma;
+    const uint32_t one = elect_one_sync();
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), ring = __shfl_sync(0xffffffffu, sring, 0);
+    const uint32_t id_s = idesc<T>(kTile, false) | (a.negate << 13), id_o = idesc<T>(C::kCols, true);
+    const uint64_t q_desc = smem_desc_sw128(__shfl_sync(0xffffffffu, sq, 0), 1024);
+    const uint64_t k_desc = smem_desc_sw128(ring, 1024), v_desc = desc_values(ring, C::kValueRows * 128);     // of slot 0
+    uint32_t units = 0, g = 0;                       // units of the tiles before, steps so far
+    int q_used = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int m = 0; ok; ++m) {
+      const Work w = next_work(m, ok);
+      if (!ok || !w.any) break;
+      Span span[C::kTiles];
+      int lo, hi;
+      spans_of(w, a, span, lo, hi);
+      const uint32_t blocks = hi - lo;
+      if (blocks == 0) continue;
+      if (of_scores) {
+        ok = __all_sync(0xffffffffu, wait(&ctl.q_full[0], q_used++ & 1, ctl, a.err, 34));
+        for (uint32_t j = 0; j < blocks && ok; ++j, ++g) {
+          // the product with the weights that the buffer held
+          if (g >= 2) ok = __all_sync(0xffffffffu, wait(&ctl.o_done[0][g & 1], ((g >> 1) - 1) & 1, ctl, a.err, 33));
+          uint32_t u = units + (j < 2 ? j : 2 * j - 1) * 4;
+          uint32_t slot = u % C::kUnits, parity = (u / C::kUnits) & 1;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            if (ok) ok = __all_sync(0xffffffffu, wait(&ctl.full[slot], parity, ctl, a.err, 33));
+            if (!ok) break;
+            if (p == 0) tc_fence_after();
+            const uint64_t qd = q_desc + (uint32_t)(p * 16384 / 16), kd = k_desc + slot * (C::kUnit / 16);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) mma_ss(one, base + (g & 1) * C::kKeys, qd + s * 2, kd + s * 2, id_s, p + s > 0);
+            commit(one, &ctl.empty[slot]);
+            if (++slot == C::kUnits) slot = 0, parity ^= 1;
+          }
+          if (ok) commit(one, &ctl.s_full[0][g & 1]);
+        }
+        if (ok) commit(one, &ctl.q_empty);
+      } else {
+        for (uint32_t j = 0; j < blocks && ok; ++j, ++g) {
+          uint32_t u = units + min(2 + 2 * j, blocks + j) * 4;
+          uint32_t slot = u % C::kUnits, parity = (u / C::kUnits) & 1;
+          bool skip = false;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {              // keys 64 (p / 2) on, values 128 (p % 2) on
+            if (ok) ok = __all_sync(0xffffffffu, wait(&ctl.full[slot], parity, ctl, a.err, 33));
+            if (!ok) break;
+            if (p == 0) {
+              // the softmax may look at the values; all their units, where it does
+              if (one) mbar_arrive(&ctl.v_here[0]);
+              ok = __all_sync(0xffffffffu, wait(&ctl.p_full[0][g & 1], (g >> 1) & 1, ctl, a.err, 35));
+              if (!ok) break;
+              tc_fence_after();
+              skip = __any_sync(0xffffffffu, *(volatile int*)&ctl.skip[0][g & 1]);
+            }
+            const uint64_t vd = v_desc + slot * (C::kUnit / 16);
+            if (!skip)
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                mma_ts(one, base + C::kO + (p & 1) * 128, base + (g & 1) * C::kKeys + ((p >> 1) * 4 + s) * 8, vd + s * 128, id_o,
+                       j > 0 || p > 1 || s > 0);
+            commit(one, &ctl.empty[slot]);
+            if (++slot == C::kUnits) slot = 0, parity ^= 1;
+          }
+          if (ok) commit(one, &ctl.o_done[0][g & 1]);
+        }
+      }
+      units += 2 * blocks * C::kPer;
+    }
   } else if (warp >= kMma) {
     const int t = warp - kMma;                       // this warp's tile
     // The whole warp goes the same way, one elected lane issues: descriptors stay in uniform registers.
@@ -497,7 +602,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), ring = __shfl_sync(0xffffffffu, sring, 0);
     const uint32_t id_s = idesc<T>(C::kKeys, false) | (a.negate << 13), id_o = idesc<T>(C::kCols, true);
     const uint64_t q_desc = smem_desc_sw128(__shfl_sync(0xffffffffu, sq, 0), 1024);
-    const uint64_t k_desc = smem_desc_sw128(ring, 1024), v_desc = desc_values(ring);     // of slot 0
+    const uint64_t k_desc = smem_desc_sw128(ring, 1024), v_desc = desc_values(ring, C::kValueRows * 128);     // of slot 0
     // The ring: the next unit's slot, and the parity of its phase.
     uint32_t slot = 0, parity = 0;
     uint32_t made = 0, met = 0;                      // steps: scores made, values met (buffer: the lowest bit)
@@ -524,7 +629,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       const uint32_t d = base + t * 128 + buf * C::kKeys;
 #pragma unroll
       for (int p = 0; p < C::kPer; ++p) {
-        const uint64_t qd = q_desc + (uint32_t)((t * C::kQ + p * 32768) / 16);
+        const uint64_t qd = q_desc + (uint32_t)(t * C::kQ / 16);
         const uint64_t kd = k_desc + after(u, p) * (C::kUnit / 16) + (uint32_t)(sub * (C::kKeys * 128) / 16);
 #pragma unroll
         for (int s = 0; s < C::kCols / 16; ++s) {
@@ -578,10 +683,11 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
           if (!ok) break;
           if (one && in) mbar_arrive(&ctl.v_here[t]);
         }
-        if (i + 2 < steps && (i + 2) % C::kSub == 0) uk = arrived();
-        if (ok && in) values(i % C::kSub, uv, i == from);
+        if (in) values(i % C::kSub, uv, i == from);
         if (!ok) break;
         if (i % C::kSub == C::kSub - 1) release(uv);
+        if (i + 2 < steps && (i + 2) % C::kSub == 0) uk = arrived();     // (keys are waited for no sooner than used)
+        if (!ok) break;
         if (i + 2 >= from && i + 2 < to) scores(i % C::kSub, uk);       // (two steps on: the same part)
         if (i + 2 < steps && (i + 2) % C::kSub == C::kSub - 1) release(uk);
         if (i + 3 == steps) commit(one, &ctl.q_empty);
@@ -698,10 +804,13 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         // bank conflicts
         constexpr int kMine = HDP / 8 * C::kKeys / 128, kTurn = kMine < 8 ? kMine : 8;
         const int k = r % C::kKeys, first = r / C::kKeys * kMine;
-        uint8_t* const rows = smem + C::kTiles * C::kQ + ((i0 + n) % C::kSub * C::kKeys + k) * 128;
+        const int key = (i0 + n) % C::kSub * C::kKeys + k;                        // of the block
+        uint8_t* const rows = smem + C::kTiles * C::kQ + key % C::kValueRows * 128;
+        const int unit_k = unit + key / C::kValueRows * 2;
         const auto piece = [&](int i) {
           const int x = first + (i & ~(kTurn - 1)) + ((i + k) & (kTurn - 1));     // of HDP / 8
-          return reinterpret_cast<uint4*>(rows + (unit + (x >> 4)) % C::kUnits * C::kUnit + ((x >> 3) & 1) * 16384 + ((x & 7) << 4));
+          return reinterpret_cast<uint4*>(rows + (unit_k + (x >> 4)) % C::kUnits * C::kUnit +
+                                          ((x >> 3) & 1) * (C::kValueRows * 128) + ((x & 7) << 4));
         };
         uint32_t most = 0;                           // the largest bits, in halves
 #pragma unroll
@@ -795,13 +904,14 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
   __syncwarp();
   __syncthreads();                                   // every role has ended
   if (*(volatile int*)&ctl.abort) {                  // a wait gave up: loads and MMAs in flight land first
-    if (warp == kLoad && lane == 0) {
-      for (int u = issued > C::kUnits ? issued - C::kUnits : 0; u < issued; ++u)
+    if (warp == kLoad) {
+      // a slot is loaded again only when its last load has been used: each lane's last units remain
+      for (int u = last; u >= 0 && u > last - C::kUnits; u -= C::kPer)
         settle(&ctl.full[u % C::kUnits], (uint32_t)(u / C::kUnits) & 1);
-      if (q_loads > 0)
+      if (q_loads > 0 && lane == 0)
         for (int t = 0; t < C::kTiles; ++t) settle(&ctl.q_full[t], (uint32_t)(q_loads - 1) & 1);
     }
-    if (warp >= kMma && elect_one_sync()) {          // the lane that issued
+    if (warp >= kMma && elect_one_sync()) {          // the lanes that issued
       mma_commit(&ctl.drain);
       settle(&ctl.drain, 0);
     }
@@ -966,7 +1076,7 @@ extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v
   PromptMaps m;
   int st = encode_rows(&m.q, dt, q, head_dim, heads, rows, q_head, q_row, p.hp, p.ntok);
   if (!st) st = encode_rows(&m.k, dt, k, head_dim, kv_heads, kv_rows, k_head, k_row, 1, kTile);
-  if (!st) st = encode_rows(&m.v, dt, v, head_dim, kv_heads, kv_rows, v_head, v_row, 1, kTile);
+  if (!st) st = encode_rows(&m.v, dt, v, head_dim, kv_heads, kv_rows, v_head, v_row, 1, head_dim > 128 ? 64 : kTile);
   if (st) return st;
   cudaStream_t s = as_stream(stream);
   if (head_dim <= 64) return dtype == FBFP_BF16 ? launch<64, __nv_bfloat16>(a, m, p, s) : launch<64, __half>(a, m, p, s);
