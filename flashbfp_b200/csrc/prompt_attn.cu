@@ -738,8 +738,13 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       bool skip = false;
       if (cut) {
 #pragma unroll
-        for (int i = 0; i < C::kKeys; ++i)
-          if (i > h || i < l) s[i] = -INFINITY;
+        for (int c = 0; c < C::kKeys; c += 32) {     // a bit for each key that is seen
+          const int up = h - c, down = l - c;
+          const uint32_t seen = (up >= 31 ? ~0u : up < 0 ? 0u : (2u << up) - 1) & (down <= 0 ? ~0u : down > 31 ? 0u : ~0u << down);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(seen >> i & 1)) s[c + i] = -INFINITY;
+        }
       }
       float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
