@@ -28,7 +28,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kTok = 32;                 // positions of a tile
-constexpr int kLeast = 16;               // tiles that are worth a CTA
+constexpr int kLeast = 12;               // tiles that are worth a CTA
 constexpr int kSms = 148;
 constexpr int kAccumulators = 8;         // 32 dims x 8 columns each, of a warp at most: 64 registers of a thread
 
@@ -65,45 +65,44 @@ __device__ __forceinline__ Reach reach_of(const Args& a, int b) {
 // so many tiles each (at least one, so that each item has a CTA). Where every item, cut into parts of kLeast
 // tiles, fits the SMs at once, a CTA takes one part (the list is padded to whole parts); else each CTA takes the
 // same length of the list, as many items or parts of items as that is. What a CTA does of one item
-// is a segment; segment number = CTA + item, each its own.
+// is a segment; segment number = CTA + item, each its own. (A cache has fewer than 2^26 tiles, so that the list
+// counts in 32 bits for up to 32 blocks of columns: the call checks.)
 struct Schedule {
   bool parts;
-  int64_t share, total;                  // tiles a CTA, of all (padded)
+  uint32_t share, total;                 // tiles a CTA, of all (padded)
 };
-__device__ __forceinline__ int64_t padded(int tiles, const Schedule& s) {
-  const int n = max(tiles, 1);
-  return s.parts ? (n + kLeast - 1) / kLeast * kLeast : n;
+__device__ __forceinline__ uint32_t padded(int tiles, bool parts) {
+  const uint32_t n = max(tiles, 1);
+  return parts ? (n + kLeast - 1) / kLeast * kLeast : n;
 }
-// By this warp.
-__device__ __forceinline__ Schedule schedule_of(const Args& a) {
-  int64_t total = 0, parts = 0;
+// By this warp. `mine`: the tiles of sequence `lane`.
+__device__ __forceinline__ Schedule schedule_of(const Args& a, int& mine) {
+  uint32_t total = 0, parts = 0;
   for (int b = threadIdx.x & 31; b < a.c.seqs; b += 32) {
-    const int n = max(reach_of(a, b).tiles, 1);
-    total += n;
-    parts += (n + kLeast - 1) / kLeast;
+    const int n = reach_of(a, b).tiles;
+    if (b < 32) mine = n;
+    total += padded(n, false);
+    parts += padded(n, true) / kLeast;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    parts += __shfl_xor_sync(0xffffffffu, parts, o);
-  }
-  const int64_t per = (int64_t)a.c.nkv * a.blocks;
-  total *= per, parts *= per;
-  if (parts <= a.slots) return {true, kLeast, parts * kLeast};
-  return {false, max((total + a.slots - 1) / a.slots, (int64_t)kLeast), total};
+  const uint32_t per = a.c.nkv * a.blocks;
+  total = __reduce_add_sync(0xffffffffu, total) * per;
+  parts = __reduce_add_sync(0xffffffffu, parts) * per;
+  if (parts <= (uint32_t)a.slots) return {true, kLeast, parts * kLeast};
+  return {false, max((total + a.slots - 1) / a.slots, (uint32_t)kLeast), total};
 }
 // The sequence that place `at` (below the total) of the list is in, and where its first item begins.
-__device__ __forceinline__ void find_sequence(const Args& a, const Schedule& s, int64_t at, int& seq, int64_t& begin) {
+__device__ __forceinline__ void find_sequence(const Args& a, const Schedule& s, uint32_t at, int mine, int& seq,
+                                              uint32_t& begin) {
   const int lane = threadIdx.x & 31;
-  const int64_t per = (int64_t)a.c.nkv * a.blocks;
-  int64_t before = 0;
+  const uint32_t per = a.c.nkv * a.blocks;
+  uint32_t before = 0;
   for (int b0 = 0; b0 < a.c.seqs; b0 += 32) {
     const int b = b0 + lane;
-    const int64_t n = b < a.c.seqs ? padded(reach_of(a, b).tiles, s) * per : 0;
-    int64_t sum = n;
+    const uint32_t n = b < a.c.seqs ? padded(b0 == 0 ? mine : reach_of(a, b).tiles, s.parts) * per : 0;
+    uint32_t sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
     const uint32_t who = __ballot_sync(0xffffffffu, at >= before + sum - n && at < before + sum);
@@ -122,10 +121,11 @@ struct Piece {
   int b, head, block;
 };
 
-template <int NG, int NT>
+template <int NG, int NT, int WARPS>
 struct Cfg {
-  // Two CTAs of six warps an SM: 168 registers a thread.
-  static constexpr int kCtas = 2, kWarps = 6, kThreads = kWarps * 32;
+  // Twelve warps an SM, 168 registers a thread: two CTAs of six, one's start and end beside the other's tiles; or
+  // one of twelve, where each CTA has a part of at most twelve tiles and the time is that of one tile.
+  static constexpr int kWarps = WARPS, kCtas = 12 / WARPS, kThreads = kWarps * 32;
   static constexpr int kValues = kTok * 16 * NG, kScales = kTok * 2 * NG;       // bytes of a tile, keys or values
   static constexpr int kMostDepth = NG > 6 ? 4 : 8;
   static constexpr int kEntry = kValues + kScales;          // keys and values of a tile are entries of their own
@@ -133,14 +133,14 @@ struct Cfg {
   static constexpr int kColumns = 8 * NT * 4;
   // of 228 KB shared memory an SM, 1 KB of it each CTA's own
   static constexpr int kMore = kFrag + kColumns + kWarps * 8 * kMostDepth + 16;  // barriers, the word that says that a wait gave up
-  static constexpr int kRoom = 115712 - kMore;
+  static constexpr int kMost = kCtas == 2 ? 115712 : 232448, kRoom = kMost - kMore;
   static constexpr int kFit = kRoom / (kWarps * kEntry);
   static constexpr int kDepth = kFit > kMostDepth ? kMostDepth : kFit;
   static constexpr int kRing = kWarps * kDepth * kEntry;
   static constexpr int kJoin = (kWarps * 8 * NT * (32 * NG + 4) + kWarps * 8 * NT * 2) * 4;      // where the warps join
   static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kMore;
   static_assert(kDepth >= 3, "keys, values and the next keys");
-  static_assert(kSmem <= 115712, "shared memory of a CTA");
+  static_assert(kSmem <= kMost, "shared memory of a CTA");
   static constexpr int kMask = NG == 8 ? 7 : NG == 4 ? 3 : NG == 2 ? 1 : 0;     // swizzle: 16-byte piece ^ 128-byte line
 };
 
@@ -263,11 +263,11 @@ __device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts) {
 
 // O += (p s) n of 32 positions. The weights p carry a power of two that brings (p s) into fp16's range.
 // CUT: some column does not see some position, whose scale may be anything.
-template <int NG, int NT, bool CUT>
+template <int NG, int NT, int WARPS, bool CUT>
 __device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float (&p)[2][NT][4],
                                            uint32_t vss, uint32_t vb, uint32_t half, int p0,
                                            const int (&at_c)[NT], const int (&low_c)[NT]) {
-  using C = Cfg<NG, NT>;
+  using C = Cfg<NG, NT, WARPS>;
   const int t = threadIdx.x & 3;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -311,10 +311,10 @@ __device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float
   }
 }
 
-template <int NG, int NT, typename T>
-__global__ void __launch_bounds__((Cfg<NG, NT>::kThreads), (Cfg<NG, NT>::kCtas))
+template <int NG, int NT, int WARPS, typename T>
+__global__ void __launch_bounds__((Cfg<NG, NT, WARPS>::kThreads), (Cfg<NG, NT, WARPS>::kCtas))
 kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
-  using C = Cfg<NG, NT>;
+  using C = Cfg<NG, NT, WARPS>;
   constexpr int kWarps = C::kWarps, kThreads = C::kThreads;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t smem[];   // (no other shared memory in front of it)
@@ -330,34 +330,35 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
     fence_mbar_init();
   }
   pdl_prologue();
-  const Schedule sch = schedule_of(a);
+  int tiles0 = 0;                                     // of sequence `lane`
+  const Schedule sch = schedule_of(a, tiles0);
   // a warp's ring: the values of all entries first (swizzled rows), then their scales; the keys and
   // the values of a tile are entries that follow each other
   uint64_t* bar = bars + warp * C::kDepth;
   uint8_t* const ring = smem + warp * C::kDepth * C::kValues;
   uint8_t* const ring_s = smem + kWarps * C::kDepth * C::kValues + warp * C::kDepth * C::kScales;
   int base = 0;                                       // entries of the segments before
-  const int64_t end = min((int64_t)(blockIdx.x + 1) * sch.share, sch.total);
+  const uint32_t end = min((blockIdx.x + 1) * sch.share, sch.total);
 #pragma unroll 1
-  for (int64_t at = (int64_t)blockIdx.x * sch.share; at < end;) {
+  for (uint32_t at = blockIdx.x * sch.share; at < end;) {
   Piece pc;
-  int64_t begin;
-  find_sequence(a, sch, at, pc.b, begin);
+  uint32_t begin;
+  find_sequence(a, sch, at, tiles0, pc.b, begin);
   const Reach reach = reach_of(a, pc.b);
   const int64_t pos = __ldg(a.pos + pc.b);
-  const int64_t n_item = padded(reach.tiles, sch);
-  const int64_t nth = (at - begin) / n_item, in_item = (at - begin) - nth * n_item;
+  const uint32_t n_item = padded(reach.tiles, sch.parts);
+  const uint32_t nth = (at - begin) / n_item, in_item = (at - begin) - nth * n_item;
   const int64_t item = (int64_t)pc.b * a.c.nkv * a.blocks + nth;
   pc.head = (int)(nth / a.blocks);
-  pc.block = (int)(nth - (int64_t)pc.head * a.blocks);
-  const int64_t length = min(n_item - in_item, end - at);
+  pc.block = (int)(nth - pc.head * a.blocks);
+  const uint32_t length = min(n_item - in_item, end - at);
   at += length;
   const bool whole = length == n_item;
   int t0, t1;                                         // tiles of the sequence
   if (sch.parts) {                                    // parts of even length
-    const int64_t parts = n_item / kLeast, part = in_item / kLeast;
-    t0 = reach.first + (int)(reach.tiles * part / parts);
-    t1 = reach.first + (int)(reach.tiles * (part + 1) / parts);
+    const uint32_t parts = n_item / kLeast, part = in_item / kLeast;
+    t0 = reach.first + (int)((uint64_t)reach.tiles * part / parts);
+    t1 = reach.first + (int)((uint64_t)reach.tiles * (part + 1) / parts);
   } else {
     t0 = reach.first + (int)in_item;
     t1 = reach.first + min((int)(in_item + length), reach.tiles);
@@ -566,8 +567,8 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
           l[n] += p[h][n][e];
         }
     }
-    if (cut) add_values<NG, NT, true>(o, p, vss, vb, half, p0, at_c, low_c);
-    else add_values<NG, NT, false>(o, p, vss, vb, half, p0, at_c, low_c);
+    if (cut) add_values<NG, NT, WARPS, true>(o, p, vss, vb, half, p0, at_c, low_c);
+    else add_values<NG, NT, WARPS, false>(o, p, vss, vb, half, p0, at_c, low_c);
     __syncwarp();
     if (lane == 0 && done + C::kDepth < 2 * mine) load(done + C::kDepth);
   }
@@ -624,7 +625,7 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
       r.x += x.x * fw, r.y += x.y * fw, r.z += x.z * fw, r.w += x.w * fw;
     }
     if (!whole) {
-      const int64_t to = (blockIdx.x + item) * (8 * NT) + c;
+      const int64_t to = ((int64_t)blockIdx.x + item) * (8 * NT) + c;
       *reinterpret_cast<float4*>(a.part + to * hd + d) = r;
       if (d == 0) a.ml[to * 2] = M, a.ml[to * 2 + 1] = L;
     } else {
@@ -655,19 +656,19 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Args a, int block_c
   const int64_t per_seq = (int64_t)a.c.nkv * a.columns;
   if (w >= per_seq * a.c.seqs) return;
   const int b = (int)(w / per_seq), rest = (int)(w - b * per_seq), head = rest / a.columns, col = rest % a.columns;
-  const Schedule sch = schedule_of(a);
-  const int64_t n_item = padded(reach_of(a, b).tiles, sch);
-  int64_t before = 0;
-  for (int i = lane; i < b; i += 32) before += padded(reach_of(a, i).tiles, sch);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  const int64_t nth = (int64_t)head * a.blocks + col / block_columns;
-  const int64_t begin = before * a.c.nkv * a.blocks + nth * n_item;
-  const int64_t first = begin / sch.share;
+  int tiles0;
+  const Schedule sch = schedule_of(a, tiles0);
+  const uint32_t n_item = padded(reach_of(a, b).tiles, sch.parts);
+  uint32_t before = 0;
+  for (int i = lane; i < b; i += 32) before += padded(reach_of(a, i).tiles, sch.parts);
+  before = __reduce_add_sync(0xffffffffu, before);
+  const uint32_t nth = head * a.blocks + col / block_columns;
+  const uint32_t begin = before * a.c.nkv * a.blocks + nth * n_item;
+  const uint32_t first = begin / sch.share;
   const int parts = (int)((begin + n_item - 1) / sch.share - first) + 1;
   if (parts == 1) return;
   const int64_t item = (int64_t)b * a.c.nkv * a.blocks + nth;
-  const int64_t from = (first + item) * block_columns + col % block_columns;
+  const int64_t from = ((int64_t)first + item) * block_columns + col % block_columns;
   float M = -INFINITY, L = 0.f, r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < parts; ++i) M = fmaxf(M, a.ml[(from + (int64_t)i * block_columns) * 2]);
   for (int i = 0; i < parts; ++i) {
@@ -703,8 +704,8 @@ int column_tiles(int64_t columns, int groups) {
 }
 
 struct Plan {
-  int nt, blocks, slots;
-  int64_t ctas, segments;
+  int nt, blocks, slots, warps;
+  int64_t ctas, segments, list;
   bool joins;
 };
 Plan plan_of(const Kv4& c, int64_t rows, int64_t heads, int64_t window) {
@@ -712,28 +713,32 @@ Plan plan_of(const Kv4& c, int64_t rows, int64_t heads, int64_t window) {
   const int64_t columns = rows * (heads / c.nkv);
   p.nt = column_tiles(columns, c.groups);
   p.blocks = (int)((columns + 8 * p.nt - 1) / (8 * p.nt));
-  p.slots = kSms * 2;                                // Cfg::kCtas
   const int64_t items = (int64_t)c.seqs * c.nkv * p.blocks;
   int64_t tiles = c.positions / kTok;                     // of a sequence at most
   if (window > 0 && (window + rows + kTok - 2) / kTok + 1 < tiles) tiles = (window + rows + kTok - 2) / kTok + 1;
   const int64_t parts = (tiles + kLeast - 1) / kLeast * items;
+  // One CTA of twelve warps an SM where that many hold all parts: a part's tiles at once. (One sequence of 384, 8
+  // heads of 256: 10.7 -> %ONE% us.)
+  p.warps = p.nt == 1 && parts <= kSms ? 12 : 6;
+  p.slots = kSms * 12 / p.warps;
   p.ctas = parts < p.slots ? parts : p.slots;
+  p.list = (tiles + kLeast) * items;
   p.joins = parts > items || parts > p.slots;
   p.segments = p.ctas + items;
   return p;
 }
 
-template <int NG, int NT, typename T>
+template <int NG, int NT, int WARPS, typename T>
 int launch(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
-  auto kernel = kv4_attn_kernel<NG, NT, T>;
+  auto kernel = kv4_attn_kernel<NG, NT, WARPS, T>;
   static bool set[64];
   int dev = 0;
   FBFP_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !set[dev]) {
-    FBFP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NG, NT>::kSmem));
+    FBFP_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NG, NT, WARPS>::kSmem));
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  FBFP_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(Cfg<NG, NT>::kThreads), (size_t)Cfg<NG, NT>::kSmem, st, a, m));
+  FBFP_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(Cfg<NG, NT, WARPS>::kThreads), (size_t)Cfg<NG, NT, WARPS>::kSmem, st, a, m));
   FBFP_LAUNCH_CHECK("kv4_attn_kernel");
   if (p.joins) {
     const int64_t warps = (int64_t)a.c.seqs * a.c.nkv * a.columns;
@@ -745,10 +750,10 @@ int launch(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
 template <int NG, typename T>
 int launch_nt(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
   if constexpr (4 * NG <= kAccumulators)
-    if (p.nt == 4) return launch<NG, 4, T>(a, m, p, st);
+    if (p.nt == 4) return launch<NG, 4, 6, T>(a, m, p, st);
   if constexpr (2 * NG <= kAccumulators)
-    if (p.nt == 2) return launch<NG, 2, T>(a, m, p, st);
-  return launch<NG, 1, T>(a, m, p, st);
+    if (p.nt == 2) return launch<NG, 2, 6, T>(a, m, p, st);
+  return p.warps == 12 ? launch<NG, 1, 12, T>(a, m, p, st) : launch<NG, 1, 6, T>(a, m, p, st);
 }
 template <typename T>
 int launch_ng(const Args& a, const Maps& m, const Plan& p, cudaStream_t st) {
@@ -795,6 +800,7 @@ extern "C" int fbfp_kv4_attention(const fbfp_kv4_cache* cache, const void* q, in
   FBFP_CHECK_ARG((int64_t)c.seqs * c.nkv * c.positions < ((int64_t)1 << 31), "the cache has 2^31 rows or more");
   if (window > c.positions + rows) window = 0;              // sees everything
   const Plan p = plan_of(c, rows, heads, window);
+  FBFP_CHECK_ARG(p.list < ((int64_t)1 << 31), "too many positions, heads and rows");
   FBFP_CHECK_ARG((int64_t)c.seqs * heads * rows < ((int64_t)1 << 31), "too many rows");
   const int64_t need = p.joins ? p.segments * 8 * p.nt * (c.hd + 2) * 4 : 0;
   FBFP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
