@@ -3,15 +3,26 @@
 //
 // A tile is 128 rows: `ntok` tokens of one sequence x the `hp` query heads that share a key/value head,
 // so that grouped heads read keys and values once and a few tokens fill a tile. Keys and values are
-// loaded in blocks of 128 keys. Roles: a warp loads (TMA), a thread issues the MMAs, four warps per tile
-// hold one row a thread: scores from tensor memory, running maximum and sum, weights back. Each tile has
-// two score buffers, so that its next scores are made under its softmax. Heads of up to 128 values: a CTA
-// takes two tiles, of 64 keys a step. Heads of up to 256: one tile (its O fills half of tensor memory), 128 keys
-// a step.
+// loaded in blocks of 128 keys (TMA). Heads of up to 128 values: a CTA takes two tiles over the same blocks;
+// heads of up to 256: one, whose O fills half of tensor memory. Each tile has two score buffers, of 64 or 128
+// keys, so that the next scores are made under this step's softmax. Roles: a warp loads; two warps issue MMAs,
+// one per tile, or one the scores and one the products with the values (a wait costs an issuing warp some
+// hundred cycles, and one warp's waits and issues in a row took longer than the MMAs themselves); four warps
+// per tile hold one row a thread: scores from tensor memory, running maximum and sum, weights back. The grid
+// has a CTA per tile (or two), longest first; a CTA that is done takes over the work of one that has not
+// started, so that its next loads and first scores come under its last softmax and output.
 //
-// softmax: weights are 2^(s c - r), c = scaling log2(e), r the row's reference: its first block's
+// softmax: weights are 2^(s c - r), c = scaling log2(e), r the row's reference: its first step's
 // maximum, raised (and O and the sum rescaled) only when a score comes out 2^8 above it, which leaves
 // the quotient O / sum what it is. fp16 weights carry a factor 2^6 that keeps small ones normal.
+//
+// Bound by the tensor cores and what feeds them from shared memory: at 256 values a block's two products read
+// 192 KB and its loads write 128 KB (of 128 bytes a clock: 2500 clocks, the MMAs take 2048), at 128 the score
+// MMAs of 64 keys read 6 KB in 32 clocks. Measured per block of 128 keys and SM (148 CTAs, a long axis): two
+// tiles x 128 values 1.95 us (1270 TFLOP/s over all SMs), one tile x 256 values 1.63 us (1520). 8192 rows x 64
+// heads of 128, fp16: 1.13 ms (971 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44 us; 128 rows over 32128 keys:
+// 84 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
+// scores of 128 keys at once for heads of 128 (fewer bytes from shared memory, but no buffer to run ahead in).
 #include <cuda.h>
 
 #include "common.cuh"
@@ -276,13 +287,12 @@ __device__ __noinline__ void add_seen(uint32_t o_at, uint32_t p_at, const T* v, 
 }
 
 // CTA `index` of all tiles: the sequences' tiles from last to first, so that a prompt's longest tiles
-// start first. Every warp finds it by itself.
-__device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int toks) {
+// start first. By the loading warp; `total`: all tiles, counted at the first call (0 before).
+__device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int toks, int& total) {
   const int lane = threadIdx.x & 31;
-  int total = 0;
   Work w{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
+  for (int pass = total > 0; pass < 2; ++pass) {
     int before = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.seqs; b0 += 32) {
@@ -317,7 +327,7 @@ __device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int to
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    total = before;
+    if (pass == 0) total = before;
     if (index >= total) return w;
   }
   return w;
@@ -450,7 +460,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const uint32_t q_bytes = (uint32_t)a.ntok * a.hp * 128 * (HDP / 64);
     uint32_t x = blockIdx.x, y = blockIdx.y;
     bool ok = true, more = true;
-    int m = 0;                                       // tiles made known
+    int m = 0, total = 0;                            // tiles made known, tiles of the call
     const auto tell = [&](const Work& w) {
       if (m >= 2) ok = __all_sync(0xffffffffu, wait(&ctl.info_empty[m & 1], (uint32_t)((m >> 1) - 1) & 1, ctl, a.err, 44));
       if (lane == 0 && ok) {
@@ -461,7 +471,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     };
 #pragma unroll 1
     for (uint32_t asked = 0; more && ok; ++asked) {
-      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles);
+      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles, total);
       w.hb = x % a.head_blocks, w.split = y;
       if (w.any) {
         tell(w);
