@@ -20,7 +20,7 @@
 // 192 KB and its loads write 128 KB (of 128 bytes a clock: 2500 clocks, the MMAs take 2048), at 128 the score
 // MMAs of 64 keys read 6 KB in 32 clocks. Measured per block of 128 keys and SM (148 CTAs, a long axis): two
 // tiles x 128 values 1.95 us (1270 TFLOP/s over all SMs), one tile x 256 values 1.63 us (1520). 8192 rows x 64
-// heads of 128, fp16: 1.13 ms (971 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44 us; 128 rows over 32128 keys:
+// heads of 128, fp16: 1.15 ms (957 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44 us; 128 rows over 32128 keys:
 // 84 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
 // scores of 128 keys at once for heads of 128 (fewer bytes from shared memory, but no buffer to run ahead in).
 #include <cuda.h>
@@ -205,7 +205,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
-// 32 columns of this warp's 32 lanes, usable at once.
+// 32 columns of this warp's 32 lanes; they may be used behind tmem_arrived.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
   uint32_t r[32];
   asm volatile(
@@ -286,49 +286,47 @@ __device__ __noinline__ void add_seen(uint32_t o_at, uint32_t p_at, const T* v, 
   tmem_wait_st();
 }
 
+// Where the search for a tile goes on: tiles of the sequences from b1 on come before, that many.
+struct Cursor {
+  int b1, before;
+};
 // CTA `index` of all tiles: the sequences' tiles from last to first, so that a prompt's longest tiles
-// start first. By the loading warp; `total`: all tiles, counted at the first call (0 before).
-__device__ __forceinline__ Work find_work(const PromptArgs& a, int index, int toks, int& total) {
+// start first. By the loading warp. A CTA's indexes mostly ascend, and then all its searches together look at
+// each sequence once. (Out of line: inlined, 8192 rows x 64 heads of 128 take 1.175 ms instead of 1.149, where one
+// tile's call gains 0.2 us.)
+__device__ __noinline__ Work find_work(const PromptArgs& a, int index, int toks, Cursor& cur) {
   const int lane = threadIdx.x & 31;
   Work w{0, 0, 0, 0, 0, 0, 0, 0};
+  if (index < cur.before) cur = {a.seqs, 0};
 #pragma unroll 1
-  for (int pass = total > 0; pass < 2; ++pass) {
-    int before = 0;
-#pragma unroll 1
-    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
-      const int b = b0 + lane;
-      int s0 = 0, s1 = 0;
-      if (b < a.seqs) {
-        s0 = min((int64_t)max(__ldg(a.starts + b), 0), a.rows);
-        s1 = min((int64_t)max(__ldg(a.starts + b + 1), s0), a.rows);
-      }
-      const int n = (s1 - s0 + toks - 1) / toks;
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      if (pass == 1) {
-        const int want = total - 1 - index;
-        const bool mine = want >= before + sum - n && want < before + sum;
-        const uint32_t who = __ballot_sync(0xffffffffu, mine);
-        if (who) {
-          const int src = __ffs(who) - 1;
-          w.q0 = __shfl_sync(0xffffffffu, s0, src);
-          w.len = __shfl_sync(0xffffffffu, s1, src) - w.q0;
-          w.tok0 = (want - __shfl_sync(0xffffffffu, before + sum - n, src)) * toks;
-          const int bb = b0 + src;
-          w.k0 = min((int64_t)max(__ldg(a.kv_starts + bb), 0), a.kv_rows);
-          w.klen = (int)min((int64_t)max(__ldg(a.kv_starts + bb + 1), w.k0), a.kv_rows) - w.k0;
-          w.any = 1;
-          return w;
-        }
-      }
-      before += __shfl_sync(0xffffffffu, sum, 31);
+  for (; cur.b1 > 0; cur.b1 -= 32) {
+    const int b = cur.b1 - 1 - lane;
+    int s0 = 0, s1 = 0;
+    if (b >= 0) {
+      s0 = min((int64_t)max(__ldg(a.starts + b), 0), a.rows);
+      s1 = min((int64_t)max(__ldg(a.starts + b + 1), s0), a.rows);
     }
-    if (pass == 0) total = before;
-    if (index >= total) return w;
+    const int n = (s1 - s0 + toks - 1) / toks;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const int place = index - cur.before - (sum - n);        // among the tiles of this lane's sequence
+    const uint32_t who = __ballot_sync(0xffffffffu, place >= 0 && place < n);
+    if (who) {
+      const int src = __ffs(who) - 1;
+      w.q0 = __shfl_sync(0xffffffffu, s0, src);
+      w.len = __shfl_sync(0xffffffffu, s1, src) - w.q0;
+      w.tok0 = __shfl_sync(0xffffffffu, n - 1 - place, src) * toks;
+      const int bb = cur.b1 - 1 - src;
+      w.k0 = min((int64_t)max(__ldg(a.kv_starts + bb), 0), a.kv_rows);
+      w.klen = (int)min((int64_t)max(__ldg(a.kv_starts + bb + 1), w.k0), a.kv_rows) - w.k0;
+      w.any = 1;
+      return w;
+    }
+    cur.before += __shfl_sync(0xffffffffu, sum, 31);
   }
   return w;
 }
@@ -460,7 +458,8 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const uint32_t q_bytes = (uint32_t)a.ntok * a.hp * 128 * (HDP / 64);
     uint32_t x = blockIdx.x, y = blockIdx.y;
     bool ok = true, more = true;
-    int m = 0, total = 0;                            // tiles made known, tiles of the call
+    int m = 0;                                       // tiles made known
+    Cursor cur{a.seqs, 0};
     const auto tell = [&](const Work& w) {
       if (m >= 2) ok = __all_sync(0xffffffffu, wait(&ctl.info_empty[m & 1], (uint32_t)((m >> 1) - 1) & 1, ctl, a.err, 44));
       if (lane == 0 && ok) {
@@ -471,7 +470,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     };
 #pragma unroll 1
     for (uint32_t asked = 0; more && ok; ++asked) {
-      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles, total);
+      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles, cur);
       w.hb = x % a.head_blocks, w.split = y;
       if (w.any) {
         tell(w);

@@ -187,3 +187,30 @@ def test_starts_of_any_contents_stay_inside():
                               ([500, 600, 700], [0, 1, 2])):
         attention.prompt_attention(q, k, v, ints(starts), kv_starts=ints(kv_starts))
     attention.check_device_errors()
+
+
+def test_many_sequences():
+    """More sequences than a warp looks through at once, a third of them empty."""
+    lens = [(0, 3, 1)[i % 3] for i in range(700)]
+    kv_lens = [n + 7 * (i % 5) for i, n in enumerate(lens)]
+    q = normal((sum(lens), 4, 64), torch.bfloat16, 1)
+    k, v = (normal((sum(kv_lens), 2, 64), torch.bfloat16, i) for i in (2, 3))
+    check(q, k, v, lens, kv_lens=kv_lens)
+    check(q, k, v, lens, kv_lens=kv_lens, window=4)
+
+
+def test_broadcast_keys():
+    """Keys and values of one head expanded to several: a stride of zero."""
+    q = normal((130, 4, 64), torch.bfloat16, 1)
+    k, v = (normal((130, 1, 64), torch.bfloat16, i) for i in (2, 3))
+    a = check(q, k, v, [130])
+    b = check(q, k.expand(130, 4, 64), v.expand(130, 4, 64), [130])
+    assert a.shape == b.shape
+
+
+def test_out_in_place_of_padding():
+    """Rows of a wider buffer as the result: what lies between them stays."""
+    q, k, v = (normal((70, h, 128), torch.float16, i) for i, h in enumerate((4, 2, 2)))
+    buf = torch.full((70, 5, 136), 3.0, dtype=torch.float16, device=DEV)
+    check(q, k, v, [70], out=buf[:, :4, :128])
+    assert bool((buf[:, 4] == 3).all()) and bool((buf[:, :, 128:] == 3).all())
