@@ -3,7 +3,7 @@
 Rows of several sequences lie back to back, without padding: ``starts`` (int32 [sequences + 1], on the
 device) holds where each begins, and after the last where it ends. Lengths stay on the device, so a
 call reads nothing back. Forward only: results carry no gradient, whatever their inputs; ``out`` must
-not require one while gradients are recorded, and counts as modified for autograd.
+not require one while gradients are recorded, must not overlap the inputs, and counts as modified for autograd.
 """
 from __future__ import annotations
 

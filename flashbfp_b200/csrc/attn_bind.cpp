@@ -172,6 +172,17 @@ PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// kv4_check(cache, out): refuses a cache that is not one, and tensors that must not be written.
+PyObject* kv4_check(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arity(n, 2)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Cache c = cache_of(a[0]);
+    for (int i = 0; i < 4; ++i) check_written(*c.t[i], "cache");
+    check_out(on(a[1], "q_out", c.index), "q_out");
+    Py_RETURN_NONE;
+  });
+}
+
 // kv4_write(cache, k, v, pos, starts, err)
 PyObject* kv4_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 6)) return nullptr;
@@ -275,4 +286,5 @@ PyObject* attn_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }  // namespace
 
 PyMethodDef attn_methods[] = {FAST(prompt_attention), FAST(kv4_write), FAST(kv4_read), FAST(kv4_attention),
+                              FAST(kv4_check),
                               FAST(attn_setup), {nullptr, nullptr, 0, nullptr}};

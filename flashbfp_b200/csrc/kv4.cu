@@ -88,27 +88,6 @@ __device__ __forceinline__ Place place_of(int64_t r, const Kv4& c, int64_t rows,
   return p;
 }
 
-// Up to R rows of one sequence that follow each other: rows first .. first + n - 1, the first at a position
-// that is in the cache as the others are. Calls f(row, n, sequence, position) for every such run of rows
-// row0 .. row0 + R - 1; usually there is one.
-template <int R, typename F>
-__device__ __forceinline__ void runs_of(int64_t row0, const Kv4& c, int64_t rows, const int32_t* base,
-                                        const int32_t* starts, int32_t* err, bool tell, F f) {
-  const Place a = place_of(row0, c, rows, base, starts, err, tell && R == 1);
-  if constexpr (R > 1) {
-    const Place z = place_of(row0 + R - 1, c, rows, base, starts, err, false);
-    if (a.b < 0 || a.b != z.b || z.at - a.at != R - 1) {
-#pragma unroll 1
-      for (int i = 0; i < R; ++i) {
-        const Place p = place_of(row0 + i, c, rows, base, starts, err, tell);
-        if (p.b >= 0) f(row0 + i, 1, p.b, p.at);
-      }
-      return;
-    }
-  }
-  if (a.b >= 0) f(row0, R, a.b, a.at);
-}
-
 // A piece as it is in memory, its largest magnitude's bits (as fp32), and its values.
 template <typename T>
 struct Raw {
@@ -248,12 +227,14 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4 c, RowsArg r, Sh
     for (int k = 0; k < R; ++k) store_values<T, VEC>(to + k * step, word[k], s[k]);
     return;
   }
+  if constexpr (R > 1) {
 #pragma unroll 1
-  for (int k = 0; k < R; ++k) {
-    const Place p = place_of(row0 + k, c, r.rows, first, starts, err, i == 0);
-    if (p.b < 0) continue;
-    const int64_t from = c.at(p.b, head, p.at) * NG;
-    store_values<T, VEC>(to + k * step, __ldg(values + from * 4), __ldg(scales + from));
+    for (int k = 0; k < R; ++k) {
+      const Place p = place_of(row0 + k, c, r.rows, first, starts, err, i == 0);
+      if (p.b < 0) continue;
+      const int64_t from = c.at(p.b, head, p.at) * NG;
+      store_values<T, VEC>(to + k * step, __ldg(values + from * 4), __ldg(scales + from));
+    }
   }
 }
 

@@ -7,13 +7,16 @@
 // fp32, and the softmax weights before those go to the values' product. So the cache is read once for
 // all columns of a block, and unpacked once.
 //
-// Bound by HBM, and close behind it by instruction issue: 4.5 bits a value arrive at 44 values per
-// clock and SM, and a value takes some two instructions (unpack, product, scale).
+// Bound by instruction issue, close behind it by HBM: a warp takes some 1300 instructions for a tile of 32
+// positions x 256 values (unpack, products, scales), 2.5 issue in a clock and SM, the integer pipe busy half the
+// time; the loads alone take two thirds as long. 16 sequences of 9000 to 32700 positions, 8 heads of 256 for 16
+// query heads: 172 us, 4.0 TB/s. 12 sequences of 2000 to 8000 positions with 4 rows each, 64 query heads on 8 of 128:
+// 256 us, where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
 // mma.sync and not tcgen05: its operands come from registers, where the unpacked values are; for
 // tcgen05 each would have to be written to shared memory once more for at most 16 columns.
 //
 // Work: all tiles of 32 positions in one list, of which each CTA takes an even share, so that the SMs fill
-// and end together whatever the lengths are, which only the device knows. A warp takes every sixth tile
+// and end together whatever the lengths are, which only the device knows. A warp takes every sixth (twelfth) tile
 // through a ring of its own (TMA: values swizzled so that fragments read without bank conflicts),
 // with a running maximum and sum; the warps join in shared memory, parts of a sequence in a second
 // launch.
@@ -718,7 +721,7 @@ Plan plan_of(const Kv4& c, int64_t rows, int64_t heads, int64_t window) {
   if (window > 0 && (window + rows + kTok - 2) / kTok + 1 < tiles) tiles = (window + rows + kTok - 2) / kTok + 1;
   const int64_t parts = (tiles + kLeast - 1) / kLeast * items;
   // One CTA of twelve warps an SM where that many hold all parts: a part's tiles at once. (One sequence of 384, 8
-  // heads of 256: 10.7 -> %ONE% us.)
+  // heads of 256: 10.7 -> 9.0 us.)
   p.warps = p.nt == 1 && parts <= kSms ? 12 : 6;
   p.slots = kSms * 12 / p.warps;
   p.ctas = parts < p.slots ? parts : p.slots;

@@ -9,7 +9,8 @@ is, so a row that is read back and written again is held as it was.
 
 ``KV4Cache`` holds keys and values [sequences, kv_heads, positions, ...]. Positions are int32 tensors on
 the device, and so are lengths: calls read nothing back and can be captured. A position outside the
-cache is skipped and recorded (``check_device_errors`` raises it). Forward only, as ``attention``.
+cache is skipped and recorded (``check_device_errors`` raises it). Forward only, as ``attention``; what a
+call writes must not overlap what it reads.
 """
 from __future__ import annotations
 
@@ -72,6 +73,7 @@ def kv4_append(cache: KV4Cache, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm:
     RMSNorm (weights 1 + w) of every q and k head, the rotary embedding with the bf16 rows cos, sin
     [positions, D] at the row's position, q to q_out [T, heads, D], k and v into the cache as ``kv4_write``
     puts them. D is a multiple of 16."""
+    _module().kv4_check(cache, q_out)
     values, d = cache.k_values, cache.head_dim
     kvh = values.shape[1]
     what = {"qkv": qkv, "q_norm": q_norm, "k_norm": k_norm, "cos": cos, "sin": sin, "q_out": q_out}

@@ -108,3 +108,39 @@ def test_written_tensors_count_as_modified():
     out = [torch.zeros(1, 1, 32, device=DEV) for _ in range(2)]
     kv4.kv4_read(c, ints([0]), ints([0, 1]), out=out)
     assert all(t._version > 0 for t in out)
+
+
+def test_append_refuses():
+    from flashbfp_b200 import kv4
+    bf = dict(dtype=torch.bfloat16, device=DEV)
+    c = kv4.empty_cache(2, 1, 32, 32, DEV)
+    qkv, w, angles, out = torch.zeros(2, 4 * 32, **bf), torch.zeros(32, **bf), torch.zeros(32, 32, **bf), torch.zeros(2, 2, 32, **bf)
+    pos = ints([0, 0])
+
+    def f(cache=c, qkv=qkv, w=w, angles=angles, pos=pos, out=out, starts=None):
+        kv4.kv4_append(cache, qkv, w, w, 1e-6, angles, angles, pos, out, starts=starts)
+
+    f()
+    wide = kv4.empty_cache(2, 1, 64, 32, DEV)
+    for i, name in enumerate(("k_values", "k_scales", "v_values", "v_scales")):
+        with pytest.raises(ValueError, match=name):              # a tensor of another length, a view, another type
+            f(cache=kv4.KV4Cache(*[(wide if i and j == i else c)[j] for j in range(4)], 32) if i else
+              kv4.KV4Cache(wide.k_values[:, :, :32], *c[1:4], 32))
+        with pytest.raises(ValueError, match=name):
+            f(cache=kv4.KV4Cache(*[t.to(torch.float16) if j == i else t for j, t in enumerate(c[:4])], 32))
+    with pytest.raises(ValueError, match="do not hold heads"):
+        f(qkv=qkv[:, :64].contiguous())
+    with pytest.raises(ValueError, match="q_out"):
+        f(out=out[:, :1])
+    with pytest.raises(ValueError, match="positions"):
+        f(angles=angles[:31])
+    with pytest.raises(ValueError, match="pos"):
+        f(pos=pos.long())
+    with pytest.raises(ValueError, match="pass starts"):
+        f(qkv=qkv[:1], out=out[:1])
+    with pytest.raises(ValueError, match="starts"):
+        f(starts=ints([0, 2]))
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        f(out=torch.zeros(2, 2, 32, requires_grad=True, **bf))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(qkv=qkv.cpu())

@@ -202,3 +202,31 @@ def test_offsets_beyond_32_bits():
     k, v = (rows((300, 1, 256), torch.bfloat16, 30 + i).to(DEV).clamp(-30, 30) for i in range(2))
     kv4.kv4_write(cache, k, v, ints([n - 300]), starts=ints([0, 300]))
     check(queries((1, 2, 256), torch.bfloat16, 32), cache, [n - 1], window=290)
+
+
+def test_many_sequences():
+    """More sequences than a warp looks through at once."""
+    seqs = 150
+    cache = filled(seqs, 2, 96, 64, 40)
+    pos = [(37 * b) % 96 for b in range(seqs)]
+    check(queries((seqs, 4, 64), torch.bfloat16, 42), cache, pos)
+    check(queries((seqs, 2, 4, 64), torch.bfloat16, 43), cache, [max(0, p - 1) for p in pos], window=33)
+
+
+def test_two_streams_at_once():
+    """Calls whose sequences are joined from parts, each with a workspace of its own."""
+    from flashbfp_b200 import kv4
+    cache = filled(2, 2, 6016, 128, 44)
+    qs = [queries((2, 4, 128), torch.bfloat16, 46 + i) for i in range(2)]
+    pos = ints([6000, 5000])
+    want = [kv4.kv4_attention(q, cache, pos) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for q, st in zip(qs, streams):
+            with torch.cuda.stream(st):
+                got.append(kv4.kv4_attention(q, cache, pos))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    kv4.check_device_errors()
