@@ -10,7 +10,7 @@
 // Bound by instruction issue, close behind it by HBM: a warp takes some 1300 instructions for a tile of 32
 // positions x 256 values (unpack, products, scales), 2.5 issue in a clock and SM, the integer pipe busy half the
 // time; the loads alone take two thirds as long. 16 sequences of 9000 to 32700 positions, 8 heads of 256 for 16
-// query heads: 172 us, 4.0 TB/s. 12 sequences of 2000 to 8000 positions with 4 rows each, 64 query heads on 8 of 128:
+// query heads: 172-174 us, 4.0 TB/s. 64 sequences of 500 to 8100 positions with 4 rows each, 64 query heads on 8 of 128:
 // 256 us, where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
 // mma.sync and not tcgen05: its operands come from registers, where the unpacked values are; for
 // tcgen05 each would have to be written to shared memory once more for at most 16 columns.
