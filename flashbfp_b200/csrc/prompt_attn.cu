@@ -42,7 +42,7 @@ struct PromptArgs {
   uint32_t negate;             // scaling < 0
   const void* v;
   void* out;
-  float* part;                 // splits > 1: O / sum [split][row][head][hd], then log2 of the sums [split][row][head]
+  float* part;                 // splits > 1: O / sum [split][hd / 8][head][row][8], then log2 of the sums [split][head][row]
   float* lse;
   int32_t* err;
 };
@@ -301,10 +301,11 @@ __device__ __noinline__ Work find_work(const PromptArgs& a, int index, int toks,
 #pragma unroll 1
   for (; cur.b1 > 0; cur.b1 -= 32) {
     const int b = cur.b1 - 1 - lane;
-    int s0 = 0, s1 = 0;
+    int s0 = 0, s1 = 0, k0 = 0, k1 = 0;
     if (b >= 0) {
-      s0 = min((int64_t)max(__ldg(a.starts + b), 0), a.rows);
-      s1 = min((int64_t)max(__ldg(a.starts + b + 1), s0), a.rows);
+      s0 = __ldg(a.starts + b), s1 = __ldg(a.starts + b + 1), k0 = __ldg(a.kv_starts + b), k1 = __ldg(a.kv_starts + b + 1);
+      s0 = min((int64_t)max(s0, 0), a.rows), s1 = min((int64_t)max(s1, s0), a.rows);
+      k0 = min((int64_t)max(k0, 0), a.kv_rows), k1 = min((int64_t)max(k1, k0), a.kv_rows);
     }
     const int n = (s1 - s0 + toks - 1) / toks;
     int sum = n;
@@ -320,9 +321,8 @@ __device__ __noinline__ Work find_work(const PromptArgs& a, int index, int toks,
       w.q0 = __shfl_sync(0xffffffffu, s0, src);
       w.len = __shfl_sync(0xffffffffu, s1, src) - w.q0;
       w.tok0 = __shfl_sync(0xffffffffu, n - 1 - place, src) * toks;
-      const int bb = cur.b1 - 1 - src;
-      w.k0 = min((int64_t)max(__ldg(a.kv_starts + bb), 0), a.kv_rows);
-      w.klen = (int)min((int64_t)max(__ldg(a.kv_starts + bb + 1), w.k0), a.kv_rows) - w.k0;
+      w.k0 = __shfl_sync(0xffffffffu, k0, src);
+      w.klen = __shfl_sync(0xffffffffu, k1, src) - w.k0;
       w.any = 1;
       return w;
     }
@@ -424,10 +424,19 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     ctl.abort = 0;
     fence_mbar_init();
   }
+  if (warp == kLoad && lane == 0) {
+    prefetch_tmap(&M.q);
+    prefetch_tmap(&M.k);
+    prefetch_tmap(&M.v);
+  }
   grid_dependency_wait();                            // before tensor memory is taken: the kernel before may hold some
-  if (warp == kLoad) {                               // 512 columns, one CTA per SM
+  Cursor cur{a.seqs, 0};
+  Work w0{0, 0, 0, 0, 0, 0, 0, 0};                   // the loading warp: this CTA's own tile
+  if (warp == kMma) {                                // 512 columns, one CTA per SM
     tmem_alloc(&ctl.tmem, 512);
     tmem_relinquish();
+  } else if (warp == kLoad) {
+    w0 = find_work(a, blockIdx.x / a.head_blocks, a.ntok * C::kTiles, cur);
   }
   tc_fence_before();
   __syncthreads();
@@ -450,16 +459,10 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
 
   int issued = 0, q_loads = 0, last = -1;            // loading: units and queries issued; this lane's last unit
   if (warp == kLoad) {
-    if (lane == 0) {
-      prefetch_tmap(&M.q);
-      prefetch_tmap(&M.k);
-      prefetch_tmap(&M.v);
-    }
     const uint32_t q_bytes = (uint32_t)a.ntok * a.hp * 128 * (HDP / 64);
     uint32_t x = blockIdx.x, y = blockIdx.y;
     bool ok = true, more = true;
     int m = 0;                                       // tiles made known
-    Cursor cur{a.seqs, 0};
     const auto tell = [&](const Work& w) {
       if (m >= 2) ok = __all_sync(0xffffffffu, wait(&ctl.info_empty[m & 1], (uint32_t)((m >> 1) - 1) & 1, ctl, a.err, 44));
       if (lane == 0 && ok) {
@@ -470,7 +473,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     };
 #pragma unroll 1
     for (uint32_t asked = 0; more && ok; ++asked) {
-      Work w = find_work(a, x / a.head_blocks, a.ntok * C::kTiles, cur);
+      Work w = asked == 0 ? w0 : find_work(a, x / a.head_blocks, a.ntok * C::kTiles, cur);
       w.hb = x % a.head_blocks, w.split = y;
       if (w.any) {
         tell(w);
@@ -870,7 +873,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);        // NaN stays
     const int64_t row = w.q0 + tok;
     if (a.splits > 1 && mine)
-      a.lse[((int64_t)w.split * a.rows + row) * a.heads + head] = sum > 0.f ? lg2(sum) + ref - shift : (sum == 0.f ? -INFINITY : sum);
+      a.lse[((int64_t)w.split * a.heads + head) * a.rows + row] = sum > 0.f ? lg2(sum) + ref - shift : (sum == 0.f ? -INFINITY : sum);
 #pragma unroll 1
     for (int d = 0; d < HDP; d += 32) {
       float o[32];
@@ -885,14 +888,16 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
       for (int i = 0; i < 32; ++i) o[i] *= inv;
       if (mine) {
         if (a.splits > 1) {
-          float* p = a.part + (((int64_t)w.split * a.rows + row) * a.heads + head) * a.hd + d;
+          // the tile's rows follow each other: whole lines (4.4 -> 2.6 us for 128 x 256 values)
+          const int64_t step = (int64_t)a.heads * a.rows * 8;
+          float* p = a.part + ((int64_t)w.split * (a.hd / 8) + d / 8) * step + ((int64_t)head * a.rows + row) * 8;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
+          for (int i = 0; i < 32; i += 8, p += step)
             if (d + i < a.hd) {
               uint32_t x[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(o[i + e]);
-              store32(p + i, x);
+              store32(p, x);
             }
         } else {
           T* p = (T*)a.out + row * a.o_row + head * a.o_head + d;
@@ -931,50 +936,57 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     }
     __syncthreads();
   }
-  if (warp == kLoad) {
+  if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
-// Joins the splits: weights 2^(lse - max) over the parts of a (row, head); a thread per 4 values.
+// Joins the splits: weights 2^(lse - max) over the parts of a (row, head). A thread has 8 values; a warp 4 rows of a
+// head x 8 such pieces, so that it reads and writes whole lines.
 template <typename T>
-__global__ void prompt_join_kernel(const PromptArgs a) {
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs a) {
   pdl_prologue();
-  const int per = a.hd / 4;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t rh = i / per;
-  const int d = (int)(i - rh * per) * 4;
-  if (rh >= a.rows * a.heads) return;
-  const int64_t row = rh / a.heads;
-  // rows of no sequence have no parts
+  const int pieces = a.hd / 8;
+  const int64_t quads = (a.rows + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t hq = (i >> 2) / pieces, head = hq / quads, row = (hq - head * quads) * 4 + (i & 3);
+  const int piece = (int)((i >> 2) - hq * pieces);
+  if (head >= a.heads || row >= a.rows) return;
   int lo = 0, hi = a.seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (__ldg(a.starts + mid) <= row) lo = mid;
     else hi = mid;
   }
-  if (row < __ldg(a.starts + lo) || row >= __ldg(a.starts + lo + 1)) return;
-  const int64_t step = a.rows * a.heads;
+  const int from = __ldg(a.starts + lo), to = __ldg(a.starts + lo + 1);
+  const int64_t step = (int64_t)a.heads * a.rows;
+  const float* const lse = a.lse + head * a.rows + row;
   float m = -INFINITY;
   bool nan = false;
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
-    const float l = a.lse[s * step + rh];
+    const float l = lse[s * step];
     nan |= l != l;
     m = fmaxf(m, l);
   }
-  float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = a.lse[s * step + rh];
-    if (l == -INFINITY) continue;
+  float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float* p = a.part + (piece * step + head * a.rows + row) * 8;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s, p += pieces * step * 8) {
+    const float l = lse[s * step];
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    if (l == -INFINITY) continue;                    // (nothing of this split: 0 all the same where nothing was seen)
     const float f = nan ? NAN : ex2(l - m);
-    const float4 p = *reinterpret_cast<const float4*>(a.part + (s * step + rh) * a.hd + d);
     sum += f;
-    o[0] += f * p.x, o[1] += f * p.y, o[2] += f * p.z, o[3] += f * p.w;
+    o[0] += f * x.x, o[1] += f * x.y, o[2] += f * x.z, o[3] += f * x.w;
+    o[4] += f * y.x, o[5] += f * y.y, o[6] += f * y.z, o[7] += f * y.w;
   }
+  if (row < from || row >= to) return;               // rows of no sequence have no parts
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* p = (T*)a.out + row * a.o_row + (rh - row * a.heads) * a.o_head + d;
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack2(o[0] * inv, o[1] * inv, p), pack2(o[2] * inv, o[3] * inv, p));
+  T* const out = (T*)a.out + row * a.o_row + head * a.o_head + piece * 8;
+  *reinterpret_cast<uint4*>(out) = make_uint4(pack2(o[0] * inv, o[1] * inv, out), pack2(o[2] * inv, o[3] * inv, out),
+                                              pack2(o[4] * inv, o[5] * inv, out), pack2(o[6] * inv, o[7] * inv, out));
 }
 
 // How a call is cut: heads of a tile (the largest divisor of a group that a tile holds), its tokens,
@@ -1018,7 +1030,7 @@ int launch(const PromptArgs& a, const PromptMaps& m, const Plan& p, cudaStream_t
                            (size_t)Cfg<HDP>::kSmem, st, a, m));
   FBFP_LAUNCH_CHECK("prompt_attn_kernel");
   if (p.splits > 1) {
-    const int64_t threads = a.rows * a.heads * (a.hd / 4);
+    const int64_t threads = (a.rows + 3) / 4 * 4 * a.heads * (a.hd / 8);
     FBFP_CUDA_TRY(launch_pdl(prompt_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a));
     FBFP_LAUNCH_CHECK("prompt_join_kernel");
   }
