@@ -875,24 +875,25 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     if (a.splits > 1 && mine)
       a.lse[((int64_t)w.split * a.heads + head) * a.rows + row] = sum > 0.f ? lg2(sum) + ref - shift : (sum == 0.f ? -INFINITY : sum);
 #pragma unroll 1
-    for (int d = 0; d < HDP; d += 32) {
-      float o[32];
+    for (int d = 0; d < HDP; d += 64) {
+      float o[64];
       if (steps > 0) {
         tmem_load32(o_at + d, o);
-        tmem_arrived<32>(o);
+        tmem_load32(o_at + d + 32, o + 32);
+        tmem_arrived<64>(o);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        for (int i = 0; i < 64; ++i) o[i] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] *= inv;
+      for (int i = 0; i < 64; ++i) o[i] *= inv;
       if (mine) {
         if (a.splits > 1) {
           // the tile's rows follow each other: whole lines (4.4 -> 2.6 us for 128 x 256 values)
           const int64_t step = (int64_t)a.heads * a.rows * 8;
           float* p = a.part + ((int64_t)w.split * (a.hd / 8) + d / 8) * step + ((int64_t)head * a.rows + row) * 8;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8, p += step)
+          for (int i = 0; i < 64; i += 8, p += step)
             if (d + i < a.hd) {
               uint32_t x[8];
 #pragma unroll
@@ -902,7 +903,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         } else {
           T* p = (T*)a.out + row * a.o_row + head * a.o_head + d;
 #pragma unroll
-          for (int i = 0; i < 32; i += 16) {
+          for (int i = 0; i < 64; i += 16) {
             uint32_t x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = pack2(o[i + 2 * e], o[i + 2 * e + 1], p);
