@@ -10,8 +10,8 @@
 // Bound by instruction issue, close behind it by HBM: a warp takes some 1300 instructions for a tile of 32
 // positions x 256 values (unpack, products, scales), 2.5 issue in a clock and SM, the integer pipe busy half the
 // time; the loads alone take two thirds as long. 16 sequences of 9000 to 32700 positions, 8 heads of 256 for 16
-// query heads: 172-174 us, 4.0 TB/s. 64 sequences of 500 to 8100 positions with 4 rows each, 64 query heads on 8 of 128:
-// 256 us, where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
+// query heads: 171-176 us, 4.0 TB/s. 64 sequences of 500 to 8100 positions with 4 rows each, 64 query heads on 8 of 128:
+// 245 us, where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
 // mma.sync and not tcgen05: its operands come from registers, where the unpacked values are; for
 // tcgen05 each would have to be written to shared memory once more for at most 16 columns.
 //
@@ -367,6 +367,22 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
     t1 = reach.first + min((int)(in_item + length), reach.tiles);
   }
   const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;       // this warp's tiles
+  // The queries are asked for before the tiles, which fill what is under way to memory (16 long sequences: 5.9 us
+  // from here to the fragments, 3.5 this way; 64 sequences with 4 rows each 256 -> 245 us in all). With one tile of
+  // columns a lane's row is the same for all its fragments.
+  constexpr int kRounds = (NT * NG + kWarps - 1) / kWarps, kRows = NT == 1 ? 1 : kRounds;
+  uint4 raw[kRows][NG];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = warp + r * kWarps, col = pc.block * 8 * NT + (NT == 1 ? 0 : i / NG * 8) + g;
+    const T* row = (const T*)a.q + pc.b * a.q_seq + col / a.group * a.q_row + (pc.head * a.group + col % a.group) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const int d = 32 * k + 8 * t;
+      raw[r][k] = make_uint4(0, 0, 0, 0);
+      if (i < NT * NG && col < a.columns && d < hd) raw[r][k] = *reinterpret_cast<const uint4*>(row + d);
+    }
+  }
   __syncthreads();                                    // the barriers are there; the last segment's join is read
   const int64_t row0 = a.c.at(pc.b, pc.head, 0);
   const auto load = [&](int e) {                      // lane 0: entry e of the segment
@@ -382,16 +398,15 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
   // the queries as the MMA's column operand: of group j, lane (g, t) holds column g's values 8 t + (0, 4),
   // (1, 5), (2, 6), (3, 7). A power of two per column brings its largest value to 2^12: bf16 values down to 2^-29
   // of the largest are exact in fp16.
-  for (int i = warp; i < NT * NG; i += kWarps) {
-    const int j = i % NG, col = pc.block * 8 * NT + i / NG * 8 + g;
-    const T* row = (const T*)a.q + pc.b * a.q_seq + col / a.group * a.q_row + (pc.head * a.group + col % a.group) * a.q_head;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int i = warp + r * kWarps, j = i % NG;
+    if (i >= NT * NG) break;
     float x[8];
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-      const int d = 32 * k + 8 * t;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (col < a.columns && d < hd) u = *reinterpret_cast<const uint4*>(row + d);
+      const uint4 u = raw[NT == 1 ? 0 : r][k];
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
