@@ -20,8 +20,8 @@
 // 192 KB and its loads write 128 KB (of 128 bytes a clock: 2500 clocks, the MMAs take 2048), at 128 the score
 // MMAs of 64 keys read 6 KB in 32 clocks. Measured per block of 128 keys and SM (148 CTAs, a long axis): two
 // tiles x 128 values 1.95 us (1270 TFLOP/s over all SMs), one tile x 256 values 1.63 us (1520). 8192 rows x 64
-// heads of 128, fp16: 1.15 ms (957 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44 us; 128 rows over 32128 keys:
-// 84 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
+// heads of 128, fp16: 1.13-1.15 ms (957-978 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44.5 us; 128 rows over 32128
+// keys: 84-88 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
 // scores of 128 keys at once for heads of 128 (fewer bytes from shared memory, but no buffer to run ahead in).
 #include <cuda.h>
 
