@@ -17,14 +17,14 @@
 //   warps 4-7   epilogue (one per tensor-memory lane quarter): drain the double-buffered fp32
 //               accumulator of each (row group, CTA) segment while the next segment streams,
 //               scale by 1/15, add outlier sums, then write y or reduce across CTAs;
-//   warps 8-23  dequantisers (4 per tensor-memory lane quarter, one 4-block substage each):
+//   warps 8-19  dequantisers (3 per tensor-memory lane quarter, every third stage each):
 //               one row per lane; each block becomes 8 bf16 pairs s*m*2^e built
 //               exactly with bit operations (PRMT/LOP3 magic pair minus its offset, HSUB2) and
 //               stored into a tensor-memory ring with tcgen05.st;
-//               outliers ride along: the producer stages each stage's outlier entries and
-//               per-row starts, and the dequantisers accumulate v * x in fp32 for the row's
-//               outliers (x read from the stage's activation tile; for M <= 4 the 4 warps of
-//               a row split its entries) and hand the sums to the epilogue through shared memory.
+//   warps 20-23 outliers (one per lane quarter): the producer stages each stage's outlier entries
+//               and per-row starts, and these warps accumulate v * x in fp32 for the row's
+//               outliers (x read from the stage's activation tile) and hand the sums to the
+//               epilogue through shared memory.
 // Work: stream-K over units (128-row group, 16-block stage); each CTA takes a contiguous
 // range. Every mbarrier wait is bounded: on timeout the CTA records an error code in the
 // workspace and winds down (waiting, bounded, for its own copies) before freeing TMEM.
@@ -57,7 +57,14 @@ constexpr uint32_t kWeightTx = kXOff;                        // payload + signs 
 constexpr int kSegCache = 1024;                               // segment pointers cached per CTA
 constexpr int kDqPerQuarter = 3;                 // dequantiser warps per tensor-memory lane quarter
 constexpr int kDq = 4 * kDqPerQuarter;
-static_assert(kASlots == 4 * kDqPerQuarter, "dequantiser warp p of a quarter owns A slots 4p..4p+3");                         // dequantiser warps (2..17), 4 per lane quarter
+static_assert(kASlots == 4 * kDqPerQuarter, "dequantiser warp p of a quarter owns A slots 4p..4p+3");
+// Barriers of the stages' landings: unit i's is full[i % kFull], phase i / kFull. A wait sees a phase's parity
+// only, so whoever waits on a barrier has to take every phase of it. Loads land in any order, and a dequantiser
+// takes every third unit: with a barrier per stage (five) it could pass on the phase two before its own
+// while the unit between, another warp's, had not landed, and read what the stage held before.
+constexpr int kFull = kStages * kDqPerQuarter;
+static_assert(kFull % kStages == 0 && kFull % kDqPerQuarter == 0,
+              "a barrier belongs to one stage and to one dequantiser of each quarter");
 constexpr int kEpiWarp0 = 4;                    // epilogue warpgroup: warps 4-7
 constexpr int kDqWarp0 = 8;                     // dequantisers: warps 8 .. 8 + kDq - 1
 constexpr int kOutWarp0 = kDqWarp0 + kDq;       // outlier warpgroup: warps 20-23
@@ -76,7 +83,7 @@ constexpr size_t kOaccBytes = 2 * 16 * 128 * sizeof(float);
 constexpr size_t kXvOff = kOaccOff + kOaccBytes;
 constexpr size_t kXvBytes = 4 * 16 * 32 * sizeof(float);
 constexpr size_t kBarOff = kXvOff + kXvBytes;
-constexpr int kNumBars = 2 * kStages + 2 * kASlots + 9;
+constexpr int kNumBars = kFull + kStages + 2 * kASlots + 9;
 constexpr size_t kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;   // + alignment slack
 static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA may opt in to");
 }  // namespace tc
@@ -106,7 +113,7 @@ __device__ __forceinline__ TcShared tc_shared(uint8_t* smem_raw) {
   S.seg = reinterpret_cast<int32_t*>(smem + tc::kSegOff);
   uint64_t* b = reinterpret_cast<uint64_t*>(smem + tc::kBarOff);
   S.full = b;
-  S.empty = S.full + tc::kStages;
+  S.empty = S.full + tc::kFull;
   S.afull = S.empty + tc::kStages;
   S.aempty = S.afull + tc::kASlots;
   S.dfull = S.aempty + tc::kASlots;
@@ -162,23 +169,24 @@ __device__ __forceinline__ OutRange out_range(const TcShared& S, const TcArgs& a
 __device__ __forceinline__ void tc_issue_weights(const TcShared& S, const TcArgs& a, const TcMaps& M,
                                                  int64_t u0, int64_t i, int64_t u, int s, uint32_t xbytes) {
   uint8_t* sb = S.stage + (size_t)s * tc::kStageBytes;
+  uint64_t* const full = &S.full[i % tc::kFull];
   const OutRange orr = out_range(S, a, u0, i);
   const int rg = (int)(u / a.n_stages), st = (int)(u % a.n_stages);
-  mbar_arrive_expect_tx(&S.full[s], tc::kWeightTx + xbytes + (uint32_t)orr.n * 4 +
+  mbar_arrive_expect_tx(full, tc::kWeightTx + xbytes + (uint32_t)orr.n * 4 +
                                         (a.entries ? tc::kRoffBytes : 0));
-  tma_2d_g2s(sb + tc::kPayOff, &M.pay, st * 128, rg * 128, &S.full[s]);
-  tma_2d_g2s(sb + tc::kSgnOff, &M.sgn, st * kStageKb, rg * 128, &S.full[s]);
-  tma_2d_g2s(sb + tc::kExpOff, &M.exp, st * kStageKb, rg * 128, &S.full[s]);
-  if (orr.n) bulk_g2s(sb + tc::kOutOff, a.entries + orr.lo4, (uint32_t)orr.n * 4, &S.full[s]);
-  if (a.entries) bulk_g2s(sb + tc::kRoffOff, roff_block(a, u), tc::kRoffBytes, &S.full[s]);
+  tma_2d_g2s(sb + tc::kPayOff, &M.pay, st * 128, rg * 128, full);
+  tma_2d_g2s(sb + tc::kSgnOff, &M.sgn, st * kStageKb, rg * 128, full);
+  tma_2d_g2s(sb + tc::kExpOff, &M.exp, st * kStageKb, rg * 128, full);
+  if (orr.n) bulk_g2s(sb + tc::kOutOff, a.entries + orr.lo4, (uint32_t)orr.n * 4, full);
+  if (a.entries) bulk_g2s(sb + tc::kRoffOff, roff_block(a, u), tc::kRoffBytes, full);
 }
 __device__ __forceinline__ void tc_issue_x(const TcShared& S, const TcArgs& a, const TcMaps& M,
-                                           int64_t u, int s) {
+                                           int64_t i, int64_t u, int s) {
   uint8_t* sb = S.stage + (size_t)s * tc::kStageBytes;
   const int st = (int)(u % a.n_stages);
 #pragma unroll
   for (int b = 0; b < 4; ++b)
-    tma_2d_g2s(sb + tc::kXOff + b * tc::kXBox, &M.x, st * 256 + b * 64, 0, &S.full[s]);
+    tma_2d_g2s(sb + tc::kXOff + b * tc::kXBox, &M.x, st * 256 + b * 64, 0, &S.full[i % tc::kFull]);
 }
 
 __device__ void tc_producer(const TcShared& S, const TcArgs& a, const TcMaps& M, int64_t u0, int64_t u1) {
@@ -192,14 +200,14 @@ __device__ void tc_producer(const TcShared& S, const TcArgs& a, const TcMaps& M,
     const int64_t npre = (u1 - u0) < tc::kStages ? (u1 - u0) : tc::kStages;
     for (int64_t j = 0; j < npre; ++j) tc_issue_weights(S, a, M, u0, j, u0 + j, (int)j, xbytes);
     grid_dependency_wait();
-    for (int64_t j = 0; j < npre; ++j) tc_issue_x(S, a, M, u0 + j, (int)j);
+    for (int64_t j = 0; j < npre; ++j) tc_issue_x(S, a, M, j, u0 + j, (int)j);
     i = npre;
     int s = (int)(npre % tc::kStages);
     uint32_t ph = npre == tc::kStages ? 1u : 0u;
     for (int64_t u = u0 + npre; u < u1; ++u, ++i) {
       if (!tc_wait(S, a, &S.empty[s], ph ^ 1, 1)) break;
       tc_issue_weights(S, a, M, u0, i, u, s, xbytes);
-      tc_issue_x(S, a, M, u, s);
+      tc_issue_x(S, a, M, i, u, s);
       if (++s == tc::kStages) { s = 0; ph ^= 1; }
     }
     // wind down: every stage issued so far must have landed before the CTA may exit, and,
@@ -207,7 +215,7 @@ __device__ void tc_producer(const TcShared& S, const TcArgs& a, const TcMaps& M,
     // arrival (an MMA commit) is still due on a stage barrier when the shared memory is freed
     const int64_t j0 = i > tc::kStages ? i - tc::kStages : 0;
     for (int64_t j = j0; j < i; ++j)
-      mbar_wait(&S.full[j % tc::kStages], (uint32_t)(j / tc::kStages) & 1, 1u << 20);
+      mbar_wait(&S.full[j % tc::kFull], (uint32_t)(j / tc::kFull) & 1, 1u << 20);
     for (int64_t j = j0; j < i; ++j)
       if (*S.abort_flag || !mbar_wait(&S.empty[j % tc::kStages], (uint32_t)(j / tc::kStages) & 1, 1u << 22))
         break;
@@ -325,7 +333,7 @@ __device__ void tc_dequant(const TcShared& S, const TcArgs& a, int64_t u0, int64
   for (int64_t u = u0; u < u1; ++u, ++i) {
     if (i % tc::kDqPerQuarter != par) continue;
     const int s = i % tc::kStages;
-    if (!tc_wait(S, a, &S.full[s], (uint32_t)(i / tc::kStages) & 1, 4)) return;
+    if (!tc_wait(S, a, &S.full[i % tc::kFull], (uint32_t)(i / tc::kFull) & 1, 4)) return;
     const uint8_t* sb = S.stage + (size_t)s * tc::kStageBytes;
     const uint32_t aph = (uint32_t)(i / tc::kDqPerQuarter) & 1;
     const uint8_t* prow = sb + tc::kPayOff + lr * 128;
@@ -383,7 +391,7 @@ __device__ void tc_outliers(const TcShared& S, const TcArgs& a, int64_t u0, int6
     for (int t = 0; t < 16; ++t) oacc[t] = 0.f;
     for (; u < seg_end; ++u, ++i) {
       const int s = i % tc::kStages;
-      if (!tc_wait(S, a, &S.full[s], (uint32_t)(i / tc::kStages) & 1, 10)) return;
+      if (!tc_wait(S, a, &S.full[i % tc::kFull], (uint32_t)(i / tc::kFull) & 1, 10)) return;
       const uint8_t* sb = S.stage + (size_t)s * tc::kStageBytes;
       if (rvalid) {
         const OutRange orr = out_range(S, a, u0, i);
@@ -585,7 +593,8 @@ gemv_tc_kernel(const TcArgs a, const __grid_constant__ TcMaps M) {
     // a stage is released by the dequantiser of each lane quarter that took it, the MMA and,
     // with outliers, the 4 outlier warps
     const uint32_t rel = 4 + 1 + (a.entries ? 4 : 0);
-    for (int s = 0; s < tc::kStages; ++s) { mbar_init(&S.full[s], 1); mbar_init(&S.empty[s], rel); }
+    for (int j = 0; j < tc::kFull; ++j) mbar_init(&S.full[j], 1);
+    for (int s = 0; s < tc::kStages; ++s) mbar_init(&S.empty[s], rel);
     for (int j = 0; j < tc::kASlots; ++j) { mbar_init(&S.afull[j], 4); mbar_init(&S.aempty[j], 1); }
     for (int d = 0; d < 2; ++d) {
       mbar_init(&S.dfull[d], 1);
