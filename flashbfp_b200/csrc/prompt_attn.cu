@@ -581,6 +581,11 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
           uint32_t u = units + min(2 + 2 * j, blocks + j) * 4;
           uint32_t slot = u % C::kUnits, parity = (u / C::kUnits) & 1;
           bool skip = false;
+          // A wait sees the parity of a phase and nothing else. The first units lie where the block's last keys
+          // lay, units that this warp does not wait for: until those have landed, a wait for these would pass
+          // on the phase before them. The block's scores are made: they have.
+          ok = __all_sync(0xffffffffu, wait(&ctl.s_full[0][g & 1], (g >> 1) & 1, ctl, a.err, 47));
+          if (!ok) break;
 #pragma unroll
           for (int p = 0; p < 4; ++p) {              // keys 64 (p / 2) on, values 128 (p % 2) on
             if (ok) ok = __all_sync(0xffffffffu, wait(&ctl.full[slot], parity, ctl, a.err, 33));
