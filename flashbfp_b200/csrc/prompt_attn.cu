@@ -84,7 +84,7 @@ struct Work {
 };
 
 struct Ctl {
-  uint64_t q_full[2], q_empty, full[10], empty[10], s_full[2][2], p_full[2][2], v_here[2], o_done[2][2], voted[2], drain;
+  uint64_t q_full[2], q_empty, full[10], empty[10], s_full[2][2], p_full[2][2], v_here[2][2], o_done[2][2], voted[2], drain;
   uint64_t info_full[2], info_empty[2], next_full;
   uint4 next;                   // the answer to a request for another CTA's work
   Work info[2];                 // this tile's and the next one's, any = 0 behind the last
@@ -406,9 +406,9 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         mbar_init(&ctl.s_full[i][k], 1);
         mbar_init(&ctl.p_full[i][k], 4);
         mbar_init(&ctl.o_done[i][k], 1);
+        mbar_init(&ctl.v_here[i][k], 1);
         ctl.skip[i][k] = 0;
       }
-      mbar_init(&ctl.v_here[i], 1);
       mbar_init(&ctl.voted[i], 4);
       for (int k = 0; k < 4; ++k) ctl.vote[i][k] = 0;
       mbar_init(&ctl.info_full[i], 1);
@@ -592,7 +592,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
             if (!ok) break;
             if (p == 0) {
               // the softmax may look at the values; all their units, where it does
-              if (one) mbar_arrive(&ctl.v_here[0]);
+              if (one) mbar_arrive(&ctl.v_here[0][g & 1]);
               ok = __all_sync(0xffffffffu, wait(&ctl.p_full[0][g & 1], (g >> 1) & 1, ctl, a.err, 35));
               if (!ok) break;
               tc_fence_after();
@@ -698,7 +698,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         if (i % C::kSub == 0) {
           uv = arrived();
           if (!ok) break;
-          if (one && in) mbar_arrive(&ctl.v_here[t]);
+          if (one && in) mbar_arrive(&ctl.v_here[t][met / C::kSub & 1]);
         }
         if (in) values(i % C::kSub, uv, i == from);
         if (!ok) break;
@@ -716,7 +716,7 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t o_at = tmem + C::kO + t * HDP + lanes;
     const float shift = kType<T> ? 0.f : 6.f;        // fp16 weights are 2^6 times as large
-    uint32_t votes = 0, blocks_seen = 0, g = 0;      // votes, blocks and steps so far
+    uint32_t votes = 0, g = 0;                       // votes and steps so far
     int units = 0;                                   // units of the tiles so far
     bool ok = true;
 #pragma unroll 1
@@ -817,7 +817,11 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         // product is made here, over what each row sees.
         const int block = (i0 + n) / C::kSub - lo, blocks = hi - lo;
         const int unit = units + min(C::kAhead + 2 * block, blocks + block) * C::kPer;   // as they are loaded
-        ok = wait(&ctl.v_here[t], (blocks_seen + n / C::kSub) & 1, ctl, a.err, 39);
+        // Not every block's values are looked at, and a wait sees no more of a phase than its parity: so two
+        // barriers take turns. The values two blocks before were here when the scores of this step's keys were asked
+        // for, and those of the block before when these were told of.
+        const uint32_t b = g / C::kSub;
+        ok = wait(&ctl.v_here[t][b & 1], (b >> 1) & 1, ctl, a.err, 39);
         for (int p = 0; p < C::kPer && ok; ++p)
           ok = wait(&ctl.full[(unit + p) % C::kUnits], (uint32_t)((unit + p) / C::kUnits) & 1, ctl, a.err, 40);
         ok = __all_sync(0xffffffffu, ok);
@@ -868,7 +872,6 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     }
     if (!ok) break;
     units += 2 * (hi - lo) * C::kPer;
-    blocks_seen += steps / C::kSub;
     if (steps > 0) {                                 // the last step's product, and all before it
       ok = __all_sync(0xffffffffu, wait(&ctl.o_done[t][(g - 1) & 1], ((g - 1) >> 1) & 1, ctl, a.err, 38));
       if (!ok) break;

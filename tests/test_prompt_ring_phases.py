@@ -125,6 +125,15 @@ def test_products_take_what_has_landed():
             assert not early, (tiles, seed, early)
 
 
+def test_softmax_looks_at_what_has_landed():
+    after_scores, here = _source()
+    for tiles in TILES:
+        for seed in range(80):
+            early = run(after_scores, here, tiles, seed)
+            assert not early, (tiles, seed, early)
+
+
 def test_the_model_tells():
-    """Values waited for without their step's scores."""
+    """Values waited for without their step's scores, or one barrier that the softmax looks at now and then."""
     assert any(run(False, 2, TILES[2], seed, looks=0.0) for seed in range(300))
+    assert any(run(True, 1, TILES[2], seed) for seed in range(300))
