@@ -849,6 +849,9 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
         const bool odd = (most & 0xFFFFu) >= inf || (most >> 16) >= inf;
         const bool found = any_of_tile(odd, t, votes, ctl, a.err, ok);
         if (!ok) break;
+        // zeros in the place of values past the end may be the other tile's, not fenced by its threads for this
+        // tile's product
+        if (C::kTiles == 2 && !found && key0 + C::kKeys > w.klen) fence_async_proxy();
         if (found) {
           const bool past = key0 + k >= w.klen;
           if (odd && past)
