@@ -94,6 +94,7 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[8], uint32_t top, 
     } else {
       y = fmaf(fmaf(-y, t, z), inv, y);
     }
+    if (up != 1.f) y = fminf(fmaxf(y, -7.f), 7.f);   // the lowest subnormal scales may lie far below max|x| / 7
     word += __float_as_uint(y + 12582920.f) << (4 * i);
   }
 }

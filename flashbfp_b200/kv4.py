@@ -2,8 +2,9 @@
 or attended to as they are held.
 
 A cached head of D values is cut into groups of 32 (the last may be shorter). A group's scale is the
-bf16 nearest to max|x| / 7, and a value is held as x / scale rounded to a whole number in -7..7 (nearest
-even), plus 8, in 4 bits: 4.5 bits a value with the scales. A group with an infinity or a NaN reads
+bf16 nearest to max|x| / 7, and a value is held as x / scale rounded to the nearest whole number (ties to
+even), plus 8, in 4 bits: 4.5 bits a value with the scales. Whole numbers end at -7 and 7 (only a scale among
+bf16's lowest subnormals, below 2^-130, lies so far from max|x| / 7 that a quotient passes them). A group with an infinity or a NaN reads
 back as NaN. Rows that enter are plain rows of any float type; what is already rounded stays what it
 is, so a row that is read back and written again is held as it was.
 

@@ -421,8 +421,8 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
  * The cache: for keys and for values, `values` [seqs][kv_heads][positions][16 g] bytes and `scales`
  * [seqs][kv_heads][positions][g] bf16, g = ceil(head_dim / 32) groups of 32 values. A group's scale s
  * is the bf16 nearest to max|x| / 7 and a value is held as n + 8, n = x / s rounded to nearest
- * even (0 where s is 0), in 4 bits: value 2 i in the low half of byte i, value 2 i + 1 in the high
- * half. A group with an infinity or NaN has a NaN scale. All four 16-byte aligned, positions a
+ * even and cut to -7..7 (0 where s is 0), in 4 bits: value 2 i in the low half of byte i, value
+ * 2 i + 1 in the high half. A group with an infinity or NaN has a NaN scale. All four 16-byte aligned, positions a
  * multiple of 32 below 2^30.
  *
  * fbfp_kv4_write: row r of k and v (any fbfp_dtype) to position pos[b] + r - starts[b] of its sequence.
