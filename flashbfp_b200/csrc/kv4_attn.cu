@@ -647,11 +647,11 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
       *reinterpret_cast<float4*>(a.part + to * hd + d) = r;
       if (d == 0) a.ml[to * 2] = M, a.ml[to * 2 + 1] = L;
     } else {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      float inv = L == 0.f ? 0.f : 1.f / L;
       const int64_t row = col / a.group;
       T* to = (T*)a.out + pc.b * a.o_seq + row * a.o_row + (pc.head * a.group + col % a.group) * a.o_head + d;
-      if (pos + row < 0 || pos + row >= a.c.positions) {
-        r = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pos + row < 0 || pos + row >= a.c.positions) {              // (L may be NaN)
+        r = make_float4(0.f, 0.f, 0.f, 0.f), inv = 0.f;
         atomicExch(a.err, 2);
       }
       store_from_float(to, kHalf ? FBFP_F16 : FBFP_BF16, 0, r.x * inv);
