@@ -73,7 +73,7 @@ __global__ void embed_kernel(const int64_t* tok, const bf16* table, int64_t voca
   const int r = blockIdx.y;
   int64_t t = tok[r];
   if (t < 0 || t >= vocab) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) atomicExch(err, 1);
+    if (threadIdx.x == 0 && blockIdx.x == 0) atomicMax(err, 1);
     t = 0;
   }
   const float s = bfr(scale);
@@ -261,7 +261,7 @@ __global__ void qk_rope_cache_kernel(const bf16* qkv, int nh, int nkv, int hd, c
   const bool is_q = head < nh;
   const int p = *pos_p + row;
   if (p < 0 || p >= max_ctx) {
-    if (threadIdx.x == 0) atomicExch(err, 2);
+    if (threadIdx.x == 0) atomicMax(err, 2);
     return;
   }
   const int64_t qkv_row = (int64_t)row * (nh + 2 * nkv) * hd;
@@ -455,7 +455,7 @@ decode_attention_step_kernel(const bf16* qkv, int nh, int nkv, int hd, const bf1
   const int group = nh / nkv, kvh = head / group;
   const int p = pos[row];
   if (p < 0 || p >= max_ctx) {                   // the whole row is skipped (no CTA counts)
-    if (threadIdx.x == 0 && head == 0 && split == 0) atomicExch(err, 2);
+    if (threadIdx.x == 0 && head == 0 && split == 0) atomicMax(err, 2);
     return;
   }
   const int lo = (window > 0 && p - window + 1 > 0) ? p - window + 1 : 0;

@@ -82,7 +82,7 @@ __device__ __forceinline__ Place place_of(int64_t r, const Kv4& c, int64_t rows,
   if (p.b < 0) return p;
   p.at += __ldg(base + p.b);
   if (p.at < 0 || p.at >= c.positions) {
-    if (tell) atomicExch(err, 2);
+    if (tell) atomicMax(err, 2);
     p.b = -1;
   }
   return p;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(Kv4 c, const __nv_
   if (b < 0) return;
   at += pos[b];
   if (at < 0 || at >= c.positions) {
-    if (lane == 0) atomicExch(err, 2);
+    if (lane == 0) atomicMax(err, 2);
     return;
   }
   const bool act = lane * 8 < c.hd;

@@ -652,7 +652,7 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
       T* to = (T*)a.out + pc.b * a.o_seq + row * a.o_row + (pc.head * a.group + col % a.group) * a.o_head + d;
       if (pos + row < 0 || pos + row >= a.c.positions) {              // (L may be NaN)
         r = make_float4(0.f, 0.f, 0.f, 0.f), inv = 0.f;
-        atomicExch(a.err, 2);
+        atomicMax(a.err, 2);
       }
       store_from_float(to, kHalf ? FBFP_F16 : FBFP_BF16, 0, r.x * inv);
       store_from_float(to, kHalf ? FBFP_F16 : FBFP_BF16, 1, r.y * inv);
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Args a, int block_c
   const int64_t at = (int64_t)__ldg(a.pos + b) + row;
   float inv = L == 0.f ? 0.f : 1.f / L;
   const bool in = at >= 0 && at < a.c.positions;
-  if (!in && lane == 0) atomicExch(a.err, 2);
+  if (!in && lane == 0) atomicMax(a.err, 2);
   T* to = (T*)a.out + b * a.o_seq + row * a.o_row + (int64_t)(head * a.group + col % a.group) * a.o_head + lane * 8;
   if (lane * 8 < a.c.hd)
 #pragma unroll

@@ -348,7 +348,8 @@ class GemmaDecoder:
             seen = torch.where(n > 0, self.pos + n - first, torch.zeros_like(n))
             rows = sum(min(r, window - 1) + m if window else r + m for r, m in zip(self.reach, lens) if m)
             plan[kind] = (first, starts(seen), rows)
-            self.err.masked_fill_(seen.sum() > rows, 2)      # positions that were not set through reset()
+            # positions that were not set through reset()
+            torch.maximum(self.err, (seen.sum() > rows).int() * 2, out=self.err)
         most = max(plan[kind][2] for kind in set(s.layer_types)) if s.layer_types else 0
         if most and (self.back[0] is None or self.back[0].shape[0] < most):
             room = min(self.batch * self.cache4[0].positions, -(-most // 1024) * 1024)

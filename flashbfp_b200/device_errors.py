@@ -1,5 +1,6 @@
 """Per device one word in which the kernels of ``attention`` and ``kv4`` record what they met: a
-position outside a cache, or a bounded device-side wait that gave up."""
+position outside a cache (2), or a bounded device-side wait that gave up (its site, 32 or more, which a
+position does not replace)."""
 from __future__ import annotations
 
 import threading

@@ -431,7 +431,8 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
  *   every q and k head, the rotary embedding with the bf16 cos/sin rows [positions][head_dim] at the
  *   row's position (roundings as fbfp_qk_rope_cache), q to q_out [rows][heads][head_dim], k and v to
  *   the cache as fbfp_kv4_write does. head_dim a multiple of 16.
- * A position outside the cache sets *err = 2, and nothing is written for that row.
+ * A position outside the cache sets *err = 2, unless a larger code stands there (a wait that gave
+ *   up), and nothing is written for that row.
  * fbfp_kv4_attention: q [seqs][rows][heads][head_dim]; row i of sequence b, at position pos[b] + i,
  *   attends to positions up to its own (with window > 0 only to the last `window` of those):
  *   softmax(q k^T scaling) v, rounded once to the output's type (q's; bf16 or fp16). A row whose
