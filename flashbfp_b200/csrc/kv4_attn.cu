@@ -245,14 +245,15 @@ __device__ __forceinline__ void load_scales(uint32_t at, uint32_t (&w)[(NG + 1) 
 }
 
 // The bits of the largest finite scale of 32 positions' values, of those that some column of the block sees:
-// a position per lane.
+// a position per lane. `low`: a lane's smallest scale so far but 0, less one (or two) in its bits.
 template <int NG>
-__device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts) {
-  uint32_t w[(NG + 1) / 2], high = 0;                 // in halves
+__device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts, uint32_t& low) {
+  uint32_t w[(NG + 1) / 2], high = 0, least = 0xFFFFFFFFu;              // in halves
   load_scales<NG>(vss + (threadIdx.x & 31) * 2 * NG, w);
 #pragma unroll
-  for (int i = 0; i < (NG + 1) / 2; ++i) high = __vmaxu2(high, w[i]);
+  for (int i = 0; i < (NG + 1) / 2; ++i) high = __vmaxu2(high, w[i]), least = __vminu2(least, w[i] - 0x00010001u);
   high = counts ? max(high & 0xFFFFu, high >> 16) : 0;
+  low = counts ? min(low, min(least & 0xFFFFu, least >> 16)) : low;
   high = __reduce_max_sync(0xffffffffu, high);
   if (high < 0x7F80u) return high;
   high = 0;                                           // infinite and NaN scales make their own dims NaN: the rest counts
@@ -264,7 +265,10 @@ __device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts) {
   return __reduce_max_sync(0xffffffffu, counts ? high : 0u);
 }
 
-// O += (p s) n of 32 positions. The weights p carry a power of two that brings (p s) into fp16's range.
+// O += (p s) n of 32 positions. The weights p carry a power of two that brings (p s) into fp16's range: 2^15 at most,
+// 2^8 where the largest weight meets the largest scale. What is below 2^-25 vanishes, which is nothing beside a
+// result in which the largest weight meets a scale 2^-kDeep as large; where smaller ones were met, add_in_rounds
+// takes this one's place.
 // CUT: some column does not see some position, whose scale may be anything.
 template <int NG, int NT, int WARPS, bool CUT>
 __device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float (&p)[2][NT][4],
@@ -309,6 +313,66 @@ __device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float
         const uint32_t b0 = pack_h(w[0], w[1]), b1 = pack_h(w[2], w[3]);
         mma(o[j][0][n], a0, b0, b1, o[j][0][n]);
         mma(o[j][1][n], a1, b0, b1, o[j][1][n]);
+      }
+    }
+  }
+}
+
+constexpr int kDeep = 14;
+// The same in several rounds: the products from 2^-14 on, from 2^-28 on and so on, each brought up to the first one's
+// range. Out of line, on copies in memory: inlined it took registers from every tile (8 sequences in a window 17.8 ->
+// 21.4 us, 16 long sequences 172 -> 182).
+template <int NG, int NT>
+struct Rounds {
+  float o[NG][2][NT][4], p[2][NT][4];
+  int at_c[NT], low_c[NT];
+};
+template <int NG, int NT, int MASK>
+__device__ __noinline__ void add_in_rounds(Rounds<NG, NT>& m, uint32_t vss, uint32_t vb, uint32_t half, int p0, int rounds) {
+  const int t = threadIdx.x & 3;
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+    const float down = __uint_as_float((uint32_t)(127 - kDeep * round) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + kDeep * round) << 23);
+    const float least = round + 1 < rounds ? down * __uint_as_float((uint32_t)(127 - kDeep) << 23) : 0.f;
+#pragma unroll 1
+    for (int hj = 0; hj < 2 * NG; ++hj) {
+      const int h = hj / NG, j = hj % NG;
+      uint32_t x[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        constexpr uint32_t turn = MASK ? ((4 * 16 * NG >> 7) & MASK) << 4 : 0;                 // rows 4 further
+        const uint32_t w0 = lds32((MASK ? vb ^ (j << 4) : vb + (j << 4)) + (16 * h + 8 * i) * 16 * NG);
+        const uint32_t w1 = lds32((MASK ? vb ^ ((j << 4) ^ turn) : vb + (j << 4)) + (16 * h + 8 * i + 4) * 16 * NG);
+        pairs(__byte_perm(w0, w1, half), x[i]);
+      }
+      const uint32_t a0[4] = {x[0][0], x[0][1], x[1][0], x[1][1]};
+      const uint32_t a1[4] = {x[0][2], x[0][3], x[1][2], x[1][3]};
+      float s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint16_t bits;
+        asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(bits) : "r"(vss + ((16 * h + t + 4 * e) * NG + j) * 2));
+        s[e] = bf16_bits_to_float(bits);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = p0 + 16 * h + t + 4 * e;
+          const float y = m.p[h][n][e] * s[e];
+          const bool mine = round == 0 ? !(y < least) : y < down && y >= least;        // (the first takes NaN)
+          w[e] = at <= m.at_c[n] && at >= m.low_c[n] && mine ? y * up : 0.f;
+        }
+        const uint32_t b0 = pack_h(w[0], w[1]), b1 = pack_h(w[2], w[3]);
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        float d0[4], d1[4];
+        mma(d0, a0, b0, b1, zero);
+        mma(d1, a1, b0, b1, zero);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m.o[j][0][n][e] = fmaf(d0[e], down, m.o[j][0][n][e]), m.o[j][1][n][e] = fmaf(d1[e], down, m.o[j][1][n][e]);
       }
     }
   }
@@ -444,7 +508,8 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
 
   float o[NG][2][NT][4];
   float m[NT], l[NT];
-  int ev = -1000;                                     // weights are 2^(score - m + 8 - ev), ev near the scales' exponent
+  int ev = -1000;                                     // weights are 2^(score - m + 8 - ev), ev near the scales' largest exponent
+  uint32_t low = 0xFFFFu;                             // the smallest scale that this lane met
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = -INFINITY, l[n] = 0.f;
@@ -542,7 +607,7 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
             if (at_p > at_c[n] || at_p < low_c[n]) p[h][n][e] = -INFINITY;
           }
     }
-    const uint32_t high = largest_scale<NG>(vss, counts);
+    const uint32_t high = largest_scale<NG>(vss, counts, low);
     const int ex = min(max((int)(high >> 7) - 127, -90), 120);
     const bool grown = ex > ev + 3;                   // the references move when weights could pass 2^14 in fp16
     const float turn = grown ? (ev < -90 ? 0.f : ex2((float)(ev - ex))) : 1.f;
@@ -585,8 +650,36 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
           l[n] += p[h][n][e];
         }
     }
-    if (cut) add_values<NG, NT, WARPS, true>(o, p, vss, vb, half, p0, at_c, low_c);
-    else add_values<NG, NT, WARPS, false>(o, p, vss, vb, half, p0, at_c, low_c);
+    if (__any_sync(0xffffffffu, low < (uint32_t)(ev - kDeep + 127) << 7)) {
+      const uint32_t least = __reduce_min_sync(0xffffffffu, low);
+      const int deep = ev - (least < 0x80u ? -133 : (int)(least >> 7) - 127);
+      Rounds<NG, NT> r;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        r.at_c[n] = at_c[n], r.low_c[n] = low_c[n];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            r.p[h][n][e] = p[h][n][e];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) r.o[j][h][n][e] = o[j][h][n][e];
+          }
+      }
+      add_in_rounds<NG, NT, C::kMask>(r, vss, vb, half, p0, min((deep + kDeep - 1) / kDeep, 9));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < NG; ++j) o[j][h][n][e] = r.o[j][h][n][e];
+    } else if (cut) {
+      add_values<NG, NT, WARPS, true>(o, p, vss, vb, half, p0, at_c, low_c);
+    } else {
+      add_values<NG, NT, WARPS, false>(o, p, vss, vb, half, p0, at_c, low_c);
+    }
     __syncwarp();
     if (lane == 0 && done + C::kDepth < 2 * mine) load(done + C::kDepth);
   }

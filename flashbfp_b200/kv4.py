@@ -134,5 +134,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, pos: torch.Tensor, window: i
     whose position is outside the cache gives 0. The result has q's shape and type.
 
     The cached whole numbers enter the products as they are; scales, scores, softmax statistics and sums
-    are fp32."""
+    are fp32. Two roundings come before the result's own. Queries enter as fp16 under a power of two for each
+    row and head: bf16 values below 2^-29 of its largest lose bits, those below 2^-37 are 0. A softmax weight times
+    its value's scale is rounded to fp16: by 2^-11 of itself, or, where it is small beside the row's others, by
+    at most 2^-19 of the largest weight times the smallest scale."""
     return _module().kv4_attention(q, cache, pos, window, scaling, out, err)

@@ -435,7 +435,9 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
  *   up), and nothing is written for that row.
  * fbfp_kv4_attention: q [seqs][rows][heads][head_dim]; row i of sequence b, at position pos[b] + i,
  *   attends to positions up to its own (with window > 0 only to the last `window` of those):
- *   softmax(q k^T scaling) v, rounded once to the output's type (q's; bf16 or fp16). A row whose
+ *   softmax(q k^T scaling) v, rounded once to the output's type (q's; bf16 or fp16). Queries enter
+ *   as fp16 under a power of two per row and head; a weight times its value's scale is rounded to
+ *   fp16 by 2^-11 of itself, or by 2^-19 of the largest weight times the smallest scale. A row whose
  *   position is outside the cache gives 0 and sets *err = 2. `workspace`:
  *   fbfp_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, its contents of no account; not
  *   shared by calls that run at the same time.
