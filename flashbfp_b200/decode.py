@@ -92,6 +92,15 @@ def rope_tables(theta: float, head_dim: int, max_ctx: int, device) -> tuple:
     return emb.cos().to(torch.bfloat16).contiguous(), emb.sin().to(torch.bfloat16).contiguous()
 
 
+def back_rows(have: int, need: int, most: int) -> int:
+    """Rows of the buffers that a chunk's keys and values are read back into, which hold ``have`` so far: at
+    least twice as many whenever they grow, so that a long prompt in many chunks asks for few of them (and the
+    allocator, which keeps what was given back, for no more than twice the last), up to ``most`` in the cache."""
+    if need <= have:
+        return have
+    return max(need, min(max(2 * have, -(-need // 1024) * 1024), most))
+
+
 class GemmaDecoder:
     """One rank's decoder. Without ``reducer`` the layers hold whole matrices. With ``reducer``
     (an ``NVLinkAllReduce`` over the tensor-parallel ranks) they hold this rank's parts as
@@ -351,10 +360,11 @@ class GemmaDecoder:
             # positions that were not set through reset()
             torch.maximum(self.err, (seen.sum() > rows).int() * 2, out=self.err)
         most = max(plan[kind][2] for kind in set(s.layer_types)) if s.layer_types else 0
-        if most and (self.back[0] is None or self.back[0].shape[0] < most):
-            room = min(self.batch * self.cache4[0].positions, -(-most // 1024) * 1024)
-            self.back = [torch.empty(max(room, most), self.hkv, s.head_dim, dtype=torch.bfloat16, device=dev)
-                         for _ in range(2)]
+        have = 0 if self.back[0] is None else self.back[0].shape[0]
+        room = back_rows(have, most, self.batch * self.cache4[0].positions if self.cache4 else 0)
+        if room != have:
+            self.back = [None, None]                         # given back before the larger pair is asked for
+            self.back = [torch.empty(room, self.hkv, s.head_dim, dtype=torch.bfloat16, device=dev) for _ in range(2)]
         return plan
 
     def _attend4(self, li: int, ly: DecodeLayer, qkv, q, attn, m: int, plan) -> None:
