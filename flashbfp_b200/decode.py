@@ -356,6 +356,7 @@ class GemmaDecoder:
             first = (self.pos + (1 - window)).clamp_min(0) if window else torch.zeros_like(self.pos)
             seen = torch.where(n > 0, self.pos + n - first, torch.zeros_like(n))
             rows = sum(min(r, window - 1) + m if window else r + m for r, m in zip(self.reach, lens) if m)
+            rows = max(rows, 1)                              # (positions before the cache: nothing to read back)
             plan[kind] = (first, starts(seen), rows)
             # positions that were not set through reset()
             torch.maximum(self.err, (seen.sum() > rows).int() * 2, out=self.err)

@@ -30,3 +30,16 @@ def test_buffers_grow_few_times():
         assert torch.equal(x[:, :, :11000], y[:, :, :11000])
     assert torch.isfinite(many).all()
     one.release()
+
+
+def test_positions_before_the_cache_are_recorded():
+    model, dec = _decoder(5, max_ctx=64, max_prefill=8)
+    for call in (lambda: dec.step(), lambda: dec.prefill([3]), lambda: dec.prefill([3, 4, 5])):
+        dec.reset(-1)
+        call()
+        with pytest.raises(RuntimeError, match="outside"):
+            dec.check()
+    dec.reset(0)
+    dec.prefill([3])
+    dec.check()
+    dec.release()
