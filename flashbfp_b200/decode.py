@@ -438,6 +438,11 @@ class GemmaDecoder:
             _lib.check(L.fbfp_post_residual_norm(P(down), m, P(ly.post_ffn_ln), P(h), P(nxt), eps,
                                                  s.hidden, P(x), st), "fbfp_post_residual_norm")
 
+    def _bound4(self, lens: Sequence[int]) -> None:
+        """Record rows that end behind max_ctx: the 4-bit cache rounds its length up, so its calls do not."""
+        if any(n and r + n > self.max_ctx for r, n in zip(self.reach, lens)):
+            self.err.clamp_(min=2)
+
     def _embed(self, ids: torch.Tensor, m: int) -> None:
         L, s, st = self.L, self.shape, _lib.stream_ptr(self.device)
         P = _lib.ptr
@@ -468,6 +473,7 @@ class GemmaDecoder:
         logits, picks and positions of the sequences that have some."""
         m = sum(lens)
         self._embed(self.ids, m)
+        self._bound4(lens)
         plan = self._chunk4(lens)
         self._layers(m, None, plan)
         some = [b for b, n in enumerate(lens) if n]
@@ -557,6 +563,8 @@ class GemmaDecoder:
         """One token per sequence: embeds self.tok[b] at position self.pos[b], leaves the greedy
         next tokens in self.tok and the logits in self.logits, and advances every position."""
         with torch.cuda.device(self.device), torch.cuda.stream(self.stream):
+            if self.int4:
+                self._bound4([1] * self.batch)
             if self.graph is not None:
                 self.graph.replay()
             else:

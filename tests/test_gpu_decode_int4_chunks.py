@@ -32,6 +32,34 @@ def test_buffers_grow_few_times():
     one.release()
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_positions_behind_max_ctx_are_recorded(captured):
+    """max_ctx is the limit, as with the bf16 cache, though the 4-bit cache's length is a multiple of 32."""
+    model, dec = _decoder(5, max_ctx=41, max_prefill=16, batch=2)
+    assert dec.cache4[0].positions == 64
+    dec.reset([38, 0])
+    if captured:
+        dec.capture()
+    for _ in range(3):
+        dec.step()
+    dec.check()
+    dec.step()                                           # position 41
+    with pytest.raises(RuntimeError, match=r"outside the KV cache \(41\)"):
+        dec.check()
+    dec.reset([30, 0])
+    dec.prefill(_ids(11, 1))                             # up to 40
+    dec.check()
+    dec.reset([0, 30])
+    dec.prefill_packed([[], _ids(12, 1)])
+    with pytest.raises(RuntimeError, match="outside"):
+        dec.check()
+    dec.reset(41)
+    dec.prefill_packed([_ids(3, 2), []])
+    with pytest.raises(RuntimeError, match="outside"):
+        dec.check()
+    dec.release()
+
+
 def test_positions_before_the_cache_are_recorded():
     model, dec = _decoder(5, max_ctx=64, max_prefill=8)
     for call in (lambda: dec.step(), lambda: dec.prefill([3]), lambda: dec.prefill([3, 4, 5])):
