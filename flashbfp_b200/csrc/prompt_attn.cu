@@ -1028,6 +1028,8 @@ Plan plan_of(int64_t rows, int64_t kv_rows, int64_t seqs, int64_t heads, int64_t
   return p;
 }
 
+constexpr int64_t kNoWindow = 1 << 30;               // no sequence is longer
+
 template <int HDP, typename T>
 int launch(const PromptArgs& a, const PromptMaps& m, const Plan& p, cudaStream_t st) {
   auto kernel = prompt_attn_kernel<HDP, T>;
@@ -1073,6 +1075,7 @@ using namespace fbfp;
 extern "C" int64_t fbfp_prompt_attention_workspace_bytes(int64_t rows, int64_t kv_rows, int64_t seqs, int64_t heads,
                                                          int64_t kv_heads, int64_t head_dim, int64_t window) {
   if (rows < 1 || kv_rows < 1 || seqs < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1) return -1;
+  if (window > kNoWindow) window = kNoWindow;
   const Plan p = plan_of(rows, kv_rows, seqs, heads, kv_heads, head_dim, window);
   return p.splits > 1 ? p.splits * rows * heads * (head_dim + 1) * 4 : 0;
 }
@@ -1096,6 +1099,7 @@ extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v
                      o_head >= 0 && ((q_row | q_head | k_row | k_head | v_row | v_head | o_row | o_head) & 7) == 0,
                  "strides must be multiples of 8");
   FBFP_CHECK_ARG(window >= 0, "negative window");
+  if (window > kNoWindow) window = kNoWindow;        // before any sum with it
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
     return set_error(FBFP_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");
   const Plan p = plan_of(rows, kv_rows, seqs, heads, kv_heads, head_dim, window);
@@ -1104,7 +1108,6 @@ extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v
   FBFP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 31) == 0),
                  "the workspace must be %lld bytes, 32-byte aligned", (long long)need);
   const int group = (int)(heads / kv_heads);
-  if (window > (1 << 30)) window = 1 << 30;          // no longer than any sequence
   PromptArgs a{rows, kv_rows, o_row, o_head, v_row, v_head, window, starts, kv_starts ? kv_starts : starts,
                head_dim % 16 == 0 && ((uintptr_t)out & 31) == 0 && ((o_row | o_head) & 15) == 0, (int)seqs, (int)heads,
                (int)head_dim, p.hp, p.ntok, p.head_blocks, group, p.splits,

@@ -109,3 +109,11 @@ def test_empty_cache_refusals():
             kv4.empty_cache(**{**a, **bad})
     c = kv4.empty_cache(3, 1, 32, 40, "cpu")
     assert c.sequence(1).k_values.data_ptr() == c.k_values[1].data_ptr() and c.k_scales.shape[3] == 2
+
+
+def test_the_longest_window_is_none(L):
+    """A window of 2^63 - 1 plans as one that no sequence fills (the workspace follows the plan)."""
+    for n in ((16, 20000, 1, 16, 8, 256), (1, 9000, 1, 2, 1, 64), (4096, 4096, 3, 16, 8, 128)):
+        none, *others = [L.fbfp_prompt_attention_workspace_bytes(*n, w) for w in (0, (1 << 63) - 1, (1 << 63) - 200, 1 << 40)]
+        assert others == [none] * 3, (n, none, others)
+    assert L.fbfp_prompt_attention_workspace_bytes(16, 20000, 1, 16, 8, 256, 0) > 0
