@@ -21,6 +21,7 @@
 // with a running maximum and sum; the warps join in shared memory, parts of a sequence in a second
 // launch.
 #include <cuda.h>
+#include <cmath>
 
 #include "kv4.cuh"
 #include "pdl.cuh"
@@ -907,6 +908,7 @@ extern "C" int fbfp_kv4_attention(const fbfp_kv4_cache* cache, const void* q, in
                      ((q_seq | q_row | q_head | o_seq | o_row | o_head) & 7) == 0,
                  "strides must be multiples of 8");
   FBFP_CHECK_ARG(window >= 0, "negative window");
+  FBFP_CHECK_ARG(std::isfinite(scaling * 1.4426950408889634f), "scaling %g is not finite, or its base-2 form is not", (double)scaling);
   if (((uintptr_t)q | (uintptr_t)out) & 15) return set_error(FBFP_ERR_ALIGN, "q and out must be 16-byte aligned");
   FBFP_CHECK_ARG((int64_t)c.seqs * c.nkv * c.positions < ((int64_t)1 << 31), "the cache has 2^31 rows or more");
   if (window > c.positions + rows) window = 0;              // sees everything

@@ -24,6 +24,7 @@
 // keys: 84-88 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
 // scores of 128 keys at once for heads of 128 (fewer bytes from shared memory, but no buffer to run ahead in).
 #include <cuda.h>
+#include <cmath>
 
 #include "common.cuh"
 #include "pdl.cuh"
@@ -1099,6 +1100,7 @@ extern "C" int fbfp_prompt_attention(const void* q, const void* k, const void* v
                      o_head >= 0 && ((q_row | q_head | k_row | k_head | v_row | v_head | o_row | o_head) & 7) == 0,
                  "strides must be multiples of 8");
   FBFP_CHECK_ARG(window >= 0, "negative window");
+  FBFP_CHECK_ARG(std::isfinite(scaling * 1.4426950408889634f), "scaling %g is not finite, or its base-2 form is not", (double)scaling);
   if (window > kNoWindow) window = kNoWindow;        // before any sum with it
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
     return set_error(FBFP_ERR_ALIGN, "q, k, v and out must be 16-byte aligned");

@@ -117,3 +117,10 @@ def test_the_longest_window_is_none(L):
         none, *others = [L.fbfp_prompt_attention_workspace_bytes(*n, w) for w in (0, (1 << 63) - 1, (1 << 63) - 200, 1 << 40)]
         assert others == [none] * 3, (n, none, others)
     assert L.fbfp_prompt_attention_workspace_bytes(16, 20000, 1, 16, 8, 256, 0) > 0
+
+
+@pytest.mark.parametrize("scaling", [float("inf"), float("-inf"), float("nan"), 3e38, -3e38])
+def test_scalings_that_are_not_finite(L, scaling):
+    refused(L, L.fbfp_kv4_attention(cache(), P, 1, 1, 4, 256, 0, 64, P, 0, scaling, P, 256, 0, 64, P, 1 << 30, P, None), "scaling")
+    refused(L, L.fbfp_prompt_attention(P, P, P, 1, 8, 8, 1, 4, 2, 64, 256, 64, 128, 64, 128, 64, P, None, 0, scaling, P, 256,
+                                       64, P, 1 << 30, P, None), "scaling")
