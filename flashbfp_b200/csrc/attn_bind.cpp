@@ -220,6 +220,8 @@ PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (k.code != v.code) refuse(PyExc_ValueError, "k and v must have one dtype");
     check_out(*k.t, "k");
     check_out(*v.t, "v");
+    if (k.rows && k.t->const_data_ptr() == v.t->const_data_ptr())
+      refuse(PyExc_ValueError, "k and v are written to one place");
     if (k.rows) {
       int32_t* const err = error_word(a[5], c.index);
       call(c.index, "fbfp_kv4_read", [&](void* st) {

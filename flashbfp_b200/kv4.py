@@ -113,7 +113,7 @@ def kv4_read(cache: KV4Cache, first: torch.Tensor, starts: torch.Tensor, rows: O
              err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows k, v [rows, kv_heads, D] of ``dtype`` from the cache: row r of sequence b comes from position
     first[b] + r - starts[b]. ``out`` gives both tensors (any strides between rows and heads), else
-    ``rows`` and ``dtype`` make them; rows from starts[-1] on are left as they were."""
+    ``rows`` and ``dtype`` make them; rows from starts[-1] on are left as they were. The two must not overlap."""
     if out is None:
         if rows is None:
             raise ValueError("kv4_read needs the number of rows, or out")

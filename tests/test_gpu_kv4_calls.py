@@ -52,3 +52,15 @@ def test_scalings_at_the_ends_of_fp32():
             kv4.kv4_attention(q, cache, ints([0] * 4), scaling=scaling)
     for scaling in (1e-45, -1e-40, 1e30):                    # equal scores: the same mean whatever they are times
         assert torch.equal(attention.prompt_attention(q, k, k, s, scaling=scaling), q)
+
+
+def test_both_results_in_one_place():
+    from flashbfp_b200 import kv4
+    cache = kv4.empty_cache(1, 2, 32, 64, DEV)
+    x = torch.zeros(4, 2, 64, **BF)
+    with pytest.raises(ValueError, match="one place"):
+        kv4.kv4_read(cache, ints([0]), ints([0, 4]), out=[x, x])
+    rows = torch.ones(4, 6, 64, **BF)                        # two parts of fused rows are two places
+    kv4.kv4_read(cache, ints([0]), ints([0, 4]), out=[rows[:, 2:4], rows[:, 4:]])
+    assert bool((rows[:, :2] == 1).all()) and not rows[:, 2:].any()
+    kv4.kv4_read(cache, ints([0]), ints([0, 0]), out=[x[:0], x[:0]])
