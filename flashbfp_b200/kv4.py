@@ -82,11 +82,12 @@ def kv4_append(cache: KV4Cache, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm:
         _lib.require_cuda(t, name)
         if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != values.device:
             raise ValueError(f"{name} must be contiguous bfloat16 on {values.device}")
-    rows, heads = qkv.shape[0], qkv.shape[1] // d - 2 * kvh
-    if qkv.dim() != 2 or heads < 1 or qkv.shape[1] != (heads + 2 * kvh) * d or q_out.numel() != rows * heads * d:
+    rows, width = qkv.shape if qkv.dim() == 2 else (0, 0)
+    heads = width // d - 2 * kvh
+    if heads < 1 or width != (heads + 2 * kvh) * d or q_out.numel() != rows * heads * d:
         raise ValueError(f"qkv {tuple(qkv.shape)} and q_out {tuple(q_out.shape)} do not hold heads of {d} beside "
                          f"2 x {kvh}")
-    if q_norm.numel() != d or k_norm.numel() != d or cos.shape != sin.shape or cos.shape[1] != d:
+    if q_norm.numel() != d or k_norm.numel() != d or cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != d:
         raise ValueError("norm weights and cos / sin rows must have one value per value of a head")
     if cos.shape[0] < cache.positions:
         raise ValueError(f"cos and sin hold {cos.shape[0]} positions, the cache {cache.positions}")

@@ -64,3 +64,21 @@ def test_both_results_in_one_place():
     kv4.kv4_read(cache, ints([0]), ints([0, 4]), out=[rows[:, 2:4], rows[:, 4:]])
     assert bool((rows[:, :2] == 1).all()) and not rows[:, 2:].any()
     kv4.kv4_read(cache, ints([0]), ints([0, 0]), out=[x[:0], x[:0]])
+
+
+def test_append_refuses_other_shapes():
+    from flashbfp_b200 import kv4
+    d = 32
+    cache = kv4.empty_cache(2, 1, 32, d, DEV)
+    ok = dict(qkv=torch.zeros(2, 4 * d, **BF), w=torch.zeros(d, **BF), ang=torch.zeros(32, d, **BF), out=torch.zeros(2, 2, d, **BF))
+
+    def f(**kw):
+        a = {**ok, **kw}
+        kv4.kv4_append(cache, a["qkv"], a["w"], a["w"], 1e-6, a["ang"], a["ang"], ints([0, 0]), a["out"])
+
+    f()
+    for bad, text in ((dict(qkv=torch.zeros(8 * d, **BF)), "do not hold heads"), (dict(qkv=torch.zeros(2, 4, d, **BF)), "do not hold heads"),
+                      (dict(qkv=torch.zeros((), **BF)), "do not hold heads"), (dict(ang=torch.zeros(32 * d, **BF)), "one value per value"),
+                      (dict(ang=torch.zeros(32, 1, d, **BF)), "one value per value"), (dict(out=torch.zeros(2, 3, d, **BF)), "q_out")):
+        with pytest.raises(ValueError, match=text):
+            f(**bad)
