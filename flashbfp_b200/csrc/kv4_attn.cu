@@ -246,7 +246,7 @@ __device__ __forceinline__ void load_scales(uint32_t at, uint32_t (&w)[(NG + 1) 
 }
 
 // The bits of the largest finite scale of 32 positions' values, of those that some column of the block sees:
-// a position per lane. `low`: a lane's smallest scale so far but 0, less one (or two) in its bits.
+// a position per lane. `low`: the lane's smallest scale but 0, less one (or two) in its bits; 0xFFFF: none.
 template <int NG>
 __device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts, uint32_t& low) {
   uint32_t w[(NG + 1) / 2], high = 0, least = 0xFFFFFFFFu;              // in halves
@@ -254,7 +254,7 @@ __device__ __forceinline__ uint32_t largest_scale(uint32_t vss, bool counts, uin
 #pragma unroll
   for (int i = 0; i < (NG + 1) / 2; ++i) high = __vmaxu2(high, w[i]), least = __vminu2(least, w[i] - 0x00010001u);
   high = counts ? max(high & 0xFFFFu, high >> 16) : 0;
-  low = counts ? min(low, min(least & 0xFFFFu, least >> 16)) : low;
+  low = counts ? min(least & 0xFFFFu, least >> 16) : 0xFFFFu;
   high = __reduce_max_sync(0xffffffffu, high);
   if (high < 0x7F80u) return high;
   high = 0;                                           // infinite and NaN scales make their own dims NaN: the rest counts
@@ -331,14 +331,23 @@ struct Rounds {
 template <int NG, int NT, int MASK>
 __device__ __noinline__ void add_in_rounds(Rounds<NG, NT>& m, uint32_t vss, uint32_t vb, uint32_t half, int p0, int rounds) {
   const int t = threadIdx.x & 3;
+  float p[2][NT][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = p0 + 16 * h + t + 4 * e;
+        p[h][n][e] = at <= m.at_c[n] && at >= m.low_c[n] ? m.p[h][n][e] : -1.f;        // -1: not seen
+      }
 #pragma unroll 1
-  for (int round = 0; round < rounds; ++round) {
-    const float down = __uint_as_float((uint32_t)(127 - kDeep * round) << 23);
-    const float up = __uint_as_float((uint32_t)(127 + kDeep * round) << 23);
-    const float least = round + 1 < rounds ? down * __uint_as_float((uint32_t)(127 - kDeep) << 23) : 0.f;
-#pragma unroll 1
-    for (int hj = 0; hj < 2 * NG; ++hj) {
-      const int h = hj / NG, j = hj % NG;
+  for (int j = 0; j < NG; ++j) {
+    float o[2][NT][4];
+#pragma unroll
+    for (int i = 0; i < 8 * NT; ++i) (&o[0][0][0])[i] = (&m.o[j][0][0][0])[i];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       uint32_t x[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -356,26 +365,39 @@ __device__ __noinline__ void add_in_rounds(Rounds<NG, NT>& m, uint32_t vss, uint
         asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(bits) : "r"(vss + ((16 * h + t + 4 * e) * NG + j) * 2));
         s[e] = bf16_bits_to_float(bits);
       }
+#pragma unroll 1
+      for (int round = 0; round < rounds; ++round) {
+        const float down = __uint_as_float((uint32_t)(127 - kDeep * round) << 23);
+        const float up = __uint_as_float((uint32_t)(127 + kDeep * round) << 23);
+        const float least = round + 1 < rounds ? down * __uint_as_float((uint32_t)(127 - kDeep) << 23) : 0.f;
+        bool none = true;
+        uint32_t b[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at = p0 + 16 * h + t + 4 * e;
-          const float y = m.p[h][n][e] * s[e];
-          const bool mine = round == 0 ? !(y < least) : y < down && y >= least;        // (the first takes NaN)
-          w[e] = at <= m.at_c[n] && at >= m.low_c[n] && mine ? y * up : 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const float y = p[h][n][e] * s[e];
+            const bool mine = round == 0 ? !(y < least) : y < down && y >= least;      // (the first takes NaN)
+            w[e] = p[h][n][e] != -1.f && mine ? y * up : 0.f;
+          }
+          b[n][0] = pack_h(w[0], w[1]), b[n][1] = pack_h(w[2], w[3]);
+          none &= (b[n][0] | b[n][1]) == 0;
         }
-        const uint32_t b0 = pack_h(w[0], w[1]), b1 = pack_h(w[2], w[3]);
-        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        float d0[4], d1[4];
-        mma(d0, a0, b0, b1, zero);
-        mma(d1, a1, b0, b1, zero);
+        if (__all_sync(0xffffffffu, none)) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          m.o[j][0][n][e] = fmaf(d0[e], down, m.o[j][0][n][e]), m.o[j][1][n][e] = fmaf(d1[e], down, m.o[j][1][n][e]);
+        for (int n = 0; n < NT; ++n) {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+          float d0[4], d1[4];
+          mma(d0, a0, b[n][0], b[n][1], zero);
+          mma(d1, a1, b[n][0], b[n][1], zero);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[0][n][e] = fmaf(d0[e], down, o[0][n][e]), o[1][n][e] = fmaf(d1[e], down, o[1][n][e]);
+        }
       }
     }
+#pragma unroll
+    for (int i = 0; i < 8 * NT; ++i) (&m.o[j][0][0][0])[i] = (&o[0][0][0])[i];
   }
 }
 
@@ -608,7 +630,9 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
             if (at_p > at_c[n] || at_p < low_c[n]) p[h][n][e] = -INFINITY;
           }
     }
-    const uint32_t high = largest_scale<NG>(vss, counts, low);
+    uint32_t here;
+    const uint32_t high = largest_scale<NG>(vss, counts, here);
+    low = min(low, here);
     const int ex = min(max((int)(high >> 7) - 127, -90), 120);
     const bool grown = ex > ev + 3;                   // the references move when weights could pass 2^14 in fp16
     const float turn = grown ? (ev < -90 ? 0.f : ex2((float)(ev - ex))) : 1.f;
@@ -651,9 +675,23 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
           l[n] += p[h][n][e];
         }
     }
+    // Rounds, where scales met lie so far below the largest, and this tile's products reach so low.
+    int rounds = 1;
     if (__any_sync(0xffffffffu, low < (uint32_t)(ev - kDeep + 127) << 7)) {
-      const uint32_t least = __reduce_min_sync(0xffffffffu, low);
-      const int deep = ev - (least < 0x80u ? -133 : (int)(least >> 7) - 127);
+      float p_low = INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p_low = fminf(p_low, p[h][n][e] == 0.f ? INFINITY : p[h][n][e]);
+      p_low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(p_low)));
+      if (!(p_low * bf16_bits_to_float(__reduce_min_sync(0xffffffffu, here)) >= __uint_as_float((uint32_t)(127 - kDeep) << 23))) {
+        const uint32_t least = __reduce_min_sync(0xffffffffu, low);
+        rounds = min((ev - (least < 0x80u ? -133 : (int)(least >> 7) - 127) + kDeep - 1) / kDeep, 9);
+      }
+    }
+    if (rounds > 1) {                                 // the same in all lanes
       Rounds<NG, NT> r;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -667,7 +705,7 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
             for (int j = 0; j < NG; ++j) r.o[j][h][n][e] = o[j][h][n][e];
           }
       }
-      add_in_rounds<NG, NT, C::kMask>(r, vss, vb, half, p0, min((deep + kDeep - 1) / kDeep, 9));
+      add_in_rounds<NG, NT, C::kMask>(r, vss, vb, half, p0, rounds);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
