@@ -169,7 +169,7 @@ __device__ __forceinline__ OutRange out_range(const TcShared& S, const TcArgs& a
 __device__ __forceinline__ void tc_issue_weights(const TcShared& S, const TcArgs& a, const TcMaps& M,
                                                  int64_t u0, int64_t i, int64_t u, int s, uint32_t xbytes) {
   uint8_t* sb = S.stage + (size_t)s * tc::kStageBytes;
-  uint64_t* const full = &S.full[i % tc::kFull];
+  uint64_t* const full = &S.full[(uint32_t)i % tc::kFull];
   const OutRange orr = out_range(S, a, u0, i);
   const int rg = (int)(u / a.n_stages), st = (int)(u % a.n_stages);
   mbar_arrive_expect_tx(full, tc::kWeightTx + xbytes + (uint32_t)orr.n * 4 +
@@ -186,7 +186,7 @@ __device__ __forceinline__ void tc_issue_x(const TcShared& S, const TcArgs& a, c
   const int st = (int)(u % a.n_stages);
 #pragma unroll
   for (int b = 0; b < 4; ++b)
-    tma_2d_g2s(sb + tc::kXOff + b * tc::kXBox, &M.x, st * 256 + b * 64, 0, &S.full[i % tc::kFull]);
+    tma_2d_g2s(sb + tc::kXOff + b * tc::kXBox, &M.x, st * 256 + b * 64, 0, &S.full[(uint32_t)i % tc::kFull]);
 }
 
 __device__ void tc_producer(const TcShared& S, const TcArgs& a, const TcMaps& M, int64_t u0, int64_t u1) {

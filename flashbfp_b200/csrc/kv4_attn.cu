@@ -7,11 +7,12 @@
 // fp32, and the softmax weights before those go to the values' product. So the cache is read once for
 // all columns of a block, and unpacked once.
 //
-// Bound by instruction issue, close behind it by HBM: a warp takes some 1300 instructions for a tile of 32
-// positions x 256 values (unpack, products, scales), 2.5 issue in a clock and SM, the integer pipe busy half the
-// time; the loads alone take two thirds as long. 16 sequences of 9000 to 32700 positions, 8 heads of 256 for 16
-// query heads: 171-176 us, 4.0 TB/s. 64 sequences of 500 to 8100 positions with 4 rows each, 64 query heads on 8 of 128:
-// 245 us, where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
+// Bound by the latency of dependent instructions in twelve warps an SM: a warp takes some 1300 instructions for a
+// tile of 32 positions x 256 values (unpack, products, scales), of which 2.5 issue in a clock and SM (58% of the
+// slots, the integer pipe busy half the time), and 168 registers a thread leave no room for more warps; the loads
+// alone take two thirds as long. 16 sequences of 9000 to 32700 positions, 8 heads of 256 for 16 query heads: 175-177
+// us, 3.9 TB/s. 64 sequences of 500 to 8100 positions with 4 rows each, 64 query heads on 8 of 128: 250 us,
+// where the unpacked values meet 32 columns in two blocks of 16 and the softmax of those counts as much.
 // mma.sync and not tcgen05: its operands come from registers, where the unpacked values are; for
 // tcgen05 each would have to be written to shared memory once more for at most 16 columns.
 //
@@ -154,11 +155,6 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   atomicExch(err, 48);
   return false;
 }
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
-__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
-  for (uint32_t it = 0; it < (1u << 14); ++it)
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return;
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm volatile(
@@ -175,11 +171,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
   return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // a & mask | 1024 in each half, in one instruction.
 __device__ __forceinline__ uint32_t in_1024(uint32_t a, uint32_t mask) {
@@ -198,7 +189,9 @@ __device__ __forceinline__ uint32_t half2_add(uint32_t a, uint32_t c) {
   return r;
 }
 // Nibbles n = 0..3 of each half of a word as fp16 pairs n - 8: in the first four bits of 1024's mantissa a
-// nibble makes it 1024 + n, in the next four 1024 + 16 n; - 1032, or / 16 - 72, is exact.
+// nibble makes it 1024 + n, in the next four 1024 + 16 n; - 1032, or / 16 - 72, is exact. (The conversion of
+// 4-bit weights by one logic operation and one of fp16 arithmetic: Kim, Henry, Fahim and Awadalla, "Who Says
+// Elephants Can't Run", 2022.)
 __device__ __forceinline__ void pairs(uint32_t w, uint32_t (&x)[4]) {
   const uint32_t h = w >> 8;
   x[0] = half2_add(in_1024(w, 0x000F000Fu), 0xE408E408u);
@@ -322,7 +315,8 @@ __device__ __forceinline__ void add_values(float (&o)[NG][2][NT][4], const float
 constexpr int kDeep = 14;
 // The same in several rounds: the products from 2^-14 on, from 2^-28 on and so on, each brought up to the first one's
 // range. Out of line, on copies in memory: inlined it took registers from every tile (8 sequences in a window 17.8 ->
-// 21.4 us, 16 long sequences 172 -> 182).
+// 21.4 us, 16 long sequences 172 -> 182). 16 sequences of 20000 positions with scales 2^16 apart in every tile: 484
+// us, in one tile 192, in none 186.
 template <int NG, int NT>
 struct Rounds {
   float o[NG][2][NT][4], p[2][NT][4];
@@ -723,7 +717,7 @@ kv4_attn_kernel(const Args a, const __grid_constant__ Maps M) {
     if (lane == 0 && done + C::kDepth < 2 * mine) load(done + C::kDepth);
   }
   if (done < 2 * mine && lane == 0)                   // a wait gave up: the loads in flight land first
-    for (int e = done; e < min(done + C::kDepth, 2 * mine); ++e) settle(&bar[(base + e) % C::kDepth], (uint32_t)((base + e) / C::kDepth) & 1);
+    for (int e = done; e < min(done + C::kDepth, 2 * mine); ++e) mbar_settle(&bar[(base + e) % C::kDepth], (uint32_t)((base + e) / C::kDepth) & 1);
   base += 2 * mine;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {

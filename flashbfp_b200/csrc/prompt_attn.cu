@@ -14,14 +14,15 @@
 //
 // softmax: weights are 2^(s c - r), c = scaling log2(e), r the row's reference: its first step's
 // maximum, raised (and O and the sum rescaled) only when a score comes out 2^8 above it, which leaves
-// the quotient O / sum what it is. fp16 weights carry a factor 2^6 that keeps small ones normal.
+// the quotient O / sum what it is (the lazily rescaled online softmax, published for attention on Blackwell). fp16
+// weights carry a factor 2^6 that keeps small ones normal.
 //
 // Bound by the tensor cores and what feeds them from shared memory: at 256 values a block's two products read
 // 192 KB and its loads write 128 KB (of 128 bytes a clock: 2500 clocks, the MMAs take 2048), at 128 the score
 // MMAs of 64 keys read 6 KB in 32 clocks. Measured per block of 128 keys and SM (148 CTAs, a long axis): two
 // tiles x 128 values 1.95 us (1270 TFLOP/s over all SMs), one tile x 256 values 1.63 us (1520). 8192 rows x 64
-// heads of 128, fp16: 1.13-1.15 ms (957-978 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44.5 us; 128 rows over 32128
-// keys: 84-88 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
+// heads of 128, fp16: 1.13-1.15 ms (953-970 TFLOP/s); 2048 rows x 16 heads of 256, bf16: 44.5 us; 128 rows over 32128
+// keys: 86-88 us. Tried and left out: two teams of four warps for each tile (the softmax is not what is waited for),
 // scores of 128 keys at once for heads of 128 (fewer bytes from shared memory, but no buffer to run ahead in).
 #include <cuda.h>
 #include <cmath>
@@ -115,11 +116,6 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Ctl& ctl, i
   if (__builtin_expect(ok != 0, 1)) return true;
   return wait_long(bar, parity, ctl, err, site);
 }
-// After a wait gave up: what is in flight lands first (a bound of its own again, some 0.3 s).
-__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
-  for (uint32_t it = 0; it < (1u << 14); ++it)
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return;
-}
 
 __device__ __forceinline__ void tma_3d_g2s(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -173,11 +169,6 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t n, bool b_n_major) {
          ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -235,7 +226,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const float* v) {
   tmem_st_32x32b_x32(addr, r);
 }
 
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 // Whether `x` holds for any of a tile's 128 rows: vote number `k` of tile t, whose rows all take part, with
 // a bounded wait. A slot is cleared two votes before it is used again.
 __device__ __forceinline__ bool any_of_tile(bool x, int t, uint32_t& k, Ctl& ctl, int32_t* err, bool& ok) {
@@ -939,13 +929,13 @@ prompt_attn_kernel(const PromptArgs a, const __grid_constant__ PromptMaps M) {
     if (warp == kLoad) {
       // a slot is loaded again only when its last load has been used: each lane's last units remain
       for (int u = last; u >= 0 && u > last - C::kUnits; u -= C::kPer)
-        settle(&ctl.full[u % C::kUnits], (uint32_t)(u / C::kUnits) & 1);
+        mbar_settle(&ctl.full[u % C::kUnits], (uint32_t)(u / C::kUnits) & 1);
       if (q_loads > 0 && lane == 0)
-        for (int t = 0; t < C::kTiles; ++t) settle(&ctl.q_full[t], (uint32_t)(q_loads - 1) & 1);
+        for (int t = 0; t < C::kTiles; ++t) mbar_settle(&ctl.q_full[t], (uint32_t)(q_loads - 1) & 1);
     }
     if (warp >= kMma && elect_one_sync()) {          // the lanes that issued
       mma_commit(&ctl.drain);
-      settle(&ctl.drain, 0);
+      mbar_settle(&ctl.drain, 0);
     }
     __syncthreads();
   }

@@ -75,6 +75,20 @@ __device__ __forceinline__ bool mbar_wait_second(uint64_t* bar, uint32_t parity,
   }
 }
 
+// After a wait gave up: what is in flight lands first (a bound of its own again, some 0.3 s).
+__device__ __forceinline__ void mbar_settle(uint64_t* bar, uint32_t parity) {
+  for (uint32_t it = 0; it < (1u << 14); ++it)
+    if (mbar_try_wait_sleep(bar, parity, 20000u)) return;
+}
+// What threads read or wrote in shared memory comes before copies and MMAs that use it.
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---------------------------------------------------------------- bulk copies
 // 1-D bulk copy global -> shared completing on an mbarrier (size and both addresses
 // must be multiples of 16 bytes); the destination is this CTA's shared memory.
