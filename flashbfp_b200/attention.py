@@ -30,7 +30,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     ``out``: undefined). ``scaling`` is 1 / sqrt(D) by default.
 
     Scores, softmax statistics and sums are fp32; the weights are rounded to the inputs' type for the
-    product with v, the result once to it. ``err``: an int32 that records a device-side wait which gave up,
+    product with v (fp16: by 2^-11 of themselves, or by 2^-31 of the row's largest), the result once to it. ``err``: an int32 that records a device-side wait which gave up,
     by default one per device that ``check_device_errors`` reads."""
     return (device_errors._bind or device_errors.module()).prompt_attention(q, k, v, starts, kv_starts, window,
                                                                             scaling, out, err)

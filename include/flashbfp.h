@@ -414,8 +414,8 @@ int fbfp_fp8_linear(const void* x, int64_t m, int64_t k, int64_t ldx, const void
 /* ------------------------------------------------------------------------------------
  * Attention of packed prompts, and the key/value cache held in 4 bits (no counterpart in the
  * reference). Packed rows: `starts` holds seqs + 1 ascending int32; rows starts[b] ..
- * starts[b + 1] - 1 are sequence b's, rows from starts[seqs] on nobody's: they are neither read
- * nor written. A null `starts`: row r is sequence r. Heads of head_dim values, a multiple of 8 up to
+ * starts[b + 1] - 1 are sequence b's, rows from starts[seqs] on nobody's: their values count for
+ * nothing, and they are not written. A null `starts`: row r is sequence r. Heads of head_dim values, a multiple of 8 up to
  * 256; query head h reads key/value head h / (heads / kv_heads). Strides in elements.
  *
  * The cache: for keys and for values, `values` [seqs][kv_heads][positions][16 g] bytes and `scales`
